@@ -398,6 +398,82 @@ int wn_dense_decode_attention(
     float scale, int pages_per_split, int num_splits,
     void* stream, void* ev_begin, void* ev_end);
 
+/* ---- a speculative decoding step: a tree of drafted tokens over the packed cache ---- */
+
+/* Split count of wn_tree_attention for this shape on the current device (max_len: the
+ * longest sequence, drafted tokens included; any count 1 .. 4096 is valid). */
+int wn_tree_plan(int B, int Hq, int Hkv, int T, int D, int S, int bw_k, int bw_v, int exact, int max_len,
+                 int* num_splits);
+
+/* Bytes of scratch wn_tree_attention needs for this shape: the rotated queries, the nodes'
+ * visible sets and num_splits (acc, m, l) partials per row. -1 for invalid sizes. */
+int64_t wn_tree_workspace_bytes(int B, int Hq, int Hkv, int T, int D, int exact, int num_splits);
+
+/* Attention of T <= 64 drafted tokens (nodes of a tree) per sequence over paged packed K/V.
+ * The cache already holds the nodes: node i of sequence b is position seq_lens[b] - T + i.
+ * It sees every position before the tree and, of the nodes, itself and its ancestors; a
+ * node that would lie before position 0 (seq_lens[b] < T) does not exist as a key, and a
+ * query that sees no key gives 0.
+ *   q        (B, Hq, T, D) with element strides, last dim contiguous, type q_dtype
+ *   parents  (B, T) int32, row stride parents_stride_b (0: one tree for all): the node's
+ *            parent, which comes before it; any other value (-1) hangs the node on the
+ *            last position before the tree
+ *   out      (B, Hq, T, D) contiguous, type out_dtype
+ * The algebra, pages, norms, table and rotations are those of wn_decode_attention; head_dim
+ * 16 .. 256 (powers of two), every pair of widths, any n_rep with n_rep * T <= 2^20, S a
+ * power of two >= 16. Pages 4-byte aligned in base and strides, Pi_K 16-byte aligned.
+ * exact != 0: products of two fp16 terms per factor, fp32 accuracy; exact = 0: one fp16
+ * term (11 significant bits, rounded to nearest), fp32 accumulation.
+ * num_pages: pages the strides address; max_pages: width of page_table. Lengths are taken
+ * as within [0, max_pages * S] and page ids as within [0, num_pages) (a page id outside
+ * reads the last page: the Python layer refuses both before the call). ev_begin / ev_end
+ * (hipEvent_t or NULL) are recorded around the scan kernel. */
+int wn_tree_attention(
+    const void* q, int q_dtype, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_t,
+    const float* pi_k, const float* pi_v, const float* codebook_k, const float* codebook_v,
+    const uint8_t* k_pages, int64_t k_stride_p, int64_t k_stride_h,
+    const uint8_t* v_pages, int64_t v_stride_p, int64_t v_stride_h,
+    const uint16_t* k_norms, int64_t kn_stride_p, int64_t kn_stride_h,
+    const uint16_t* v_norms, int64_t vn_stride_p, int64_t vn_stride_h,
+    const int32_t* page_table, int64_t table_stride_b, const int32_t* seq_lens,
+    const int32_t* parents, int64_t parents_stride_b,
+    void* out, int out_dtype, void* workspace, int64_t workspace_bytes,
+    int B, int Hq, int Hkv, int T, int D, int S, int bw_k, int bw_v, int num_pages, int max_pages,
+    float scale, int exact, int num_splits, void* stream, void* ev_begin, void* ev_end);
+
+/* Keeps the accepted branch of a tree: for i < counts[b] (clipped to [0, A]) the row of node
+ * path[b, i], position start_pos[b] + path[b, i], moves to position start_pos[b] + i, in every
+ * layer and kv head, K and V, and lengths[b] = start_pos[b] + counts[b]. Every source is read
+ * before a position is written, so a branch may move onto itself. Rows are k_row / v_row bytes
+ * at pages + layer * stride_l + page * stride_p + head * stride_h + slot * row (bytes); fp16
+ * norms with strides in elements, or both null (an unquantized cache). A node outside
+ * [0, nodes), a position outside the table or a page outside [0, num_pages) moves nothing.
+ * 1 <= A <= nodes <= 64, S a power of two; lengths may not be start_pos. */
+int wn_commit_kv(
+    uint8_t* k_pages, int64_t k_stride_l, int64_t k_stride_p, int64_t k_stride_h, int k_row,
+    uint8_t* v_pages, int64_t v_stride_l, int64_t v_stride_p, int64_t v_stride_h, int v_row,
+    uint16_t* k_norms, int64_t kn_stride_l, int64_t kn_stride_p, int64_t kn_stride_h,
+    uint16_t* v_norms, int64_t vn_stride_l, int64_t vn_stride_p, int64_t vn_stride_h,
+    const int32_t* page_table, int64_t table_stride_b, const int32_t* start_pos,
+    const int32_t* path, int64_t path_stride_b, const int32_t* counts, int32_t* lengths,
+    int layers, int B, int Hkv, int S, int A, int nodes, int num_pages, int max_pages, void* stream);
+
+/* Log probabilities of given tokens, entropy and the `top` most likely alternatives of N rows
+ * of V logits (row r at logits + (r / inner) * stride_outer + (r % inner) * stride_inner
+ * elements, contiguous along V).
+ *   logprob (N)            x[tokens[r]] - logsumexp(x); NaN for a token outside [0, V).
+ *                          tokens and logprob may both be null
+ *   entropy (N)            -sum p log p (may be null)
+ *   top_logprobs, top_ids  (N, top), the largest first, equal logits by the lowest index
+ * Logits of -inf have probability 0; a row with a NaN or +inf, or without a finite logit,
+ * gives NaN. top <= 64 and <= V. The workspace is wn_token_logprobs_workspace_bytes (0: none
+ * needed), 256-byte aligned. */
+int64_t wn_token_logprobs_workspace_bytes(int64_t N, int V, int top);
+int wn_token_logprobs(const void* logits, int dtype, int64_t stride_outer, int64_t stride_inner, int64_t inner,
+                      const int64_t* tokens, float* logprob, float* entropy, float* top_logprobs,
+                      int64_t* top_ids, int64_t N, int V, int top, void* workspace, int64_t workspace_bytes,
+                      void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -151,6 +151,36 @@ SIGNATURES = {
         _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i,   # B Hq Hkv Q D S bwk bwv
         _c_f, _c_i,                                 # scale, num_splits
         _c_p, _c_p, _c_p]),                         # stream, ev_begin, ev_end
+    "wn_tree_plan": (_c_i, [_c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, ctypes.POINTER(_c_i)]),
+    "wn_tree_workspace_bytes": (_c_i64, [_c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i]),
+    "wn_tree_attention": (_c_i, [
+        _c_p, _c_i, _c_i64, _c_i64, _c_i64,         # q, dtype, strides (b, h, t)
+        _c_p, _c_p, _c_p, _c_p,                     # pi_k, pi_v, codebooks
+        _c_p, _c_i64, _c_i64,                       # k pages
+        _c_p, _c_i64, _c_i64,                       # v pages
+        _c_p, _c_i64, _c_i64,                       # k norms
+        _c_p, _c_i64, _c_i64,                       # v norms
+        _c_p, _c_i64, _c_p,                         # table, stride, seq_lens
+        _c_p, _c_i64,                               # parents, stride
+        _c_p, _c_i, _c_p, _c_i64,                   # out, out dtype, workspace
+        _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i,   # B Hq Hkv T D S bwk bwv num_pages max_pages
+        _c_f, _c_i, _c_i,                           # scale, exact, num_splits
+        _c_p, _c_p, _c_p]),                         # stream, ev_begin, ev_end
+    "wn_commit_kv": (_c_i, [
+        _c_p, _c_i64, _c_i64, _c_i64, _c_i,         # k pages, strides (layer, page, head), row bytes
+        _c_p, _c_i64, _c_i64, _c_i64, _c_i,         # v pages
+        _c_p, _c_i64, _c_i64, _c_i64,               # k norms
+        _c_p, _c_i64, _c_i64, _c_i64,               # v norms
+        _c_p, _c_i64, _c_p,                         # table, stride, start_pos
+        _c_p, _c_i64, _c_p, _c_p,                   # path, stride, counts, lengths
+        _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i,   # layers B Hkv S A nodes num_pages max_pages
+        _c_p]),
+    "wn_token_logprobs_workspace_bytes": (_c_i64, [_c_i64, _c_i, _c_i]),
+    "wn_token_logprobs": (_c_i, [
+        _c_p, _c_i, _c_i64, _c_i64, _c_i64,         # logits, dtype, strides (outer, inner), inner
+        _c_p, _c_p, _c_p, _c_p, _c_p,               # tokens, logprob, entropy, top_logprobs, top_ids
+        _c_i64, _c_i, _c_i, _c_p, _c_i64,           # N, V, top, workspace, bytes
+        _c_p]),
 }
 
 # bench.py's measurement probes (include/winnow_probe.h): libwinnow_probe.so beside

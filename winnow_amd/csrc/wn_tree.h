@@ -1,0 +1,112 @@
+// Attention of a tree of drafted tokens over paged packed K/V for gfx950: up to 64
+// drafted tokens (nodes) per sequence, whose K and V are the last T positions of the
+// cache. Node i sees every position before the tree and, among the nodes, itself and
+// its ancestors; with s = scale q . k_hat and k_hat = n_K (c_K Pi_K),
+//   out = softmax(s) v_hat = (sum_j p_j n_V,j c_V,j) Pi_V / sum_j p_j,
+// so the query is rotated once (q' = q Pi_K^T), keys and values are read as codes and
+// norms, and the value sum is rotated back once per row.
+//
+// Three launches on the caller's stream:
+//   1. tree_rotate_kernel  q' of every row (row r of a (sequence, kv head) is node
+//                          r / n_rep, head r % n_rep of the group) as fp16, or as two
+//                          fp16 terms, with a power-of-two scale per row; and every
+//                          node's 64-bit word of visible nodes, from the parents;
+//   2. tree_scan_kernel    one work-group per (sequence, kv head, row block, split of the
+//                          tokens): online softmax over its chunks, an (acc, m, l)
+//                          partial per row;
+//   3. tree_merge_kernel   per row the max-stable merge of its splits, 1/l, Pi_V, cast.
+//
+// The scan, per chunk of 64 tokens (32 at head_dim 256): all threads turn the packed rows
+// into fp16 tiles in LDS, K as [token][dim] and V as [dim][token], each code looked up
+// once per work-group in a table of (high, low) fp16 terms of 2^8 c, one copy per bank;
+// then wave (rg, tg) takes row group rg and token group tg. Per 16 x 16 tile (lane
+// 16 g + c) scores have A = K (row c = token tile_row(t, c), k-slots = 8 dims) and B = q'
+// (column c = query row), so that a lane's score registers of tiles 2ks, 2ks + 1 are the
+// consecutive tokens 32 ks + 8 g .. + 7 of one row: as the value product's B operand P
+// never leaves the registers, and A is one 16-byte read of the V tile.
+//
+// Precision. EX = true: every factor is a sum of two fp16 terms (22 bits), and each product
+// the three larger of their four products (what is left out is below 2^-22 of a term):
+// fp32 accuracy for fp16 and fp32 results. EX = false: one fp16 term per factor (rounded to
+// nearest, 2^-12 of a factor at most, three bits finer than a bf16 result's own rounding),
+// a third of the matrix work. Sums, maxima and partials are fp32 either way.
+#pragma once
+
+#include <cstdint>
+#include <utility>
+
+#include "wn_common.h"
+
+namespace wn {
+
+struct TreeArgs {
+  const _Float16* qh;  // (B Hkv nrp, D) high terms of q' 2^e
+  const _Float16* ql;  // low terms (EX)
+  const float* qs;     // (B Hkv nrp) scale log2(e) 2^-(e + 8)
+  const uint64_t* vis; // (B T) visible nodes of a node
+  const uint8_t* k_pages;
+  const uint8_t* v_pages;
+  const uint16_t* k_norms;
+  const uint16_t* v_norms;
+  const float* cb_k;
+  const float* cb_v;
+  const int32_t* table;
+  const int32_t* seq_lens;
+  float* part_acc;             // (items, 16, D), item = ((b Hkv + kvh) nsplit + s) nrp / 16 + row block
+  float* part_ml;              // (items, 16, 2): maximum (log2 units), sum
+  int64_t ksp, ksh, vsp, vsh;  // page strides, bytes
+  int64_t knp, knh, vnp, vnh;  // norm strides, elements
+  int64_t tsb;                 // page-table row stride, elements
+  int B, Hkv, n_rep, T, nrp, ncg, nsplit, log2S, max_pages, num_pages, bwk, bwv;
+};
+
+struct TreeRotArgs {
+  const void* q;
+  int64_t qsb, qsh, qsq;  // element strides of q (B, Hq, T, D)
+  const float* pi;
+  const int32_t* parents;
+  int64_t psb;  // parents' row stride, elements
+  _Float16* qh;
+  _Float16* ql;
+  float* qs;
+  uint64_t* vis;
+  float scale;  // scale log2(e)
+  int Hkv, n_rep, T, nrp, q_dtype, exact;
+};
+
+struct TreeMergeArgs {
+  const float* part_acc;
+  const float* part_ml;
+  const float* pi_v;
+  void* out;  // (B, Hq, T, D) contiguous
+  int out_dtype, Hkv, n_rep, T, nrp, nsplit;
+};
+
+using TreeScanFn = void (*)(TreeArgs);
+using TreeRotFn = void (*)(TreeRotArgs);
+using TreeMergeFn = void (*)(TreeMergeArgs);
+
+struct TreeScan {
+  TreeScanFn fn = nullptr;
+  int rows = 0, threads = 0;  // query rows and threads of a work-group
+  int lds = 0;                // bytes without the codebook tables
+};
+
+struct TreeKernels {
+  TreeScan scan[3];  // for up to 32, up to 64 and more rows per kv head
+  TreeRotFn rotate = nullptr;
+  TreeMergeFn merge = nullptr;
+};
+
+// Bytes of one side's codebook table in LDS: 2^bw entries of (high, low), a copy per bank
+// (16 of 6-bit tables, 8 of 8-bit ones: their size).
+__host__ __device__ constexpr int tree_copies(int bw) { return bw <= 5 ? 32 : bw == 6 ? 16 : 8; }
+__host__ __device__ constexpr int tree_table_bytes(int bw) { return (4 << bw) * tree_copies(bw); }
+
+TreeKernels tree_kernels_16(bool exact);
+TreeKernels tree_kernels_32(bool exact);
+TreeKernels tree_kernels_64(bool exact);
+TreeKernels tree_kernels_128(bool exact);
+TreeKernels tree_kernels_256(bool exact);
+
+}  // namespace wn

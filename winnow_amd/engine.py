@@ -13,6 +13,9 @@ machine-readable ``reason``), ``Request``, ``EngineConfig``, and ``Engine`` with
 * decoding is greedy, so a request's tokens depend on its prompt alone and a batched
   run equals the request run by itself.
 
+A request that sets ``top_logprobs`` also gets a ``TokenScore`` per generated token (in
+``logprobs`` and in the token events), from ``logprobs.token_logprobs`` over the step's logits.
+
 Structure (this module's own):
 
 * Running requests sit in ``max_batch`` fixed batch slots; a finished request frees
@@ -37,6 +40,7 @@ from dataclasses import dataclass, field
 
 import torch
 
+from winnow_amd.logprobs import MAX_TOP, token_logprobs
 from winnow_amd.packed_backend import PagedPackedCache
 from winnow_amd.page_pool import PoolExhausted, default_fence
 
@@ -47,6 +51,15 @@ class Refused(RuntimeError):
     def __init__(self, reason: str, detail: str = ""):
         super().__init__(f"{reason}: {detail}" if detail else reason)
         self.reason = reason
+
+
+@dataclass(frozen=True)
+class TokenScore:
+    """How likely a generated token was under the model, and what else was."""
+
+    logprob: float
+    entropy: float
+    alternatives: tuple[tuple[int, float], ...]   # (token, log probability), most likely first
 
 
 @dataclass
@@ -71,6 +84,9 @@ class Request:
     finished_at: float | None = None
     cancel_requested: bool = False
     done: threading.Event = field(default_factory=threading.Event)
+    # not in the reference: score each generated token, with so many alternatives (None: not)
+    top_logprobs: int | None = None
+    logprobs: list[TokenScore] = field(default_factory=list)
 
 
 @dataclass
@@ -94,6 +110,8 @@ _RULES = (
      lambda e, r: f"{len(r.prompt_ids)} > {e.cfg.max_prompt_tokens}"),
     ("bad_max_new_tokens", lambda e, r: not 1 <= r.max_new_tokens <= e.cfg.max_new_tokens_cap,
      lambda e, r: f"must be 1..{e.cfg.max_new_tokens_cap}"),
+    ("bad_top_logprobs", lambda e, r: r.top_logprobs is not None and not 0 <= r.top_logprobs <= MAX_TOP,
+     lambda e, r: f"must be 0..{MAX_TOP}"),
     ("exceeds_request_cap", lambda e, r: e._worst_pages(r) > e.pool.max_pages_per_request,
      lambda e, r: f"{e._worst_pages(r)} pages > {e.pool.max_pages_per_request}"),
 )
@@ -249,13 +267,28 @@ class Engine:
             self.on_logits(reqs, logits)
         return logits
 
-    def _take_token(self, req: Request, token: int, now: float) -> str | None:
+    def _scores(self, reqs: list[Request], logits: torch.Tensor, tokens: list[int]) -> list[TokenScore | None]:
+        """The score of each request's token where it asked for one, in one pass over the logits."""
+        top = max((r.top_logprobs for r in reqs if r.top_logprobs is not None), default=None)
+        if top is None:
+            return [None] * len(reqs)
+        s = token_logprobs(logits, torch.tensor(tokens, device=logits.device), top=min(top, logits.shape[-1]))
+        rows = zip(s.logprob.tolist(), s.entropy.tolist(), s.top_ids.tolist() if top else [[]] * len(reqs),
+                   s.top_logprobs.tolist() if top else [[]] * len(reqs))
+        return [None if r.top_logprobs is None else
+                TokenScore(lp, h, tuple(zip(ids[:r.top_logprobs], lps[:r.top_logprobs])))
+                for r, (lp, h, ids, lps) in zip(reqs, rows)]
+
+    def _take_token(self, req: Request, token: int, now: float, score: TokenScore | None = None) -> str | None:
         """Record a generated token; the reason the request stops, if it does."""
         req.generated.append(token)
+        if score is not None:
+            req.logprobs.append(score)
         req.token_times.append(now)
         if req.first_token_at is None:
             req.first_token_at = now
-        self._notify(req, kind="token", index=len(req.generated) - 1, token_id=token, t=now)
+        self._notify(req, kind="token", index=len(req.generated) - 1, token_id=token, t=now,
+                     **({"score": score} if score is not None else {}))
         if token in self.eos and not req.ignore_eos:
             return "eos"
         return "length" if len(req.generated) >= req.max_new_tokens else None
@@ -268,14 +301,17 @@ class Engine:
         req = min(pending, key=lambda r: self._admitted_at[r.request_id])
         lo = req.stored
         hi = min(lo + self.cfg.prefill_chunk, len(req.prompt_ids))
+        last = hi == len(req.prompt_ids)
         try:
             logits = self._forward([req], [req.prompt_ids[lo:hi]])
+            token = int(logits[0].argmax()) if last else -1
+            score = self._scores([req], logits, [token])[0] if last else None
         except Exception as exc:  # noqa: BLE001 - reported on the request
             self._retire(req, "error", f"{type(exc).__name__}: {exc}", default_fence(self.device))
             return True
-        if hi == len(req.prompt_ids):
+        if last:
             req.state = "decode"
-            why = self._take_token(req, int(logits[0].argmax()), self.clock())
+            why = self._take_token(req, token, self.clock(), score)
             if why:
                 ended[req.request_id] = (req, why)
         return True
@@ -286,15 +322,17 @@ class Engine:
         if not batch:
             return False
         try:
-            tokens = self._forward(batch, [[r.generated[-1]] for r in batch]).argmax(-1).tolist()
+            logits = self._forward(batch, [[r.generated[-1]] for r in batch])
+            tokens = logits.argmax(-1).tolist()
+            scores = self._scores(batch, logits, tokens)
         except Exception as exc:  # noqa: BLE001 - reported on every request of the batch
             fence = default_fence(self.device)
             for r in batch:
                 self._retire(r, "error", f"{type(exc).__name__}: {exc}", fence)
             return True
         now = self.clock()
-        for r, t in zip(batch, tokens):
-            why = self._take_token(r, int(t), now)
+        for r, t, score in zip(batch, tokens, scores):
+            why = self._take_token(r, int(t), now, score)
             if why:
                 ended[r.request_id] = (r, why)
         return True

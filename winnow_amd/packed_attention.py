@@ -506,6 +506,144 @@ def packed_prefill_attention(q: torch.Tensor, kv: PackedKV, scale: float, *,
     return out
 
 
+TREE_NODES = 64      # drafted tokens per sequence: a node's visible nodes are one 64-bit word
+
+
+def check_tree(q: torch.Tensor, kv: PackedKV, parents: torch.Tensor) -> None:
+    """What ``packed_tree_attention`` needs beyond ``check_contract``."""
+    B, _, T, D = q.shape
+    if not 1 <= T <= TREE_NODES:
+        raise UnsupportedLayout(f"tree attention takes 1 to {TREE_NODES} drafted tokens, got {T}")
+    if not _lib.is_hip(q):
+        raise UnsupportedLayout("tree attention needs tensors on a HIP device")
+    if D not in SUPPORTED_HEAD_DIMS or not _pow2(kv.page_size):
+        raise UnsupportedLayout(f"tree attention: head_dim {D} (compiled: {SUPPORTED_HEAD_DIMS}), page size "
+                                f"{kv.page_size} (a power of two >= 16)")
+    if q.dtype not in _lib.DTYPE_CODE or q.stride(-1) != 1:
+        raise UnsupportedLayout("q must be fp32/fp16/bf16 with a contiguous head_dim")
+    if q.requires_grad and torch.is_grad_enabled():
+        raise UnsupportedLayout("tree attention has no gradient: call it under torch.no_grad() or detach q")
+    for pages, norms in ((kv.k_pages, kv.k_norms), (kv.v_pages, kv.v_norms)):
+        if pages.stride(-1) != 1 or pages.stride(-2) != pages.shape[-1]:
+            raise UnsupportedLayout("pages need contiguous (S, NB) rows")
+        if pages.data_ptr() % 4 or pages.stride(0) % 4 or pages.stride(1) % 4:
+            raise UnsupportedLayout("page base and strides must be 4-byte aligned")
+        if norms.stride(-1) != 1:
+            raise UnsupportedLayout("norms need a contiguous slot axis")
+    for quant in (kv.k_quant, kv.v_quant):
+        if not quant.Pi.is_contiguous() or quant.Pi.data_ptr() % 16 or not quant.centroids.is_contiguous():
+            raise UnsupportedLayout("rotations (16-byte aligned) and codebooks must be contiguous")
+    if kv.page_table.stride(-1) != 1 or not kv.seq_lens.is_contiguous():
+        raise UnsupportedLayout("page_table rows and seq_lens must be contiguous")
+    if kv.page_table.shape[1] < 1 or kv.page_table.shape[1] * kv.page_size > 2 ** 31 - 257:
+        raise UnsupportedLayout("page_table must hold 1 to 2^31 - 257 positions per sequence")
+    if kv.k_pages.shape[0] < 1:
+        raise UnsupportedLayout("the pool has no pages")
+    if parents.shape != (B, T) or parents.dtype != torch.int32 or parents.device != q.device \
+            or (T > 1 and parents.stride(1) != 1):
+        raise UnsupportedLayout(f"parents must be ({B}, {T}) int32 on {q.device} with contiguous rows")
+
+
+def check_parents(parents: torch.Tensor) -> None:
+    """Every node's parent comes before it, or is -1. Reads a host copy."""
+    p = parents.detach().to("cpu").numpy()
+    bad = (p < -1) | (p >= np.arange(p.shape[1])[None, :])
+    if bad.any():
+        b, i = (int(x[0]) for x in np.nonzero(bad))
+        raise UnsupportedLayout(f"sequence {b}: node {i} has parent {int(p[b, i])}, not -1 or an earlier node")
+
+
+@functools.lru_cache(maxsize=1024)
+def _tree_plan(device_index: int, *shape) -> int:
+    ns = ctypes.c_int(0)
+    with torch.cuda.device(device_index):
+        _lib.call("wn_tree_plan", *shape, ctypes.byref(ns))
+    return ns.value
+
+
+@functools.lru_cache(maxsize=1024)
+def tree_workspace_bytes(batch: int, num_q_heads: int, num_kv_heads: int, nodes: int, head_dim: int, exact: bool,
+                         num_splits: int) -> int:
+    return int(_lib.lib().wn_tree_workspace_bytes(batch, num_q_heads, num_kv_heads, nodes, head_dim, int(exact),
+                                                  num_splits))
+
+
+def tree_exact(q: torch.Tensor, out_dtype: torch.dtype, allow_tf32: bool = False) -> bool:
+    """Whether ``packed_tree_attention`` takes two fp16 terms per factor (fp32 accuracy): unless
+    the result is bf16 of a bf16 query, whose own rounding is eight times coarser than a single
+    term's, or the caller allows TF32-class products."""
+    return not (allow_tf32 or q.dtype == out_dtype == torch.bfloat16)
+
+
+def tree_plan_for(q: torch.Tensor, kv: PackedKV, exact: bool) -> int:
+    """Split count of the tree attention for this query and handle (wn_tree_plan)."""
+    B, Hq, T, D = q.shape
+    lens = kv.seq_lens_host if kv.seq_lens_host is not None else kv.seq_lens.cpu()
+    # the plan counts 64-token chunks of the longest sequence
+    longest = max(lens.tolist(), default=0)
+    return _tree_plan(q.get_device(), B, Hq, kv.num_kv_heads, T, D, kv.page_size, kv.k_quant.bit_width,
+                      kv.v_quant.bit_width, int(exact), -(-max(longest, 0) // 64) * 64)
+
+
+def packed_tree_attention(q: torch.Tensor, kv: PackedKV, scale: float, parents: torch.Tensor, *,
+                          allow_tf32: bool = False, num_splits: int | None = None,
+                          out_dtype: torch.dtype | None = None, workspace: torch.Tensor | None = None,
+                          parents_host: torch.Tensor | None = None, check_ranges: bool = True,
+                          timing_events=None) -> torch.Tensor:
+    """Attention of a tree of drafted tokens over packed pages: q (B, Hq, T, D) ->
+    (B, Hq, T, D) in q.dtype (``wn_tree_attention``).
+
+    The cache already holds the T <= 64 drafted tokens (nodes) of each sequence, as after
+    ``append_kv``: node i is position ``seq_lens[b] - T + i``. ``parents`` (B, T) int32 on
+    q's device gives each node's parent, a node before it, or -1 for a child of the last
+    token before the tree; a row stride of 0 (``expand``) shares one tree. Node i attends
+    to every position before the tree, to its ancestors and to itself. Nodes that would
+    lie before position 0 do not exist as keys; a query that sees no key gives 0.
+
+    A chain (``parents[i] = i - 1``) is the causal mask of ``packed_prefill_attention``.
+    Every head_dim, width pair, n_rep and page size of ``packed_decode_attention`` is
+    served. Products have fp32 accuracy, or, where the query and the result are bf16 or
+    ``allow_tf32`` is given, TF32-class accuracy (single fp16 operands, fp32 accumulation).
+    ``num_splits`` replaces the library's split count, ``out_dtype`` the result's type,
+    ``workspace`` is a caller-owned uint8 buffer of at least ``tree_workspace_bytes``,
+    ``timing_events`` a pair of raw ``hipEvent_t`` handles recorded around the scan.
+
+    Raises ``UnsupportedLayout`` before any launch for what ``check_contract`` and
+    ``check_tree`` reject; ``check_ranges`` covers lengths, page ids and parents, read from
+    ``parents_host`` and the handle's host mirrors when given, else copied to the host."""
+    check_contract(q, kv, check_ranges=check_ranges)
+    check_tree(q, kv, parents)
+    if check_ranges:
+        check_parents(parents if parents_host is None else parents_host)
+        if parents_host is not None and parents_host.shape != parents.shape:
+            raise UnsupportedLayout(f"parents_host is {tuple(parents_host.shape)}, parents {tuple(parents.shape)}")
+    B, Hq, T, D = q.shape
+    Hkv = kv.num_kv_heads
+    out_dtype = out_dtype or q.dtype
+    if out_dtype not in _lib.DTYPE_CODE:
+        raise UnsupportedLayout(f"output dtype {out_dtype} is not supported")
+    exact = tree_exact(q, out_dtype, allow_tf32)
+    out = torch.empty(B, Hq, T, D, dtype=out_dtype, device=q.device)
+    if B == 0:
+        return out
+    ns = int(num_splits) if num_splits else tree_plan_for(q, kv, exact)
+    need = tree_workspace_bytes(B, Hq, Hkv, T, D, exact, ns)
+    if need < 0:
+        raise UnsupportedLayout(f"bad tree sizes B={B} Hq={Hq} Hkv={Hkv} T={T} splits={ns}")
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    elif workspace.numel() * workspace.element_size() < need or workspace.device != q.device:
+        raise UnsupportedLayout(f"workspace needs {need} bytes on {q.device}")
+    ev0, ev1 = timing_events or (None, None)
+    with torch.cuda.device(q.device):
+        _lib.call("wn_tree_attention", _lib.ptr(q), _lib.DTYPE_CODE[q.dtype], q.stride(0), q.stride(1), q.stride(2),
+                  *_operands(q, kv)[4:], _lib.ptr(parents), parents.stride(0), _lib.ptr(out),
+                  _lib.DTYPE_CODE[out_dtype], _lib.ptr(workspace), workspace.numel() * workspace.element_size(),
+                  B, Hq, Hkv, T, D, kv.page_size, kv.k_quant.bit_width, kv.v_quant.bit_width, kv.k_pages.shape[0],
+                  kv.page_table.shape[1], float(scale), int(exact), ns, _lib.stream_of(q.device), ev0, ev1)
+    return out
+
+
 DENSE_PAGE_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 

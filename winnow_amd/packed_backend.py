@@ -283,6 +283,93 @@ def append_kv(k: torch.Tensor, v: torch.Tensor | None, k_tq, v_tq,
     plan.launch(bound, timing_events)
 
 
+def _check_commit_side(name: str, pages: torch.Tensor, norms, lead) -> None:
+    if pages.dim() not in (4, 5) or pages.shape[:-1] != lead:
+        raise pa.UnsupportedLayout(f"commit: {name} pages must be ([layers,] P, Hkv, S, row), got {tuple(pages.shape)}")
+    if pages.dtype not in (torch.uint8, *pa.DENSE_PAGE_DTYPES) or (pages.dtype == torch.uint8) != (norms is not None):
+        raise pa.UnsupportedLayout(f"commit: {name} pages are uint8 with norms, or fp32/fp16/bf16 without")
+    if pages.stride(-1) != 1 or pages.stride(-2) != pages.shape[-1]:
+        raise pa.UnsupportedLayout("commit: pages need contiguous (S, row) blocks")
+    if norms is not None and (norms.dtype != torch.float16 or norms.shape != lead or norms.stride(-1) != 1):
+        raise pa.UnsupportedLayout(f"commit: {name} norms must be fp16 of the pages' leading shape, slots contiguous")
+    for t in (pages, norms):
+        if t is not None and any(n > 1 and st == 0 for n, st in zip(t.shape[:-1], t.stride())):
+            raise pa.UnsupportedLayout(f"commit: {name} is written in place and may not be expanded")
+
+
+@torch.no_grad()
+def commit_kv(k_pages: torch.Tensor, v_pages: torch.Tensor, k_norms: torch.Tensor | None,
+              v_norms: torch.Tensor | None, page_table: torch.Tensor, start_pos: torch.Tensor,
+              path: torch.Tensor, counts: torch.Tensor, *, nodes: int,
+              page_table_host: torch.Tensor | None = None, start_pos_host: torch.Tensor | None = None,
+              check_ranges: bool = True) -> torch.Tensor:
+    """Keep the accepted branch of a tree of ``nodes`` drafted tokens whose K and V were
+    appended at ``start_pos`` (``append_kv``): the cache rows of node ``path[b, i]`` move to
+    position ``start_pos[b] + i`` for ``i < counts[b]``, K and V, codes and norms, in every
+    layer, in one launch (``wn_commit_kv``). Returns the new lengths ``start_pos + counts``,
+    (B,) int32; what lies behind them is as the moves left it.
+
+    Pages are one layer's (P, Hkv, S, row) or a whole pool's (layers, P, Hkv, S, row): packed
+    (uint8, with norms) or unquantized (fp32/fp16/bf16, norms None). ``path`` (B, A) and
+    ``counts`` (B,) are int32 on the device and may come straight from the acceptance; counts
+    are clipped to [0, A], and a node outside [0, nodes) moves nothing. Every row is read
+    before any is written, so the order of a path does not matter.
+
+    Raises ``UnsupportedLayout`` before the launch for operands off the GPU or of the wrong
+    shape, and (``check_ranges``) where the nodes' positions lie outside a table row or its
+    pages outside the pool, read as in ``append_kv``."""
+    packed = k_pages.dtype == torch.uint8
+    lead = k_pages.shape[:-1]
+    for name, pages, norms in (("K", k_pages, k_norms), ("V", v_pages, v_norms)):
+        _check_commit_side(name, pages, norms, lead)
+    if v_pages.dtype != k_pages.dtype:
+        raise pa.UnsupportedLayout(f"commit: K pages are {k_pages.dtype}, V pages {v_pages.dtype}")
+    ops = [k_pages, v_pages, page_table, start_pos, path, counts] + ([k_norms, v_norms] if packed else [])
+    if not all(_lib.is_hip(t) for t in ops) or len({t.device for t in ops}) != 1:
+        raise pa.UnsupportedLayout("commit: every operand must be on one HIP device")
+    layers = 1 if k_pages.dim() == 4 else k_pages.shape[0]
+    P, Hkv, S = lead[-3:]
+    if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.stride(-1) != 1:
+        raise pa.UnsupportedLayout("commit: page_table must be (B, max_pages) int32 with contiguous rows")
+    B, width = page_table.shape
+    if start_pos.dtype != torch.int32 or start_pos.shape != (B,) or not start_pos.is_contiguous():
+        raise pa.UnsupportedLayout("commit: start_pos must be (B,) int32, contiguous")
+    if counts.dtype != torch.int32 or counts.shape != (B,) or not counts.is_contiguous():
+        raise pa.UnsupportedLayout("commit: counts must be (B,) int32, contiguous")
+    if path.dim() != 2 or path.shape[0] != B or path.dtype != torch.int32 or (path.shape[1] > 1 and path.stride(1) != 1):
+        raise pa.UnsupportedLayout("commit: path must be (B, A) int32 with contiguous rows")
+    A = path.shape[1]
+    if not 1 <= A <= nodes <= pa.TREE_NODES:
+        raise pa.UnsupportedLayout(f"commit: a path of {A} of {nodes} nodes (1 <= A <= nodes <= {pa.TREE_NODES})")
+    if S & (S - 1):
+        raise pa.UnsupportedLayout(f"commit: page size {S} is not a power of two")
+    if check_ranges:
+        _positions_in_range(start_pos_host if start_pos_host is not None else start_pos.cpu(),
+                            page_table_host if page_table_host is not None else page_table.cpu(), nodes, P, S)
+    lengths = torch.empty(B, dtype=torch.int32, device=k_pages.device)
+
+    with torch.cuda.device(k_pages.device):
+        _lib.call("wn_commit_kv", *_commit_pages(k_pages), *_commit_pages(v_pages), *_commit_norms(k_norms),
+                  *_commit_norms(v_norms), _lib.ptr(page_table), page_table.stride(0), _lib.ptr(start_pos),
+                  _lib.ptr(path), path.stride(0), _lib.ptr(counts), _lib.ptr(lengths), layers, B, Hkv, S, A, nodes, P,
+                  width, _lib.stream_of(k_pages.device))
+    return lengths
+
+
+def _commit_pages(t: torch.Tensor) -> tuple:
+    """Address, layer, page and head strides in bytes, bytes of a row."""
+    size = t.element_size()
+    st = t.stride() if t.dim() == 5 else (0, *t.stride())
+    return _lib.ptr(t), st[0] * size, st[1] * size, st[2] * size, t.shape[-1] * size
+
+
+def _commit_norms(t: torch.Tensor | None) -> tuple:
+    if t is None:
+        return None, 0, 0, 0
+    st = t.stride() if t.dim() == 4 else (0, *t.stride())
+    return _lib.ptr(t), st[0], st[1], st[2]
+
+
 def _append_dense_rows(src: torch.Tensor, pages: torch.Tensor, meta: PageTable) -> None:
     """Unquantized append: row (page, h, slot) of a contiguous (P, Hkv, S, D) layer is
     flat row (page * Hkv + h) * S + slot; the addresses are formed on the device."""
@@ -304,12 +391,19 @@ class PagedPackedCache:
     tokens it already stores. A forward appends the same n tokens to every sequence
     (n = 1 for a batched decode step, a chunk for a single-sequence prefill); the
     lengths advance once the last layer has written (packed_backend.py:88-112).
+
+    ``tree`` makes the forward one over a tree of drafted tokens per sequence: the parent of
+    each of the n <= 64 tokens, (n,) for every sequence or (B, n), as a list or a host tensor
+    (``packed_attention.packed_tree_attention``; ``tree_positions`` gives the model's position
+    ids). The leases must cover the whole tree. ``commit`` then keeps the accepted branch.
     """
 
     def __init__(self, pool: PagePool, owners, lengths, *, k_quant, v_quant,
-                 head_dim: int, decode_backend: str = "auto", allow_tf32: bool = False):
+                 head_dim: int, decode_backend: str = "auto", allow_tf32: bool = False, tree=None):
         if len(owners) != len(lengths):
             raise ValueError("one length per owner")
+        self.tree = None if tree is None else _tree_parents(tree, len(owners))
+        self._tree_device: torch.Tensor | None = None
         self.pool = pool
         self.owners = list(owners)
         self.lengths = [int(L) for L in lengths]
@@ -330,9 +424,12 @@ class PagedPackedCache:
         """Page metadata of this forward: checked against the pool's leases (a short or
         released lease raises ``StalePage``; pages are never granted here), range-checked
         on the host, and uploaded to ``device`` in one copy."""
+        if self.tree is not None and self.tree.shape[1] != n:
+            raise ValueError(f"the tree has {self.tree.shape[1]} tokens, the forward {n}")
         meta = self.pool.batch_table(self.owners, self.lengths, n)
         _positions_in_range(meta.start_host, meta.table_host, n, self.pool.num_pages, self.pool.page_size)
         self.meta = meta.to(device)
+        self._tree_device = None if self.tree is None else self.tree.to(device)
         return self.meta
 
     @torch.no_grad()
@@ -358,9 +455,64 @@ class PagedPackedCache:
                                  seq_lens_host=meta.seq_host, page_table_host=meta.table_host)
         handle.decode_backend = self.decode_backend
         handle.allow_tf32 = self.allow_tf32
+        if self.tree is not None:
+            handle.tree, handle.tree_host = self._tree_device, self.tree
         if layer_idx == pool.num_layers - 1:
             self.lengths = meta.seq_host.tolist()
         return handle, handle
+
+    @torch.no_grad()
+    def commit(self, paths) -> list[int]:
+        """Keep one branch of each sequence's tree after a forward over it: ``paths[b]`` are the
+        accepted nodes from a child of the last stored token down, each the next one's parent
+        (empty: none). Their rows move to the positions right behind the history in one launch
+        over every layer (``commit_kv``), the cache forgets the rest, and ``lengths`` are the
+        tokens kept. The next forward takes a new tree or none."""
+        meta, pool = self.meta, self.pool
+        if self.tree is None or meta is None or self.lengths != meta.seq_host.tolist():
+            raise RuntimeError("commit follows a forward over a tree")
+        B, T = self.tree.shape
+        paths = [[int(i) for i in p] for p in paths]
+        if len(paths) != B:
+            raise ValueError(f"{len(paths)} paths for {B} sequences")
+        for b, p in enumerate(paths):
+            parent = -1
+            for i in p:
+                if not 0 <= i < T or int(self.tree[b, i]) != parent:
+                    raise ValueError(f"sequence {b}: {p} is not a branch of its tree from the root down")
+                parent = i
+        A = max([1] + [len(p) for p in paths])
+        host = torch.tensor([p + [0] * (A - len(p)) + [len(p)] for p in paths], dtype=torch.int32).reshape(B, A + 1)
+        if B:
+            dev = host.to(pool.device)
+            commit_kv(pool.k_pages, pool.v_pages, pool.k_norms, pool.v_norms, meta.table, meta.start, dev[:, :A],
+                      dev[:, A].contiguous(), nodes=T, page_table_host=meta.table_host, start_pos_host=meta.start_host)
+        self.lengths = (meta.start_host + host[:, A]).tolist()
+        self.meta = self.tree = self._tree_device = None
+        return self.lengths
+
+
+def _tree_parents(tree, batch: int) -> torch.Tensor:
+    """(batch, n) int32 parents on the host; ``UnsupportedLayout`` unless they make a tree."""
+    t = torch.as_tensor(tree).to("cpu", torch.int32)
+    if t.dim() == 1:
+        t = t[None].expand(batch, -1)
+    if t.dim() != 2 or t.shape[0] != batch or not 1 <= t.shape[1] <= pa.TREE_NODES:
+        raise pa.UnsupportedLayout(f"tree must be (n,) or ({batch}, n) parents, 1 <= n <= {pa.TREE_NODES}, got {tuple(t.shape)}")
+    pa.check_parents(t)
+    return t.contiguous()
+
+
+def tree_positions(tree, lengths) -> torch.Tensor:
+    """Position ids (B, n) int64 of a tree's tokens behind histories of ``lengths`` tokens: a
+    token's position is its depth in the tree, not its place in the cache."""
+    lengths = torch.as_tensor(lengths, dtype=torch.int64)
+    parents = _tree_parents(tree, lengths.numel()).to(torch.int64)
+    depth = torch.zeros_like(parents)
+    for i in range(parents.shape[1]):
+        up = parents[:, i]
+        depth[:, i] = torch.where(up >= 0, depth.gather(1, up.clamp(min=0)[:, None])[:, 0] + 1, 0)
+    return lengths[:, None] + depth
 
 
 # ---------------------------------------------------------------------------- attention
@@ -478,10 +630,13 @@ def _offset_causal(lens: torch.Tensor, Q: int, Lmax: int, device):
     return mask[:, None].to(device), (last >= 0)[:, None, :, None].to(device)
 
 
-def _padded_sdpa(query, k, v, lens, scaling):
+def _padded_sdpa(query, k, v, lens, scaling, tree=None):
     """One SDPA call over histories padded to the longest; rows without a key are 0."""
     B, Hq, Q, _ = query.shape
-    mask, live = _offset_causal(lens, Q, k.shape[2], query.device)
+    if tree is None:
+        mask, live = _offset_causal(lens, Q, k.shape[2], query.device)
+    else:
+        mask, live = _tree_mask(tree, lens, k.shape[2], query.device)
     out = F.scaled_dot_product_attention(query, k, v, attn_mask=mask, scale=scaling,
                                          enable_gqa=Hq != k.shape[1])
     return torch.where(live, out, torch.zeros((), dtype=out.dtype, device=out.device))
@@ -616,9 +771,25 @@ def _library_sdpa(query, kv: pa.PackedKV, lens: torch.Tensor, Lmax: int, scaling
     return _padded_sdpa(query, hist[0], hist[1], lens, scaling)
 
 
+def _tree_mask(parents: torch.Tensor, lens: torch.Tensor, Lmax: int, device):
+    """(B, 1, T, Lmax) mask of a tree's tokens over histories that end with them, and whether a
+    row sees any key; ``parents`` and ``lens`` on the host."""
+    B, T = parents.shape
+    sees = torch.eye(T, dtype=torch.bool).repeat(B, 1, 1)
+    for i in range(T):
+        up = parents[:, i].to(torch.int64)
+        rows = sees[torch.arange(B), up.clamp(min=0)]
+        sees[:, i] |= rows & (up >= 0)[:, None]
+    node = torch.arange(Lmax)[None, :] - (lens[:, None] - T)                              # (B, Lmax)
+    mask = sees.gather(2, node.clamp(0, T - 1)[:, None, :].expand(B, T, Lmax)) & (node < T)[:, None, :]
+    mask |= (node < 0)[:, None, :]
+    return mask[:, None].to(device), mask.any(-1)[:, None, :, None].to(device)
+
+
 def _dense_sdpa(query, kv: pa.DenseKV, scaling):
     """Gather every sequence's unquantized rows into one padded (B, Hkv, Lmax, D) pair with
-    one indexed read per side, then one offset-causal SDPA (packed_backend.py:229-246)."""
+    one indexed read per side, then one SDPA under the offset-causal mask
+    (packed_backend.py:229-246) or the handle's tree."""
     B, Hq, Q, D = query.shape
     lens = _host_lens(kv).to(torch.int64)
     Lmax = int(lens.max()) if B else 0
@@ -632,7 +803,7 @@ def _dense_sdpa(query, kv: pa.DenseKV, scaling):
     slot = (t % S).to(query.device)[None, :].expand(B, Lmax)
     k = kv.k_pages[page, :, slot].permute(0, 2, 1, 3).to(query.dtype)         # (B, Hkv, Lmax, D)
     v = kv.v_pages[page, :, slot].permute(0, 2, 1, 3).to(query.dtype)
-    return _padded_sdpa(query, k, v, lens, scaling)
+    return _padded_sdpa(query, k, v, lens, scaling, getattr(kv, "tree_host", None))
 
 
 def _hip_packed(query, kv, scaling):
@@ -641,6 +812,11 @@ def _hip_packed(query, kv, scaling):
 
 def _hip_dense(query, kv, scaling):
     return pa.dense_decode_attention(query, kv, scaling)
+
+
+def _hip_tree(query, kv, scaling):
+    return pa.packed_tree_attention(query, kv, scaling, kv.tree, allow_tf32=getattr(kv, "allow_tf32", False),
+                                    parents_host=kv.tree_host)
 
 
 def _hip_prefill(query, kv, scaling):
@@ -655,10 +831,14 @@ _ROUTES = {
     "hip_dense": _hip_dense,
     "dense_sdpa": _dense_sdpa,
     "prefill_dense_sdpa": _dense_sdpa,
+    "tree_hip_packed": _hip_tree,
+    "tree_dense_sdpa": _dense_sdpa,
 }
 
 
 def _route(query, kv) -> str:
+    if getattr(kv, "tree", None) is not None:
+        return "tree_dense_sdpa" if isinstance(kv, pa.DenseKV) else "tree_hip_packed"
     if query.shape[2] > 1:
         if isinstance(kv, pa.DenseKV):
             return "prefill_dense_sdpa"
