@@ -11,13 +11,13 @@ namespace {
 
 constexpr int kTreeNodes = 64;
 
-TreeKernels pick_tree(int D, bool exact) {
+TreeKernels pick_tree(int D, bool exact, int bw_k, int bw_v) {
   switch (D) {
-    case 16: return tree_kernels_16(exact);
-    case 32: return tree_kernels_32(exact);
-    case 64: return tree_kernels_64(exact);
-    case 128: return tree_kernels_128(exact);
-    case 256: return tree_kernels_256(exact);
+    case 16: return tree_kernels_16(exact, bw_k, bw_v);
+    case 32: return tree_kernels_32(exact, bw_k, bw_v);
+    case 64: return tree_kernels_64(exact, bw_k, bw_v);
+    case 128: return tree_kernels_128(exact, bw_k, bw_v);
+    case 256: return tree_kernels_256(exact, bw_k, bw_v);
     default: return TreeKernels{};
   }
 }
@@ -66,7 +66,9 @@ int tree_slots(const TreeScan& s, int lds) {
   return n;
 }
 
-int tree_lds(const TreeScan& s, int bw_k, int bw_v) { return s.lds + tree_table_bytes(bw_k) + tree_table_bytes(bw_v); }
+int tree_lds(const TreeScan& s, int bw_k, int bw_v) {
+  return std::max(s.give, s.lds + (s.tables ? s.tables : tree_table_bytes(bw_k) + tree_table_bytes(bw_v)));
+}
 
 bool tree_shape(int B, int Hq, int Hkv, int T, int D) {
   return B >= 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && T > 0 && T <= kTreeNodes && valid_head_dim(D) &&
@@ -85,7 +87,7 @@ extern "C" int wn_tree_plan(int B, int Hq, int Hkv, int T, int D, int S, int bw_
   WN_REQUIRE(is_pow2(S) && S >= 16 && valid_bw(bw_k) && valid_bw(bw_v), WN_E_UNSUPPORTED,
              "wn_tree_plan: (S=%d, bw_k=%d, bw_v=%d) not compiled", S, bw_k, bw_v);
   const int64_t rows = int64_t(Hq / Hkv) * T;
-  const TreeKernels k = pick_tree(D, exact != 0);
+  const TreeKernels k = pick_tree(D, exact != 0, bw_k, bw_v);
   const TreeScan& scan = tree_variant(k, rows);
   const int slots = tree_slots(scan, tree_lds(scan, bw_k, bw_v));
   WN_REQUIRE(slots > 0, WN_E_LAUNCH, "wn_tree_plan: cannot query the device occupancy");
@@ -99,7 +101,7 @@ extern "C" int64_t wn_tree_workspace_bytes(int B, int Hq, int Hkv, int T, int D,
   using namespace wn;
   if (!tree_shape(B, Hq, Hkv, T, D) || num_splits <= 0) return -1;
   const int64_t rows = int64_t(Hq / Hkv) * T;
-  const TreeKernels k = pick_tree(D, exact != 0);
+  const TreeKernels k = pick_tree(D, exact != 0, 4, 4);  // the rows of a work-group do not go by the widths
   return tree_layout(B, Hkv, tree_nrp(tree_variant(k, rows), rows), T, D, num_splits).total;
 }
 
@@ -141,7 +143,7 @@ extern "C" int wn_tree_attention(
              WN_E_INVALID, "tree: Pi_K 16-byte aligned, q and out aligned to their type");
   const int n_rep = Hq / Hkv;
   const int64_t rows = int64_t(n_rep) * T;
-  const TreeKernels k = pick_tree(D, exact != 0);
+  const TreeKernels k = pick_tree(D, exact != 0, bw_k, bw_v);
   const TreeScan& scan = tree_variant(k, rows);
   const int nrp = tree_nrp(scan, rows), ncg = nrp / scan.rows;
   const TreeLayout lay = tree_layout(B, Hkv, nrp, T, D, num_splits);

@@ -89,7 +89,8 @@ using TreeMergeFn = void (*)(TreeMergeArgs);
 struct TreeScan {
   TreeScanFn fn = nullptr;
   int rows = 0, threads = 0;  // query rows and threads of a work-group
-  int lds = 0;                // bytes without the codebook tables
+  int lds = 0, tables = 0;    // LDS bytes without the codebook tables; theirs (0: by the widths)
+  int give = 0;               // LDS bytes that the hand-over at the end takes
 };
 
 struct TreeKernels {
@@ -103,10 +104,10 @@ struct TreeKernels {
 __host__ __device__ constexpr int tree_copies(int bw) { return bw <= 5 ? 32 : bw == 6 ? 16 : 8; }
 __host__ __device__ constexpr int tree_table_bytes(int bw) { return (4 << bw) * tree_copies(bw); }
 
-TreeKernels tree_kernels_16(bool exact);
-TreeKernels tree_kernels_32(bool exact);
-TreeKernels tree_kernels_64(bool exact);
-TreeKernels tree_kernels_128(bool exact);
-TreeKernels tree_kernels_256(bool exact);
+TreeKernels tree_kernels_16(bool exact, int bw_k, int bw_v);
+TreeKernels tree_kernels_32(bool exact, int bw_k, int bw_v);
+TreeKernels tree_kernels_64(bool exact, int bw_k, int bw_v);
+TreeKernels tree_kernels_128(bool exact, int bw_k, int bw_v);
+TreeKernels tree_kernels_256(bool exact, int bw_k, int bw_v);
 
 }  // namespace wn

@@ -20,22 +20,41 @@ struct TreeGeo {
   static constexpr int DP = D < 32 ? 32 : D;        // K dims, padded to one K-step
   static constexpr int KS = DP / 32, MT = D / 16;   // score K-steps, value M-tiles
   static constexpr int CH = D == 256 ? 32 : 64;     // tokens per chunk
-  static constexpr int KROW = 2 * DP + 16;          // bytes of a K tile row: 16 rows in 16 bank quads
-  static constexpr int VROW = 2 * CH + 16;          // bytes of a V tile row
+  static constexpr int NG = CH / 16;                // 16-token groups, each within a page (S >= 16)
+  // K tile rows of whole 16-byte columns, swapped by a key of the token (rows of 128 bytes and
+  // more) or padded (shorter ones), so that the eight rows that eight lanes read lie in different
+  // banks; V tile rows of 2 CH bytes, swapped by a key of the dim for reads and writes alike
+  static constexpr int KROW = DP >= 64 ? 2 * DP : 2 * DP + 16;
+  static constexpr int VROW = 2 * CH;
   static constexpr int KT = CH * KROW, VT = D * VROW;
+  __device__ static uint32_t k_at(int tok, int col) {
+    if constexpr (DP >= 64) return uint32_t(tok * KROW + ((col ^ ((tok & 3) | (tok >> 1 & 4))) << 4));
+    else return uint32_t(tok * KROW + (col << 4));
+  }
+  __device__ static uint32_t v_key(int row) { return CH == 64 ? (row ^ row >> 3) & 7 : (row >> 1 ^ row >> 3) & 3; }
+  __device__ static uint32_t v_at(int row, int col) { return uint32_t(row * VROW) + ((uint32_t(col) ^ v_key(row)) << 4); }
 };
 
 // Token of row c of score tile t.
 __device__ __forceinline__ int tree_tok(int t, int c) { return 32 * (t >> 1) + 8 * (c >> 2) + 4 * (t & 1) + (c & 3); }
 
-// The raw words of one group of eight codes: the up to two 4-byte words that hold bytes
+// The raw words of one group of eight codes: the one or two 4-byte words that hold bytes
 // [o, o + bw) of a block; a word without any of them is not read.
 struct TreeRaw {
   uint32_t lo, hi;
 };
+template <int BW>
 __device__ __forceinline__ TreeRaw tree_raw(const uint8_t* block, uint32_t o, int bw) {
-  const uint32_t a = o & ~3u, b = (o + uint32_t(bw) - 1) & ~3u;
-  return TreeRaw{*reinterpret_cast<const uint32_t*>(block + a), *reinterpret_cast<const uint32_t*>(block + b)};
+  TreeRaw r;
+  r.lo = *reinterpret_cast<const uint32_t*>(block + (o & ~3u));
+  if constexpr (BW == 4) {
+    r.hi = 0;
+  } else {
+    const uint32_t last = (o + uint32_t(bw) - 1) & ~3u;
+    r.hi = r.lo;
+    if (last != (o & ~3u)) r.hi = *reinterpret_cast<const uint32_t*>(block + last);
+  }
+  return r;
 }
 
 // Table entries (high | low << 16) of the eight codes of a group that starts at byte o.
@@ -43,7 +62,7 @@ template <int BW>
 __device__ __forceinline__ void tree_entries(TreeRaw r, uint32_t o, const char* tab, uint32_t lane, uint32_t (&e)[8]) {
   constexpr int COP = tree_copies(BW);
   const uint32_t own = (lane & uint32_t(COP - 1)) << 2, sh = 8 * (o & 3);
-  const uint64_t w = (uint64_t(r.hi) << 32 | r.lo) >> sh;
+  const uint64_t w = BW == 4 ? uint64_t(r.lo) : (uint64_t(r.hi) << 32 | r.lo) >> sh;
   const uint32_t lo = uint32_t(w), hi = uint32_t(w >> 32);
 #pragma unroll
   for (int m = 0; m < 8; ++m) {
@@ -61,15 +80,20 @@ __device__ __forceinline__ void tree_entries(TreeRaw r, uint32_t o, const char* 
 __device__ __forceinline__ uint32_t pack_lo(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
 __device__ __forceinline__ uint32_t pack_hi(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 
-template <class F>
+// f(width) with the width as a constant; W: the width where the kernel is compiled for one.
+template <int W, class F>
 __device__ __forceinline__ void tree_by_width(int bw, F&& f) {
-  switch (bw) {  // wave-uniform
-    case 2: f(std::integral_constant<int, 2>{}); break;
-    case 3: f(std::integral_constant<int, 3>{}); break;
-    case 4: f(std::integral_constant<int, 4>{}); break;
-    case 5: f(std::integral_constant<int, 5>{}); break;
-    case 6: f(std::integral_constant<int, 6>{}); break;
-    default: f(std::integral_constant<int, 8>{}); break;
+  if constexpr (W != 0) {
+    f(std::integral_constant<int, W>{});
+  } else {
+    switch (bw) {  // wave-uniform
+      case 2: f(std::integral_constant<int, 2>{}); break;
+      case 3: f(std::integral_constant<int, 3>{}); break;
+      case 4: f(std::integral_constant<int, 4>{}); break;
+      case 5: f(std::integral_constant<int, 5>{}); break;
+      case 6: f(std::integral_constant<int, 6>{}); break;
+      default: f(std::integral_constant<int, 8>{}); break;
+    }
   }
 }
 
@@ -85,39 +109,96 @@ __device__ __forceinline__ void tree_stage_table(const float* cb, int bw, char* 
   }
 }
 
+// A 4-bit codebook by the byte: the fp16 values of 2^8 c of a byte's two codes, in copies. One
+// lookup then serves two codes. Sixteen copies (two lanes of 32 share a bank half of the time):
+// with a copy per bank the two sides' tables take 64 KB, and one work-group per CU is left.
+constexpr int kPairCopies = 16, kPairBytes = 256 * kPairCopies * 4;
+template <int NTHR>
+__device__ __forceinline__ void tree_stage_pairs(const float* cb, char* dst, int tid) {
+  for_strided<256 * kPairCopies, NTHR>(tid, [&](int i) {
+    const int v = i / kPairCopies;
+    const _Float16 a = _Float16(cb[v & 15] * kTreeCb), b = _Float16(cb[v >> 4] * kTreeCb);
+    reinterpret_cast<uint32_t*>(dst)[i] =
+        uint32_t(__builtin_bit_cast(uint16_t, a)) | uint32_t(__builtin_bit_cast(uint16_t, b)) << 16;
+  });
+}
+// Entry of byte J of x.
+template <int J>
+__device__ __forceinline__ uint32_t tree_pair(uint32_t x, const char* tab, uint32_t own) {
+  const uint32_t at = (J == 0 ? x << 6 : x >> (8 * J - 6)) & 0x3fc0u;
+  return *reinterpret_cast<const uint32_t*>(tab + (at | own));
+}
+
+// Largest of the sixteen lanes of a row, in each of them.
+__device__ __forceinline__ uint32_t tree_row_max(uint32_t x) {
+  x = max(x, uint32_t(__builtin_amdgcn_mov_dpp(int(x), 0x128, 0xf, 0xf, true)));  // row_ror:8, 4, 2, 1
+  x = max(x, uint32_t(__builtin_amdgcn_mov_dpp(int(x), 0x124, 0xf, 0xf, true)));
+  x = max(x, uint32_t(__builtin_amdgcn_mov_dpp(int(x), 0x122, 0xf, 0xf, true)));
+  return max(x, uint32_t(__builtin_amdgcn_mov_dpp(int(x), 0x121, 0xf, 0xf, true)));
+}
+
+// g with x < 2^g for a non-negative finite fp16 x > 0, the least such.
+__device__ __forceinline__ int tree_exponent(uint32_t bits) {
+  return bits >> 10 ? int(bits >> 10) - 14 : 8 - __builtin_clz(bits);
+}
+
+// The largest of the four lanes 16 apart, in each of them.
+__device__ __forceinline__ float tree_max16(float x) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+  x = fmaxf(__builtin_bit_cast(float, uint32_t(a[0])), __builtin_bit_cast(float, uint32_t(a[1])));
+  const auto b = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+  return fmaxf(__builtin_bit_cast(float, uint32_t(b[0])), __builtin_bit_cast(float, uint32_t(b[1])));
+}
+
 template <int D, bool EX, int NCT, int RG, int TG>
 struct TreeCfg {
   using G = TreeGeo<D>;
   static constexpr int NW = RG * TG, NTHR = 64 * NW, ROWS = 16 * NCT * RG;
   static constexpr int NTW = G::CH / 16 / TG;  // score tiles of a wave
   static constexpr int PL = EX ? 2 : 1;        // planes of a tile
-  static constexpr int KI = G::CH * D / 8, VI = KI / 2;                        // dequantization items of a chunk
-  static constexpr int NK = (KI + NTHR - 1) / NTHR, NV = (VI + NTHR - 1) / NTHR;
+  // dequantization items of a chunk: K (token, 8 dims), dims fastest; V (token pair, 8 dims), a
+  // wave taking the 8 pairs of GPW groups of 16 tokens times DGL groups of dims
+  static constexpr int KI = G::CH * D / 8, NK = (KI + NTHR - 1) / NTHR;
+  static constexpr int DGL = D / 8 < 8 ? D / 8 : 8, GPW = 8 / DGL;
+  static constexpr int VGB = (G::NG + GPW - 1) / GPW, VC = VGB * (D / 8 / DGL), NV = (VC + NW - 1) / NW;
   static constexpr int k_off = 0, v_off = k_off + PL * G::KT, n_off = v_off + PL * G::VT;
-  static constexpr int tab_off = n_off + 4 * G::CH;  // norms: K then V, fp16
-  // the waves of token group 1 hand over (acc, m, l) in the tiles' place
-  static_assert(TG == 1 || RG * NCT * 16 * (D + 2) * 4 <= tab_off, "hand-over of the token groups fits");
-  static_assert(NTW % 2 == 0 && tab_off % 16 == 0, "whole value K-steps");
+  // norms: K then V, fp16; then the largest V norm of each group of tokens
+  static constexpr int m_off = n_off + 4 * G::CH, tab_off = m_off + 16;
+  // the waves of token group 1 hand over (acc, m, l) in the tiles' place and the tables'
+  static constexpr int give = TG == 1 ? 0 : RG * NCT * 16 * (D + 2) * 4;
+  static_assert(NTW % 2 == 0 && tab_off % 16 == 0 && TG <= 2, "whole value K-steps");
 };
 
-template <int D, bool EX, int NCT, int RG, int TG>
-__global__ __launch_bounds__(64 * RG * TG) void tree_scan_kernel(TreeArgs a) {
+template <int D, bool EX, int NCT, int RG, int TG, int W>
+__global__ __launch_bounds__(64 * RG * TG, 2) void tree_scan_kernel(TreeArgs a) {
   using C = TreeCfg<D, EX, NCT, RG, TG>;
   using G = TreeGeo<D>;
   extern __shared__ __align__(16) char lds[];
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
   const int wig = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rg = wig % RG, tg = wig / RG;
+  const int bwk = W ? W : a.bwk, bwv = W ? W : a.bwv;
+  constexpr bool PAIR = W == 4 && !EX;
   char* tabk = lds + C::tab_off;
-  char* tabv = tabk + tree_table_bytes(a.bwk);
-  tree_stage_table<C::NTHR>(a.cb_k, a.bwk, tabk, tid);
-  tree_stage_table<C::NTHR>(a.cb_v, a.bwv, tabv, tid);
+  char* tabv = tabk + (PAIR ? kPairBytes : tree_table_bytes(bwk));
+  if constexpr (PAIR) {
+    tree_stage_pairs<C::NTHR>(a.cb_k, tabk, tid);
+    tree_stage_pairs<C::NTHR>(a.cb_v, tabv, tid);
+  } else {
+    tree_stage_table<C::NTHR>(a.cb_k, bwk, tabk, tid);
+    tree_stage_table<C::NTHR>(a.cb_v, bwv, tabv, tid);
+  }
   if constexpr (D < G::DP) {  // the padded dims of the K tile stay zero
     for (int i = tid; i < C::PL * G::KT / 4; i += C::NTHR) reinterpret_cast<uint32_t*>(lds + C::k_off)[i] = 0;
   }
 
-  // unit: ((b Hkv + kvh) nsplit + s) ncg + row block of ROWS
-  int u = blockIdx.x;
+  // unit: ((b Hkv + kvh) nsplit + s) ncg + row block of ROWS; the row blocks of one stretch of
+  // tokens are neighbours on one XCD (work-groups go to the eight XCDs in turn)
+  int u;
+  {
+    const int n = gridDim.x, p = blockIdx.x, q = n >> 3, r = n & 7, x = p & 7;
+    u = x * q + min(x, r) + (p >> 3);
+  }
   const int cg = u % a.ncg;
   u /= a.ncg;
   const int s = u % a.nsplit;
@@ -132,7 +213,6 @@ __global__ __launch_bounds__(64 * RG * TG) void tree_scan_kernel(TreeArgs a) {
 
   f32x4 acc[NCT][G::MT];
   float m[NCT], l[NCT], sc[NCT];
-  uint64_t vis[NCT];
   h8 qh[NCT][G::KS], ql[EX ? NCT : 1][EX ? G::KS : 1];
   int gs = kTreeNoScale;  // values are scaled by 2^(8 - gs)
 #pragma unroll
@@ -143,8 +223,6 @@ __global__ __launch_bounds__(64 * RG * TG) void tree_scan_kernel(TreeArgs a) {
     l[ct] = 0.f;
     const int64_t row = row0 + 16 * ct + c;
     sc[ct] = a.qs[row];
-    const int node = (r0 + 16 * ct + c) / a.n_rep;
-    vis[ct] = node < a.T ? a.vis[int64_t(b) * a.T + node] : 0;
 #pragma unroll
     for (int k = 0; k < G::KS; ++k) {
       const bool pad = D < 32 && g >= D / 8;  // dims past D
@@ -156,96 +234,183 @@ __global__ __launch_bounds__(64 * RG * TG) void tree_scan_kernel(TreeArgs a) {
   if (ch_lo < ch_hi) {
     const int t_hi = min(G::CH * ch_hi, L), col_hi = (t_hi - 1) >> a.log2S, smask = (1 << a.log2S) - 1;
     const int32_t* trow = a.table + int64_t(b) * a.tsb;
-    const uint32_t nbk = uint32_t(D * a.bwk / 8), nbv = uint32_t(D * a.bwv / 8), last_page = uint32_t(a.num_pages - 1);
-    // tokens past the range read its last page (and are masked): every address is one of the pool
-    auto page_of = [&](int t) { return int64_t(min(uint32_t(trow[min(t >> a.log2S, col_hi)]), last_page)); };
+    const uint32_t nbk = uint32_t(D * bwk / 8), nbv = uint32_t(D * bwv / 8), last_page = uint32_t(a.num_pages - 1);
+    // The page of each 16-token group of a chunk (wave-uniform; S >= 16). Tokens past the range
+    // read its last page (and are masked), so every address is one of the pool.
+    uint32_t pid = 0;  // lane i: group i % NG
+    auto pages = [&](int c0) { pid = min(uint32_t(trow[min((c0 + 16 * (lane % G::NG)) >> a.log2S, col_hi)]), last_page); };
+    auto page_of = [&](int grp) {
+      return int64_t(D >= 64 ? uint32_t(__builtin_amdgcn_readlane(int(pid), grp)) : uint32_t(__shfl(int(pid), grp, 64)));
+    };
+    // Item j of this thread: K (token tok, 8 dims dg), V (tokens 2 tp, 2 tp + 1, 8 dims dg); its
+    // group of tokens, wave-uniform from 64 dims on, and whether there is one. A row's address is
+    // its group's (scalar) plus the token's within the group (the same for every j).
+    constexpr bool UNI = D >= 64;
+    auto k_item = [&](int j, int* grp, int* tok, int* dg) {
+      const int it = tid + C::NTHR * j;
+      *tok = it / (D / 8);
+      *dg = it % (D / 8);
+      *grp = UNI ? (64 * wig + C::NTHR * j) / (D / 8) >> 4 : *tok >> 4;
+      return C::KI % C::NTHR == 0 || it < C::KI;
+    };
+    auto v_item = [&](int j, int* grp, int* tp, int* dg) {
+      const int combo = wig + C::NW * j, half = UNI ? 0 : (lane >> 3) / C::DGL;
+      *grp = (combo % C::VGB) * C::GPW + half;
+      *tp = 8 * *grp + (lane & 7);
+      *dg = (combo / C::VGB) * C::DGL + (lane >> 3) % C::DGL;
+      return C::VC % C::NW == 0 || combo < C::VC;
+    };
+    auto block = [&](const uint8_t* pool, int64_t sp, int64_t sh, int c0, int grp, uint32_t nb) {
+      return pool + page_of(grp) * sp + kvh * sh + uint32_t((c0 + 16 * grp) & smask) * nb;
+    };
+    // byte of an item's codes within its group's block of 16 rows
+    auto k_off = [&](int tok, int dg) { return uint32_t(tok & 15) * nbk + uint32_t(dg * bwk); };
+    auto v_off = [&](int tp, int dg) { return uint32_t(2 * tp & 15) * nbv + uint32_t(dg * bwv); };
 
     TreeRaw kr[C::NK], vr[C::NV][2];
     uint16_t nr = 0;
     auto load = [&](int c0) {
 #pragma unroll
       for (int j = 0; j < C::NK; ++j) {
-        const int it = min(tid + C::NTHR * j, C::KI - 1), tok = it / (D / 8), dg = it % (D / 8);
-        const int t = c0 + tok;
-        kr[j] = tree_raw(a.k_pages + page_of(t) * a.ksp + kvh * a.ksh, uint32_t(t & smask) * nbk + uint32_t(dg * a.bwk), a.bwk);
+        int grp, tok, dg;
+        if (k_item(j, &grp, &tok, &dg)) kr[j] = tree_raw<W>(block(a.k_pages, a.ksp, a.ksh, c0, grp, nbk), k_off(tok, dg), bwk);
       }
 #pragma unroll
       for (int j = 0; j < C::NV; ++j) {
-        const int it = min(tid + C::NTHR * j, C::VI - 1), tp = it % (G::CH / 2), dg = it / (G::CH / 2);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int t = c0 + 2 * tp + h;
-          vr[j][h] = tree_raw(a.v_pages + page_of(t) * a.vsp + kvh * a.vsh, uint32_t(t & smask) * nbv + uint32_t(dg * a.bwv), a.bwv);
-        }
+        int grp, tp, dg;
+        if (!v_item(j, &grp, &tp, &dg)) continue;
+        const uint8_t* v = block(a.v_pages, a.vsp, a.vsh, c0, grp, nbv);
+        vr[j][0] = tree_raw<W>(v, v_off(tp, dg), bwv);
+        vr[j][1] = tree_raw<W>(v, v_off(tp, dg) + nbv, bwv);
       }
-      if (tid < 2 * G::CH) {
-        const int t = c0 + tid % G::CH;
-        const int64_t pid = page_of(t);
-        const uint16_t* p = tid < G::CH ? a.k_norms + pid * a.knp + kvh * a.knh : a.v_norms + pid * a.vnp + kvh * a.vnh;
-        nr = t < t_hi ? p[t & smask] : uint16_t(0);  // what lies past the sequence may hold anything
+      if (wig < G::NG && lane < 32) {  // wave w: the norms of group w, K in lanes 0..15, V in 16..31
+        const int t = c0 + 16 * wig + c, slot = t & smask;
+        const int64_t p = page_of(wig);
+        const uint16_t* nk = a.k_norms + p * a.knp + kvh * a.knh;
+        const uint16_t* nv = a.v_norms + p * a.vnp + kvh * a.vnh;
+        nr = t < t_hi ? (lane < 16 ? nk : nv)[slot] : uint16_t(0);  // what lies past the sequence may hold anything
       }
     };
-    auto store = [&](int c0) {
-      tree_by_width(a.bwk, [&](auto bw) {
+    uint32_t k_to, v_to;  // LDS addresses of the first items
+    {
+      int grp, tok, tp, dg;
+      k_item(0, &grp, &tok, &dg);
+      k_to = uint32_t(C::k_off) + G::k_at(tok, dg);
+      v_item(0, &grp, &tp, &dg);
+      v_to = uint32_t(C::v_off) + G::v_at(8 * dg, tp >> 2) + 4 * (tp & 3);
+    }
+    auto store = [&]() {
+      // recomputed from these two each chunk: held as loop invariants, the addresses of every
+      // write would take some thirty registers
+      asm volatile("" : "+v"(k_to), "+v"(v_to));
+      const uint32_t own = uint32_t(lane & (kPairCopies - 1)) << 2;
+      // items NTHR apart are whole groups of tokens apart (but at head_dim 256: eight tokens), so
+      // the K tile's key is the first item's; so is the V tile's from 64 dims on, eight dim
+      // groups apart
+      auto k_dst = [&](int j, int tok, int dg) {
+        return lds + (D == 256 ? uint32_t(C::k_off) + G::k_at(tok, dg) : k_to + uint32_t(j * (C::NTHR / (D / 8)) * G::KROW));
+      };
+      auto v_dst = [&](int j, int d, int tp, int dg) {
+        if (j == 0 || (G::CH == 64 && C::VGB == C::NW))
+          return lds + (v_to ^ uint32_t(G::CH == 64 ? d << 4 : d >> 1 << 4)) + (d + 8 * C::DGL * j) * G::VROW;
+        return lds + C::v_off + G::v_at(8 * dg + d, tp >> 2) + 4 * (tp & 3);
+      };
+      tree_by_width<W>(bwk, [&](auto bw) {
         constexpr int BW = decltype(bw)::value;
 #pragma unroll
         for (int j = 0; j < C::NK; ++j) {
-          const int it = tid + C::NTHR * j;
-          if (C::KI % C::NTHR && it >= C::KI) break;
-          const int tok = it / (D / 8), dg = it % (D / 8);
-          uint32_t e[8];
-          tree_entries<BW>(kr[j], uint32_t((c0 + tok) & smask) * nbk + uint32_t(dg * BW), tabk, lane, e);
-          char* dst = lds + C::k_off + tok * G::KROW + 16 * dg;
-          *reinterpret_cast<u32x4*>(dst) = u32x4{pack_lo(e[0], e[1]), pack_lo(e[2], e[3]), pack_lo(e[4], e[5]), pack_lo(e[6], e[7])};
-          if constexpr (EX)
-            *reinterpret_cast<u32x4*>(dst + G::KT) = u32x4{pack_hi(e[0], e[1]), pack_hi(e[2], e[3]), pack_hi(e[4], e[5]), pack_hi(e[6], e[7])};
-        }
-      });
-      tree_by_width(a.bwv, [&](auto bw) {
-        constexpr int BW = decltype(bw)::value;
-#pragma unroll
-        for (int j = 0; j < C::NV; ++j) {
-          const int it = tid + C::NTHR * j;
-          if (C::VI % C::NTHR && it >= C::VI) break;
-          const int tp = it % (G::CH / 2), dg = it / (G::CH / 2);
-          uint32_t e0[8], e1[8];
-          const int t = c0 + 2 * tp;
-          tree_entries<BW>(vr[j][0], uint32_t(t & smask) * nbv + uint32_t(dg * BW), tabv, lane, e0);
-          tree_entries<BW>(vr[j][1], uint32_t((t + 1) & smask) * nbv + uint32_t(dg * BW), tabv, lane, e1);
-#pragma unroll
-          for (int d = 0; d < 8; ++d) {
-            char* dst = lds + C::v_off + (8 * dg + d) * G::VROW + 4 * tp;
-            *reinterpret_cast<uint32_t*>(dst) = pack_lo(e0[d], e1[d]);
-            if constexpr (EX) *reinterpret_cast<uint32_t*>(dst + G::VT) = pack_hi(e0[d], e1[d]);
+          int grp, tok, dg;
+          if (!k_item(j, &grp, &tok, &dg)) continue;
+          char* dst = k_dst(j, tok, dg);
+          if constexpr (PAIR) {
+            const uint32_t x = kr[j].lo;
+            *reinterpret_cast<u32x4*>(dst) =
+                u32x4{tree_pair<0>(x, tabk, own), tree_pair<1>(x, tabk, own), tree_pair<2>(x, tabk, own), tree_pair<3>(x, tabk, own)};
+          } else {
+            uint32_t e[8];
+            tree_entries<BW>(kr[j], k_off(tok, dg), tabk, lane, e);
+            *reinterpret_cast<u32x4*>(dst) = u32x4{pack_lo(e[0], e[1]), pack_lo(e[2], e[3]), pack_lo(e[4], e[5]), pack_lo(e[6], e[7])};
+            if constexpr (EX)
+              *reinterpret_cast<u32x4*>(dst + G::KT) = u32x4{pack_hi(e[0], e[1]), pack_hi(e[2], e[3]), pack_hi(e[4], e[5]), pack_hi(e[6], e[7])};
+            if (j & 1) __builtin_amdgcn_sched_barrier(0);  // the lookups of two items in flight
           }
         }
       });
-      if (tid < 2 * G::CH) reinterpret_cast<uint16_t*>(lds + C::n_off)[tid] = nr;
+      __builtin_amdgcn_sched_barrier(0);
+      tree_by_width<W>(bwv, [&](auto bw) {
+        constexpr int BW = decltype(bw)::value;
+#pragma unroll
+        for (int j = 0; j < C::NV; ++j) {
+          int grp, tp, dg;
+          if (!v_item(j, &grp, &tp, &dg)) continue;
+          if constexpr (PAIR) {
+            // byte i of `even`: the codes of dim 2 i of both tokens; of `odd`, of dim 2 i + 1
+            constexpr uint32_t m = 0x0f0f0f0fu;
+            const uint32_t x = vr[j][0].lo, y = vr[j][1].lo;
+            const uint32_t even = (x & m) | (y << 4 & ~m), odd = (x >> 4 & m) | (y & ~m);
+            const uint32_t e[8] = {tree_pair<0>(even, tabv, own), tree_pair<0>(odd, tabv, own), tree_pair<1>(even, tabv, own),
+                                   tree_pair<1>(odd, tabv, own),  tree_pair<2>(even, tabv, own), tree_pair<2>(odd, tabv, own),
+                                   tree_pair<3>(even, tabv, own), tree_pair<3>(odd, tabv, own)};
+#pragma unroll
+            for (int d = 0; d < 8; ++d) *reinterpret_cast<uint32_t*>(v_dst(j, d, tp, dg)) = e[d];
+          } else {
+            uint32_t e0[8], e1[8];
+            tree_entries<BW>(vr[j][0], v_off(tp, dg), tabv, lane, e0);
+            tree_entries<BW>(vr[j][1], v_off(tp, dg) + nbv, tabv, lane, e1);
+#pragma unroll
+            for (int d = 0; d < 8; ++d) {
+              char* dst = v_dst(j, d, tp, dg);
+              *reinterpret_cast<uint32_t*>(dst) = pack_lo(e0[d], e1[d]);
+              if constexpr (EX) *reinterpret_cast<uint32_t*>(dst + G::VT) = pack_hi(e0[d], e1[d]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+      });
+      if (wig < G::NG) {
+        const uint32_t size = uint32_t(nr) & 0x7fffu;
+        const uint32_t top = tree_row_max(size < 0x7c00u ? size : 0);  // of the finite ones
+        if (lane < 32) reinterpret_cast<uint16_t*>(lds + C::n_off)[(lane >> 4) * G::CH + 16 * wig + c] = nr;
+        if (lane == 16) reinterpret_cast<uint32_t*>(lds + C::m_off)[wig] = top;
+      }
     };
 
+    // LDS addresses of the products' operands: from 64 dims on the XORs of a few registers
+    uint32_t kb[G::KS], vb[4];
+    const int w0 = 16 * C::NTW * tg;  // the wave's first token of a chunk
+#pragma unroll
+    for (int k = 0; k < G::KS; ++k) kb[k] = uint32_t(C::k_off) + G::k_at(w0 + tree_tok(0, c), 4 * k + g);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) vb[i] = (uint32_t(C::v_off) + G::v_at(c, (w0 >> 3) + g)) ^ uint32_t(i << 5);
+    // row 16 mt + c, column (w0 >> 3) + 4 ks + g: the key's part of mt and ks is a swap by i
+    auto v_addr = [&](int mt, int ks) {
+      if constexpr (G::CH == 64) return vb[((2 * mt & 7) ^ 4 * ks) >> 1] + uint32_t(16 * mt * G::VROW);
+      else return (vb[0] ^ uint32_t((2 * mt & 3) << 4)) + uint32_t(16 * mt * G::VROW);
+    };
+    pages(G::CH * ch_lo);
     load(G::CH * ch_lo);
     for (int ch = ch_lo; ch < ch_hi; ++ch) {
       const int c0 = G::CH * ch;
+      pages(min(c0 + G::CH, G::CH * (ch_hi - 1)));
       __syncthreads();  // the last chunk's tiles are read (at first: the tables are staged)
-      store(c0);
+      store();
       if (ch + 1 < ch_hi) load(c0 + G::CH);
       __syncthreads();
 
       // scores of the wave's tokens: register i of tile t is token w0 + tree_tok(t, 4 g + i)
-      const int w0 = 16 * C::NTW * tg;
       f32x4 d[NCT][C::NTW];
 #pragma unroll
       for (int t = 0; t < C::NTW; ++t) {
 #pragma unroll
         for (int ct = 0; ct < NCT; ++ct) d[ct][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-        const char* kp = lds + C::k_off + (w0 + tree_tok(t, c)) * G::KROW + 16 * g;
 #pragma unroll
         for (int k = 0; k < G::KS; ++k) {
-          const h8 kh = *reinterpret_cast<const h8*>(kp + 64 * k);
+          const char* kp = lds + kb[k] + tree_tok(t, 0) * G::KROW;
+          const h8 kh = *reinterpret_cast<const h8*>(kp);
 #pragma unroll
           for (int ct = 0; ct < NCT; ++ct) d[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[ct][k], d[ct][t], 0, 0, 0);
           if constexpr (EX) {
-            const h8 kl = *reinterpret_cast<const h8*>(kp + G::KT + 64 * k);
+            const h8 kl = *reinterpret_cast<const h8*>(kp + G::KT);
 #pragma unroll
             for (int ct = 0; ct < NCT; ++ct) {
               d[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[ct][k], d[ct][t], 0, 0, 0);
@@ -254,98 +419,135 @@ __global__ __launch_bounds__(64 * RG * TG) void tree_scan_kernel(TreeArgs a) {
           }
         }
       }
-      // norms of the wave's tokens, eight consecutive ones per K-step of the values
-      h8 nk[C::NTW / 2], nv[C::NTW / 2];
-      uint32_t nmax = 0;
+      __builtin_amdgcn_sched_barrier(0);
+      // value scale: every n_V < 2^(7 + gs), so 2^kTreeRescale n_V 2^-gs < 2^15 in fp16; it
+      // follows the norms' magnitude (n_V = 2^-20 keeps its bits)
+      constexpr int KV = C::NTW / 2;
+      {
+        const uint32_t* gm = reinterpret_cast<const uint32_t*>(lds + C::m_off);
+        uint32_t top = gm[0];
 #pragma unroll
-      for (int ks = 0; ks < C::NTW / 2; ++ks) {
+        for (int i = 1; i < G::NG; ++i) top = max(top, gm[i]);
+        top = __builtin_amdgcn_readfirstlane(int(top));
+        if (top && tree_exponent(top) - 7 > gs) {  // wave-uniform, rare after the first chunk
+          const int to = tree_exponent(top) - 7;
+          const float f = ldexpf(1.f, gs - to);
+          gs = to;
+#pragma unroll
+          for (int ct = 0; ct < NCT; ++ct) {
+            l[ct] *= f;
+#pragma unroll
+            for (int mt = 0; mt < G::MT; ++mt) acc[ct][mt] *= f;
+          }
+        }
+      }
+      // norms of the wave's tokens, eight consecutive ones per K-step of the values
+      h8 nk[KV], nv[KV];
+#pragma unroll
+      for (int ks = 0; ks < KV; ++ks) {
         const uint16_t* np = reinterpret_cast<const uint16_t*>(lds + C::n_off) + w0 + 32 * ks + 8 * g;
         nk[ks] = *reinterpret_cast<const h8*>(np);
         nv[ks] = *reinterpret_cast<const h8*>(np + G::CH);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) nmax = max(nmax, min(uint32_t(__builtin_bit_cast(uint16_t, nv[ks][j])) & 0x7fffu, 0x7bffu));
       }
-      // value scale: every n_V < 2^(7 + gs), so 2^kTreeRescale n_V 2^-gs < 2^15 in fp16; it
-      // follows the norms' magnitude (n_V = 2^-20 keeps its bits)
-      {
-        int ge;
-        const float top = wave_max(f16_to_f32(uint16_t(nmax)));
-        frexpf(top, &ge);
-        if (top > 0.f && ge - 7 > gs) {  // wave-uniform, rare after the first chunk
-          const float f = ldexpf(1.f, max(gs - (ge - 7), -126));
-          gs = ge - 7;
+      // scores less the row's maximum and gs, so that p 2^-gs = 2^x. masked: some of the chunk's
+      // tokens are nodes, seen by their descendants only, or lie past the sequence; a value norm
+      // that is not finite there makes the rows that see it NaN and no other
+      const float gsf = float(gs);
+      float x[NCT][KV][8], top[NCT];
+      auto scores = [&](auto masked) {
+        constexpr bool MASK = decltype(masked)::value;
+        bool bad[KV][8];
+        if constexpr (MASK) {
 #pragma unroll
-          for (int ct = 0; ct < NCT; ++ct)
+          for (int ks = 0; ks < KV; ++ks)
 #pragma unroll
-            for (int mt = 0; mt < G::MT; ++mt) acc[ct][mt] *= f;
+            for (int j = 0; j < 8; ++j) {
+              const float v = float(nv[ks][j]);
+              bad[ks][j] = !(fabsf(v) < INFINITY);
+              if (bad[ks][j]) nv[ks][j] = _Float16(0.f);
+            }
         }
-      }
-      const float vsc = ldexpf(1.f, -gs);
-      const bool full = c0 + G::CH <= hist;  // no node among the chunk's tokens
-
-      h8 ph[NCT][C::NTW / 2], pl[EX ? NCT : 1][EX ? C::NTW / 2 : 1];
+#pragma unroll
+        for (int ct = 0; ct < NCT; ++ct) {
+          uint32_t seen[KV];  // bit j: token 8 g + j of the K-step
+          if constexpr (MASK) {
+            int row = r0 + 16 * ct + c;
+            asm volatile("" : "+v"(row));  // not ahead of the loop: once per split
+            const int node = row / a.n_rep;
+            const uint64_t vis = node < a.T ? a.vis[int64_t(b) * a.T + node] : 0;
+            const int at = hist - c0;  // the tree's first position in the chunk (or before it)
+            const uint64_t word = at >= 0 ? (vis << at | ((uint64_t(1) << at) - 1)) : at > -64 ? vis >> -at : 0;
+#pragma unroll
+            for (int ks = 0; ks < KV; ++ks) seen[ks] = uint32_t(word >> (w0 + 32 * ks + 8 * g)) & 0xffu;
+          }
+          const float m0 = (m[ct] == -INFINITY ? 0.f : m[ct]) + gsf;
+          top[ct] = -INFINITY;
+#pragma unroll
+          for (int ks = 0; ks < KV; ++ks)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              float y = fmaf(d[ct][2 * ks + (j >> 2)][j & 3] * sc[ct], float(nk[ks][j]), -m0);
+              if (MASK) y = !(seen[ks] >> j & 1) ? -INFINITY : bad[ks][j] ? __builtin_nanf("") : y;
+              x[ct][ks][j] = y;
+              top[ct] = fmaxf(top[ct], y);
+            }
+        }
+      };
+      if (c0 + G::CH <= hist) scores(std::integral_constant<bool, false>{});
+      else scores(std::integral_constant<bool, true>{});
+      // a row's maximum moves when a score exceeds it by more than kTreeRescale, and on its first key
+      bool move[NCT], any = false;
 #pragma unroll
       for (int ct = 0; ct < NCT; ++ct) {
-        // the chunk's visible tokens: bit j for token c0 + j (positions before the tree, and
-        // the node's own word of nodes, shifted to where the tree starts)
-        uint32_t seen[C::NTW / 2];
-        if (!full) {
-          const int at = hist - c0;  // the tree's first position in the chunk (or before it)
-          const uint64_t word = at >= 0 ? (vis[ct] << at | ((uint64_t(1) << at) - 1)) : at > -64 ? vis[ct] >> -at : 0;
+        top[ct] = tree_max16(top[ct]) + gsf;
+        move[ct] = top[ct] > kTreeRescale || (m[ct] == -INFINITY && top[ct] > -INFINITY);
+        any = any || move[ct];
+      }
+      if (__any(any)) {
 #pragma unroll
-          for (int ks = 0; ks < C::NTW / 2; ++ks) seen[ks] = uint32_t(word >> (w0 + 32 * ks + 8 * g)) & 0xffu;
-        }
-        const bool fresh = m[ct] == -INFINITY;
-        const float m0 = fresh ? 0.f : m[ct];
-        float x[C::NTW / 2][8], top = -INFINITY;
-#pragma unroll
-        for (int ks = 0; ks < C::NTW / 2; ++ks)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            float y = fmaf(d[ct][2 * ks + (j >> 2)][j & 3] * sc[ct], float(nk[ks][j]), -m0);
-            if (!full && !(seen[ks] >> j & 1)) y = -INFINITY;
-            x[ks][j] = y;
-            top = fmaxf(top, y);
-          }
-        top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const bool move = top > kTreeRescale || (fresh && top > -INFINITY);
-        if (__any(move)) {
-          const float shift = move ? top : 0.f;
-          const float alpha = move ? (fresh ? 0.f : __builtin_amdgcn_exp2f(-top)) : 1.f;
-          m[ct] = move ? m0 + top : m[ct];
+        for (int ct = 0; ct < NCT; ++ct) {
+          const bool fresh = m[ct] == -INFINITY;
+          const float shift = move[ct] ? top[ct] : 0.f;
+          const float alpha = move[ct] ? (fresh ? 0.f : __builtin_amdgcn_exp2f(-top[ct])) : 1.f;
+          m[ct] = move[ct] ? (fresh ? 0.f : m[ct]) + top[ct] : m[ct];
           l[ct] *= alpha;
 #pragma unroll
           for (int mt = 0; mt < G::MT; ++mt) acc[ct][mt] *= alpha;
 #pragma unroll
-          for (int ks = 0; ks < C::NTW / 2; ++ks)
+          for (int ks = 0; ks < KV; ++ks)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[ks][j] -= shift;
+            for (int j = 0; j < 8; ++j) x[ct][ks][j] -= shift;
         }
+      }
+      // weights p n_V 2^-gs (l sums p 2^-gs)
+      h8 ph[NCT][KV], pl[EX ? NCT : 1][EX ? KV : 1];
 #pragma unroll
-        for (int ks = 0; ks < C::NTW / 2; ++ks)
+      for (int ct = 0; ct < NCT; ++ct)
+#pragma unroll
+        for (int ks = 0; ks < KV; ++ks)
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const float p = __builtin_amdgcn_exp2f(x[ks][j]);
+            const float p = __builtin_amdgcn_exp2f(x[ct][ks][j]);
             l[ct] += p;
-            float w = p * (float(nv[ks][j]) * vsc);
-            if (!full && !(seen[ks] >> j & 1)) w = 0.f;  // a norm that is not finite reaches no row that does not see it
-            const _Float16 h = _Float16(w);
-            ph[ct][ks][j] = h;
-            if constexpr (EX) pl[ct][ks][j] = _Float16(w - float(h));
+            float w = p * float(nv[ks][j]);
+            // one rounded product for both terms: fused with the conversion (which rounds the exact
+            // product) the high term could differ from the one that the low term makes up for
+            if constexpr (EX) asm("" : "+v"(w));
+            ph[ct][ks][j] = _Float16(w);
+            if constexpr (EX) pl[ct][ks][j] = _Float16(w - float(ph[ct][ks][j]));
           }
-      }
+      __builtin_amdgcn_sched_barrier(0);
       // values: A row c of M-tile mt = dim 16 mt + c, k-slots of lane group g = tokens 32 ks + 8 g .. + 7
 #pragma unroll
       for (int mt = 0; mt < G::MT; ++mt) {
-        const char* vp = lds + C::v_off + (16 * mt + c) * G::VROW + 2 * (w0 + 8 * g);
 #pragma unroll
-        for (int ks = 0; ks < C::NTW / 2; ++ks) {
-          const h8 vh = *reinterpret_cast<const h8*>(vp + 64 * ks);
+        for (int ks = 0; ks < KV; ++ks) {
+          const char* vp = lds + v_addr(mt, ks);
+          const h8 vh = *reinterpret_cast<const h8*>(vp);
 #pragma unroll
           for (int ct = 0; ct < NCT; ++ct) acc[ct][mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph[ct][ks], acc[ct][mt], 0, 0, 0);
           if constexpr (EX) {
-            const h8 vl = *reinterpret_cast<const h8*>(vp + G::VT + 64 * ks);
+            const h8 vl = *reinterpret_cast<const h8*>(vp + G::VT);
 #pragma unroll
             for (int ct = 0; ct < NCT; ++ct) {
               acc[ct][mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph[ct][ks], acc[ct][mt], 0, 0, 0);
@@ -357,9 +559,10 @@ __global__ __launch_bounds__(64 * RG * TG) void tree_scan_kernel(TreeArgs a) {
     }
   }
 
-  const float f = ldexpf(1.f, max(gs, -60) - 8);
+  const float f = ldexpf(1.f, gs - 8), lf = ldexpf(1.f, gs);
 #pragma unroll
   for (int ct = 0; ct < NCT; ++ct) {
+    l[ct] *= lf;
     l[ct] += __shfl_xor(l[ct], 16, 64);
     l[ct] += __shfl_xor(l[ct], 32, 64);
 #pragma unroll
@@ -529,26 +732,34 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeMergeArgs a) {
       });
 }
 
-template <int D, bool EX, int NCT, int RG, int TG>
+template <int D, bool EX, int NCT, int RG, int TG, int W>
 TreeScan tree_scan() {
   using C = TreeCfg<D, EX, NCT, RG, TG>;
-  return TreeScan{tree_scan_kernel<D, EX, NCT, RG, TG>, C::ROWS, C::NTHR, C::tab_off};
+  return TreeScan{tree_scan_kernel<D, EX, NCT, RG, TG, W>, C::ROWS, C::NTHR, C::tab_off, W == 4 && !EX ? 2 * kPairBytes : 0, C::give};
 }
 
-template <int D, bool EX>
+template <int D, bool EX, int W>
 TreeKernels tree_kernels() {
   TreeKernels k;
   if constexpr (D == 256) {
     // 128 accumulator registers per 32 rows: sixteen rows a wave
-    k.scan[0] = k.scan[1] = k.scan[2] = tree_scan<D, EX, 1, 4, 1>();
+    k.scan[0] = k.scan[1] = k.scan[2] = tree_scan<D, EX, 1, 4, 1, W>();
   } else {
-    k.scan[0] = tree_scan<D, EX, 1, 2, 2>();
-    k.scan[1] = tree_scan<D, EX, 2, 2, 2>();
-    k.scan[2] = tree_scan<D, EX, 2, 4, 1>();
+    k.scan[0] = tree_scan<D, EX, 1, 2, 2, W>();
+    k.scan[1] = tree_scan<D, EX, 2, 2, 2, W>();
+    if constexpr (EX) k.scan[2] = k.scan[1];
+    else k.scan[2] = tree_scan<D, EX, 2, 4, 1, W>();
   }
   k.rotate = tree_rotate_kernel<D>;
   k.merge = tree_merge_kernel<D>;
   return k;
+}
+
+// Kernels for 4-bit K and V, the width that most caches take, and for any widths.
+template <int D>
+TreeKernels tree_kernels_for(bool exact, int bw_k, int bw_v) {
+  if (bw_k == 4 && bw_v == 4) return exact ? tree_kernels<D, true, 4>() : tree_kernels<D, false, 4>();
+  return exact ? tree_kernels<D, true, 0>() : tree_kernels<D, false, 0>();
 }
 
 }  // namespace
