@@ -21,17 +21,22 @@ struct TreeGeo {
   static constexpr int KS = DP / 32, MT = D / 16;   // score K-steps, value M-tiles
   static constexpr int CH = D == 256 ? 32 : 64;     // tokens per chunk
   static constexpr int NG = CH / 16;                // 16-token groups, each within a page (S >= 16)
-  // K tile rows of whole 16-byte columns, swapped by a key of the token (rows of 128 bytes and
-  // more) or padded (shorter ones), so that the eight rows that eight lanes read lie in different
-  // banks; V tile rows of 2 CH bytes, swapped by a key of the dim for reads and writes alike
+  // An operand read takes one 16-byte column of sixteen rows at once, the banks hold 256 bytes:
+  // K tile rows have their columns swapped by a key of the token that is another one (or another
+  // part of the banks) for each of a score tile's rows; rows shorter than 128 bytes are padded.
+  // V tile rows likewise by a key of the dim, which the writes (eight dim groups, two columns) spread
+  // over eight columns too. Read at 4.5 clocks a wave and CU; a key of eight rows only: 8.2.
   static constexpr int KROW = DP >= 64 ? 2 * DP : 2 * DP + 16;
   static constexpr int VROW = 2 * CH;
   static constexpr int KT = CH * KROW, VT = D * VROW;
+  __device__ static uint32_t k_key(int tok) {
+    return DP >= 128 ? (tok & 3) | (tok >> 1 & 12) : (tok >> 1 & 1) | (tok >> 2 & 6);
+  }
   __device__ static uint32_t k_at(int tok, int col) {
-    if constexpr (DP >= 64) return uint32_t(tok * KROW + ((col ^ ((tok & 3) | (tok >> 1 & 4))) << 4));
+    if constexpr (DP >= 64) return uint32_t(tok * KROW) + ((uint32_t(col) ^ k_key(tok)) << 4);
     else return uint32_t(tok * KROW + (col << 4));
   }
-  __device__ static uint32_t v_key(int row) { return CH == 64 ? (row ^ row >> 3) & 7 : (row >> 1 ^ row >> 3) & 3; }
+  __device__ static uint32_t v_key(int row) { return CH == 64 ? (row >> 1 & 7) ^ (row >> 4 & 3) : (row >> 2 & 3) ^ (row >> 4 & 1); }
   __device__ static uint32_t v_at(int row, int col) { return uint32_t(row * VROW) + ((uint32_t(col) ^ v_key(row)) << 4); }
 };
 
@@ -110,9 +115,9 @@ __device__ __forceinline__ void tree_stage_table(const float* cb, int bw, char* 
 }
 
 // A 4-bit codebook by the byte: the fp16 values of 2^8 c of a byte's two codes, in copies. One
-// lookup then serves two codes. Sixteen copies (two lanes of 32 share a bank half of the time):
-// with a copy per bank the two sides' tables take 64 KB, and one work-group per CU is left.
-constexpr int kPairCopies = 16, kPairBytes = 256 * kPairCopies * 4;
+// lookup then serves two codes. Eight copies, 8 KB: a lookup takes 4.4 clocks a wave and CU
+// (sixteen copies: 4.2; a copy per bank, 32 KB: 3.0).
+constexpr int kPairCopies = 8, kPairBytes = 256 * kPairCopies * 4;
 template <int NTHR>
 __device__ __forceinline__ void tree_stage_pairs(const float* cb, char* dst, int tid) {
   for_strided<256 * kPairCopies, NTHR>(tid, [&](int i) {
@@ -125,7 +130,9 @@ __device__ __forceinline__ void tree_stage_pairs(const float* cb, char* dst, int
 // Entry of byte J of x.
 template <int J>
 __device__ __forceinline__ uint32_t tree_pair(uint32_t x, const char* tab, uint32_t own) {
-  const uint32_t at = (J == 0 ? x << 6 : x >> (8 * J - 6)) & 0x3fc0u;
+  constexpr int SH = 5;  // 4 kPairCopies bytes an entry
+  static_assert(4 * kPairCopies == 1 << SH, "");
+  const uint32_t at = (J == 0 ? x << SH : x >> (8 * J - SH)) & (255u << SH);
   return *reinterpret_cast<const uint32_t*>(tab + (at | own));
 }
 
@@ -238,14 +245,15 @@ __global__ __launch_bounds__(64 * RG * TG, 2) void tree_scan_kernel(TreeArgs a) 
     // The page of each 16-token group of a chunk (wave-uniform; S >= 16). Tokens past the range
     // read its last page (and are masked), so every address is one of the pool.
     uint32_t pid = 0;  // lane i: group i % NG
-    auto pages = [&](int c0) { pid = min(uint32_t(trow[min((c0 + 16 * (lane % G::NG)) >> a.log2S, col_hi)]), last_page); };
+    auto page_ids = [&](int c0) { return uint32_t(trow[min((c0 + 16 * (lane % G::NG)) >> a.log2S, col_hi)]); };
+    auto pages = [&](int c0) { pid = page_ids(c0); };
     auto page_of = [&](int grp) {
-      return int64_t(D >= 64 ? uint32_t(__builtin_amdgcn_readlane(int(pid), grp)) : uint32_t(__shfl(int(pid), grp, 64)));
+      return int64_t(min(D >= 64 ? uint32_t(__builtin_amdgcn_readlane(int(pid), grp)) : uint32_t(__shfl(int(pid), grp, 64)), last_page));
     };
     // Item j of this thread: K (token tok, 8 dims dg), V (tokens 2 tp, 2 tp + 1, 8 dims dg); its
     // group of tokens, wave-uniform from 64 dims on, and whether there is one. A row's address is
     // its group's (scalar) plus the token's within the group (the same for every j).
-    constexpr bool UNI = D >= 64;
+    constexpr bool UNI = D >= 64, DP64 = D >= 64;
     auto k_item = [&](int j, int* grp, int* tok, int* dg) {
       const int it = tid + C::NTHR * j;
       *tok = it / (D / 8);
@@ -267,28 +275,34 @@ __global__ __launch_bounds__(64 * RG * TG, 2) void tree_scan_kernel(TreeArgs a) 
     auto k_off = [&](int tok, int dg) { return uint32_t(tok & 15) * nbk + uint32_t(dg * bwk); };
     auto v_off = [&](int tp, int dg) { return uint32_t(2 * tp & 15) * nbv + uint32_t(dg * bwv); };
 
-    TreeRaw kr[C::NK], vr[C::NV][2];
-    uint16_t nr = 0;
-    auto load = [&](int c0) {
+    // AHEAD sets of raw rows: chunk n is stored from one while n + 1 travels in the other, and
+    // n + 2 is loaded into the first as soon as it is stored (at any widths a row takes twice the
+    // registers: one set). Loads are issued on every step, the last ones' again at the end: behind
+    // a branch each step's waits would have to cover the path without.
+    constexpr int AHEAD = W ? 2 : 1;
+    TreeRaw kr[AHEAD][C::NK], vr[AHEAD][C::NV][2];
+    uint16_t nr[AHEAD];
+    auto load = [&](auto set, int c0) {
+      constexpr int P = decltype(set)::value;
 #pragma unroll
       for (int j = 0; j < C::NK; ++j) {
         int grp, tok, dg;
-        if (k_item(j, &grp, &tok, &dg)) kr[j] = tree_raw<W>(block(a.k_pages, a.ksp, a.ksh, c0, grp, nbk), k_off(tok, dg), bwk);
+        if (k_item(j, &grp, &tok, &dg)) kr[P][j] = tree_raw<W>(block(a.k_pages, a.ksp, a.ksh, c0, grp, nbk), k_off(tok, dg), bwk);
       }
 #pragma unroll
       for (int j = 0; j < C::NV; ++j) {
         int grp, tp, dg;
         if (!v_item(j, &grp, &tp, &dg)) continue;
         const uint8_t* v = block(a.v_pages, a.vsp, a.vsh, c0, grp, nbv);
-        vr[j][0] = tree_raw<W>(v, v_off(tp, dg), bwv);
-        vr[j][1] = tree_raw<W>(v, v_off(tp, dg) + nbv, bwv);
+        vr[P][j][0] = tree_raw<W>(v, v_off(tp, dg), bwv);
+        vr[P][j][1] = tree_raw<W>(v, v_off(tp, dg) + nbv, bwv);
       }
-      if (wig < G::NG && lane < 32) {  // wave w: the norms of group w, K in lanes 0..15, V in 16..31
-        const int t = c0 + 16 * wig + c, slot = t & smask;
+      if (C::NW <= G::NG || wig < G::NG) {  // wave w: the norms of group w, K in lanes 0..15, V in 16..31
+        const int slot = (c0 + 16 * wig + c) & smask;
         const int64_t p = page_of(wig);
         const uint16_t* nk = a.k_norms + p * a.knp + kvh * a.knh;
         const uint16_t* nv = a.v_norms + p * a.vnp + kvh * a.vnh;
-        nr = t < t_hi ? (lane < 16 ? nk : nv)[slot] : uint16_t(0);  // what lies past the sequence may hold anything
+        nr[P] = (lane & 16 ? nv : nk)[slot];
       }
     };
     uint32_t k_to, v_to;  // LDS addresses of the first items
@@ -299,20 +313,24 @@ __global__ __launch_bounds__(64 * RG * TG, 2) void tree_scan_kernel(TreeArgs a) 
       v_item(0, &grp, &tp, &dg);
       v_to = uint32_t(C::v_off) + G::v_at(8 * dg, tp >> 2) + 4 * (tp & 3);
     }
-    auto store = [&]() {
+    auto store = [&](auto set, int c0) {
+      constexpr int P = decltype(set)::value;
       // recomputed from these two each chunk: held as loop invariants, the addresses of every
       // write would take some thirty registers
       asm volatile("" : "+v"(k_to), "+v"(v_to));
       const uint32_t own = uint32_t(lane & (kPairCopies - 1)) << 2;
-      // items NTHR apart are whole groups of tokens apart (but at head_dim 256: eight tokens), so
-      // the K tile's key is the first item's; so is the V tile's from 64 dims on, eight dim
-      // groups apart
+      // An item's address from the first one's: TOK tokens further on, the key swapped by their
+      // bits (steps of 8 and more tokens add to the same bits of the first item's token only where
+      // that has none: up to 64 items of a wave lie in one group of 16); eight groups of dims
+      // further on, the V tile's key is the same
       auto k_dst = [&](int j, int tok, int dg) {
-        return lds + (D == 256 ? uint32_t(C::k_off) + G::k_at(tok, dg) : k_to + uint32_t(j * (C::NTHR / (D / 8)) * G::KROW));
+        constexpr int TOK = C::NTHR / (D / 8);
+        if (TOK >= 16 && DP64) return lds + (k_to ^ (G::k_key(TOK * j) << 4)) + uint32_t(TOK * j * G::KROW);
+        return lds + C::k_off + G::k_at(tok, dg);
       };
       auto v_dst = [&](int j, int d, int tp, int dg) {
         if (j == 0 || (G::CH == 64 && C::VGB == C::NW))
-          return lds + (v_to ^ uint32_t(G::CH == 64 ? d << 4 : d >> 1 << 4)) + (d + 8 * C::DGL * j) * G::VROW;
+          return lds + (v_to ^ uint32_t(G::CH == 64 ? d >> 1 << 4 : d >> 2 << 4)) + (d + 8 * C::DGL * j) * G::VROW;
         return lds + C::v_off + G::v_at(8 * dg + d, tp >> 2) + 4 * (tp & 3);
       };
       tree_by_width<W>(bwk, [&](auto bw) {
@@ -323,12 +341,12 @@ __global__ __launch_bounds__(64 * RG * TG, 2) void tree_scan_kernel(TreeArgs a) 
           if (!k_item(j, &grp, &tok, &dg)) continue;
           char* dst = k_dst(j, tok, dg);
           if constexpr (PAIR) {
-            const uint32_t x = kr[j].lo;
+            const uint32_t x = kr[P][j].lo;
             *reinterpret_cast<u32x4*>(dst) =
                 u32x4{tree_pair<0>(x, tabk, own), tree_pair<1>(x, tabk, own), tree_pair<2>(x, tabk, own), tree_pair<3>(x, tabk, own)};
           } else {
             uint32_t e[8];
-            tree_entries<BW>(kr[j], k_off(tok, dg), tabk, lane, e);
+            tree_entries<BW>(kr[P][j], k_off(tok, dg), tabk, lane, e);
             *reinterpret_cast<u32x4*>(dst) = u32x4{pack_lo(e[0], e[1]), pack_lo(e[2], e[3]), pack_lo(e[4], e[5]), pack_lo(e[6], e[7])};
             if constexpr (EX)
               *reinterpret_cast<u32x4*>(dst + G::KT) = u32x4{pack_hi(e[0], e[1]), pack_hi(e[2], e[3]), pack_hi(e[4], e[5]), pack_hi(e[6], e[7])};
@@ -346,7 +364,7 @@ __global__ __launch_bounds__(64 * RG * TG, 2) void tree_scan_kernel(TreeArgs a) 
           if constexpr (PAIR) {
             // byte i of `even`: the codes of dim 2 i of both tokens; of `odd`, of dim 2 i + 1
             constexpr uint32_t m = 0x0f0f0f0fu;
-            const uint32_t x = vr[j][0].lo, y = vr[j][1].lo;
+            const uint32_t x = vr[P][j][0].lo, y = vr[P][j][1].lo;
             const uint32_t even = (x & m) | (y << 4 & ~m), odd = (x >> 4 & m) | (y & ~m);
             const uint32_t e[8] = {tree_pair<0>(even, tabv, own), tree_pair<0>(odd, tabv, own), tree_pair<1>(even, tabv, own),
                                    tree_pair<1>(odd, tabv, own),  tree_pair<2>(even, tabv, own), tree_pair<2>(odd, tabv, own),
@@ -355,8 +373,8 @@ __global__ __launch_bounds__(64 * RG * TG, 2) void tree_scan_kernel(TreeArgs a) 
             for (int d = 0; d < 8; ++d) *reinterpret_cast<uint32_t*>(v_dst(j, d, tp, dg)) = e[d];
           } else {
             uint32_t e0[8], e1[8];
-            tree_entries<BW>(vr[j][0], v_off(tp, dg), tabv, lane, e0);
-            tree_entries<BW>(vr[j][1], v_off(tp, dg) + nbv, tabv, lane, e1);
+            tree_entries<BW>(vr[P][j][0], v_off(tp, dg), tabv, lane, e0);
+            tree_entries<BW>(vr[P][j][1], v_off(tp, dg) + nbv, tabv, lane, e1);
 #pragma unroll
             for (int d = 0; d < 8; ++d) {
               char* dst = v_dst(j, d, tp, dg);
@@ -367,10 +385,11 @@ __global__ __launch_bounds__(64 * RG * TG, 2) void tree_scan_kernel(TreeArgs a) 
           }
         }
       });
-      if (wig < G::NG) {
-        const uint32_t size = uint32_t(nr) & 0x7fffu;
+      if (C::NW <= G::NG || wig < G::NG) {
+        // what lies past the sequence may hold anything
+        const uint32_t n = c0 + 16 * wig + c < t_hi ? nr[P] : 0, size = n & 0x7fffu;
         const uint32_t top = tree_row_max(size < 0x7c00u ? size : 0);  // of the finite ones
-        if (lane < 32) reinterpret_cast<uint16_t*>(lds + C::n_off)[(lane >> 4) * G::CH + 16 * wig + c] = nr;
+        if (lane < 32) reinterpret_cast<uint16_t*>(lds + C::n_off)[(lane >> 4) * G::CH + 16 * wig + c] = uint16_t(n);
         if (lane == 16) reinterpret_cast<uint32_t*>(lds + C::m_off)[wig] = top;
       }
     };
@@ -381,20 +400,33 @@ __global__ __launch_bounds__(64 * RG * TG, 2) void tree_scan_kernel(TreeArgs a) 
 #pragma unroll
     for (int k = 0; k < G::KS; ++k) kb[k] = uint32_t(C::k_off) + G::k_at(w0 + tree_tok(0, c), 4 * k + g);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) vb[i] = (uint32_t(C::v_off) + G::v_at(c, (w0 >> 3) + g)) ^ uint32_t(i << 5);
-    // row 16 mt + c, column (w0 >> 3) + 4 ks + g: the key's part of mt and ks is a swap by i
+    for (int i = 0; i < 4; ++i) vb[i] = (uint32_t(C::v_off) + G::v_at(c, (w0 >> 3) + g)) ^ uint32_t(i << 4);
+    // tile t of K-step k: tokens tree_tok(t, 0) further on (bits 2 and 5: not the key's)
+    auto k_addr = [&](int t, int k) { return kb[k] + uint32_t(tree_tok(t, 0) * G::KROW); };
+    // row 16 mt + c, column (w0 >> 3) + 4 ks + g: mt's part of the key and ks are swaps
     auto v_addr = [&](int mt, int ks) {
-      if constexpr (G::CH == 64) return vb[((2 * mt & 7) ^ 4 * ks) >> 1] + uint32_t(16 * mt * G::VROW);
-      else return (vb[0] ^ uint32_t((2 * mt & 3) << 4)) + uint32_t(16 * mt * G::VROW);
+      if constexpr (G::CH == 64) return (vb[mt & 3] ^ uint32_t(ks << 6)) + uint32_t(16 * mt * G::VROW);
+      else return vb[mt & 1] + uint32_t(16 * mt * G::VROW);
     };
+    const int c_last = G::CH * (ch_hi - 1);
+    auto next = [&](int c0) { return min(c0, c_last); };  // the last chunk again past the end
+    constexpr std::integral_constant<int, 0> even;
+    constexpr std::integral_constant<int, AHEAD - 1> odd;
     pages(G::CH * ch_lo);
-    load(G::CH * ch_lo);
-    for (int ch = ch_lo; ch < ch_hi; ++ch) {
-      const int c0 = G::CH * ch;
-      pages(min(c0 + G::CH, G::CH * (ch_hi - 1)));
+    load(even, G::CH * ch_lo);
+    if constexpr (AHEAD == 2) {
+      pages(next(G::CH * (ch_lo + 1)));
+      load(odd, next(G::CH * (ch_lo + 1)));
+    }
+    pages(next(G::CH * (ch_lo + AHEAD)));
+    auto chunk = [&](auto set, int c0) {
       __syncthreads();  // the last chunk's tiles are read (at first: the tables are staged)
-      store();
-      if (ch + 1 < ch_hi) load(c0 + G::CH);
+      store(set, c0);
+      // the page ids of the chunk after are asked for ahead of the rows: waiting for them next
+      // time waits for no row
+      const uint32_t ids = page_ids(next(c0 + (AHEAD + 1) * G::CH));
+      load(set, next(c0 + AHEAD * G::CH));
+      pid = ids;
       __syncthreads();
 
       // scores of the wave's tokens: register i of tile t is token w0 + tree_tok(t, 4 g + i)
@@ -405,7 +437,7 @@ __global__ __launch_bounds__(64 * RG * TG, 2) void tree_scan_kernel(TreeArgs a) 
         for (int ct = 0; ct < NCT; ++ct) d[ct][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < G::KS; ++k) {
-          const char* kp = lds + kb[k] + tree_tok(t, 0) * G::KROW;
+          const char* kp = lds + k_addr(t, k);
           const h8 kh = *reinterpret_cast<const h8*>(kp);
 #pragma unroll
           for (int ct = 0; ct < NCT; ++ct) d[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[ct][k], d[ct][t], 0, 0, 0);
@@ -556,6 +588,10 @@ __global__ __launch_bounds__(64 * RG * TG, 2) void tree_scan_kernel(TreeArgs a) 
           }
         }
       }
+    };
+    for (int ch = ch_lo; ch < ch_hi; ch += AHEAD) {
+      chunk(even, G::CH * ch);
+      if (AHEAD == 2 && ch + 1 < ch_hi) chunk(odd, G::CH * (ch + 1));
     }
   }
 
