@@ -400,14 +400,18 @@ int wn_dense_decode_attention(
 
 /* ---- a speculative decoding step: a tree of drafted tokens over the packed cache ---- */
 
-/* Split count of wn_tree_attention for this shape on the current device (max_len: the
- * longest sequence, drafted tokens included; any count 1 .. 4096 is valid). */
-int wn_tree_plan(int B, int Hq, int Hkv, int T, int D, int S, int bw_k, int bw_v, int exact, int max_len,
-                 int* num_splits);
+/* Splits of wn_tree_attention for this shape on the current device: splits of *span tokens (a
+ * multiple of 64), *num_splits of them for the longest sequence and *parts in all, so that they
+ * fill the device in few rounds. lens: B lengths in host memory (drafted tokens included), or NULL
+ * (every sequence fills its table row). Any num_splits 1 .. 4096, span and parts >= 1 are valid for
+ * any lengths: a sequence that num_splits spans do not cover takes longer ones, and work-groups
+ * for fewer parts than there are take several. */
+int wn_tree_plan(int B, int Hq, int Hkv, int T, int D, int S, int bw_k, int bw_v, int exact, int max_pages,
+                 const int32_t* lens, int* num_splits, int* span, int* parts);
 
 /* Bytes of scratch wn_tree_attention needs for this shape: the rotated queries, the nodes'
  * visible sets and num_splits (acc, m, l) partials per row. -1 for invalid sizes. */
-int64_t wn_tree_workspace_bytes(int B, int Hq, int Hkv, int T, int D, int exact, int num_splits);
+int64_t wn_tree_workspace_bytes(int B, int Hq, int Hkv, int T, int D, int num_splits);
 
 /* Attention of T <= 64 drafted tokens (nodes of a tree) per sequence over paged packed K/V.
  * The cache already holds the nodes: node i of sequence b is position seq_lens[b] - T + i.
@@ -439,7 +443,7 @@ int wn_tree_attention(
     const int32_t* parents, int64_t parents_stride_b,
     void* out, int out_dtype, void* workspace, int64_t workspace_bytes,
     int B, int Hq, int Hkv, int T, int D, int S, int bw_k, int bw_v, int num_pages, int max_pages,
-    float scale, int exact, int num_splits, void* stream, void* ev_begin, void* ev_end);
+    float scale, int exact, int num_splits, int span, int parts, void* stream, void* ev_begin, void* ev_end);
 
 /* Keeps the accepted branch of a tree: for i < counts[b] (clipped to [0, A]) the row of node
  * path[b, i], position start_pos[b] + path[b, i], moves to position start_pos[b] + i, in every

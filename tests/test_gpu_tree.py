@@ -225,7 +225,7 @@ def test_a_workspace_of_the_callers():
     pa = _pa()
     q, kv, parents = _case(17, (50, 300), 8, 2, 128, 9, 4, 4)
     d = to_device(kv, DEV)
-    need = pa.tree_workspace_bytes(2, 8, 2, 9, 128, True, 4)
+    need = pa.tree_workspace_bytes(2, 8, 2, 9, 128, 4)
     ws = torch.full((need + 512,), 255, dtype=torch.uint8, device=DEV)
     got = pa.packed_tree_attention(q.to(DEV), d, 0.08, parents.to(DEV), num_splits=4, workspace=ws[:need])
     _check(got, q, kv, parents, 0.08, torch.float32)
@@ -250,3 +250,81 @@ def test_pages_past_four_gigabytes():
     d.page_table, d.page_table_host = table.to(DEV), table
     got = _pa().packed_tree_attention(q.to(DEV), d, 0.08, parents.to(DEV))
     _check(got, q, kv, parents, 0.08, torch.float32)
+
+
+def _wide_table(d, columns):
+    """The same sequences behind a page table with room for ``columns`` pages each: what the kernel
+    variants are chosen by."""
+    table = torch.zeros(d.page_table.shape[0], columns, dtype=torch.int32, device=DEV)
+    table[:, :d.page_table.shape[1]] = d.page_table
+    d.page_table = table
+    return d
+
+
+@pytest.mark.parametrize("bwk,bwv", [(4, 4), (4, 6), (6, 4), (6, 6)])
+@pytest.mark.parametrize("Hq,Hkv,T", [(16, 4, 1), (16, 4, 8), (28, 4, 9), (4, 4, 64)])
+def test_tree_of_long_contexts(bwk, bwv, Hq, Hkv, T):
+    """What a table with room for 5 x 4 x 32,768 positions takes (4 and 6 bits, single terms), at
+    lengths of nothing, inside the tree, across chunks and long; partial blocks of 32 rows."""
+    lens = (0, max(1, T // 2), T + 63, 700, 3001)
+    q, kv, parents = _case(1700 + T + bwk * bwv, lens, Hq, Hkv, 128, T, bwk, bwv, dtype=torch.bfloat16)
+    d = _wide_table(to_device(kv, DEV), 2048)
+    for splits in (None, 1, 13):
+        got = _pa().packed_tree_attention(q.to(DEV), d, 0.09, parents.to(DEV), num_splits=splits)
+        _check(got, q, kv, parents, 0.09, torch.bfloat16, single=True)
+    again = _pa().packed_tree_attention(q.to(DEV), d, 0.09, parents.to(DEV), num_splits=13)
+    assert torch.equal(got, again)
+
+
+def test_long_contexts_what_a_row_does_not_see_does_not_reach_it():
+    q, kv, parents = _case(18, (21, 90, 200, 40), 8, 4, 128, 12, 4, 6, dtype=torch.bfloat16)
+    parents[:] = torch.tensor([-1, 0, 0, 1, 2, 2, -1, 6, 4, 3, 7, 5], dtype=torch.int32)
+    clean = _pa().packed_tree_attention(q.to(DEV), _wide_table(to_device(kv, DEV), 2048), 0.08, parents.to(DEV))
+    for b, L in enumerate((21, 90, 200, 40)):
+        for side in ("k", "v"):
+            norms = getattr(kv, f"{side}_norms")
+            norms[int(kv.page_table[b, (L - 1) // 16]), :, (L - 1) % 16 + 1:] = float("nan")
+            node = L - 12 + 6                                       # node 6: seen by 6, 7 and 10
+            norms[int(kv.page_table[b, node // 16]), :, node % 16] = float("inf")
+    got = _pa().packed_tree_attention(q.to(DEV), _wide_table(to_device(kv, DEV), 2048), 0.08, parents.to(DEV))
+    rest = [i for i in range(12) if i not in (6, 7, 10)]
+    assert torch.equal(got[:, :, rest], clean[:, :, rest])
+    assert not torch.isfinite(got[:, :, [6, 7, 10]].float()).any(-1).all()
+
+
+@pytest.mark.parametrize("columns", [0, 2048])
+def test_a_captured_call_at_lengths_that_grow_and_end(columns):
+    """Captured at short lengths (few splits planned), replayed at longer, shorter and empty ones."""
+    pa = _pa()
+    B, T = 5, 9
+    q, kv, parents = _case(19, (3000,) * B, 8, 2, 128, T, 4, 4, dtype=torch.bfloat16)
+    d, dq, dp = to_device(kv, DEV), q.to(DEV), parents.to(DEV)
+    if columns:
+        d = _wide_table(d, 16 * columns)
+    d.seq_lens.fill_(20)
+    d.seq_lens_host = torch.full((B,), 20, dtype=torch.int32)
+    assert pa.tree_plan_for(dq, d, False)[2] <= B
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = pa.packed_tree_attention(dq, d, 0.08, dp, check_ranges=False)
+    for lens in ((20,) * B, (3000, 0, 1, 2999, 64), (0,) * B, (3000,) * B, (10, 700, 0, 0, 129)):
+        kv.seq_lens.copy_(torch.tensor(lens, dtype=kv.seq_lens.dtype))
+        d.seq_lens_host = torch.tensor(lens, dtype=torch.int32)
+        d.seq_lens.copy_(d.seq_lens_host)
+        graph.replay()
+        torch.cuda.synchronize()
+        _check(out, q, kv, parents, 0.08, torch.bfloat16, single=True)
+        _check(pa.packed_tree_attention(dq, d, 0.08, dp), q, kv, parents, 0.08, torch.bfloat16, single=True)
+
+
+@pytest.mark.parametrize("columns", [0, 1024])
+def test_many_sequences_some_of_them_empty(columns):
+    """More sequences than a wave has lanes, empty ones between and at both ends."""
+    lens = [0, 0, 5] + [(37 * i) % 90 if i % 3 else 0 for i in range(135)] + [400, 0]
+    q, kv, parents = _case(20, lens, 4, 2, 128, 3, 4, 4, dtype=torch.bfloat16)
+    d = to_device(kv, DEV)
+    if columns:
+        d = _wide_table(d, columns)
+    for splits in (None, 5):
+        got = _pa().packed_tree_attention(q.to(DEV), d, 0.08, parents.to(DEV), num_splits=splits)
+        _check(got, q, kv, parents, 0.08, torch.bfloat16, single=True)

@@ -151,17 +151,17 @@ def test_c_abi_refusals():
     tree = lambda **k: _lib.call("wn_tree_attention", *{**dict(  # noqa: E731
         q=i, dt=0, qb=0, qh=0, qt=0, pk=i, pv=i, ck=i, cv=i, kp=i, ksp=0, ksh=0, vp=i, vsp=0, vsh=0, kn=i, knp=0, knh=0, vn=i, vnp=0,
         vnh=0, table=i, tsb=0, lens=i, par=i, psb=0, out=i, odt=0, ws=i, wsb=1 << 40, B=1, Hq=4, Hkv=2, T=5, D=64, S=16, bwk=4, bwv=4,
-        P=4, maxp=4, scale=1.0, exact=1, ns=1, stream=None, e0=None, e1=None), **k}.values())
+        P=4, maxp=4, scale=1.0, exact=1, ns=1, span=64, parts=1, stream=None, e0=None, e1=None), **k}.values())
     for k, match in [(dict(T=65), "T<=64"), (dict(T=0), "T<="), (dict(D=96), "power of two"), (dict(Hq=5), "Hq"), (dict(bwk=7), "widths"),
-                     (dict(S=8), "page size"), (dict(S=24), "page size"), (dict(dt=3), "dtype"), (dict(ns=0), "num_splits"), (dict(ns=4097), "num_splits"),
+                     (dict(S=8), "page size"), (dict(S=24), "page size"), (dict(dt=3), "dtype"), (dict(ns=0), "num_splits"), (dict(ns=4097), "num_splits"), (dict(span=0), "span"), (dict(span=96), "span"), (dict(parts=0), "parts"),
                      (dict(P=0), "num_pages"), (dict(maxp=1 << 28), "max_pages"), (dict(q=None), "null"), (dict(par=None), "null"),
                      (dict(kp=i + 2), "4-byte"), (dict(vsh=6), "4-byte"), (dict(knp=-1), "negative"), (dict(pk=i + 4), "16-byte"),
                      (dict(wsb=100), "workspace"), (dict(ws=i + 16), "workspace"), (dict(ws=None), "workspace")]:
         with pytest.raises(_lib.WinnowHipError, match=match):
             tree(**k)
     tree(B=0)                                                        # nothing to do, nothing launched
-    assert _lib.lib().wn_tree_workspace_bytes(1, 4, 2, 65, 64, 1, 1) == -1
-    assert pa.tree_workspace_bytes(2, 32, 8, 16, 128, False, 4) > 2 * 32 * 16 * 4 * 128 * 4
+    assert _lib.lib().wn_tree_workspace_bytes(1, 4, 2, 65, 64, 1) == -1
+    assert pa.tree_workspace_bytes(2, 32, 8, 16, 128, 4) > 2 * 32 * 16 * 4 * 128 * 4
     commit = lambda **k: _lib.call("wn_commit_kv", *{**dict(  # noqa: E731
         k=i, kl=0, kp=64, kh=64, kr=4, v=i, vl=0, vp=64, vh=64, vr=4, kn=i, knl=0, knp=0, knh=0, vn=i, vnl=0, vnp=0, vnh=0, t=i, tsb=0,
         start=i, path=i, psb=0, counts=i, lengths=2 * i, layers=1, B=1, Hkv=1, S=16, A=1, nodes=4, P=1, maxp=1, stream=None), **k}.values())

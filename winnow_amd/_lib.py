@@ -151,8 +151,9 @@ SIGNATURES = {
         _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i,   # B Hq Hkv Q D S bwk bwv
         _c_f, _c_i,                                 # scale, num_splits
         _c_p, _c_p, _c_p]),                         # stream, ev_begin, ev_end
-    "wn_tree_plan": (_c_i, [_c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, ctypes.POINTER(_c_i)]),
-    "wn_tree_workspace_bytes": (_c_i64, [_c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i]),
+    "wn_tree_plan": (_c_i, [_c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_p,
+                            ctypes.POINTER(_c_i), ctypes.POINTER(_c_i), ctypes.POINTER(_c_i)]),
+    "wn_tree_workspace_bytes": (_c_i64, [_c_i, _c_i, _c_i, _c_i, _c_i, _c_i]),
     "wn_tree_attention": (_c_i, [
         _c_p, _c_i, _c_i64, _c_i64, _c_i64,         # q, dtype, strides (b, h, t)
         _c_p, _c_p, _c_p, _c_p,                     # pi_k, pi_v, codebooks
@@ -164,7 +165,7 @@ SIGNATURES = {
         _c_p, _c_i64,                               # parents, stride
         _c_p, _c_i, _c_p, _c_i64,                   # out, out dtype, workspace
         _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i,   # B Hq Hkv T D S bwk bwv num_pages max_pages
-        _c_f, _c_i, _c_i,                           # scale, exact, num_splits
+        _c_f, _c_i, _c_i, _c_i, _c_i,               # scale, exact, num_splits, span, parts
         _c_p, _c_p, _c_p]),                         # stream, ev_begin, ev_end
     "wn_commit_kv": (_c_i, [
         _c_p, _c_i64, _c_i64, _c_i64, _c_i,         # k pages, strides (layer, page, head), row bytes

@@ -43,6 +43,7 @@ struct TreeArgs {
   const _Float16* qh;  // (B Hkv nrp, D) high terms of q' 2^e
   const _Float16* ql;  // low terms (EX)
   const float* qs;     // (B Hkv nrp) scale log2(e) 2^-(e + 8)
+  const float* qf;     // (B Hkv nrp, 128) scale log2(e) q' in place of the three (row scan)
   const uint64_t* vis; // (B T) visible nodes of a node
   const uint8_t* k_pages;
   const uint8_t* v_pages;
@@ -57,8 +58,74 @@ struct TreeArgs {
   int64_t ksp, ksh, vsp, vsh;  // page strides, bytes
   int64_t knp, knh, vnp, vnh;  // norm strides, elements
   int64_t tsb;                 // page-table row stride, elements
-  int B, Hkv, n_rep, T, nrp, ncg, nsplit, log2S, max_pages, num_pages, bwk, bwv;
+  int B, Hkv, n_rep, T, nrp, ncg, nsplit, span, log2S, max_pages, num_pages, bwk, bwv;
 };
+
+// Tokens of a split of a sequence of L: `span` (a multiple of 64), more where nsplit of them do not
+// cover it. Long and short sequences then have splits of one size, and as many as they need.
+__host__ __device__ inline int tree_span(int L, int nsplit, int span) {
+  const int even = int((int64_t(L) + nsplit - 1) / nsplit + 63) / 64 * 64;
+  return span > even ? span : even;
+}
+
+#ifdef __HIPCC__
+// Split j of the batch, its splits counted sequence after sequence: its sequence and place there.
+// False past the last one. Every lane of a wave takes part.
+__device__ __forceinline__ bool tree_split(const TreeArgs& a, int lane, int j, int* b, int* s) {
+  int before = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int L = b0 + lane < a.B ? min(max(a.seq_lens[b0 + lane], 0), a.max_pages << a.log2S) : 0;
+    const int span = tree_span(L, a.nsplit, a.span), own = (L + span - 1) / span;
+    int upto = own;  // of this lane's sequence and those before it
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int x = __shfl_up(upto, o, 64);
+      upto += lane >= o ? x : 0;
+    }
+    const int all = __builtin_amdgcn_readlane(upto, 63);
+    if (j < before + all) {
+      const int k = __builtin_popcountll(__ballot(before + upto <= j));
+      *b = b0 + k;
+      *s = j - before - __builtin_amdgcn_readlane(upto - own, k);
+      return true;
+    }
+    before += all;
+  }
+  return false;
+}
+
+// Addresses of the rows of 16-token groups. Lane (kind, i) of the wave's first 16 holds the address of
+// group i's K rows, V rows, K norms or V norms (kind 0 .. 3): formed by one product a chunk, and read
+// from there into scalars, where a scalar product per group and kind took a sixth of the scan's
+// instructions.
+struct TreeRows {
+  uint64_t base, stride;  // of the kind: pool + head, bytes per page
+  uint32_t token;         // bytes per token
+  uint64_t at;            // of the group
+  __device__ __forceinline__ void init(const TreeArgs& a, int lane, int kvh, uint32_t nbk, uint32_t nbv) {
+    const int kind = lane >> 2 & 3;
+    base = kind == 0   ? reinterpret_cast<uint64_t>(a.k_pages) + uint64_t(kvh) * uint64_t(a.ksh)
+           : kind == 1 ? reinterpret_cast<uint64_t>(a.v_pages) + uint64_t(kvh) * uint64_t(a.vsh)
+           : kind == 2 ? reinterpret_cast<uint64_t>(a.k_norms) + uint64_t(kvh) * uint64_t(a.knh) * 2
+                       : reinterpret_cast<uint64_t>(a.v_norms) + uint64_t(kvh) * uint64_t(a.vnh) * 2;
+    stride = uint64_t(kind == 0 ? a.ksp : kind == 1 ? a.vsp : kind == 2 ? a.knp * 2 : a.vnp * 2);
+    token = kind == 0 ? nbk : kind == 1 ? nbv : 2;
+  }
+  __device__ __forceinline__ void set(uint32_t page, int slot) {
+    at = base + uint64_t(page) * stride + uint32_t(slot) * token;
+  }
+  __device__ __forceinline__ const uint8_t* rows(int kind, int group) const {  // wave-uniform
+    const int l = 4 * kind + group;
+    return reinterpret_cast<const uint8_t*>(uint64_t(uint32_t(__builtin_amdgcn_readlane(int(at >> 32), l))) << 32 |
+                                            uint32_t(__builtin_amdgcn_readlane(int(uint32_t(at)), l)));
+  }
+  __device__ __forceinline__ const uint8_t* rows_lane(int kind, int group) const {  // by the lane
+    const int l = 4 * kind + group;
+    return reinterpret_cast<const uint8_t*>(uint64_t(uint32_t(__shfl(int(at >> 32), l, 64))) << 32 |
+                                            uint32_t(__shfl(int(uint32_t(at)), l, 64)));
+  }
+};
+#endif
 
 struct TreeRotArgs {
   const void* q;
@@ -69,6 +136,7 @@ struct TreeRotArgs {
   _Float16* qh;
   _Float16* ql;
   float* qs;
+  float* qf;  // not null: fp32 rows, no terms
   uint64_t* vis;
   float scale;  // scale log2(e)
   int Hkv, n_rep, T, nrp, q_dtype, exact;
@@ -79,7 +147,8 @@ struct TreeMergeArgs {
   const float* part_ml;
   const float* pi_v;
   void* out;  // (B, Hq, T, D) contiguous
-  int out_dtype, Hkv, n_rep, T, nrp, nsplit;
+  const int32_t* seq_lens;
+  int out_dtype, Hkv, n_rep, T, nrp, nsplit, span, max_len;
 };
 
 using TreeScanFn = void (*)(TreeArgs);
@@ -91,18 +160,23 @@ struct TreeScan {
   int rows = 0, threads = 0;  // query rows and threads of a work-group
   int lds = 0, tables = 0;    // LDS bytes without the codebook tables; theirs (0: by the widths)
   int give = 0;               // LDS bytes that the hand-over at the end takes
+  int waves = 0;              // > 0: the row scan, so many waves a work-group, each with its own rows
 };
 
 struct TreeKernels {
   TreeScan scan[3];  // for up to 32, up to 64 and more rows per kv head
   TreeRotFn rotate = nullptr;
-  TreeMergeFn merge = nullptr;
+  int rotate_threads = 0;
+  TreeMergeFn merge[2] = {};  // of four and of sixteen rows a work-group
 };
 
 // Bytes of one side's codebook table in LDS: 2^bw entries of (high, low), a copy per bank
 // (16 of 6-bit tables, 8 of 8-bit ones: their size).
 __host__ __device__ constexpr int tree_copies(int bw) { return bw <= 5 ? 32 : bw == 6 ? 16 : 8; }
 __host__ __device__ constexpr int tree_table_bytes(int bw) { return (4 << bw) * tree_copies(bw); }
+
+// The row scan (tree_rows.hip): head_dim 128, 4 and 6-bit K and V, single-term products.
+TreeScan tree_rows_scan(int bw_k, int bw_v);
 
 TreeKernels tree_kernels_16(bool exact, int bw_k, int bw_v);
 TreeKernels tree_kernels_32(bool exact, int bw_k, int bw_v);

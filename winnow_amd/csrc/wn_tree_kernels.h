@@ -171,8 +171,9 @@ struct TreeCfg {
   static constexpr int k_off = 0, v_off = k_off + PL * G::KT, n_off = v_off + PL * G::VT;
   // norms: K then V, fp16; then the largest V norm of each group of tokens
   static constexpr int m_off = n_off + 4 * G::CH, tab_off = m_off + 16;
-  // the waves of token group 1 hand over (acc, m, l) in the tiles' place and the tables'
-  static constexpr int give = TG == 1 ? 0 : RG * NCT * 16 * (D + 2) * 4;
+  // the waves of token group 1 hand over (acc, m, l) in the tiles' place, sixteen rows at a time
+  static constexpr int give = RG * 16 * (D + 2) * 4;
+  static_assert(TG == 1 || give <= tab_off, "hand-over fits");
   static_assert(NTW % 2 == 0 && tab_off % 16 == 0 && TG <= 2, "whole value K-steps");
 };
 
@@ -199,478 +200,476 @@ __global__ __launch_bounds__(64 * RG * TG, 2) void tree_scan_kernel(TreeArgs a) 
     for (int i = tid; i < C::PL * G::KT / 4; i += C::NTHR) reinterpret_cast<uint32_t*>(lds + C::k_off)[i] = 0;
   }
 
-  // unit: ((b Hkv + kvh) nsplit + s) ncg + row block of ROWS; the row blocks of one stretch of
-  // tokens are neighbours on one XCD (work-groups go to the eight XCDs in turn)
-  int u;
-  {
-    const int n = gridDim.x, p = blockIdx.x, q = n >> 3, r = n & 7, x = p & 7;
-    u = x * q + min(x, r) + (p >> 3);
-  }
-  const int cg = u % a.ncg;
-  u /= a.ncg;
-  const int s = u % a.nsplit;
-  u /= a.nsplit;
-  const int kvh = u % a.Hkv, b = u / a.Hkv;
-  const int L = min(max(const_view(a.seq_lens)[b], 0), a.max_pages << a.log2S);
-  const int hist = L - a.T;  // position of node 0
-  const int nch = (L + G::CH - 1) / G::CH;
-  const int ch_lo = int(int64_t(nch) * s / a.nsplit), ch_hi = int(int64_t(nch) * (s + 1) / a.nsplit);
-  const int r0 = cg * C::ROWS + rg * 16 * NCT;  // the wave's first row
-  const int64_t row0 = (int64_t(b) * a.Hkv + kvh) * a.nrp + r0;
+  // Unit (split of the batch, kv head), and its row block of ROWS. Work-groups go to the eight XCDs
+  // in turn: a unit's row blocks, which read the same rows, share one, and units go round. A grid of
+  // fewer units than there are (lengths that have grown since it was planned) goes over them again.
+  const int cg = int(blockIdx.x >> 3) % a.ncg, step = int(gridDim.x) / a.ncg;
+  for (int u = (int(blockIdx.x >> 3) / a.ncg) * 8 + int(blockIdx.x & 7);; u += step) {
+    int b, s;
+    if (!tree_split(a, lane, u / a.Hkv, &b, &s)) break;  // the whole work-group
+    const int kvh = u % a.Hkv;
+    const int L = min(max(const_view(a.seq_lens)[b], 0), a.max_pages << a.log2S);
+    const int span = tree_span(L, a.nsplit, a.span);
+    const int ch_lo = s * (span / G::CH), ch_hi = (min(L, s * span + span) + G::CH - 1) / G::CH;
+    const int hist = L - a.T;  // position of node 0
+    const int rows = a.n_rep * a.T, r0 = cg * C::ROWS + rg * 16 * NCT;  // the wave's first row
+    const int64_t row0 = (int64_t(b) * a.Hkv + kvh) * a.nrp + r0;
 
-  f32x4 acc[NCT][G::MT];
-  float m[NCT], l[NCT], sc[NCT];
-  h8 qh[NCT][G::KS], ql[EX ? NCT : 1][EX ? G::KS : 1];
-  int gs = kTreeNoScale;  // values are scaled by 2^(8 - gs)
+    f32x4 acc[NCT][G::MT];
+    float m[NCT], l[NCT], sc[NCT];
+    h8 qh[NCT][G::KS], ql[EX ? NCT : 1][EX ? G::KS : 1];
+    int gs = kTreeNoScale;  // values are scaled by 2^(8 - gs)
 #pragma unroll
-  for (int ct = 0; ct < NCT; ++ct) {
+    for (int ct = 0; ct < NCT; ++ct) {
 #pragma unroll
-    for (int mt = 0; mt < G::MT; ++mt) acc[ct][mt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    m[ct] = -INFINITY;
-    l[ct] = 0.f;
-    const int64_t row = row0 + 16 * ct + c;
-    sc[ct] = a.qs[row];
+      for (int mt = 0; mt < G::MT; ++mt) acc[ct][mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      m[ct] = -INFINITY;
+      l[ct] = 0.f;
+      const int64_t row = row0 + 16 * ct + c;
+      sc[ct] = a.qs[row];
 #pragma unroll
-    for (int k = 0; k < G::KS; ++k) {
-      const bool pad = D < 32 && g >= D / 8;  // dims past D
-      qh[ct][k] = pad ? h8{} : *reinterpret_cast<const h8*>(a.qh + row * D + 32 * k + 8 * g);
-      if constexpr (EX) ql[ct][k] = pad ? h8{} : *reinterpret_cast<const h8*>(a.ql + row * D + 32 * k + 8 * g);
+      for (int k = 0; k < G::KS; ++k) {
+        const bool pad = D < 32 && g >= D / 8;  // dims past D
+        qh[ct][k] = pad ? h8{} : *reinterpret_cast<const h8*>(a.qh + row * D + 32 * k + 8 * g);
+        if constexpr (EX) ql[ct][k] = pad ? h8{} : *reinterpret_cast<const h8*>(a.ql + row * D + 32 * k + 8 * g);
+      }
     }
-  }
 
-  if (ch_lo < ch_hi) {
-    const int t_hi = min(G::CH * ch_hi, L), col_hi = (t_hi - 1) >> a.log2S, smask = (1 << a.log2S) - 1;
-    const int32_t* trow = a.table + int64_t(b) * a.tsb;
-    const uint32_t nbk = uint32_t(D * bwk / 8), nbv = uint32_t(D * bwv / 8), last_page = uint32_t(a.num_pages - 1);
-    // The page of each 16-token group of a chunk (wave-uniform; S >= 16). Tokens past the range
-    // read its last page (and are masked), so every address is one of the pool.
-    uint32_t pid = 0;  // lane i: group i % NG
-    auto page_ids = [&](int c0) { return uint32_t(trow[min((c0 + 16 * (lane % G::NG)) >> a.log2S, col_hi)]); };
-    auto pages = [&](int c0) { pid = page_ids(c0); };
-    auto page_of = [&](int grp) {
-      return int64_t(min(D >= 64 ? uint32_t(__builtin_amdgcn_readlane(int(pid), grp)) : uint32_t(__shfl(int(pid), grp, 64)), last_page));
-    };
-    // Item j of this thread: K (token tok, 8 dims dg), V (tokens 2 tp, 2 tp + 1, 8 dims dg); its
-    // group of tokens, wave-uniform from 64 dims on, and whether there is one. A row's address is
-    // its group's (scalar) plus the token's within the group (the same for every j).
-    constexpr bool UNI = D >= 64, DP64 = D >= 64;
-    auto k_item = [&](int j, int* grp, int* tok, int* dg) {
-      const int it = tid + C::NTHR * j;
-      *tok = it / (D / 8);
-      *dg = it % (D / 8);
-      *grp = UNI ? (64 * wig + C::NTHR * j) / (D / 8) >> 4 : *tok >> 4;
-      return C::KI % C::NTHR == 0 || it < C::KI;
-    };
-    auto v_item = [&](int j, int* grp, int* tp, int* dg) {
-      const int combo = wig + C::NW * j, half = UNI ? 0 : (lane >> 3) / C::DGL;
-      *grp = (combo % C::VGB) * C::GPW + half;
-      *tp = 8 * *grp + (lane & 7);
-      *dg = (combo / C::VGB) * C::DGL + (lane >> 3) % C::DGL;
-      return C::VC % C::NW == 0 || combo < C::VC;
-    };
-    auto block = [&](const uint8_t* pool, int64_t sp, int64_t sh, int c0, int grp, uint32_t nb) {
-      return pool + page_of(grp) * sp + kvh * sh + uint32_t((c0 + 16 * grp) & smask) * nb;
-    };
-    // byte of an item's codes within its group's block of 16 rows
-    auto k_off = [&](int tok, int dg) { return uint32_t(tok & 15) * nbk + uint32_t(dg * bwk); };
-    auto v_off = [&](int tp, int dg) { return uint32_t(2 * tp & 15) * nbv + uint32_t(dg * bwv); };
-
-    // AHEAD sets of raw rows: chunk n is stored from one while n + 1 travels in the other, and
-    // n + 2 is loaded into the first as soon as it is stored (at any widths a row takes twice the
-    // registers: one set). Loads are issued on every step, the last ones' again at the end: behind
-    // a branch each step's waits would have to cover the path without.
-    constexpr int AHEAD = W ? 2 : 1;
-    TreeRaw kr[AHEAD][C::NK], vr[AHEAD][C::NV][2];
-    uint16_t nr[AHEAD];
-    auto load = [&](auto set, int c0) {
-      constexpr int P = decltype(set)::value;
-#pragma unroll
-      for (int j = 0; j < C::NK; ++j) {
-        int grp, tok, dg;
-        if (k_item(j, &grp, &tok, &dg)) kr[P][j] = tree_raw<W>(block(a.k_pages, a.ksp, a.ksh, c0, grp, nbk), k_off(tok, dg), bwk);
-      }
-#pragma unroll
-      for (int j = 0; j < C::NV; ++j) {
-        int grp, tp, dg;
-        if (!v_item(j, &grp, &tp, &dg)) continue;
-        const uint8_t* v = block(a.v_pages, a.vsp, a.vsh, c0, grp, nbv);
-        vr[P][j][0] = tree_raw<W>(v, v_off(tp, dg), bwv);
-        vr[P][j][1] = tree_raw<W>(v, v_off(tp, dg) + nbv, bwv);
-      }
-      if (C::NW <= G::NG || wig < G::NG) {  // wave w: the norms of group w, K in lanes 0..15, V in 16..31
-        const int slot = (c0 + 16 * wig + c) & smask;
-        const int64_t p = page_of(wig);
-        const uint16_t* nk = a.k_norms + p * a.knp + kvh * a.knh;
-        const uint16_t* nv = a.v_norms + p * a.vnp + kvh * a.vnh;
-        nr[P] = (lane & 16 ? nv : nk)[slot];
-      }
-    };
-    uint32_t k_to, v_to;  // LDS addresses of the first items
     {
-      int grp, tok, tp, dg;
-      k_item(0, &grp, &tok, &dg);
-      k_to = uint32_t(C::k_off) + G::k_at(tok, dg);
-      v_item(0, &grp, &tp, &dg);
-      v_to = uint32_t(C::v_off) + G::v_at(8 * dg, tp >> 2) + 4 * (tp & 3);
-    }
-    auto store = [&](auto set, int c0) {
-      constexpr int P = decltype(set)::value;
-      // recomputed from these two each chunk: held as loop invariants, the addresses of every
-      // write would take some thirty registers
-      asm volatile("" : "+v"(k_to), "+v"(v_to));
-      const uint32_t own = uint32_t(lane & (kPairCopies - 1)) << 2;
-      // An item's address from the first one's: TOK tokens further on, the key swapped by their
-      // bits (steps of 8 and more tokens add to the same bits of the first item's token only where
-      // that has none: up to 64 items of a wave lie in one group of 16); eight groups of dims
-      // further on, the V tile's key is the same
-      auto k_dst = [&](int j, int tok, int dg) {
-        constexpr int TOK = C::NTHR / (D / 8);
-        if (TOK >= 16 && DP64) return lds + (k_to ^ (G::k_key(TOK * j) << 4)) + uint32_t(TOK * j * G::KROW);
-        return lds + C::k_off + G::k_at(tok, dg);
+      const int t_hi = min(G::CH * ch_hi, L), col_hi = (t_hi - 1) >> a.log2S, smask = (1 << a.log2S) - 1;
+      const int32_t* trow = a.table + int64_t(b) * a.tsb;
+      const uint32_t nbk = uint32_t(D * bwk / 8), nbv = uint32_t(D * bwv / 8), last_page = uint32_t(a.num_pages - 1);
+      // The rows of each 16-token group of a chunk (S >= 16: they lie in one page). Tokens past the
+      // range read its last page (and are masked), so every address is one of the pool.
+      TreeRows at;
+      at.init(a, lane, kvh, nbk, nbv);
+      auto page_ids = [&](int c0) { return uint32_t(trow[min((c0 + 16 * (lane & 3 & (G::NG - 1))) >> a.log2S, col_hi)]); };
+      auto pages = [&](uint32_t ids, int c0) { at.set(min(ids, last_page), (c0 + 16 * (lane & 3)) & smask); };
+      // Item j of this thread: K (token tok, 8 dims dg), V (tokens 2 tp, 2 tp + 1, 8 dims dg); its
+      // group of tokens, wave-uniform from 64 dims on, and whether there is one. A row's address is
+      // its group's (scalar) plus the token's within the group (the same for every j).
+      constexpr bool UNI = D >= 64, DP64 = D >= 64;
+      auto k_item = [&](int j, int* grp, int* tok, int* dg) {
+        const int it = tid + C::NTHR * j;
+        *tok = it / (D / 8);
+        *dg = it % (D / 8);
+        *grp = UNI ? (64 * wig + C::NTHR * j) / (D / 8) >> 4 : *tok >> 4;
+        return C::KI % C::NTHR == 0 || it < C::KI;
       };
-      auto v_dst = [&](int j, int d, int tp, int dg) {
-        if (j == 0 || (G::CH == 64 && C::VGB == C::NW))
-          return lds + (v_to ^ uint32_t(G::CH == 64 ? d >> 1 << 4 : d >> 2 << 4)) + (d + 8 * C::DGL * j) * G::VROW;
-        return lds + C::v_off + G::v_at(8 * dg + d, tp >> 2) + 4 * (tp & 3);
+      auto v_item = [&](int j, int* grp, int* tp, int* dg) {
+        const int combo = wig + C::NW * j, half = UNI ? 0 : (lane >> 3) / C::DGL;
+        *grp = (combo % C::VGB) * C::GPW + half;
+        *tp = 8 * *grp + (lane & 7);
+        *dg = (combo / C::VGB) * C::DGL + (lane >> 3) % C::DGL;
+        return C::VC % C::NW == 0 || combo < C::VC;
       };
-      tree_by_width<W>(bwk, [&](auto bw) {
-        constexpr int BW = decltype(bw)::value;
+      auto block = [&](int kind, int grp) { return UNI ? at.rows(kind, grp) : at.rows_lane(kind, grp); };
+      // byte of an item's codes within its group's block of 16 rows
+      auto k_off = [&](int tok, int dg) { return uint32_t(tok & 15) * nbk + uint32_t(dg * bwk); };
+      auto v_off = [&](int tp, int dg) { return uint32_t(2 * tp & 15) * nbv + uint32_t(dg * bwv); };
+
+      // AHEAD sets of raw rows: chunk n is stored from one while n + 1 travels in the other, and
+      // n + 2 is loaded into the first as soon as it is stored (at any widths a row takes twice the
+      // registers: one set). Loads are issued on every step, the last ones' again at the end: behind
+      // a branch each step's waits would have to cover the path without.
+      constexpr int AHEAD = W ? 2 : 1;
+      TreeRaw kr[AHEAD][C::NK], vr[AHEAD][C::NV][2];
+      uint16_t nr[AHEAD];
+      auto load = [&](auto set) {
+        constexpr int P = decltype(set)::value;
 #pragma unroll
         for (int j = 0; j < C::NK; ++j) {
           int grp, tok, dg;
-          if (!k_item(j, &grp, &tok, &dg)) continue;
-          char* dst = k_dst(j, tok, dg);
-          if constexpr (PAIR) {
-            const uint32_t x = kr[P][j].lo;
-            *reinterpret_cast<u32x4*>(dst) =
-                u32x4{tree_pair<0>(x, tabk, own), tree_pair<1>(x, tabk, own), tree_pair<2>(x, tabk, own), tree_pair<3>(x, tabk, own)};
-          } else {
-            uint32_t e[8];
-            tree_entries<BW>(kr[P][j], k_off(tok, dg), tabk, lane, e);
-            *reinterpret_cast<u32x4*>(dst) = u32x4{pack_lo(e[0], e[1]), pack_lo(e[2], e[3]), pack_lo(e[4], e[5]), pack_lo(e[6], e[7])};
-            if constexpr (EX)
-              *reinterpret_cast<u32x4*>(dst + G::KT) = u32x4{pack_hi(e[0], e[1]), pack_hi(e[2], e[3]), pack_hi(e[4], e[5]), pack_hi(e[6], e[7])};
-            if (j & 1) __builtin_amdgcn_sched_barrier(0);  // the lookups of two items in flight
-          }
+          if (k_item(j, &grp, &tok, &dg)) kr[P][j] = tree_raw<W>(block(0, grp), k_off(tok, dg), bwk);
         }
-      });
-      __builtin_amdgcn_sched_barrier(0);
-      tree_by_width<W>(bwv, [&](auto bw) {
-        constexpr int BW = decltype(bw)::value;
 #pragma unroll
         for (int j = 0; j < C::NV; ++j) {
           int grp, tp, dg;
           if (!v_item(j, &grp, &tp, &dg)) continue;
-          if constexpr (PAIR) {
-            // byte i of `even`: the codes of dim 2 i of both tokens; of `odd`, of dim 2 i + 1
-            constexpr uint32_t m = 0x0f0f0f0fu;
-            const uint32_t x = vr[P][j][0].lo, y = vr[P][j][1].lo;
-            const uint32_t even = (x & m) | (y << 4 & ~m), odd = (x >> 4 & m) | (y & ~m);
-            const uint32_t e[8] = {tree_pair<0>(even, tabv, own), tree_pair<0>(odd, tabv, own), tree_pair<1>(even, tabv, own),
-                                   tree_pair<1>(odd, tabv, own),  tree_pair<2>(even, tabv, own), tree_pair<2>(odd, tabv, own),
-                                   tree_pair<3>(even, tabv, own), tree_pair<3>(odd, tabv, own)};
-#pragma unroll
-            for (int d = 0; d < 8; ++d) *reinterpret_cast<uint32_t*>(v_dst(j, d, tp, dg)) = e[d];
-          } else {
-            uint32_t e0[8], e1[8];
-            tree_entries<BW>(vr[P][j][0], v_off(tp, dg), tabv, lane, e0);
-            tree_entries<BW>(vr[P][j][1], v_off(tp, dg) + nbv, tabv, lane, e1);
-#pragma unroll
-            for (int d = 0; d < 8; ++d) {
-              char* dst = v_dst(j, d, tp, dg);
-              *reinterpret_cast<uint32_t*>(dst) = pack_lo(e0[d], e1[d]);
-              if constexpr (EX) *reinterpret_cast<uint32_t*>(dst + G::VT) = pack_hi(e0[d], e1[d]);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-          }
+          const uint8_t* v = block(1, grp);
+          vr[P][j][0] = tree_raw<W>(v, v_off(tp, dg), bwv);
+          vr[P][j][1] = tree_raw<W>(v, v_off(tp, dg) + nbv, bwv);
         }
-      });
-      if (C::NW <= G::NG || wig < G::NG) {
-        // what lies past the sequence may hold anything
-        const uint32_t n = c0 + 16 * wig + c < t_hi ? nr[P] : 0, size = n & 0x7fffu;
-        const uint32_t top = tree_row_max(size < 0x7c00u ? size : 0);  // of the finite ones
-        if (lane < 32) reinterpret_cast<uint16_t*>(lds + C::n_off)[(lane >> 4) * G::CH + 16 * wig + c] = uint16_t(n);
-        if (lane == 16) reinterpret_cast<uint32_t*>(lds + C::m_off)[wig] = top;
-      }
-    };
-
-    // LDS addresses of the products' operands: from 64 dims on the XORs of a few registers
-    uint32_t kb[G::KS], vb[4];
-    const int w0 = 16 * C::NTW * tg;  // the wave's first token of a chunk
-#pragma unroll
-    for (int k = 0; k < G::KS; ++k) kb[k] = uint32_t(C::k_off) + G::k_at(w0 + tree_tok(0, c), 4 * k + g);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) vb[i] = (uint32_t(C::v_off) + G::v_at(c, (w0 >> 3) + g)) ^ uint32_t(i << 4);
-    // tile t of K-step k: tokens tree_tok(t, 0) further on (bits 2 and 5: not the key's)
-    auto k_addr = [&](int t, int k) { return kb[k] + uint32_t(tree_tok(t, 0) * G::KROW); };
-    // row 16 mt + c, column (w0 >> 3) + 4 ks + g: mt's part of the key and ks are swaps
-    auto v_addr = [&](int mt, int ks) {
-      if constexpr (G::CH == 64) return (vb[mt & 3] ^ uint32_t(ks << 6)) + uint32_t(16 * mt * G::VROW);
-      else return vb[mt & 1] + uint32_t(16 * mt * G::VROW);
-    };
-    const int c_last = G::CH * (ch_hi - 1);
-    auto next = [&](int c0) { return min(c0, c_last); };  // the last chunk again past the end
-    constexpr std::integral_constant<int, 0> even;
-    constexpr std::integral_constant<int, AHEAD - 1> odd;
-    pages(G::CH * ch_lo);
-    load(even, G::CH * ch_lo);
-    if constexpr (AHEAD == 2) {
-      pages(next(G::CH * (ch_lo + 1)));
-      load(odd, next(G::CH * (ch_lo + 1)));
-    }
-    pages(next(G::CH * (ch_lo + AHEAD)));
-    auto chunk = [&](auto set, int c0) {
-      __syncthreads();  // the last chunk's tiles are read (at first: the tables are staged)
-      store(set, c0);
-      // the page ids of the chunk after are asked for ahead of the rows: waiting for them next
-      // time waits for no row
-      const uint32_t ids = page_ids(next(c0 + (AHEAD + 1) * G::CH));
-      load(set, next(c0 + AHEAD * G::CH));
-      pid = ids;
-      __syncthreads();
-
-      // scores of the wave's tokens: register i of tile t is token w0 + tree_tok(t, 4 g + i)
-      f32x4 d[NCT][C::NTW];
-#pragma unroll
-      for (int t = 0; t < C::NTW; ++t) {
-#pragma unroll
-        for (int ct = 0; ct < NCT; ++ct) d[ct][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int k = 0; k < G::KS; ++k) {
-          const char* kp = lds + k_addr(t, k);
-          const h8 kh = *reinterpret_cast<const h8*>(kp);
-#pragma unroll
-          for (int ct = 0; ct < NCT; ++ct) d[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[ct][k], d[ct][t], 0, 0, 0);
-          if constexpr (EX) {
-            const h8 kl = *reinterpret_cast<const h8*>(kp + G::KT);
-#pragma unroll
-            for (int ct = 0; ct < NCT; ++ct) {
-              d[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[ct][k], d[ct][t], 0, 0, 0);
-              d[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, ql[ct][k], d[ct][t], 0, 0, 0);
-            }
-          }
-        }
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      // value scale: every n_V < 2^(7 + gs), so 2^kTreeRescale n_V 2^-gs < 2^15 in fp16; it
-      // follows the norms' magnitude (n_V = 2^-20 keeps its bits)
-      constexpr int KV = C::NTW / 2;
-      {
-        const uint32_t* gm = reinterpret_cast<const uint32_t*>(lds + C::m_off);
-        uint32_t top = gm[0];
-#pragma unroll
-        for (int i = 1; i < G::NG; ++i) top = max(top, gm[i]);
-        top = __builtin_amdgcn_readfirstlane(int(top));
-        if (top && tree_exponent(top) - 7 > gs) {  // wave-uniform, rare after the first chunk
-          const int to = tree_exponent(top) - 7;
-          const float f = ldexpf(1.f, gs - to);
-          gs = to;
-#pragma unroll
-          for (int ct = 0; ct < NCT; ++ct) {
-            l[ct] *= f;
-#pragma unroll
-            for (int mt = 0; mt < G::MT; ++mt) acc[ct][mt] *= f;
-          }
-        }
-      }
-      // norms of the wave's tokens, eight consecutive ones per K-step of the values
-      h8 nk[KV], nv[KV];
-#pragma unroll
-      for (int ks = 0; ks < KV; ++ks) {
-        const uint16_t* np = reinterpret_cast<const uint16_t*>(lds + C::n_off) + w0 + 32 * ks + 8 * g;
-        nk[ks] = *reinterpret_cast<const h8*>(np);
-        nv[ks] = *reinterpret_cast<const h8*>(np + G::CH);
-      }
-      // scores less the row's maximum and gs, so that p 2^-gs = 2^x. masked: some of the chunk's
-      // tokens are nodes, seen by their descendants only, or lie past the sequence; a value norm
-      // that is not finite there makes the rows that see it NaN and no other
-      const float gsf = float(gs);
-      float x[NCT][KV][8], top[NCT];
-      auto scores = [&](auto masked) {
-        constexpr bool MASK = decltype(masked)::value;
-        bool bad[KV][8];
-        if constexpr (MASK) {
-#pragma unroll
-          for (int ks = 0; ks < KV; ++ks)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float v = float(nv[ks][j]);
-              bad[ks][j] = !(fabsf(v) < INFINITY);
-              if (bad[ks][j]) nv[ks][j] = _Float16(0.f);
-            }
-        }
-#pragma unroll
-        for (int ct = 0; ct < NCT; ++ct) {
-          uint32_t seen[KV];  // bit j: token 8 g + j of the K-step
-          if constexpr (MASK) {
-            int row = r0 + 16 * ct + c;
-            asm volatile("" : "+v"(row));  // not ahead of the loop: once per split
-            const int node = row / a.n_rep;
-            const uint64_t vis = node < a.T ? a.vis[int64_t(b) * a.T + node] : 0;
-            const int at = hist - c0;  // the tree's first position in the chunk (or before it)
-            const uint64_t word = at >= 0 ? (vis << at | ((uint64_t(1) << at) - 1)) : at > -64 ? vis >> -at : 0;
-#pragma unroll
-            for (int ks = 0; ks < KV; ++ks) seen[ks] = uint32_t(word >> (w0 + 32 * ks + 8 * g)) & 0xffu;
-          }
-          const float m0 = (m[ct] == -INFINITY ? 0.f : m[ct]) + gsf;
-          top[ct] = -INFINITY;
-#pragma unroll
-          for (int ks = 0; ks < KV; ++ks)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              float y = fmaf(d[ct][2 * ks + (j >> 2)][j & 3] * sc[ct], float(nk[ks][j]), -m0);
-              if (MASK) y = !(seen[ks] >> j & 1) ? -INFINITY : bad[ks][j] ? __builtin_nanf("") : y;
-              x[ct][ks][j] = y;
-              top[ct] = fmaxf(top[ct], y);
-            }
+        if (C::NW <= G::NG || wig < G::NG) {  // wave w: the norms of group w, K in lanes 0..15, V in 16..31
+          nr[P] = reinterpret_cast<const uint16_t*>(lane & 16 ? at.rows(3, wig) : at.rows(2, wig))[c];
         }
       };
-      if (c0 + G::CH <= hist) scores(std::integral_constant<bool, false>{});
-      else scores(std::integral_constant<bool, true>{});
-      // a row's maximum moves when a score exceeds it by more than kTreeRescale, and on its first key
-      bool move[NCT], any = false;
-#pragma unroll
-      for (int ct = 0; ct < NCT; ++ct) {
-        top[ct] = tree_max16(top[ct]) + gsf;
-        move[ct] = top[ct] > kTreeRescale || (m[ct] == -INFINITY && top[ct] > -INFINITY);
-        any = any || move[ct];
+      uint32_t k_to, v_to;  // LDS addresses of the first items
+      {
+        int grp, tok, tp, dg;
+        k_item(0, &grp, &tok, &dg);
+        k_to = uint32_t(C::k_off) + G::k_at(tok, dg);
+        v_item(0, &grp, &tp, &dg);
+        v_to = uint32_t(C::v_off) + G::v_at(8 * dg, tp >> 2) + 4 * (tp & 3);
       }
-      if (__any(any)) {
+      auto store = [&](auto set, int c0) {
+        constexpr int P = decltype(set)::value;
+        // recomputed from these two each chunk: held as loop invariants, the addresses of every
+        // write would take some thirty registers
+        asm volatile("" : "+v"(k_to), "+v"(v_to));
+        const uint32_t own = uint32_t(lane & (kPairCopies - 1)) << 2;
+        // An item's address from the first one's: TOK tokens further on, the key swapped by their
+        // bits (steps of 8 and more tokens add to the same bits of the first item's token only where
+        // that has none: up to 64 items of a wave lie in one group of 16); eight groups of dims
+        // further on, the V tile's key is the same
+        auto k_dst = [&](int j, int tok, int dg) {
+          constexpr int TOK = C::NTHR / (D / 8);
+          if (TOK >= 16 && DP64) return lds + (k_to ^ (G::k_key(TOK * j) << 4)) + uint32_t(TOK * j * G::KROW);
+          return lds + C::k_off + G::k_at(tok, dg);
+        };
+        auto v_dst = [&](int j, int d, int tp, int dg) {
+          if (j == 0 || (G::CH == 64 && C::VGB == C::NW))
+            return lds + (v_to ^ uint32_t(G::CH == 64 ? d >> 1 << 4 : d >> 2 << 4)) + (d + 8 * C::DGL * j) * G::VROW;
+          return lds + C::v_off + G::v_at(8 * dg + d, tp >> 2) + 4 * (tp & 3);
+        };
+        tree_by_width<W>(bwk, [&](auto bw) {
+          constexpr int BW = decltype(bw)::value;
 #pragma unroll
-        for (int ct = 0; ct < NCT; ++ct) {
-          const bool fresh = m[ct] == -INFINITY;
-          const float shift = move[ct] ? top[ct] : 0.f;
-          const float alpha = move[ct] ? (fresh ? 0.f : __builtin_amdgcn_exp2f(-top[ct])) : 1.f;
-          m[ct] = move[ct] ? (fresh ? 0.f : m[ct]) + top[ct] : m[ct];
-          l[ct] *= alpha;
-#pragma unroll
-          for (int mt = 0; mt < G::MT; ++mt) acc[ct][mt] *= alpha;
-#pragma unroll
-          for (int ks = 0; ks < KV; ++ks)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[ct][ks][j] -= shift;
-        }
-      }
-      // weights p n_V 2^-gs (l sums p 2^-gs)
-      h8 ph[NCT][KV], pl[EX ? NCT : 1][EX ? KV : 1];
-#pragma unroll
-      for (int ct = 0; ct < NCT; ++ct)
-#pragma unroll
-        for (int ks = 0; ks < KV; ++ks)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float p = __builtin_amdgcn_exp2f(x[ct][ks][j]);
-            l[ct] += p;
-            float w = p * float(nv[ks][j]);
-            // one rounded product for both terms: fused with the conversion (which rounds the exact
-            // product) the high term could differ from the one that the low term makes up for
-            if constexpr (EX) asm("" : "+v"(w));
-            ph[ct][ks][j] = _Float16(w);
-            if constexpr (EX) pl[ct][ks][j] = _Float16(w - float(ph[ct][ks][j]));
+          for (int j = 0; j < C::NK; ++j) {
+            int grp, tok, dg;
+            if (!k_item(j, &grp, &tok, &dg)) continue;
+            char* dst = k_dst(j, tok, dg);
+            if constexpr (PAIR) {
+              const uint32_t x = kr[P][j].lo;
+              *reinterpret_cast<u32x4*>(dst) =
+                  u32x4{tree_pair<0>(x, tabk, own), tree_pair<1>(x, tabk, own), tree_pair<2>(x, tabk, own), tree_pair<3>(x, tabk, own)};
+            } else {
+              uint32_t e[8];
+              tree_entries<BW>(kr[P][j], k_off(tok, dg), tabk, lane, e);
+              *reinterpret_cast<u32x4*>(dst) = u32x4{pack_lo(e[0], e[1]), pack_lo(e[2], e[3]), pack_lo(e[4], e[5]), pack_lo(e[6], e[7])};
+              if constexpr (EX)
+                *reinterpret_cast<u32x4*>(dst + G::KT) = u32x4{pack_hi(e[0], e[1]), pack_hi(e[2], e[3]), pack_hi(e[4], e[5]), pack_hi(e[6], e[7])};
+              if (j & 1) __builtin_amdgcn_sched_barrier(0);  // the lookups of two items in flight
+            }
           }
-      __builtin_amdgcn_sched_barrier(0);
-      // values: A row c of M-tile mt = dim 16 mt + c, k-slots of lane group g = tokens 32 ks + 8 g .. + 7
+        });
+        __builtin_amdgcn_sched_barrier(0);
+        tree_by_width<W>(bwv, [&](auto bw) {
+          constexpr int BW = decltype(bw)::value;
 #pragma unroll
-      for (int mt = 0; mt < G::MT; ++mt) {
+          for (int j = 0; j < C::NV; ++j) {
+            int grp, tp, dg;
+            if (!v_item(j, &grp, &tp, &dg)) continue;
+            if constexpr (PAIR) {
+              // byte i of `even`: the codes of dim 2 i of both tokens; of `odd`, of dim 2 i + 1
+              constexpr uint32_t m = 0x0f0f0f0fu;
+              const uint32_t x = vr[P][j][0].lo, y = vr[P][j][1].lo;
+              const uint32_t even = (x & m) | (y << 4 & ~m), odd = (x >> 4 & m) | (y & ~m);
+              const uint32_t e[8] = {tree_pair<0>(even, tabv, own), tree_pair<0>(odd, tabv, own), tree_pair<1>(even, tabv, own),
+                                     tree_pair<1>(odd, tabv, own),  tree_pair<2>(even, tabv, own), tree_pair<2>(odd, tabv, own),
+                                     tree_pair<3>(even, tabv, own), tree_pair<3>(odd, tabv, own)};
 #pragma unroll
-        for (int ks = 0; ks < KV; ++ks) {
-          const char* vp = lds + v_addr(mt, ks);
-          const h8 vh = *reinterpret_cast<const h8*>(vp);
+              for (int d = 0; d < 8; ++d) *reinterpret_cast<uint32_t*>(v_dst(j, d, tp, dg)) = e[d];
+            } else {
+              uint32_t e0[8], e1[8];
+              tree_entries<BW>(vr[P][j][0], v_off(tp, dg), tabv, lane, e0);
+              tree_entries<BW>(vr[P][j][1], v_off(tp, dg) + nbv, tabv, lane, e1);
 #pragma unroll
-          for (int ct = 0; ct < NCT; ++ct) acc[ct][mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph[ct][ks], acc[ct][mt], 0, 0, 0);
-          if constexpr (EX) {
-            const h8 vl = *reinterpret_cast<const h8*>(vp + G::VT);
+              for (int d = 0; d < 8; ++d) {
+                char* dst = v_dst(j, d, tp, dg);
+                *reinterpret_cast<uint32_t*>(dst) = pack_lo(e0[d], e1[d]);
+                if constexpr (EX) *reinterpret_cast<uint32_t*>(dst + G::VT) = pack_hi(e0[d], e1[d]);
+              }
+              __builtin_amdgcn_sched_barrier(0);
+            }
+          }
+        });
+        if (C::NW <= G::NG || wig < G::NG) {
+          // what lies past the sequence may hold anything
+          const uint32_t n = c0 + 16 * wig + c < t_hi ? nr[P] : 0, size = n & 0x7fffu;
+          const uint32_t top = tree_row_max(size < 0x7c00u ? size : 0);  // of the finite ones
+          if (lane < 32) reinterpret_cast<uint16_t*>(lds + C::n_off)[(lane >> 4) * G::CH + 16 * wig + c] = uint16_t(n);
+          if (lane == 16) reinterpret_cast<uint32_t*>(lds + C::m_off)[wig] = top;
+        }
+      };
+
+      // LDS addresses of the products' operands: from 64 dims on the XORs of a few registers
+      uint32_t kb[G::KS], vb[4];
+      const int w0 = 16 * C::NTW * tg;  // the wave's first token of a chunk
 #pragma unroll
-            for (int ct = 0; ct < NCT; ++ct) {
-              acc[ct][mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph[ct][ks], acc[ct][mt], 0, 0, 0);
-              acc[ct][mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl[ct][ks], acc[ct][mt], 0, 0, 0);
+      for (int k = 0; k < G::KS; ++k) kb[k] = uint32_t(C::k_off) + G::k_at(w0 + tree_tok(0, c), 4 * k + g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) vb[i] = (uint32_t(C::v_off) + G::v_at(c, (w0 >> 3) + g)) ^ uint32_t(i << 4);
+      // tile t of K-step k: tokens tree_tok(t, 0) further on (bits 2 and 5: not the key's)
+      auto k_addr = [&](int t, int k) { return kb[k] + uint32_t(tree_tok(t, 0) * G::KROW); };
+      // row 16 mt + c, column (w0 >> 3) + 4 ks + g: mt's part of the key and ks are swaps
+      auto v_addr = [&](int mt, int ks) {
+        if constexpr (G::CH == 64) return (vb[mt & 3] ^ uint32_t(ks << 6)) + uint32_t(16 * mt * G::VROW);
+        else return vb[mt & 1] + uint32_t(16 * mt * G::VROW);
+      };
+      const int c_last = G::CH * (ch_hi - 1);
+      auto next = [&](int c0) { return min(c0, c_last); };  // the last chunk again past the end
+      constexpr std::integral_constant<int, 0> even;
+      constexpr std::integral_constant<int, AHEAD - 1> odd;
+      pages(page_ids(G::CH * ch_lo), G::CH * ch_lo);
+      load(even);
+      if constexpr (AHEAD == 2) {
+        pages(page_ids(next(G::CH * (ch_lo + 1))), next(G::CH * (ch_lo + 1)));
+        load(odd);
+      }
+      uint32_t ids = page_ids(next(G::CH * (ch_lo + AHEAD)));
+      auto chunk = [&](auto set, int c0) {
+        __syncthreads();  // the last chunk's tiles are read (at first: the tables are staged)
+        store(set, c0);
+        // the page ids of the chunk after are asked for ahead of the rows: waiting for them next
+        // time waits for no row
+        pages(ids, next(c0 + AHEAD * G::CH));
+        ids = page_ids(next(c0 + (AHEAD + 1) * G::CH));
+        load(set);
+        __syncthreads();
+        if (r0 >= rows) return;  // padding: the wave has only its part of the tiles to do
+
+        // scores of the wave's tokens: register i of tile t is token w0 + tree_tok(t, 4 g + i)
+        f32x4 d[NCT][C::NTW];
+#pragma unroll
+        for (int t = 0; t < C::NTW; ++t) {
+#pragma unroll
+          for (int ct = 0; ct < NCT; ++ct) d[ct][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < G::KS; ++k) {
+            const char* kp = lds + k_addr(t, k);
+            const h8 kh = *reinterpret_cast<const h8*>(kp);
+#pragma unroll
+            for (int ct = 0; ct < NCT; ++ct) d[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[ct][k], d[ct][t], 0, 0, 0);
+            if constexpr (EX) {
+              const h8 kl = *reinterpret_cast<const h8*>(kp + G::KT);
+#pragma unroll
+              for (int ct = 0; ct < NCT; ++ct) {
+                d[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[ct][k], d[ct][t], 0, 0, 0);
+                d[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, ql[ct][k], d[ct][t], 0, 0, 0);
+              }
             }
           }
         }
+        __builtin_amdgcn_sched_barrier(0);
+        // value scale: every n_V < 2^(7 + gs), so 2^kTreeRescale n_V 2^-gs < 2^15 in fp16; it
+        // follows the norms' magnitude (n_V = 2^-20 keeps its bits)
+        constexpr int KV = C::NTW / 2;
+        {
+          const uint32_t* gm = reinterpret_cast<const uint32_t*>(lds + C::m_off);
+          uint32_t top = gm[0];
+#pragma unroll
+          for (int i = 1; i < G::NG; ++i) top = max(top, gm[i]);
+          top = __builtin_amdgcn_readfirstlane(int(top));
+          if (top && tree_exponent(top) - 7 > gs) {  // wave-uniform, rare after the first chunk
+            const int to = tree_exponent(top) - 7;
+            const float f = ldexpf(1.f, gs - to);
+            gs = to;
+#pragma unroll
+            for (int ct = 0; ct < NCT; ++ct) {
+              l[ct] *= f;
+#pragma unroll
+              for (int mt = 0; mt < G::MT; ++mt) acc[ct][mt] *= f;
+            }
+          }
+        }
+        // norms of the wave's tokens, eight consecutive ones per K-step of the values
+        h8 nk[KV], nv[KV];
+#pragma unroll
+        for (int ks = 0; ks < KV; ++ks) {
+          const uint16_t* np = reinterpret_cast<const uint16_t*>(lds + C::n_off) + w0 + 32 * ks + 8 * g;
+          nk[ks] = *reinterpret_cast<const h8*>(np);
+          nv[ks] = *reinterpret_cast<const h8*>(np + G::CH);
+        }
+        // scores less the row's maximum and gs, so that p 2^-gs = 2^x. masked: some of the chunk's
+        // tokens are nodes, seen by their descendants only, or lie past the sequence; a value norm
+        // that is not finite there makes the rows that see it NaN and no other
+        const float gsf = float(gs);
+        float x[NCT][KV][8], top[NCT];
+        auto scores = [&](auto masked) {
+          constexpr bool MASK = decltype(masked)::value;
+          bool bad[KV][8];
+          if constexpr (MASK) {
+#pragma unroll
+            for (int ks = 0; ks < KV; ++ks)
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const float v = float(nv[ks][j]);
+                bad[ks][j] = !(fabsf(v) < INFINITY);
+                if (bad[ks][j]) nv[ks][j] = _Float16(0.f);
+              }
+          }
+#pragma unroll
+          for (int ct = 0; ct < NCT; ++ct) {
+            uint32_t seen[KV];  // bit j: token 8 g + j of the K-step
+            if constexpr (MASK) {
+              int row = r0 + 16 * ct + c;
+              asm volatile("" : "+v"(row));  // not ahead of the loop: once per split
+              const int node = row / a.n_rep;
+              const uint64_t vis = node < a.T ? a.vis[int64_t(b) * a.T + node] : 0;
+              const int at = hist - c0;  // the tree's first position in the chunk (or before it)
+              const uint64_t word = at >= 0 ? (vis << at | ((uint64_t(1) << at) - 1)) : at > -64 ? vis >> -at : 0;
+#pragma unroll
+              for (int ks = 0; ks < KV; ++ks) seen[ks] = uint32_t(word >> (w0 + 32 * ks + 8 * g)) & 0xffu;
+            }
+            const float m0 = (m[ct] == -INFINITY ? 0.f : m[ct]) + gsf;
+            top[ct] = -INFINITY;
+#pragma unroll
+            for (int ks = 0; ks < KV; ++ks)
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                float y = fmaf(d[ct][2 * ks + (j >> 2)][j & 3] * sc[ct], float(nk[ks][j]), -m0);
+                if (MASK) y = !(seen[ks] >> j & 1) ? -INFINITY : bad[ks][j] ? __builtin_nanf("") : y;
+                x[ct][ks][j] = y;
+                top[ct] = fmaxf(top[ct], y);
+              }
+          }
+        };
+        if (c0 + G::CH <= hist) scores(std::integral_constant<bool, false>{});
+        else scores(std::integral_constant<bool, true>{});
+        // a row's maximum moves when a score exceeds it by more than kTreeRescale, and on its first key
+        bool move[NCT], any = false;
+#pragma unroll
+        for (int ct = 0; ct < NCT; ++ct) {
+          top[ct] = tree_max16(top[ct]) + gsf;
+          move[ct] = top[ct] > kTreeRescale || (m[ct] == -INFINITY && top[ct] > -INFINITY);
+          any = any || move[ct];
+        }
+        if (__any(any)) {
+#pragma unroll
+          for (int ct = 0; ct < NCT; ++ct) {
+            const bool fresh = m[ct] == -INFINITY;
+            const float shift = move[ct] ? top[ct] : 0.f;
+            const float alpha = move[ct] ? (fresh ? 0.f : __builtin_amdgcn_exp2f(-top[ct])) : 1.f;
+            m[ct] = move[ct] ? (fresh ? 0.f : m[ct]) + top[ct] : m[ct];
+            l[ct] *= alpha;
+#pragma unroll
+            for (int mt = 0; mt < G::MT; ++mt) acc[ct][mt] *= alpha;
+#pragma unroll
+            for (int ks = 0; ks < KV; ++ks)
+#pragma unroll
+              for (int j = 0; j < 8; ++j) x[ct][ks][j] -= shift;
+          }
+        }
+        // weights p n_V 2^-gs (l sums p 2^-gs)
+        h8 ph[NCT][KV], pl[EX ? NCT : 1][EX ? KV : 1];
+#pragma unroll
+        for (int ct = 0; ct < NCT; ++ct)
+#pragma unroll
+          for (int ks = 0; ks < KV; ++ks)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float p = __builtin_amdgcn_exp2f(x[ct][ks][j]);
+              l[ct] += p;
+              float w = p * float(nv[ks][j]);
+              // one rounded product for both terms: fused with the conversion (which rounds the exact
+              // product) the high term could differ from the one that the low term makes up for
+              if constexpr (EX) asm("" : "+v"(w));
+              ph[ct][ks][j] = _Float16(w);
+              if constexpr (EX) pl[ct][ks][j] = _Float16(w - float(ph[ct][ks][j]));
+            }
+        __builtin_amdgcn_sched_barrier(0);
+        // values: A row c of M-tile mt = dim 16 mt + c, k-slots of lane group g = tokens 32 ks + 8 g .. + 7
+#pragma unroll
+        for (int mt = 0; mt < G::MT; ++mt) {
+#pragma unroll
+          for (int ks = 0; ks < KV; ++ks) {
+            const char* vp = lds + v_addr(mt, ks);
+            const h8 vh = *reinterpret_cast<const h8*>(vp);
+#pragma unroll
+            for (int ct = 0; ct < NCT; ++ct) acc[ct][mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph[ct][ks], acc[ct][mt], 0, 0, 0);
+            if constexpr (EX) {
+              const h8 vl = *reinterpret_cast<const h8*>(vp + G::VT);
+#pragma unroll
+              for (int ct = 0; ct < NCT; ++ct) {
+                acc[ct][mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph[ct][ks], acc[ct][mt], 0, 0, 0);
+                acc[ct][mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl[ct][ks], acc[ct][mt], 0, 0, 0);
+              }
+            }
+          }
+        }
+      };
+      for (int ch = ch_lo; ch < ch_hi; ch += AHEAD) {
+        chunk(even, G::CH * ch);
+        if (AHEAD == 2 && ch + 1 < ch_hi) chunk(odd, G::CH * (ch + 1));
       }
-    };
-    for (int ch = ch_lo; ch < ch_hi; ch += AHEAD) {
-      chunk(even, G::CH * ch);
-      if (AHEAD == 2 && ch + 1 < ch_hi) chunk(odd, G::CH * (ch + 1));
     }
-  }
 
-  const float f = ldexpf(1.f, gs - 8), lf = ldexpf(1.f, gs);
+    const float f = ldexpf(1.f, gs - 8), lf = ldexpf(1.f, gs);
 #pragma unroll
-  for (int ct = 0; ct < NCT; ++ct) {
-    l[ct] *= lf;
-    l[ct] += __shfl_xor(l[ct], 16, 64);
-    l[ct] += __shfl_xor(l[ct], 32, 64);
+    for (int ct = 0; ct < NCT; ++ct) {
+      l[ct] *= lf;
+      l[ct] += __shfl_xor(l[ct], 16, 64);
+      l[ct] += __shfl_xor(l[ct], 32, 64);
 #pragma unroll
-    for (int mt = 0; mt < G::MT; ++mt) acc[ct][mt] *= f;
-  }
-  if constexpr (TG == 2) {  // the second token group's waves hand over to the first's
-    __syncthreads();  // the tiles are read
-    float* give = reinterpret_cast<float*>(lds) + (rg * NCT * 16) * (D + 2);
-    if (tg == 1) {
+      for (int mt = 0; mt < G::MT; ++mt) acc[ct][mt] *= f;
+    }
+    if constexpr (TG == 2) {  // the second token group's waves hand over to the first's
+      float* o = reinterpret_cast<float*>(lds) + (rg * 16 + c) * (D + 2);
 #pragma unroll
       for (int ct = 0; ct < NCT; ++ct) {
-        float* o = give + (16 * ct + c) * (D + 2);
+        __syncthreads();  // the tiles, or what was handed over before, are read
+        if (tg == 1) {
 #pragma unroll
-        for (int mt = 0; mt < G::MT; ++mt)
+          for (int mt = 0; mt < G::MT; ++mt)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) o[16 * mt + 4 * g + i] = acc[ct][mt][i];
-        if (g == 0) {
-          o[D] = m[ct];
-          o[D + 1] = l[ct];
+            for (int i = 0; i < 4; ++i) o[16 * mt + 4 * g + i] = acc[ct][mt][i];
+          if (g == 0) {
+            o[D] = m[ct];
+            o[D + 1] = l[ct];
+          }
+        }
+        __syncthreads();
+        if (tg == 0) {
+          const float m1 = o[D], l1 = o[D + 1], M = fmaxf(m[ct], m1);
+          const float w0 = m[ct] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[ct] - M);
+          const float w1 = m1 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m1 - M);
+          m[ct] = M;
+          l[ct] = l[ct] * w0 + l1 * w1;
+#pragma unroll
+          for (int mt = 0; mt < G::MT; ++mt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[ct][mt][i] = acc[ct][mt][i] * w0 + o[16 * mt + 4 * g + i] * w1;
         }
       }
     }
-    __syncthreads();
-    if (tg == 1) return;
+    // items of 16 rows: ((b Hkv + kvh) nsplit + s) nrp / 16 + row block
+    if (tg == 0 && r0 < rows) {
 #pragma unroll
-    for (int ct = 0; ct < NCT; ++ct) {
-      const float* o = give + (16 * ct + c) * (D + 2);
-      const float m1 = o[D], l1 = o[D + 1], M = fmaxf(m[ct], m1);
-      const float w0 = m[ct] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[ct] - M);
-      const float w1 = m1 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m1 - M);
-      m[ct] = M;
-      l[ct] = l[ct] * w0 + l1 * w1;
+      for (int ct = 0; ct < NCT; ++ct) {
+        const int64_t item = ((int64_t(b) * a.Hkv + kvh) * a.nsplit + s) * (a.nrp / 16) + r0 / 16 + ct;
+        float* o = a.part_acc + (item * 16 + c) * D + 4 * g;
 #pragma unroll
-      for (int mt = 0; mt < G::MT; ++mt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[ct][mt][i] = acc[ct][mt][i] * w0 + o[16 * mt + 4 * g + i] * w1;
+        for (int mt = 0; mt < G::MT; ++mt) *reinterpret_cast<f32x4*>(o + 16 * mt) = acc[ct][mt];
+        if (g == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * (item * 16 + c)) = make_float2(m[ct], l[ct]);
+      }
     }
-  }
-  // items of 16 rows: ((b Hkv + kvh) nsplit + s) nrp / 16 + row block
-#pragma unroll
-  for (int ct = 0; ct < NCT; ++ct) {
-    const int64_t item = ((int64_t(b) * a.Hkv + kvh) * a.nsplit + s) * (a.nrp / 16) + r0 / 16 + ct;
-    float* o = a.part_acc + (item * 16 + c) * D + 4 * g;
-#pragma unroll
-    for (int mt = 0; mt < G::MT; ++mt) *reinterpret_cast<f32x4*>(o + 16 * mt) = acc[ct][mt];
-    if (g == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * (item * 16 + c)) = make_float2(m[ct], l[ct]);
+    __syncthreads();  // the tiles and what was handed over are read
   }
 }
 
-// Columns j of 16 rows of x (LDS rows of D + 4 floats) times a D x D matrix on
-// v_mfma_f32_16x16x4f32: wave w takes column tiles w, w + 4, ...; K-step (s, e), slot g is
-// column 16 s + 4 g + e of x. mat(j, k4) gives rows k4 .. k4 + 3 of column j. Lane 16 g + c
-// ends with columns 16 t + 4 g .. + 3 of row c.
-template <int D, class Mat, class Out>
-__device__ __forceinline__ void tree_rows_product(const float* x, int wave, int lane, Mat&& mat, Out&& out) {
-  const int g = lane >> 4, c = lane & 15;
-  for (int t = wave; t < D / 16; t += 4) {
-    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+// 16 rows times a D x D matrix on v_mfma_f32_16x16x4f32, a tile of 16 columns a wave: K-step (s, e),
+// slot g is column 16 s + 4 g + e of the rows. mat(j, k4) gives rows k4 .. k4 + 3 of column j; the
+// operands are loaded ahead of the rows, whose loads they hide behind. Lane 16 g + c ends with
+// columns 16 wave + 4 g .. + 3 of row c.
+template <int D>
+struct TreeProduct {
+  f32x4 m[D / 16];
+  template <class Mat>
+  __device__ __forceinline__ void load(int wave, int lane, Mat&& mat) {
+    if (wave >= D / 16) return;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) m[s] = mat(16 * wave + (lane & 15), 16 * s + 4 * (lane >> 4));
+  }
+  // x: LDS, row c's D floats (16-byte aligned)
+  __device__ __forceinline__ f32x4 run(const float* x, int lane) const {
+    f32x4 y[2] = {};
 #pragma unroll
     for (int s = 0; s < D / 16; ++s) {
-      const f32x4 av = mat(16 * t + c, 16 * s + 4 * g), bv = *reinterpret_cast<const f32x4*>(x + c * (D + 4) + 16 * s + 4 * g);
+      const f32x4 bv = *reinterpret_cast<const f32x4*>(x + 16 * s + 4 * (lane >> 4));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y = __builtin_amdgcn_mfma_f32_16x16x4f32(av[e], bv[e], y, 0, 0, 0);
+      for (int e = 0; e < 4; ++e) y[s & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(m[s][e], bv[e], y[s & 1], 0, 0, 0);
     }
-    out(t, y);
+    return y[0] + y[1];
   }
-}
+};
+
+__host__ __device__ constexpr int tree_rotate_threads(int D) { return 4 * D > 256 ? 4 * D : 256; }
 
 // q' of sixteen rows per work-group (rows past n_rep T: zero), and the nodes' words.
 template <int D>
-__global__ __launch_bounds__(256) void tree_rotate_kernel(TreeRotArgs a) {
-  constexpr int XS = D + 4;
+__global__ __launch_bounds__(tree_rotate_threads(D)) void tree_rotate_kernel(TreeRotArgs a) {
+  constexpr int XS = D + 4, NTHR = tree_rotate_threads(D);
   __shared__ __align__(16) float x[16 * XS];
   __shared__ __align__(16) float y[16 * XS];
   __shared__ int par[64];
@@ -680,13 +679,22 @@ __global__ __launch_bounds__(256) void tree_rotate_kernel(TreeRotArgs a) {
   const int r0 = 16 * int(blockIdx.x % tiles), kvh = int(unit % a.Hkv), rows = a.n_rep * a.T;
   const int64_t b = unit / a.Hkv;
   const bool words = kvh == 0 && r0 == 0;  // one work-group per sequence
+  TreeProduct<D> pi;
+  pi.load(wave, lane, [&](int j, int k) { return *reinterpret_cast<const f32x4*>(a.pi + j * D + k); });
   if (words && tid < 64) par[tid] = tid < a.T ? a.parents[b * a.psb + tid] : -1;
-  for (int i = tid; i < 16 * D; i += 256) {
-    const int r = r0 + i / D, d = i % D;
-    float v = 0.f;
-    if (r < rows) v = load_elem(a.q, b * a.qsb + (kvh * a.n_rep + r % a.n_rep) * a.qsh + (r / a.n_rep) * a.qsq + d, a.q_dtype);
-    x[(i / D) * XS + d] = v;
-  }
+  // all loads of a thread at once: the type is asked for outside
+  const auto fetch = [&](auto&& load) {
+#pragma unroll
+    for (int i0 = 0; i0 < 16 * D; i0 += NTHR) {
+      const int i = i0 + tid, r = r0 + i / D, d = i % D;
+      float v = 0.f;
+      if (r < rows) v = load(b * a.qsb + (kvh * a.n_rep + r % a.n_rep) * a.qsh + (r / a.n_rep) * a.qsq + d);
+      x[(i / D) * XS + d] = v;
+    }
+  };
+  if (a.q_dtype == WN_F32) fetch([&](int64_t o) { return static_cast<const float*>(a.q)[o]; });
+  else if (a.q_dtype == WN_BF16) fetch([&](int64_t o) { return bf16_to_f32(static_cast<const uint16_t*>(a.q)[o]); });
+  else fetch([&](int64_t o) { return f16_to_f32(static_cast<const uint16_t*>(a.q)[o]); });
   __syncthreads();
   if (words && tid < a.T) {
     // a parent comes before its child: any other value ends the walk, as -1 does
@@ -695,11 +703,16 @@ __global__ __launch_bounds__(256) void tree_rotate_kernel(TreeRotArgs a) {
     a.vis[b * a.T + tid] = w;
   }
   const int g = lane >> 4, c = lane & 15;
-  tree_rows_product<D>(
-      x, wave, lane, [&](int j, int k) { return *reinterpret_cast<const f32x4*>(a.pi + j * D + k); },
-      [&](int t, f32x4 v) { *reinterpret_cast<f32x4*>(y + c * XS + 16 * t + 4 * g) = v; });
+  if (wave < D / 16) *reinterpret_cast<f32x4*>(y + c * XS + 16 * wave + 4 * g) = pi.run(x + c * XS, lane);
   __syncthreads();
+  if (a.qf) {
+#pragma unroll
+    for (int i = tid; i < 16 * D; i += NTHR)
+      a.qf[(unit * a.nrp + r0 + i / D) * D + i % D] = y[(i / D) * XS + i % D] * a.scale;
+    return;
+  }
   // sixteen threads a row: its largest magnitude, then the fp16 terms of q' 2^e (below 2^15)
+  if (tid >= 256) return;
   const int r = tid >> 4, k = tid & 15;
   float top = 0.f;
 #pragma unroll
@@ -721,57 +734,97 @@ __global__ __launch_bounds__(256) void tree_rotate_kernel(TreeRotArgs a) {
   }
 }
 
-// Sixteen rows per work-group: the splits' partials merged (weights 2^(m_s - max m)),
-// divided by the sum, times Pi_V, cast. A row that saw no key is 0.
-template <int D>
-__global__ __launch_bounds__(256) void tree_merge_kernel(TreeMergeArgs a) {
-  constexpr int XS = D + 4, DPT = D / 16;  // dims per thread
-  __shared__ __align__(16) float x[16 * XS];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int tiles = a.nrp / 16;
-  const int64_t unit = blockIdx.x / tiles;
-  const int blk = int(blockIdx.x % tiles), rows = a.n_rep * a.T;
-  const int r = tid >> 4, k = tid & 15;
-  const int64_t first = (unit * a.nsplit * tiles + blk) * 16 + r, step = int64_t(tiles) * 16;
-  float M = -INFINITY;
-  for (int s = 0; s < a.nsplit; ++s) M = fmaxf(M, a.part_ml[2 * (first + s * step)]);
-  float den = 0.f, num[DPT];
+// R rows per work-group of 16 waves, 16 / R waves a row: the splits' partials merged (weights
+// 2^(m_s - max m)), divided by the sum, times Pi_V, cast. A row that saw no key is 0. The statistics
+// come a split to a lane, the accumulators a split to a load, eight of them in flight; the first of
+// both, and Pi_V's operands, are asked for before anything is known of the sequence: what bounds
+// these few rows is one round trip after another.
+template <int D, int R>
+__global__ __launch_bounds__(1024) void tree_merge_kernel(TreeMergeArgs a) {
+  constexpr int XS = D + 4, LD = D < 64 ? D : 64, VEC = D / LD;  // lanes a split, dims a lane
+  constexpr int SUB = 64 / LD, PARTS = 16 / R * SUB;              // splits are taken in PARTS residue classes
+  __shared__ __align__(16) float x[PARTS][R][XS];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int rows = a.n_rep * a.T, blocks = (rows + R - 1) / R;
+  const int64_t unit = blockIdx.x / blocks;
+  const int blk = int(blockIdx.x % blocks);
+  const int r = wave % R, part = wave / R * SUB + lane / LD, d0 = VEC * (lane % LD);
+  const int64_t first = unit * a.nsplit * a.nrp + min(blk * R + r, rows - 1);
+  const auto stats = [&](int s) { return *reinterpret_cast<const float2*>(a.part_ml + 2 * (first + int64_t(min(s, a.nsplit - 1)) * a.nrp)); };
+  float v[8][VEC];
+  const auto fetch = [&](int s0) {  // splits s0 + part, s0 + PARTS + part, ...
 #pragma unroll
-  for (int i = 0; i < DPT; ++i) num[i] = 0.f;
-  if (M != -INFINITY) {
-    for (int s = 0; s < a.nsplit; ++s) {
-      const int64_t p = first + s * step;
-      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * p);
-      const float w = __builtin_amdgcn_exp2f(ml.x - M);  // 0 for a split that saw no key
-      den = fmaf(w, ml.y, den);
+    for (int j = 0; j < 8; ++j) {
+      const float* p = a.part_acc + (first + int64_t(min(s0 + PARTS * j + part, a.nsplit - 1)) * a.nrp) * D + d0;
 #pragma unroll
-      for (int i = 0; i < DPT; ++i) num[i] = fmaf(w, a.part_acc[p * D + k + 16 * i], num[i]);
+      for (int e = 0; e < VEC; ++e) v[j][e] = p[e];
+    }
+  };
+  const float2 ml0 = stats(lane);
+  fetch(0);
+  TreeProduct<D> pi;
+  pi.load(wave, lane, [&](int j, int kk) {
+    return f32x4{a.pi_v[kk * D + j], a.pi_v[(kk + 1) * D + j], a.pi_v[(kk + 2) * D + j], a.pi_v[(kk + 3) * D + j]};
+  });
+  const int L = min(max(a.seq_lens[unit / a.Hkv], 0), a.max_len), span = tree_span(L, a.nsplit, a.span);
+  const int live = (L + span - 1) / max(span, 1);  // splits that the sequence has: the others' partials are not its own
+  float M = lane < live ? ml0.x : -INFINITY;
+  for (int s = 64 + lane; s < live; s += 64) M = fmaxf(M, stats(s).x);
+  M = wave_max(M);
+  if (M == -INFINITY) M = 0.f;  // no split saw a key: every weight is 0
+  float den = 0.f, num[VEC] = {};
+  for (int s0 = 0; s0 < live; s0 += 64) {
+    const float2 ml = s0 ? stats(s0 + lane) : ml0;
+    const bool own = s0 + lane < live;
+    const float w = own ? __builtin_amdgcn_exp2f(ml.x - M) : 0.f;  // split s0 + lane's; 0 for one that saw no key
+    den = own ? fmaf(w, ml.y, den) : den;
+    const int n = min(64, live - s0);
+    for (int i = 0; i < n; i += 8 * PARTS) {
+      if (s0 + i) fetch(s0 + i);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int s = i + PARTS * j + part;
+        const float ws = __shfl(w, s & 63, 64);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) num[e] = s < n ? fmaf(ws, v[j][e], num[e]) : num[e];
+      }
     }
   }
+  den = wave_sum(den);
   const float inv = den != 0.f ? 1.f / den : 0.f;
 #pragma unroll
-  for (int i = 0; i < DPT; ++i) x[r * XS + k + 16 * i] = num[i] * inv;
+  for (int e = 0; e < VEC; ++e) x[part][r][d0 + e] = num[e] * inv;
   __syncthreads();
-  const int g = lane >> 4, c = lane & 15, rr = 16 * blk + c;
+  if constexpr (PARTS > 1) {
+    for (int i = tid; i < R * D; i += 1024) {
+      float t = 0.f;
+#pragma unroll
+      for (int q = 0; q < PARTS; ++q) t += x[q][i / D][i % D];
+      x[0][i / D][i % D] = t;
+    }
+    __syncthreads();
+  }
+  const int g = lane >> 4, c = lane & 15, rr = R * blk + c;
+  if (wave >= D / 16) return;
+  const f32x4 y = pi.run(x[0][c % R], lane);
+  if (c >= R || rr >= rows) return;
   const int kvh = int(unit % a.Hkv), Hq = a.Hkv * a.n_rep;
   const int64_t b = unit / a.Hkv;
-  const int64_t o = ((b * Hq + kvh * a.n_rep + rr % a.n_rep) * a.T + rr / a.n_rep) * D + 4 * g;
-  tree_rows_product<D>(
-      x, wave, lane,
-      [&](int j, int kk) {
-        return f32x4{a.pi_v[kk * D + j], a.pi_v[(kk + 1) * D + j], a.pi_v[(kk + 2) * D + j], a.pi_v[(kk + 3) * D + j]};
-      },
-      [&](int t, f32x4 v) {
-        if (rr >= rows) return;
+  const int64_t o = ((b * Hq + kvh * a.n_rep + rr % a.n_rep) * a.T + rr / a.n_rep) * D + 16 * wave + 4 * g;
+  if (a.out_dtype == WN_F32) {
+    __builtin_memcpy(static_cast<float*>(a.out) + o, &y, 16);
+  } else {
+    uint16_t h[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) store_elem(a.out, o + 16 * t + i, a.out_dtype, v[i]);
-      });
+    for (int i = 0; i < 4; ++i) h[i] = a.out_dtype == WN_BF16 ? f32_to_bf16(y[i]) : f32_to_f16(y[i]);
+    __builtin_memcpy(static_cast<uint16_t*>(a.out) + o, h, 8);
+  }
 }
 
 template <int D, bool EX, int NCT, int RG, int TG, int W>
 TreeScan tree_scan() {
   using C = TreeCfg<D, EX, NCT, RG, TG>;
-  return TreeScan{tree_scan_kernel<D, EX, NCT, RG, TG, W>, C::ROWS, C::NTHR, C::tab_off, W == 4 && !EX ? 2 * kPairBytes : 0, C::give};
+  return TreeScan{tree_scan_kernel<D, EX, NCT, RG, TG, W>, C::ROWS, C::NTHR, C::tab_off, W == 4 && !EX ? 2 * kPairBytes : 0, C::give, 0};
 }
 
 template <int D, bool EX, int W>
@@ -787,7 +840,9 @@ TreeKernels tree_kernels() {
     else k.scan[2] = tree_scan<D, EX, 2, 4, 1, W>();
   }
   k.rotate = tree_rotate_kernel<D>;
-  k.merge = tree_merge_kernel<D>;
+  k.merge[0] = tree_merge_kernel<D, 4>;
+  k.merge[1] = tree_merge_kernel<D, 16>;
+  k.rotate_threads = tree_rotate_threads(D);
   return k;
 }
 

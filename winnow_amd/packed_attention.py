@@ -554,18 +554,9 @@ def check_parents(parents: torch.Tensor) -> None:
 
 
 @functools.lru_cache(maxsize=1024)
-def _tree_plan(device_index: int, *shape) -> int:
-    ns = ctypes.c_int(0)
-    with torch.cuda.device(device_index):
-        _lib.call("wn_tree_plan", *shape, ctypes.byref(ns))
-    return ns.value
-
-
-@functools.lru_cache(maxsize=1024)
-def tree_workspace_bytes(batch: int, num_q_heads: int, num_kv_heads: int, nodes: int, head_dim: int, exact: bool,
+def tree_workspace_bytes(batch: int, num_q_heads: int, num_kv_heads: int, nodes: int, head_dim: int,
                          num_splits: int) -> int:
-    return int(_lib.lib().wn_tree_workspace_bytes(batch, num_q_heads, num_kv_heads, nodes, head_dim, int(exact),
-                                                  num_splits))
+    return int(_lib.lib().wn_tree_workspace_bytes(batch, num_q_heads, num_kv_heads, nodes, head_dim, num_splits))
 
 
 def tree_exact(q: torch.Tensor, out_dtype: torch.dtype, allow_tf32: bool = False) -> bool:
@@ -575,14 +566,21 @@ def tree_exact(q: torch.Tensor, out_dtype: torch.dtype, allow_tf32: bool = False
     return not (allow_tf32 or q.dtype == out_dtype == torch.bfloat16)
 
 
-def tree_plan_for(q: torch.Tensor, kv: PackedKV, exact: bool) -> int:
-    """Split count of the tree attention for this query and handle (wn_tree_plan)."""
+def tree_plan_for(q: torch.Tensor, kv: PackedKV, exact: bool, *, read_lens: bool = True) -> tuple[int, int, int]:
+    """(num_splits, span, parts) of the tree attention for this query and handle (wn_tree_plan), from the
+    lengths' host mirror, or, without one, a host copy (``read_lens``) or the width of the table."""
     B, Hq, T, D = q.shape
-    lens = kv.seq_lens_host if kv.seq_lens_host is not None else kv.seq_lens.cpu()
-    # the plan counts 64-token chunks of the longest sequence
-    longest = max(lens.tolist(), default=0)
-    return _tree_plan(q.get_device(), B, Hq, kv.num_kv_heads, T, D, kv.page_size, kv.k_quant.bit_width,
-                      kv.v_quant.bit_width, int(exact), -(-max(longest, 0) // 64) * 64)
+    lens = kv.seq_lens_host
+    if lens is None and read_lens:
+        lens = kv.seq_lens.cpu()
+    if lens is not None and (lens.dtype != torch.int32 or lens.shape != (B,) or not lens.is_contiguous()):
+        lens = lens.to(torch.int32).reshape(B).contiguous()
+    ns, span, parts = ctypes.c_int(0), ctypes.c_int(0), ctypes.c_int(0)
+    with torch.cuda.device(q.device):
+        _lib.call("wn_tree_plan", B, Hq, kv.num_kv_heads, T, D, kv.page_size, kv.k_quant.bit_width, kv.v_quant.bit_width,
+                  int(exact), kv.page_table.shape[1], _lib.ptr(lens), ctypes.byref(ns), ctypes.byref(span),
+                  ctypes.byref(parts))
+    return ns.value, span.value, parts.value
 
 
 def packed_tree_attention(q: torch.Tensor, kv: PackedKV, scale: float, parents: torch.Tensor, *,
@@ -626,8 +624,8 @@ def packed_tree_attention(q: torch.Tensor, kv: PackedKV, scale: float, parents: 
     out = torch.empty(B, Hq, T, D, dtype=out_dtype, device=q.device)
     if B == 0:
         return out
-    ns = int(num_splits) if num_splits else tree_plan_for(q, kv, exact)
-    need = tree_workspace_bytes(B, Hq, Hkv, T, D, exact, ns)
+    ns, span, parts = (int(num_splits), 64, B * int(num_splits)) if num_splits else tree_plan_for(q, kv, exact, read_lens=check_ranges)
+    need = tree_workspace_bytes(B, Hq, Hkv, T, D, ns)
     if need < 0:
         raise UnsupportedLayout(f"bad tree sizes B={B} Hq={Hq} Hkv={Hkv} T={T} splits={ns}")
     if workspace is None:
@@ -640,7 +638,7 @@ def packed_tree_attention(q: torch.Tensor, kv: PackedKV, scale: float, parents: 
                   *_operands(q, kv)[4:], _lib.ptr(parents), parents.stride(0), _lib.ptr(out),
                   _lib.DTYPE_CODE[out_dtype], _lib.ptr(workspace), workspace.numel() * workspace.element_size(),
                   B, Hq, Hkv, T, D, kv.page_size, kv.k_quant.bit_width, kv.v_quant.bit_width, kv.k_pages.shape[0],
-                  kv.page_table.shape[1], float(scale), int(exact), ns, _lib.stream_of(q.device), ev0, ev1)
+                  kv.page_table.shape[1], float(scale), int(exact), ns, span, parts, _lib.stream_of(q.device), ev0, ev1)
     return out
 
 
