@@ -445,6 +445,14 @@ int wn_tree_attention(
     int B, int Hq, int Hkv, int T, int D, int S, int bw_k, int bw_v, int num_pages, int max_pages,
     float scale, int exact, int num_splits, int span, int parts, void* stream, void* ev_begin, void* ev_end);
 
+/* Host checks of host memory, no launch: 1 if every sequence's positions lie in its page table row
+ * and on pages 0 .. num_pages - 1, else 0. lengths != 0: positions 0 .. start[b] - 1 (n unused), else
+ * start[b] .. start[b] + n - 1. */
+int wn_positions_in_range(const int32_t* start, int lengths, int n, const int32_t* page_table, int64_t table_stride_b,
+                          int B, int max_pages, int num_pages, int S);
+/* 1 if every parents[b, i] is -1 or in 0 .. i - 1, else 0. Host memory. */
+int wn_parents_in_order(const int32_t* parents, int64_t parents_stride_b, int B, int T);
+
 /* Keeps the accepted branch of a tree: for i < counts[b] (clipped to [0, A]) the row of node
  * path[b, i], position start_pos[b] + path[b, i], moves to position start_pos[b] + i, in every
  * layer and kv head, K and V, and lengths[b] = start_pos[b] + counts[b]. Every source is read

@@ -224,3 +224,43 @@ def test_engine_refuses_too_many_alternatives():
         with pytest.raises(Refused, match="bad_top_logprobs"):
             e.submit(Request("r", [1], 2, top_logprobs=n))
     assert e.submit(Request("r", [1], 2, top_logprobs=0)).logprobs == []
+
+
+def test_the_native_range_checks_agree_with_the_plain_ones(monkeypatch):
+    """Positions of lengths and of appended tokens, and parents: random small metadata, some of it
+    out of range, strided tables, other types; the message names what the plain check finds."""
+    import random
+
+    from winnow_amd import packed_attention as pa
+    from winnow_amd import packed_backend as pb
+    _lib.lib()
+    r = random.Random(5)
+
+    def said(check, *args):
+        try:
+            return check(*args)
+        except pa.UnsupportedLayout as e:
+            return str(e)
+
+    refused = 0
+    for k in range(600):
+        B, W, S, P = r.randint(0, 5), r.choice([1, 2, 7]), r.choice([1, 16, 12]), r.choice([1, 5])
+        odd = [-1, P, 2 ** 31 - 1, -2 ** 31]
+        ids = [[r.choice(odd) if r.random() < 0.03 else r.randrange(P) for _ in range(W + 2)] for _ in range(B)]
+        table = torch.tensor(ids, dtype=torch.int32).reshape(B, W + 2)[:, 1:1 + W]
+        start = torch.tensor([r.choice([0, W * S, W * S + 1, -1, 2 ** 31 - 1]) if r.random() < 0.2 else r.randint(0, W * S)
+                              for _ in range(B)], dtype=torch.int32)
+        n = r.choice([0, 1, 2, S, 2 ** 31 - 1])
+        parents = torch.tensor([[r.choice([-2, i, i + 1, 2 ** 31 - 1]) if r.random() < 0.03 else r.randint(-1, i - 1)
+                                 for i in range(W)] for _ in range(B)], dtype=torch.int32).reshape(B, W)
+        if k % 3 == 0:
+            table, start = table.long(), start.long()  # not the mirrors' type: the plain checks look
+        calls = [(pa.check_page_ranges, start, table, P, S), (pb._positions_in_range, start, table, n, P, S),
+                 (pa.check_parents, parents)]
+        got = [said(*c) for c in calls]
+        with monkeypatch.context() as m:
+            m.setattr(_lib, "positions_in_range", lambda *a: False)
+            m.setattr(_lib, "parents_in_order", lambda *a: False)
+            assert got == [said(*c) for c in calls], (start, table, n, P, S, parents)
+        refused += sum(x is not None for x in got)
+    assert 300 < refused < 1500

@@ -6,6 +6,7 @@ to host code. Build it with ``python -m winnow_amd.build``.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import threading
 from pathlib import Path
@@ -167,6 +168,8 @@ SIGNATURES = {
         _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i,   # B Hq Hkv T D S bwk bwv num_pages max_pages
         _c_f, _c_i, _c_i, _c_i, _c_i,               # scale, exact, num_splits, span, parts
         _c_p, _c_p, _c_p]),                         # stream, ev_begin, ev_end
+    "wn_positions_in_range": (_c_i, [_c_p, _c_i, _c_i, _c_p, _c_i64, _c_i, _c_i, _c_i, _c_i]),
+    "wn_parents_in_order": (_c_i, [_c_p, _c_i64, _c_i, _c_i]),
     "wn_commit_kv": (_c_i, [
         _c_p, _c_i64, _c_i64, _c_i64, _c_i,         # k pages, strides (layer, page, head), row bytes
         _c_p, _c_i64, _c_i64, _c_i64, _c_i,         # v pages
@@ -278,6 +281,37 @@ def ptr(t: torch.Tensor | None):
     """A tensor's device address for a ``void*`` argument (a plain integer: ctypes
     converts it faster than a c_void_p object built in Python)."""
     return None if t is None else t.data_ptr()
+
+
+_here = contextlib.nullcontext()
+
+
+def on(device: torch.device):
+    """``torch.cuda.device(device)``, or nothing where that is the current one already."""
+    return _here if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _host_int32(t: torch.Tensor) -> bool:
+    return t.dtype is torch.int32 and t.device.type == "cpu" and (t.shape[-1] <= 1 or t.stride(-1) == 1)
+
+
+def positions_in_range(start: torch.Tensor, table: torch.Tensor, n: int | None, num_pages: int, page_size: int) -> bool:
+    """Whether the loaded library finds positions start[b] .. start[b] + n - 1 (n None: 0 .. start[b] - 1)
+    inside row b of the table and on pages of the pool (``wn_positions_in_range``, int32 host tensors).
+    False also where it cannot say: the caller then looks for itself, and names the sequence."""
+    if _lib is None or table.dim() != 2 or start.shape != table.shape[:1] or not (_host_int32(start) and _host_int32(table)):
+        return False
+    B, width = table.shape
+    return bool(_lib.wn_positions_in_range(start.data_ptr(), n is None, n or 0, table.data_ptr(), table.stride(0),
+                                           B, width, num_pages, page_size))
+
+
+def parents_in_order(parents: torch.Tensor) -> bool:
+    """Whether the loaded library finds every parent -1 or an earlier node (``wn_parents_in_order``)."""
+    if _lib is None or parents.dim() != 2 or not _host_int32(parents):
+        return False
+    B, T = parents.shape
+    return bool(_lib.wn_parents_in_order(parents.data_ptr(), parents.stride(0), B, T))
 
 
 def stream_of(device: torch.device):

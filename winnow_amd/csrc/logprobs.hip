@@ -10,14 +10,18 @@
 //
 // Bound: HBM, one read of the logits. A work-group of four waves takes a row, or a segment
 // of it where there are few rows (a second launch then joins the segments): each lane keeps
-// its own running (m, l, t), rescaled once per 16-byte piece.
+// its own running (m, l, t), rescaled once per batch of four 16-byte pieces, while the next
+// batch travels.
 //
 // The alternatives of a wave are a sorted list across its lanes (lane i: the i-th best),
 // as 64-bit keys (value in the order of unsigned numbers, then ~index), so that one
 // comparison orders equal logits too and the result does not depend on who came first. A
-// piece whose largest logit cannot beat the list's last is skipped with one comparison per
-// lane; the waves of a work-group share the best of their last keys, each of which is a
-// lower bound of the row's.
+// batch whose largest logit cannot beat the list's bound is skipped with one comparison per
+// lane; of a piece that can, only the lanes that do are looked at. What keeps those few:
+//   - where many lanes of a piece have a hit (the first piece, rising logits), the bound goes up
+//     to the top-th largest of the lanes' best before any is inserted;
+//   - the waves publish their ceil(top / 4)-th best: the least of the four is no larger than
+//     the row's top-th, and far nearer to it than any wave's own top-th.
 #include <algorithm>
 
 #include "wn_common.h"
@@ -61,22 +65,33 @@ __device__ __forceinline__ uint64_t lp_read(uint64_t v, int lane) {
          uint32_t(__builtin_amdgcn_readlane(int(uint32_t(v)), lane));
 }
 
+// x of the lane before (lane 0 keeps its own).
+__device__ __forceinline__ uint32_t lp_before(uint32_t x) {
+  return uint32_t(__builtin_amdgcn_update_dpp(int(x), int(x), 0x138, 0xf, 0xf, false));  // wave_shr:1
+}
+
 // The best keys a wave has met: lane i holds the i-th best (0: none yet).
 struct LpList {
-  uint64_t mine = 0, last = 0;  // last: the least key worth taking is above this (wave-uniform)
+  uint64_t mine = 0, last = 0;  // last: a key must be above this to be worth taking (wave-uniform)
   int top;
   // takes every lane's key that belongs in the list
   __device__ __forceinline__ void offer(uint64_t key, int lane) {
     uint64_t hit = __ballot(key > last);
     while (hit) {
       const uint64_t k = lp_read(key, __builtin_ctzll(hit));
-      hit &= hit - 1;
-      if (k <= last) continue;  // wave-uniform: the list has moved on
       const int pos = __popcll(__ballot(mine > k));
-      const uint64_t up = __shfl_up(mine, 1, 64);
+      const uint64_t up = uint64_t(lp_before(uint32_t(mine >> 32))) << 32 | lp_before(uint32_t(mine));
       mine = lane < pos ? mine : lane == pos ? k : up;
       last = max(last, lp_read(mine, top - 1));
+      hit &= __ballot(key > last) & ~(hit & -hit);
     }
+  }
+  // raises the bound to just below the top-th largest of the hit lanes' keys (each of some element)
+  __device__ __forceinline__ void tighten(uint64_t key, uint64_t hit) {
+    int above = 0;
+    for (uint64_t h = hit; h; h &= h - 1) above += lp_read(key, __builtin_ctzll(h)) > key;
+    const uint64_t at = __ballot(above == top - 1) & hit;
+    if (at) last = max(last, lp_read(key, __builtin_ctzll(at)) - 1);
   }
 };
 
@@ -112,12 +127,9 @@ __device__ __forceinline__ float lp_elem(uint32_t w, int half) {
   else return f16_to_f32(uint16_t(half ? w >> 16 : w));
 }
 
-// N values (those of x at index i0 ..) into a lane's sums and the wave's list.
+// N values into a lane's sums; their maximum `top`.
 template <int N>
-__device__ __forceinline__ void lp_take(const float (&x)[N], uint32_t i0, int n, LpSum& s, LpList& list, int lane) {
-  float top = -INFINITY;
-#pragma unroll
-  for (int j = 0; j < N; ++j) top = fmaxf(top, x[j]);  // what lies past n is -inf
+__device__ __forceinline__ void lp_add(const float (&x)[N], float top, LpSum& s) {
   const float mn = fmaxf(s.m, top);
   const float mz = mn == -INFINITY ? 0.f : mn;
   const float d0 = s.m == -INFINITY ? 0.f : s.m - mz;
@@ -130,12 +142,6 @@ __device__ __forceinline__ void lp_take(const float (&x)[N], uint32_t i0, int n,
     const float d = x[j] - mz, p = __builtin_amdgcn_exp2f(d * kLog2e);
     s.l += p;
     s.t = fmaf(p, fmaxf(d, -1000.f), s.t);  // e^-1000 is 0: -inf and overflows add nothing
-  }
-  if (list.top) {
-    if (__any(n > 0 && lp_key(top, i0) > list.last)) {  // no element of the piece has a better key
-#pragma unroll
-      for (int j = 0; j < N; ++j) list.offer(j < n ? lp_key(x[j], i0 + j) : 0, lane);
-    }
   }
 }
 
@@ -169,12 +175,12 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LpArgs a) {
   constexpr int VEC = LpType<DT>::VEC;
   __shared__ uint64_t lists[kLpWaves * kTopMost];
   __shared__ float sums[kLpWaves * 3];
-  __shared__ uint64_t floor_key;  // the largest `last` of the work-group's waves
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ __align__(16) uint64_t shared_best[kLpWaves];  // of each wave, its ceil(top / 4)-th best
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t row = blockIdx.x / a.nseg;
   const int seg = int(blockIdx.x % a.nseg);
   const T* x = static_cast<const T*>(a.x) + (row / a.inner) * a.outer_stride + (row % a.inner) * a.row_stride;
-  if (tid == 0) floor_key = 0;
+  if (tid < kLpWaves) shared_best[tid] = 0;
   __syncthreads();
 
   // segments are cut where the row's memory is 16-byte aligned: element head + k seg
@@ -187,14 +193,18 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LpArgs a) {
   LpSum s;
   LpList list;
   list.top = a.top;
+  const int quarter = (a.top + kLpWaves - 1) / kLpWaves - 1;
+  uint64_t told = 0;
   auto share = [&]() {
-    if (!a.top) return;
-    const uint64_t f = lp_read(__hip_atomic_load(&floor_key, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP), 0);
-    if (f < list.last) {
-      if (lane == 0) atomicMax(reinterpret_cast<unsigned long long*>(&floor_key), (unsigned long long)list.last);
-    } else {
-      list.last = f;
-    }
+    const uint64_t own = lp_read(list.mine, max(quarter, 0));
+    if (own != told && lane == 0)
+      __hip_atomic_store(&shared_best[wave], own, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    told = own;
+    uint64_t least = own;
+#pragma unroll
+    for (int w = 0; w < kLpWaves; ++w)
+      least = min(least, __hip_atomic_load(&shared_best[w], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
+    list.last = max(list.last, lp_read(least, 0));
   };
   // the ends, at most 2 VEC - 2 elements: one per lane of wave 0
   if (wave == 0) {
@@ -206,24 +216,91 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LpArgs a) {
       if constexpr (DT == WN_F32) v[0] = x[i];
       else v[0] = lp_elem<DT>(x[i], 0);
     }
-    lp_take<1>(v, uint32_t(i), live ? 1 : 0, s, list, lane);
+    lp_add<1>(v, v[0], s);
+    if (a.top) list.offer(live ? lp_key(v[0], uint32_t(i)) : 0, lane);
   }
-  constexpr int STEP = 64 * VEC;  // a wave's piece of the row
-  for (int p = body + wave * STEP; p < whole; p += kLpWaves * STEP) {
-    const int i = p + lane * VEC;
-    float v[VEC];
-    const bool live = i < whole;
-    if (live) {
-      const uint4 w = *reinterpret_cast<const uint4*>(x + i);
-      const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+  // batches of U pieces a wave; piece u of the batch at p starts at p + u kLpWaves STEP
+  constexpr int STEP = 64 * VEC, U = 4, BATCH = U * kLpWaves * STEP;
+  uint4 w[U];
+  // unsigned: a position past the end may pass 2^31
+  const uint32_t end = uint32_t(whole);
+  auto load = [&](uint32_t p) {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) v[j] = DT == WN_F32 ? lp_elem<DT>(ws[j], 0) : lp_elem<DT>(ws[j / 2], j & 1);
+    for (int u = 0; u < U; ++u) {
+      const uint32_t i = p + u * kLpWaves * STEP + lane * VEC;
+      if (i < end) w[u] = *reinterpret_cast<const uint4*>(x + i);
+    }
+  };
+  auto values = [&](const uint4& q, float (&v)[VEC]) {
+    const uint32_t ws[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[j] = DT == WN_F32 ? lp_elem<DT>(ws[j], 0) : lp_elem<DT>(ws[j / 2], j & 1);
+  };
+  // the hits of a piece at i0 (of lane 0), top: each lane's largest value in it
+  auto collect = [&](const uint4& q, float top, uint32_t i0) {
+    const uint32_t i = i0 + lane * VEC;
+    const bool live = i < end;
+    // no element of the lane has a key above the first's index with the largest value
+    uint64_t hit = __ballot(live && lp_key(top, i) > list.last);
+    if (__popcll(hit) > max(a.top, 8)) {
+      list.tighten(live ? lp_key(top, i + VEC - 1) : 0, hit);
+      hit = __ballot(live && lp_key(top, i) > list.last);
+    }
+    while (hit) {
+      const int from = __builtin_ctzll(hit);
+      const uint32_t ws[4] = {uint32_t(__builtin_amdgcn_readlane(int(q.x), from)), uint32_t(__builtin_amdgcn_readlane(int(q.y), from)),
+                              uint32_t(__builtin_amdgcn_readlane(int(q.z), from)), uint32_t(__builtin_amdgcn_readlane(int(q.w), from))};
+      const int word = lane / (VEC / 4);  // lane j: element j of the piece
+      const uint32_t mine = word == 0 ? ws[0] : word == 1 ? ws[1] : word == 2 ? ws[2] : ws[3];
+      list.offer(lane < VEC ? lp_key(lp_elem<DT>(mine, lane & 1), i0 + from * VEC + lane) : 0, lane);
+      hit &= __ballot(live && lp_key(top, i) > list.last) & ~(hit & -hit);
+    }
+  };
+  uint32_t p = uint32_t(body + wave * STEP);
+  if (p < end) load(p);
+  for (; p < end; p += BATCH) {
+    uint4 q[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) q[u] = w[u];
+    load(p + BATCH);
+    float tops[U];
+    if (p + (U - 1) * kLpWaves * STEP + STEP <= end) {  // every piece is whole
+      float v[U][VEC], all[U * VEC], top = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        values(q[u], v[u]);
+        tops[u] = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          tops[u] = fmaxf(tops[u], v[u][j]);
+          all[u * VEC + j] = v[u][j];
+        }
+        top = fmaxf(top, tops[u]);
+      }
+      lp_add<U * VEC>(all, top, s);
+      if (!a.top) continue;
+      if (__any(lp_key(top, p + lane * VEC) > list.last)) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) collect(q[u], tops[u], p + u * kLpWaves * STEP);
+      }
     } else {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) v[j] = -INFINITY;
+      for (int u = 0; u < U; ++u) {
+        const uint32_t i0 = p + u * kLpWaves * STEP;
+        if (i0 >= end) break;
+        float v[VEC], top = -INFINITY;
+        values(q[u], v);
+        const bool live = i0 + lane * VEC < end;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          v[j] = live ? v[j] : -INFINITY;
+          top = fmaxf(top, v[j]);
+        }
+        lp_add<VEC>(v, top, s);
+        if (a.top) collect(q[u], top, i0);
+      }
     }
-    lp_take<VEC>(v, uint32_t(i), live ? VEC : 0, s, list, lane);
-    share();
+    if (a.top) share();
   }
 
   // the lanes' sums, then the waves'
@@ -252,13 +329,20 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LpArgs a) {
   if (lane < a.top) a.keys[part * a.top + lane] = list.mine;
 }
 
-// Joins the segments of a row: one wave per row.
+// Joins the segments of a row: one wave per row, its keys by 64, each 64 narrowed to those that
+// can be among the best before any is inserted.
 template <int DT>
 __global__ __launch_bounds__(64) void logprobs_join_kernel(LpArgs a) {
   using T = typename LpType<DT>::T;
   const int lane = threadIdx.x;
   const int64_t row = blockIdx.x;
   const T* x = static_cast<const T*>(a.x) + (row / a.inner) * a.outer_stride + (row % a.inner) * a.row_stride;
+  const int n = a.nseg * a.top;
+  const uint64_t* keys = a.keys + row * n;
+  constexpr int U = 6;
+  uint64_t key[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) key[u] = 64 * u + lane < n ? keys[64 * u + lane] : 0;
   const float given = lane == 0 ? lp_given<DT>(a, row, x) : 0.f;
   LpSum s;
   for (int g = lane; g < a.nseg; g += 64) {
@@ -269,16 +353,37 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(LpArgs a) {
   for (int o = 32; o > 0; o >>= 1) s.join(__shfl_xor(s.m, o, 64), __shfl_xor(s.l, o, 64), __shfl_xor(s.t, o, 64));
   LpList list;
   list.top = a.top;
-  const int n = a.nseg * a.top;
-  for (int i0 = 0; i0 < n; i0 += 64) list.offer(i0 + lane < n ? a.keys[row * n + i0 + lane] : 0, lane);
+  for (int i0 = 0; i0 < n; i0 += 64 * U) {
+    uint64_t best = key[0];
+#pragma unroll
+    for (int u = 1; u < U; ++u) best = max(best, key[u]);
+    const uint64_t hit = __ballot(best > list.last);
+    if (__popcll(hit) > a.top) list.tighten(best, hit);
+#pragma unroll
+    for (int u = 0; u < U; ++u) list.offer(key[u], lane);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + 64 * (U + u) + lane;
+      key[u] = i < n ? keys[i] : 0;
+    }
+  }
   lp_finish(a, row, s, list.mine, lane, given);
 }
 
-// Segments of a row: one for as many rows as fill the device with a few work-groups per
-// CU, else as many as that takes, of 2,048 elements at least.
+// Segments of a row, of 2,048 elements at least: the count that takes the least time for 1,024
+// work-groups at a time (four per CU), a work-group taking the time of its elements and 2,000
+// more, the second launch that of 10,000 (5 us).
 int lp_segments(int64_t N, int V) {
-  const int64_t want = (1024 + N - 1) / std::max<int64_t>(N, 1);
-  return int(std::max<int64_t>(1, std::min<int64_t>(want, (int64_t(V) + 2047) / 2048)));
+  const int64_t most = std::min<int64_t>(1024, (int64_t(V) + 2047) / 2048);
+  int64_t best = 1, least = INT64_MAX;
+  for (int64_t n = 1; n <= most; ++n) {
+    const int64_t cost = (N * n + 1023) / 1024 * ((V + n - 1) / n + 2000) + (n > 1 ? 10000 : 0);
+    if (cost < least) {
+      best = n;
+      least = cost;
+    }
+  }
+  return int(best);
 }
 
 int64_t align256(int64_t x) { return (x + 255) & ~int64_t(255); }

@@ -64,7 +64,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
     outer, inner, n_inner = (st[0], st[1], rows[1]) if len(rows) == 2 else (0, st[0] if rows else 0, N)
     need = int(_lib.lib().wn_token_logprobs_workspace_bytes(N, V, top))
     workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    with torch.cuda.device(dev):
+    with _lib.on(dev):
         _lib.call("wn_token_logprobs", _lib.ptr(logits), _lib.DTYPE_CODE[logits.dtype], outer, inner, n_inner,
                   _lib.ptr(tokens), _lib.ptr(logprob), _lib.ptr(entropy), _lib.ptr(top_lp), _lib.ptr(top_id), N, V, top,
                   _lib.ptr(workspace), need, _lib.stream_of(dev))

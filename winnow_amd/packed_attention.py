@@ -204,11 +204,11 @@ def check_contract(q: torch.Tensor, kv: PackedKV, *, check_ranges: bool = True) 
         raise UnsupportedLayout("seq_lens must be (B,)")
     if kv.page_table.dtype != torch.int32 or kv.seq_lens.dtype != torch.int32:
         raise UnsupportedLayout("page_table and seq_lens must be int32")
-    devices = {t.device for t in (q, kv.k_pages, kv.v_pages, kv.k_norms, kv.v_norms,
-                                  kv.page_table, kv.seq_lens, kv.k_quant.Pi, kv.v_quant.Pi,
-                                  kv.k_quant.centroids, kv.v_quant.centroids)}
-    if len(devices) != 1:
-        raise UnsupportedLayout(f"all operands must share a device, got {devices}")
+    dev = q.device
+    operands = (kv.k_pages, kv.v_pages, kv.k_norms, kv.v_norms, kv.page_table, kv.seq_lens, kv.k_quant.Pi, kv.v_quant.Pi,
+                kv.k_quant.centroids, kv.v_quant.centroids)
+    if any(t.device != dev for t in operands):
+        raise UnsupportedLayout(f"all operands must share a device, got { {dev, *(t.device for t in operands)} }")
     if not check_ranges:
         return
     lens = kv.seq_lens_host if kv.seq_lens_host is not None else kv.seq_lens
@@ -222,7 +222,9 @@ def check_page_ranges(seq_lens: torch.Tensor, page_table: torch.Tensor, num_page
     cdiv(len, page_size)) lies in [0, num_pages): the scan kernels index pages with
     these ids unchecked. Copies the two small tensors to the host (host mirrors are
     read in place); the checks run in numpy, whose small-array operations cost far
-    less host time than torch's."""
+    less host time than torch's, and natively for int32 mirrors."""
+    if _lib.positions_in_range(seq_lens, page_table, None, num_pages, page_size):
+        return
     lens = seq_lens.detach().to("cpu").numpy().astype(np.int64)
     table = page_table.detach().to("cpu").numpy()
     width = table.shape[1]
@@ -524,9 +526,10 @@ def check_tree(q: torch.Tensor, kv: PackedKV, parents: torch.Tensor) -> None:
     if q.requires_grad and torch.is_grad_enabled():
         raise UnsupportedLayout("tree attention has no gradient: call it under torch.no_grad() or detach q")
     for pages, norms in ((kv.k_pages, kv.k_norms), (kv.v_pages, kv.v_norms)):
-        if pages.stride(-1) != 1 or pages.stride(-2) != pages.shape[-1]:
+        st = pages.stride()
+        if st[3] != 1 or st[2] != pages.shape[3]:
             raise UnsupportedLayout("pages need contiguous (S, NB) rows")
-        if pages.data_ptr() % 4 or pages.stride(0) % 4 or pages.stride(1) % 4:
+        if pages.data_ptr() % 4 or st[0] % 4 or st[1] % 4:
             raise UnsupportedLayout("page base and strides must be 4-byte aligned")
         if norms.stride(-1) != 1:
             raise UnsupportedLayout("norms need a contiguous slot axis")
@@ -535,9 +538,10 @@ def check_tree(q: torch.Tensor, kv: PackedKV, parents: torch.Tensor) -> None:
             raise UnsupportedLayout("rotations (16-byte aligned) and codebooks must be contiguous")
     if kv.page_table.stride(-1) != 1 or not kv.seq_lens.is_contiguous():
         raise UnsupportedLayout("page_table rows and seq_lens must be contiguous")
-    if kv.page_table.shape[1] < 1 or kv.page_table.shape[1] * kv.page_size > 2 ** 31 - 257:
+    P, _, S, _ = kv.k_pages.shape
+    if not 1 <= kv.page_table.shape[1] <= (2 ** 31 - 257) // S:
         raise UnsupportedLayout("page_table must hold 1 to 2^31 - 257 positions per sequence")
-    if kv.k_pages.shape[0] < 1:
+    if P < 1:
         raise UnsupportedLayout("the pool has no pages")
     if parents.shape != (B, T) or parents.dtype != torch.int32 or parents.device != q.device \
             or (T > 1 and parents.stride(1) != 1):
@@ -546,6 +550,8 @@ def check_tree(q: torch.Tensor, kv: PackedKV, parents: torch.Tensor) -> None:
 
 def check_parents(parents: torch.Tensor) -> None:
     """Every node's parent comes before it, or is -1. Reads a host copy."""
+    if _lib.parents_in_order(parents):
+        return
     p = parents.detach().to("cpu").numpy()
     bad = (p < -1) | (p >= np.arange(p.shape[1])[None, :])
     if bad.any():
@@ -576,7 +582,7 @@ def tree_plan_for(q: torch.Tensor, kv: PackedKV, exact: bool, *, read_lens: bool
     if lens is not None and (lens.dtype != torch.int32 or lens.shape != (B,) or not lens.is_contiguous()):
         lens = lens.to(torch.int32).reshape(B).contiguous()
     ns, span, parts = ctypes.c_int(0), ctypes.c_int(0), ctypes.c_int(0)
-    with torch.cuda.device(q.device):
+    with _lib.on(q.device):
         _lib.call("wn_tree_plan", B, Hq, kv.num_kv_heads, T, D, kv.page_size, kv.k_quant.bit_width, kv.v_quant.bit_width,
                   int(exact), kv.page_table.shape[1], _lib.ptr(lens), ctypes.byref(ns), ctypes.byref(span),
                   ctypes.byref(parts))
@@ -633,12 +639,17 @@ def packed_tree_attention(q: torch.Tensor, kv: PackedKV, scale: float, parents: 
     elif workspace.numel() * workspace.element_size() < need or workspace.device != q.device:
         raise UnsupportedLayout(f"workspace needs {need} bytes on {q.device}")
     ev0, ev1 = timing_events or (None, None)
-    with torch.cuda.device(q.device):
-        _lib.call("wn_tree_attention", _lib.ptr(q), _lib.DTYPE_CODE[q.dtype], q.stride(0), q.stride(1), q.stride(2),
-                  *_operands(q, kv)[4:], _lib.ptr(parents), parents.stride(0), _lib.ptr(out),
-                  _lib.DTYPE_CODE[out_dtype], _lib.ptr(workspace), workspace.numel() * workspace.element_size(),
-                  B, Hq, Hkv, T, D, kv.page_size, kv.k_quant.bit_width, kv.v_quant.bit_width, kv.k_pages.shape[0],
-                  kv.page_table.shape[1], float(scale), int(exact), ns, span, parts, _lib.stream_of(q.device), ev0, ev1)
+    kq, vq, table = kv.k_quant, kv.v_quant, kv.page_table
+    kp, vp, kn, vn = kv.k_pages.stride(), kv.v_pages.stride(), kv.k_norms.stride(), kv.v_norms.stride()
+    with _lib.on(q.device):
+        _lib.call("wn_tree_attention", q.data_ptr(), _lib.DTYPE_CODE[q.dtype], *q.stride()[:3],
+                  kq.Pi.data_ptr(), vq.Pi.data_ptr(), kq.centroids.data_ptr(), vq.centroids.data_ptr(),
+                  kv.k_pages.data_ptr(), kp[0], kp[1], kv.v_pages.data_ptr(), vp[0], vp[1],
+                  kv.k_norms.data_ptr(), kn[0], kn[1], kv.v_norms.data_ptr(), vn[0], vn[1],
+                  table.data_ptr(), table.stride(0), kv.seq_lens.data_ptr(), parents.data_ptr(), parents.stride(0),
+                  out.data_ptr(), _lib.DTYPE_CODE[out_dtype], workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+                  B, Hq, Hkv, T, D, kv.page_size, kq.bit_width, vq.bit_width, kv.k_pages.shape[0],
+                  table.shape[1], float(scale), int(exact), ns, span, parts, _lib.stream_of(q.device), ev0, ev1)
     return out
 
 

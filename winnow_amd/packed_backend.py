@@ -108,7 +108,9 @@ def _positions_in_range(start: torch.Tensor, table: torch.Tensor, n: int, num_pa
                         page_size: int) -> None:
     """Every position start[b] + i (i < n) lies inside row b of the table and names a
     page in [0, num_pages). Reads host tensors only (in numpy: small-array operations
-    cost far less host time there than in torch)."""
+    cost far less host time there than in torch; int32 mirrors natively)."""
+    if _lib.positions_in_range(start, table, n, num_pages, page_size):
+        return
     start = start.detach().numpy().astype(np.int64)
     width = table.shape[1]
     if n == 0 or start.size == 0:
@@ -284,17 +286,22 @@ def append_kv(k: torch.Tensor, v: torch.Tensor | None, k_tq, v_tq,
 
 
 def _check_commit_side(name: str, pages: torch.Tensor, norms, lead) -> None:
-    if pages.dim() not in (4, 5) or pages.shape[:-1] != lead:
-        raise pa.UnsupportedLayout(f"commit: {name} pages must be ([layers,] P, Hkv, S, row), got {tuple(pages.shape)}")
+    shape, st = pages.shape, pages.stride()
+    if len(shape) not in (4, 5) or shape[:-1] != lead:
+        raise pa.UnsupportedLayout(f"commit: {name} pages must be ([layers,] P, Hkv, S, row), got {tuple(shape)}")
     if pages.dtype not in (torch.uint8, *pa.DENSE_PAGE_DTYPES) or (pages.dtype == torch.uint8) != (norms is not None):
         raise pa.UnsupportedLayout(f"commit: {name} pages are uint8 with norms, or fp32/fp16/bf16 without")
-    if pages.stride(-1) != 1 or pages.stride(-2) != pages.shape[-1]:
+    if st[-1] != 1 or st[-2] != shape[-1]:
         raise pa.UnsupportedLayout("commit: pages need contiguous (S, row) blocks")
-    if norms is not None and (norms.dtype != torch.float16 or norms.shape != lead or norms.stride(-1) != 1):
-        raise pa.UnsupportedLayout(f"commit: {name} norms must be fp16 of the pages' leading shape, slots contiguous")
-    for t in (pages, norms):
-        if t is not None and any(n > 1 and st == 0 for n, st in zip(t.shape[:-1], t.stride())):
-            raise pa.UnsupportedLayout(f"commit: {name} is written in place and may not be expanded")
+    nst = (1,)
+    if norms is not None:
+        nst = norms.stride()
+        if norms.dtype != torch.float16 or norms.shape != lead or nst[-1] != 1:
+            raise pa.UnsupportedLayout(f"commit: {name} norms must be fp16 of the pages' leading shape, slots contiguous")
+    if 0 in st or 0 in nst:  # an axis of one entry may have any stride
+        for t in (pages, norms):
+            if t is not None and any(n > 1 and s == 0 for n, s in zip(t.shape[:-1], t.stride())):
+                raise pa.UnsupportedLayout(f"commit: {name} is written in place and may not be expanded")
 
 
 @torch.no_grad()
@@ -324,8 +331,9 @@ def commit_kv(k_pages: torch.Tensor, v_pages: torch.Tensor, k_norms: torch.Tenso
         _check_commit_side(name, pages, norms, lead)
     if v_pages.dtype != k_pages.dtype:
         raise pa.UnsupportedLayout(f"commit: K pages are {k_pages.dtype}, V pages {v_pages.dtype}")
-    ops = [k_pages, v_pages, page_table, start_pos, path, counts] + ([k_norms, v_norms] if packed else [])
-    if not all(_lib.is_hip(t) for t in ops) or len({t.device for t in ops}) != 1:
+    dev = k_pages.device
+    if not _lib.is_hip(k_pages) or v_pages.device != dev or page_table.device != dev or start_pos.device != dev \
+            or path.device != dev or counts.device != dev or (packed and (k_norms.device != dev or v_norms.device != dev)):
         raise pa.UnsupportedLayout("commit: every operand must be on one HIP device")
     layers = 1 if k_pages.dim() == 4 else k_pages.shape[0]
     P, Hkv, S = lead[-3:]
@@ -346,13 +354,12 @@ def commit_kv(k_pages: torch.Tensor, v_pages: torch.Tensor, k_norms: torch.Tenso
     if check_ranges:
         _positions_in_range(start_pos_host if start_pos_host is not None else start_pos.cpu(),
                             page_table_host if page_table_host is not None else page_table.cpu(), nodes, P, S)
-    lengths = torch.empty(B, dtype=torch.int32, device=k_pages.device)
-
-    with torch.cuda.device(k_pages.device):
+    lengths = torch.empty(B, dtype=torch.int32, device=dev)
+    with _lib.on(dev):
         _lib.call("wn_commit_kv", *_commit_pages(k_pages), *_commit_pages(v_pages), *_commit_norms(k_norms),
                   *_commit_norms(v_norms), _lib.ptr(page_table), page_table.stride(0), _lib.ptr(start_pos),
                   _lib.ptr(path), path.stride(0), _lib.ptr(counts), _lib.ptr(lengths), layers, B, Hkv, S, A, nodes, P,
-                  width, _lib.stream_of(k_pages.device))
+                  width, _lib.stream_of(dev))
     return lengths
 
 
