@@ -17,11 +17,13 @@
 // as 64-bit keys (value in the order of unsigned numbers, then ~index), so that one
 // comparison orders equal logits too and the result does not depend on who came first. A
 // batch whose largest logit cannot beat the list's bound is skipped with one comparison per
-// lane; of a piece that can, only the lanes that do are looked at. What keeps those few:
-//   - where many lanes of a piece have a hit (the first piece, rising logits), the bound goes up
-//     to the top-th largest of the lanes' best before any is inserted;
-//   - the waves publish their ceil(top / 4)-th best: the least of the four is no larger than
-//     the row's top-th, and far nearer to it than any wave's own top-th.
+// lane; of a piece that can, only the lanes that do are looked at. An insertion costs 36
+// instructions, so what counts is how few there are, and the bound is what keeps them few:
+//   - it starts from the first batch: a wave's ceil(top / 4)-th largest of its lanes' maxima, the
+//     least of the four waves' (at least `top` logits are no smaller);
+//   - later the waves publish their ceil(top / 4)-th best: again the least of the four;
+//   - where many lanes of a batch have a hit all the same (rising logits) it goes up to the
+//     top-th largest of the lanes' maxima before any is inserted.
 #include <algorithm>
 
 #include "wn_common.h"
@@ -86,14 +88,45 @@ struct LpList {
       hit &= __ballot(key > last) & ~(hit & -hit);
     }
   }
-  // raises the bound to just below the top-th largest of the hit lanes' keys (each of some element)
-  __device__ __forceinline__ void tighten(uint64_t key, uint64_t hit) {
-    int above = 0;
-    for (uint64_t h = hit; h; h &= h - 1) above += lp_read(key, __builtin_ctzll(h)) > key;
-    const uint64_t at = __ballot(above == top - 1) & hit;
-    if (at) last = max(last, lp_read(key, __builtin_ctzll(at)) - 1);
-  }
+  // at least `top` keys are known to be `bound` or above (0: nothing is known)
+  __device__ __forceinline__ void raise(uint64_t bound) { last = bound ? max(last, bound - 1) : last; }
 };
+
+// The largest b, its low 44 bits 0, such that `rank` lanes have keys of b or above (0: fewer have any).
+__device__ __forceinline__ uint64_t lp_bound(uint64_t key, int rank) {
+  const uint32_t k = uint32_t(key >> 32);
+  uint32_t b = 0;
+#pragma unroll
+  for (uint32_t bit = 1u << 31; bit >= 1u << 12; bit >>= 1) b = __popcll(__ballot(k >= (b | bit))) >= rank ? b | bit : b;
+  return uint64_t(b) << 32;
+}
+
+// The work-group's waves agree on a bound: the least of what each has published (a rank of
+// ceil(top / 4) in its own).
+__device__ __forceinline__ uint64_t lp_least(const uint64_t* best) {
+  uint64_t least = best[0];
+#pragma unroll
+  for (int w = 1; w < kLpWaves; ++w) least = min(least, best[w]);
+  return lp_read(least, 0);
+}
+
+// The waves' sorted lists merged: a key's place is its place in its own list plus the keys above it
+// in the others'. lists: kLpWaves of 64, out: 64, zero. Every wave calls.
+__device__ __forceinline__ void lp_merge(uint64_t mine, int top, int wave, int lane, uint64_t* lists, uint64_t* out) {
+  lists[wave * 64 + lane] = mine;
+  __syncthreads();
+  int place = lane;
+#pragma unroll
+  for (int o = 1; o < kLpWaves; ++o) {
+    const uint64_t* l = lists + (wave + o) % kLpWaves * 64;
+    int n = 0;
+#pragma unroll
+    for (int step = 32; step > 0; step >>= 1) n += l[n + step - 1] > mine ? step : 0;
+    place += n + (l[n] > mine);
+  }
+  if (mine && place < top) out[place] = mine;
+  __syncthreads();
+}
 
 struct LpSum {
   float m = -INFINITY, l = 0.f, t = 0.f;
@@ -173,15 +206,14 @@ template <int DT>
 __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LpArgs a) {
   using T = typename LpType<DT>::T;
   constexpr int VEC = LpType<DT>::VEC;
-  __shared__ uint64_t lists[kLpWaves * kTopMost];
+  __shared__ uint64_t lists[kLpWaves * 64], merged[64];
   __shared__ float sums[kLpWaves * 3];
-  __shared__ __align__(16) uint64_t shared_best[kLpWaves];  // of each wave, its ceil(top / 4)-th best
+  __shared__ uint64_t best[kLpWaves], agreed;  // of each wave, its ceil(top / 4)-th best; the bound from them
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t row = blockIdx.x / a.nseg;
   const int seg = int(blockIdx.x % a.nseg);
   const T* x = static_cast<const T*>(a.x) + (row / a.inner) * a.outer_stride + (row % a.inner) * a.row_stride;
-  if (tid < kLpWaves) shared_best[tid] = 0;
-  __syncthreads();
+  if (wave == 0) merged[lane] = 0;
 
   // segments are cut where the row's memory is 16-byte aligned: element head + k seg
   const int head = min(a.V, int((16 - reinterpret_cast<uintptr_t>(x) % 16) % 16 / sizeof(T)));
@@ -193,32 +225,6 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LpArgs a) {
   LpSum s;
   LpList list;
   list.top = a.top;
-  const int quarter = (a.top + kLpWaves - 1) / kLpWaves - 1;
-  uint64_t told = 0;
-  auto share = [&]() {
-    const uint64_t own = lp_read(list.mine, max(quarter, 0));
-    if (own != told && lane == 0)
-      __hip_atomic_store(&shared_best[wave], own, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-    told = own;
-    uint64_t least = own;
-#pragma unroll
-    for (int w = 0; w < kLpWaves; ++w)
-      least = min(least, __hip_atomic_load(&shared_best[w], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
-    list.last = max(list.last, lp_read(least, 0));
-  };
-  // the ends, at most 2 VEC - 2 elements: one per lane of wave 0
-  if (wave == 0) {
-    const int before = body - lo, after = hi - whole;
-    const int i = lane < before ? lo + lane : whole + (lane - before);
-    const bool live = lane < before + after;
-    float v[1] = {-INFINITY};
-    if (live) {
-      if constexpr (DT == WN_F32) v[0] = x[i];
-      else v[0] = lp_elem<DT>(x[i], 0);
-    }
-    lp_add<1>(v, v[0], s);
-    if (a.top) list.offer(live ? lp_key(v[0], uint32_t(i)) : 0, lane);
-  }
   // batches of U pieces a wave; piece u of the batch at p starts at p + u kLpWaves STEP
   constexpr int STEP = 64 * VEC, U = 4, BATCH = U * kLpWaves * STEP;
   uint4 w[U];
@@ -236,16 +242,21 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LpArgs a) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) v[j] = DT == WN_F32 ? lp_elem<DT>(ws[j], 0) : lp_elem<DT>(ws[j / 2], j & 1);
   };
-  // the hits of a piece at i0 (of lane 0), top: each lane's largest value in it
+  // lanes whose largest value, in a piece or batch from i on, can be among the best: no element of
+  // the lane has a key above the first index's with that value
+  auto hits = [&](float top, uint32_t i, bool live) {
+    uint64_t hit = __ballot(live && lp_key(top, i) > list.last);
+    if (__popcll(hit) > max(a.top, 8)) {
+      list.raise(lp_bound(live ? lp_key(top, 0) : 0, a.top));
+      hit = __ballot(live && lp_key(top, i) > list.last);
+    }
+    return hit;
+  };
+  // takes those of a piece at i0 (of lane 0), top: each lane's largest value in it
   auto collect = [&](const uint4& q, float top, uint32_t i0) {
     const uint32_t i = i0 + lane * VEC;
     const bool live = i < end;
-    // no element of the lane has a key above the first's index with the largest value
-    uint64_t hit = __ballot(live && lp_key(top, i) > list.last);
-    if (__popcll(hit) > max(a.top, 8)) {
-      list.tighten(live ? lp_key(top, i + VEC - 1) : 0, hit);
-      hit = __ballot(live && lp_key(top, i) > list.last);
-    }
+    uint64_t hit = hits(top, i, live);
     while (hit) {
       const int from = __builtin_ctzll(hit);
       const uint32_t ws[4] = {uint32_t(__builtin_amdgcn_readlane(int(q.x), from)), uint32_t(__builtin_amdgcn_readlane(int(q.y), from)),
@@ -257,12 +268,44 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LpArgs a) {
     }
   };
   uint32_t p = uint32_t(body + wave * STEP);
-  if (p < end) load(p);
+  load(p);
+  const int rank = (a.top + kLpWaves - 1) / kLpWaves;
+  uint64_t told = 0;
+  if (a.top) {
+    uint64_t first = 0;  // a bound of the lane's largest key in its first batch
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float v[VEC], top = -INFINITY;
+      values(w[u], v);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) top = fmaxf(top, v[j]);
+      if (p + u * kLpWaves * STEP + lane * VEC < end) first = max(first, lp_key(top, 0xffffffffu));
+    }
+    told = lp_bound(first, rank);
+    if (lane == 0) best[wave] = told;
+    if (tid == 0) agreed = 0;
+    __syncthreads();
+    list.raise(lp_least(best));
+  }
+  // the ends, at most 2 VEC - 2 elements: one per lane of wave 0
+  if (wave == 0) {
+    const int before = body - lo, after = hi - whole;
+    const int i = lane < before ? lo + lane : whole + (lane - before);
+    const bool live = lane < before + after;
+    float v[1] = {-INFINITY};
+    if (live) {
+      if constexpr (DT == WN_F32) v[0] = x[i];
+      else v[0] = lp_elem<DT>(x[i], 0);
+    }
+    lp_add<1>(v, v[0], s);
+    if (a.top) list.offer(live ? lp_key(v[0], uint32_t(i)) : 0, lane);
+  }
   for (; p < end; p += BATCH) {
     uint4 q[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) q[u] = w[u];
     load(p + BATCH);
+    const uint64_t bound = a.top ? __hip_atomic_load(&agreed, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) : 0;
     float tops[U];
     if (p + (U - 1) * kLpWaves * STEP + STEP <= end) {  // every piece is whole
       float v[U][VEC], all[U * VEC], top = -INFINITY;
@@ -279,11 +322,12 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LpArgs a) {
       }
       lp_add<U * VEC>(all, top, s);
       if (!a.top) continue;
-      if (__any(lp_key(top, p + lane * VEC) > list.last)) {
+      list.raise(lp_read(bound, 0));
+      if (!hits(top, p + lane * VEC, true)) continue;
 #pragma unroll
-        for (int u = 0; u < U; ++u) collect(q[u], tops[u], p + u * kLpWaves * STEP);
-      }
+      for (int u = 0; u < U; ++u) collect(q[u], tops[u], p + u * kLpWaves * STEP);
     } else {
+      if (a.top) list.raise(lp_read(bound, 0));
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const uint32_t i0 = p + u * kLpWaves * STEP;
@@ -300,7 +344,18 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LpArgs a) {
         if (a.top) collect(q[u], top, i0);
       }
     }
-    if (a.top) share();
+    if (a.top) {
+      const uint64_t own = lp_read(list.mine, rank - 1);
+      if (own > told) {
+        told = own;
+        if (lane == 0) __hip_atomic_store(&best[wave], own, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        uint64_t least = own;
+#pragma unroll
+        for (int o = 0; o < kLpWaves; ++o)
+          least = min(least, o == wave ? own : __hip_atomic_load(&best[o], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
+        if (lane == 0) atomicMax(reinterpret_cast<unsigned long long*>(&agreed), (unsigned long long)least);
+      }
+    }
   }
 
   // the lanes' sums, then the waves'
@@ -311,63 +366,65 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LpArgs a) {
     sums[3 * wave + 1] = s.l;
     sums[3 * wave + 2] = s.t;
   }
-  lists[wave * kTopMost + lane] = list.mine;
-  __syncthreads();
+  if (a.top) lp_merge(list.mine, a.top, wave, lane, lists, merged);
+  else __syncthreads();
   if (wave != 0) return;
 #pragma unroll
   for (int w = 1; w < kLpWaves; ++w) s.join(sums[3 * w], sums[3 * w + 1], sums[3 * w + 2]);
-  if (a.top) {
-    list.last = lp_read(list.mine, a.top - 1);
-    for (int w = 1; w < kLpWaves; ++w) list.offer(lane < a.top ? lists[w * kTopMost + lane] : 0, lane);
-  }
+  const uint64_t key = merged[lane];
   if (a.nseg == 1) {
-    lp_finish(a, row, s, list.mine, lane, lane == 0 ? lp_given<DT>(a, row, x) : 0.f);
+    lp_finish(a, row, s, key, lane, lane == 0 ? lp_given<DT>(a, row, x) : 0.f);
     return;
   }
   const int64_t part = row * a.nseg + seg;
   if (lane == 0) a.part[part] = make_float4(s.m, s.l, s.t, 0.f);
-  if (lane < a.top) a.keys[part * a.top + lane] = list.mine;
+  if (lane < a.top) a.keys[part * a.top + lane] = key;
 }
 
-// Joins the segments of a row: one wave per row, its keys by 64, each 64 narrowed to those that
-// can be among the best before any is inserted.
+// Joins the segments of a row: a work-group per row, a quarter of the segments' keys to a wave, with
+// the bound of the waves' lanes' maxima as above.
 template <int DT>
-__global__ __launch_bounds__(64) void logprobs_join_kernel(LpArgs a) {
+__global__ __launch_bounds__(kLpThreads) void logprobs_join_kernel(LpArgs a) {
   using T = typename LpType<DT>::T;
-  const int lane = threadIdx.x;
+  __shared__ uint64_t lists[kLpWaves * 64], merged[64], best[kLpWaves];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t row = blockIdx.x;
   const T* x = static_cast<const T*>(a.x) + (row / a.inner) * a.outer_stride + (row % a.inner) * a.row_stride;
   const int n = a.nseg * a.top;
   const uint64_t* keys = a.keys + row * n;
-  constexpr int U = 6;
-  uint64_t key[U];
+  constexpr int U = 4;  // kept in registers, 1,024 keys of the row; the rest is read again
+  uint64_t key[U], first = 0;
 #pragma unroll
-  for (int u = 0; u < U; ++u) key[u] = 64 * u + lane < n ? keys[64 * u + lane] : 0;
-  const float given = lane == 0 ? lp_given<DT>(a, row, x) : 0.f;
+  for (int u = 0; u < U; ++u) key[u] = kLpThreads * u + tid < n ? keys[kLpThreads * u + tid] : 0;
   LpSum s;
-  for (int g = lane; g < a.nseg; g += 64) {
-    const float4 p = a.part[row * a.nseg + g];
-    s.join(p.x, p.y, p.z);
+  float given = 0.f;
+  if (wave == 0) {
+    if (lane == 0) given = lp_given<DT>(a, row, x);
+    for (int g = lane; g < a.nseg; g += 64) {
+      const float4 p = a.part[row * a.nseg + g];
+      s.join(p.x, p.y, p.z);
+    }
+    merged[lane] = 0;
   }
+  if (a.top) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) s.join(__shfl_xor(s.m, o, 64), __shfl_xor(s.l, o, 64), __shfl_xor(s.t, o, 64));
-  LpList list;
-  list.top = a.top;
-  for (int i0 = 0; i0 < n; i0 += 64 * U) {
-    uint64_t best = key[0];
-#pragma unroll
-    for (int u = 1; u < U; ++u) best = max(best, key[u]);
-    const uint64_t hit = __ballot(best > list.last);
-    if (__popcll(hit) > a.top) list.tighten(best, hit);
+    for (int u = 0; u < U; ++u) first = max(first, key[u]);
+    for (int i = kLpThreads * U + tid; i < n; i += kLpThreads) first = max(first, keys[i]);
+    const uint64_t own = lp_bound(first, (a.top + kLpWaves - 1) / kLpWaves);
+    if (lane == 0) best[wave] = own;
+    __syncthreads();
+    LpList list;
+    list.top = a.top;
+    list.raise(lp_least(best));
 #pragma unroll
     for (int u = 0; u < U; ++u) list.offer(key[u], lane);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + 64 * (U + u) + lane;
-      key[u] = i < n ? keys[i] : 0;
-    }
+    for (int i = kLpThreads * U; i < n; i += kLpThreads) list.offer(i + tid < n ? keys[i + tid] : 0, lane);
+    lp_merge(list.mine, a.top, wave, lane, lists, merged);
   }
-  lp_finish(a, row, s, list.mine, lane, given);
+  if (wave != 0) return;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s.join(__shfl_xor(s.m, o, 64), __shfl_xor(s.l, o, 64), __shfl_xor(s.t, o, 64));
+  lp_finish(a, row, s, merged[lane], lane, given);
 }
 
 // Segments of a row, of 2,048 elements at least: the count that takes the least time for 1,024
@@ -437,7 +494,7 @@ extern "C" int wn_token_logprobs(const void* logits, int dtype, int64_t stride_o
   const dim3 grid(unsigned(N * nseg)), join(static_cast<unsigned>(N));
   auto run = [&](auto scan, auto joined) {
     hipLaunchKernelGGL(scan, grid, dim3(kLpThreads), 0, st, a);
-    if (nseg > 1) hipLaunchKernelGGL(joined, join, dim3(64), 0, st, a);
+    if (nseg > 1) hipLaunchKernelGGL(joined, join, dim3(kLpThreads), 0, st, a);
   };
   if (dtype == WN_F32) run(logprobs_kernel<WN_F32>, logprobs_join_kernel<WN_F32>);
   else if (dtype == WN_F16) run(logprobs_kernel<WN_F16>, logprobs_join_kernel<WN_F16>);
