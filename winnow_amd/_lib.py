@@ -315,7 +315,10 @@ def parents_in_order(parents: torch.Tensor) -> bool:
 
 
 def stream_of(device: torch.device):
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    """The handle of the device's current stream, as a plain integer (0: the default stream)."""
+    if device.index is None:
+        return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def is_hip(t: torch.Tensor) -> bool:

@@ -98,6 +98,9 @@ __device__ __forceinline__ bool tree_split(const TreeArgs& a, int lane, int j, i
 // group i's K rows, V rows, K norms or V norms (kind 0 .. 3): formed by one product a chunk, and read
 // from there into scalars, where a scalar product per group and kind took a sixth of the scan's
 // instructions.
+// Of global memory, by type: through a pointer that the compiler must take for any memory's, every wait
+// for LDS waits for the rows too.
+using TreeBytes = const __attribute__((address_space(1))) uint8_t*;
 struct TreeRows {
   uint64_t base, stride;  // of the kind: pool + head, bytes per page
   uint32_t token;         // bytes per token
@@ -114,14 +117,14 @@ struct TreeRows {
   __device__ __forceinline__ void set(uint32_t page, int slot) {
     at = base + uint64_t(page) * stride + uint32_t(slot) * token;
   }
-  __device__ __forceinline__ const uint8_t* rows(int kind, int group) const {  // wave-uniform
+  __device__ __forceinline__ TreeBytes rows(int kind, int group) const {  // wave-uniform
     const int l = 4 * kind + group;
-    return reinterpret_cast<const uint8_t*>(uint64_t(uint32_t(__builtin_amdgcn_readlane(int(at >> 32), l))) << 32 |
+    return TreeBytes(uint64_t(uint32_t(__builtin_amdgcn_readlane(int(at >> 32), l))) << 32 |
                                             uint32_t(__builtin_amdgcn_readlane(int(uint32_t(at)), l)));
   }
-  __device__ __forceinline__ const uint8_t* rows_lane(int kind, int group) const {  // by the lane
+  __device__ __forceinline__ TreeBytes rows_lane(int kind, int group) const {  // by the lane
     const int l = 4 * kind + group;
-    return reinterpret_cast<const uint8_t*>(uint64_t(uint32_t(__shfl(int(at >> 32), l, 64))) << 32 |
+    return TreeBytes(uint64_t(uint32_t(__shfl(int(at >> 32), l, 64))) << 32 |
                                             uint32_t(__shfl(int(uint32_t(at)), l, 64)));
   }
 };

@@ -44,21 +44,18 @@ struct TreeGeo {
 __device__ __forceinline__ int tree_tok(int t, int c) { return 32 * (t >> 1) + 8 * (c >> 2) + 4 * (t & 1) + (c & 3); }
 
 // The raw words of one group of eight codes: the one or two 4-byte words that hold bytes
-// [o, o + bw) of a block; a word without any of them is not read.
+// [o, o + bw) of a block; no other word is read.
 struct TreeRaw {
   uint32_t lo, hi;
 };
 template <int BW>
-__device__ __forceinline__ TreeRaw tree_raw(const uint8_t* block, uint32_t o, int bw) {
+__device__ __forceinline__ TreeRaw tree_raw(TreeBytes block, uint32_t o, int bw) {
+  using Words = const __attribute__((address_space(1))) uint32_t*;
   TreeRaw r;
-  r.lo = *reinterpret_cast<const uint32_t*>(block + (o & ~3u));
-  if constexpr (BW == 4) {
-    r.hi = 0;
-  } else {
-    const uint32_t last = (o + uint32_t(bw) - 1) & ~3u;
-    r.hi = r.lo;
-    if (last != (o & ~3u)) r.hi = *reinterpret_cast<const uint32_t*>(block + last);
-  }
+  r.lo = *Words(block + (o & ~3u));
+  // the same word again where one holds them all: a branch would wait for the load before it
+  if constexpr (BW == 4) r.hi = 0;
+  else r.hi = *Words(block + ((o + uint32_t(bw) - 1) & ~3u));
   return r;
 }
 
@@ -286,12 +283,12 @@ __global__ __launch_bounds__(64 * RG * TG, 2) void tree_scan_kernel(TreeArgs a) 
         for (int j = 0; j < C::NV; ++j) {
           int grp, tp, dg;
           if (!v_item(j, &grp, &tp, &dg)) continue;
-          const uint8_t* v = block(1, grp);
+          const TreeBytes v = block(1, grp);
           vr[P][j][0] = tree_raw<W>(v, v_off(tp, dg), bwv);
           vr[P][j][1] = tree_raw<W>(v, v_off(tp, dg) + nbv, bwv);
         }
         if (C::NW <= G::NG || wig < G::NG) {  // wave w: the norms of group w, K in lanes 0..15, V in 16..31
-          nr[P] = reinterpret_cast<const uint16_t*>(lane & 16 ? at.rows(3, wig) : at.rows(2, wig))[c];
+          nr[P] = ((const __attribute__((address_space(1))) uint16_t*)(lane & 16 ? at.rows(3, wig) : at.rows(2, wig)))[c];
         }
       };
       uint32_t k_to, v_to;  // LDS addresses of the first items
@@ -422,25 +419,34 @@ __global__ __launch_bounds__(64 * RG * TG, 2) void tree_scan_kernel(TreeArgs a) 
         // scores of the wave's tokens: register i of tile t is token w0 + tree_tok(t, 4 g + i)
         f32x4 d[NCT][C::NTW];
 #pragma unroll
-        for (int t = 0; t < C::NTW; ++t) {
+        for (int t = 0; t < C::NTW; ++t)
 #pragma unroll
           for (int ct = 0; ct < NCT; ++ct) d[ct][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        // two tiles at a time, so that an accumulator's next product is 2 NCT instructions off
+#pragma unroll
+        for (int t0 = 0; t0 < C::NTW; t0 += 2)
 #pragma unroll
           for (int k = 0; k < G::KS; ++k) {
-            const char* kp = lds + k_addr(t, k);
-            const h8 kh = *reinterpret_cast<const h8*>(kp);
+            const char* kp[2] = {lds + k_addr(t0, k), lds + k_addr(t0 + 1, k)};
+            h8 kh[2], kl[2];
 #pragma unroll
-            for (int ct = 0; ct < NCT; ++ct) d[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[ct][k], d[ct][t], 0, 0, 0);
+            for (int t = 0; t < 2; ++t) {
+              kh[t] = *reinterpret_cast<const h8*>(kp[t]);
+              if constexpr (EX) kl[t] = *reinterpret_cast<const h8*>(kp[t] + G::KT);
+            }
+            auto products = [&](const h8 (&x)[2], const auto& y) {
+#pragma unroll
+              for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int ct = 0; ct < NCT; ++ct)
+                  d[ct][t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[t], y[ct][k], d[ct][t0 + t], 0, 0, 0);
+            };
+            products(kh, qh);
             if constexpr (EX) {
-              const h8 kl = *reinterpret_cast<const h8*>(kp + G::KT);
-#pragma unroll
-              for (int ct = 0; ct < NCT; ++ct) {
-                d[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[ct][k], d[ct][t], 0, 0, 0);
-                d[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, ql[ct][k], d[ct][t], 0, 0, 0);
-              }
+              products(kl, qh);
+              products(kh, ql);
             }
           }
-        }
         __builtin_amdgcn_sched_barrier(0);
         // value scale: every n_V < 2^(7 + gs), so 2^kTreeRescale n_V 2^-gs < 2^15 in fp16; it
         // follows the norms' magnitude (n_V = 2^-20 keeps its bits)
@@ -560,24 +566,31 @@ __global__ __launch_bounds__(64 * RG * TG, 2) void tree_scan_kernel(TreeArgs a) 
             }
         __builtin_amdgcn_sched_barrier(0);
         // values: A row c of M-tile mt = dim 16 mt + c, k-slots of lane group g = tokens 32 ks + 8 g .. + 7
+        constexpr int MP = G::MT > 1 ? 2 : 1;  // M-tiles at a time, as above
 #pragma unroll
-        for (int mt = 0; mt < G::MT; ++mt) {
+        for (int m0 = 0; m0 < G::MT; m0 += MP)
 #pragma unroll
           for (int ks = 0; ks < KV; ++ks) {
-            const char* vp = lds + v_addr(mt, ks);
-            const h8 vh = *reinterpret_cast<const h8*>(vp);
+            h8 vh[MP], vl[MP];
 #pragma unroll
-            for (int ct = 0; ct < NCT; ++ct) acc[ct][mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph[ct][ks], acc[ct][mt], 0, 0, 0);
+            for (int i = 0; i < MP; ++i) {
+              const char* vp = lds + v_addr(m0 + i, ks);
+              vh[i] = *reinterpret_cast<const h8*>(vp);
+              if constexpr (EX) vl[i] = *reinterpret_cast<const h8*>(vp + G::VT);
+            }
+            auto products = [&](const h8 (&x)[MP], const auto& y) {
+#pragma unroll
+              for (int i = 0; i < MP; ++i)
+#pragma unroll
+                for (int ct = 0; ct < NCT; ++ct)
+                  acc[ct][m0 + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[i], y[ct][ks], acc[ct][m0 + i], 0, 0, 0);
+            };
+            products(vh, ph);
             if constexpr (EX) {
-              const h8 vl = *reinterpret_cast<const h8*>(vp + G::VT);
-#pragma unroll
-              for (int ct = 0; ct < NCT; ++ct) {
-                acc[ct][mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph[ct][ks], acc[ct][mt], 0, 0, 0);
-                acc[ct][mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl[ct][ks], acc[ct][mt], 0, 0, 0);
-              }
+              products(vl, ph);
+              products(vh, pl);
             }
           }
-        }
       };
       for (int ch = ch_lo; ch < ch_hi; ch += AHEAD) {
         chunk(even, G::CH * ch);

@@ -174,41 +174,45 @@ def check_contract(q: torch.Tensor, kv: PackedKV, *, check_ranges: bool = True) 
     B, Hq, _, D = q.shape
     if D != kv.head_dim:
         raise UnsupportedLayout(f"q head_dim {D} != cache head_dim {kv.head_dim}")
-    for name, quant in (("k", kv.k_quant), ("v", kv.v_quant)):
+    kq, vq, k_pages, v_pages, k_norms, v_norms = kv.k_quant, kv.v_quant, kv.k_pages, kv.v_pages, kv.k_norms, kv.v_norms
+    table, seq_lens = kv.page_table, kv.seq_lens
+    for name, quant in (("k", kq), ("v", vq)):
         if quant.Pi.shape != (D, D) or quant.Pi.dtype != torch.float32:
             raise UnsupportedLayout(f"{name} rotation must be fp32 ({D}, {D})")
         if quant.centroids.dtype != torch.float32 or quant.centroids.numel() != 2 ** quant.bit_width:
             raise UnsupportedLayout(f"{name} codebook must be fp32 with 2**bw entries")
     try:
-        nb_k = packed_bytes(D, kv.k_quant.bit_width)
-        nb_v = packed_bytes(D, kv.v_quant.bit_width)
+        nb_k = packed_bytes(D, kq.bit_width)
+        nb_v = packed_bytes(D, vq.bit_width)
     except ValueError as e:
         raise UnsupportedLayout(str(e)) from e
-    P, Hkv, S = kv.k_pages.shape[:3]
-    if kv.k_pages.dtype != torch.uint8 or kv.v_pages.dtype != torch.uint8:
+    if k_pages.dtype != torch.uint8 or v_pages.dtype != torch.uint8:
         raise UnsupportedLayout("packed pages must be uint8")
-    if kv.k_pages.shape != (P, Hkv, S, nb_k) or kv.v_pages.shape[:3] != (P, Hkv, S) \
-            or kv.v_pages.shape[3] != nb_v:
+    lead = k_pages.shape[:3]
+    P, Hkv, S = lead
+    if k_pages.shape != (P, Hkv, S, nb_k) or v_pages.shape != (P, Hkv, S, nb_v):
         raise UnsupportedLayout(
-            f"page shapes {tuple(kv.k_pages.shape)}/{tuple(kv.v_pages.shape)} do not "
+            f"page shapes {tuple(k_pages.shape)}/{tuple(v_pages.shape)} do not "
             f"match (P, Hkv, S, NB) with NB={nb_k}/{nb_v}")
-    if kv.k_norms.shape != (P, Hkv, S) or kv.v_norms.shape != (P, Hkv, S):
+    if k_norms.shape != lead or v_norms.shape != lead:
         raise UnsupportedLayout("norms must be (P, Hkv, S)")
-    if kv.k_norms.dtype != torch.float16 or kv.v_norms.dtype != torch.float16:
+    if k_norms.dtype != torch.float16 or v_norms.dtype != torch.float16:
         raise UnsupportedLayout("norms must be fp16")
     if Hq % Hkv:
         raise UnsupportedLayout(f"Hq={Hq} is not a multiple of Hkv={Hkv}")
-    if kv.page_table.dim() != 2 or kv.page_table.shape[0] != B:
+    if table.dim() != 2 or table.shape[0] != B:
         raise UnsupportedLayout("page_table must be (B, max_pages)")
-    if kv.seq_lens.shape != (B,):
+    if seq_lens.shape != (B,):
         raise UnsupportedLayout("seq_lens must be (B,)")
-    if kv.page_table.dtype != torch.int32 or kv.seq_lens.dtype != torch.int32:
+    if table.dtype != torch.int32 or seq_lens.dtype != torch.int32:
         raise UnsupportedLayout("page_table and seq_lens must be int32")
     dev = q.device
-    operands = (kv.k_pages, kv.v_pages, kv.k_norms, kv.v_norms, kv.page_table, kv.seq_lens, kv.k_quant.Pi, kv.v_quant.Pi,
-                kv.k_quant.centroids, kv.v_quant.centroids)
-    if any(t.device != dev for t in operands):
-        raise UnsupportedLayout(f"all operands must share a device, got { {dev, *(t.device for t in operands)} }")
+    if k_pages.device != dev or v_pages.device != dev or k_norms.device != dev or v_norms.device != dev \
+            or table.device != dev or seq_lens.device != dev or kq.Pi.device != dev or vq.Pi.device != dev \
+            or kq.centroids.device != dev or vq.centroids.device != dev:
+        devices = {t.device for t in (q, k_pages, v_pages, k_norms, v_norms, table, seq_lens, kq.Pi, vq.Pi,
+                                      kq.centroids, vq.centroids)}
+        raise UnsupportedLayout(f"all operands must share a device, got {devices}")
     if not check_ranges:
         return
     lens = kv.seq_lens_host if kv.seq_lens_host is not None else kv.seq_lens

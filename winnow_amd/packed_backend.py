@@ -304,7 +304,6 @@ def _check_commit_side(name: str, pages: torch.Tensor, norms, lead) -> None:
                 raise pa.UnsupportedLayout(f"commit: {name} is written in place and may not be expanded")
 
 
-@torch.no_grad()
 def commit_kv(k_pages: torch.Tensor, v_pages: torch.Tensor, k_norms: torch.Tensor | None,
               v_norms: torch.Tensor | None, page_table: torch.Tensor, start_pos: torch.Tensor,
               path: torch.Tensor, counts: torch.Tensor, *, nodes: int,
