@@ -228,6 +228,8 @@ extern "C" int wn_tree_attention(
   ra.nrp = nrp;
   ra.q_dtype = q_dtype;
   ra.exact = exact != 0;
+  const int per = q_dtype == WN_F32 ? 4 : 8;  // elements of 16 bytes
+  ra.vec = aligned(q, 16) && q_stride_b % per == 0 && q_stride_h % per == 0 && q_stride_t % per == 0;
   hipLaunchKernelGGL(k.rotate, dim3(unsigned(tiles)), dim3(k.rotate_threads), 0, st, ra);
 
   TreeArgs a;

@@ -143,6 +143,7 @@ struct TreeRotArgs {
   uint64_t* vis;
   float scale;  // scale log2(e)
   int Hkv, n_rep, T, nrp, q_dtype, exact;
+  int vec;  // q's base and strides are multiples of 16 bytes
 };
 
 struct TreeMergeArgs {

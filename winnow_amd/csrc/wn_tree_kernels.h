@@ -679,7 +679,7 @@ struct TreeProduct {
 
 __host__ __device__ constexpr int tree_rotate_threads(int D) { return 4 * D > 256 ? 4 * D : 256; }
 
-// q' of sixteen rows per work-group (rows past n_rep T: zero), and the nodes' words.
+// q' of sixteen rows per work-group (rows past n_rep T: zero, up to a multiple of 32), and the nodes' words.
 template <int D>
 __global__ __launch_bounds__(tree_rotate_threads(D)) void tree_rotate_kernel(TreeRotArgs a) {
   constexpr int XS = D + 4, NTHR = tree_rotate_threads(D);
@@ -691,23 +691,53 @@ __global__ __launch_bounds__(tree_rotate_threads(D)) void tree_rotate_kernel(Tre
   const int64_t unit = blockIdx.x / tiles;  // b Hkv + kvh
   const int r0 = 16 * int(blockIdx.x % tiles), kvh = int(unit % a.Hkv), rows = a.n_rep * a.T;
   const int64_t b = unit / a.Hkv;
+  if (r0 >= (rows + 31) / 32 * 32) return;  // of no wave that computes
   const bool words = kvh == 0 && r0 == 0;  // one work-group per sequence
   TreeProduct<D> pi;
   pi.load(wave, lane, [&](int j, int k) { return *reinterpret_cast<const f32x4*>(a.pi + j * D + k); });
   if (words && tid < 64) par[tid] = tid < a.T ? a.parents[b * a.psb + tid] : -1;
-  // all loads of a thread at once: the type is asked for outside
-  const auto fetch = [&](auto&& load) {
+  // a thread's share of a row by 16 bytes where q is laid out for it (a.vec)
+  const auto fetch = [&](auto vec, auto&& load) {
+    constexpr int V = decltype(vec)::value, PER = D / V;  // elements a load, loads a row
 #pragma unroll
-    for (int i0 = 0; i0 < 16 * D; i0 += NTHR) {
-      const int i = i0 + tid, r = r0 + i / D, d = i % D;
-      float v = 0.f;
-      if (r < rows) v = load(b * a.qsb + (kvh * a.n_rep + r % a.n_rep) * a.qsh + (r / a.n_rep) * a.qsq + d);
-      x[(i / D) * XS + d] = v;
+    for (int i0 = 0; i0 < 16 * PER; i0 += NTHR) {
+      const int i = i0 + tid, r = r0 + i / PER, d = V * (i % PER);
+      if (16 * PER % NTHR != 0 && i >= 16 * PER) break;
+      float v[V] = {};
+      if (r < rows) load(b * a.qsb + (kvh * a.n_rep + r % a.n_rep) * a.qsh + (r / a.n_rep) * a.qsq + d, v);
+#pragma unroll
+      for (int e = 0; e < V; ++e) x[(i / PER) * XS + d + e] = v[e];
     }
   };
-  if (a.q_dtype == WN_F32) fetch([&](int64_t o) { return static_cast<const float*>(a.q)[o]; });
-  else if (a.q_dtype == WN_BF16) fetch([&](int64_t o) { return bf16_to_f32(static_cast<const uint16_t*>(a.q)[o]); });
-  else fetch([&](int64_t o) { return f16_to_f32(static_cast<const uint16_t*>(a.q)[o]); });
+  const auto words16 = [&](auto vec, auto&& value) {
+    fetch(vec, [&](int64_t o, float (&v)[decltype(vec)::value]) {
+      constexpr int V = decltype(vec)::value;
+      uint16_t h[V];
+      __builtin_memcpy(h, __builtin_assume_aligned(static_cast<const uint16_t*>(a.q) + o, 2 * V), 2 * V);
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = value(h[e]);
+    });
+  };
+  const auto words32 = [&](auto vec) {
+    fetch(vec, [&](int64_t o, float (&v)[decltype(vec)::value]) {
+      constexpr int V = decltype(vec)::value;
+      __builtin_memcpy(v, __builtin_assume_aligned(static_cast<const float*>(a.q) + o, 4 * V), 4 * V);
+    });
+  };
+  constexpr std::integral_constant<int, 1> one;
+  constexpr std::integral_constant<int, 4> four;
+  constexpr std::integral_constant<int, 8> eight;
+  const auto bf16 = [](uint16_t h) { return bf16_to_f32(h); };
+  const auto fp16 = [](uint16_t h) { return f16_to_f32(h); };
+  if (a.vec) {
+    if (a.q_dtype == WN_F32) words32(four);
+    else if (a.q_dtype == WN_BF16) words16(eight, bf16);
+    else words16(eight, fp16);
+  } else {
+    if (a.q_dtype == WN_F32) words32(one);
+    else if (a.q_dtype == WN_BF16) words16(one, bf16);
+    else words16(one, fp16);
+  }
   __syncthreads();
   if (words && tid < a.T) {
     // a parent comes before its child: any other value ends the walk, as -1 does
@@ -720,16 +750,20 @@ __global__ __launch_bounds__(tree_rotate_threads(D)) void tree_rotate_kernel(Tre
   __syncthreads();
   if (a.qf) {
 #pragma unroll
-    for (int i = tid; i < 16 * D; i += NTHR)
-      a.qf[(unit * a.nrp + r0 + i / D) * D + i % D] = y[(i / D) * XS + i % D] * a.scale;
+    for (int i = 4 * tid; i < 16 * D; i += 4 * NTHR) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(y + (i / D) * XS + i % D) * a.scale;
+      *reinterpret_cast<f32x4*>(a.qf + (unit * a.nrp + r0 + i / D) * D + i % D) = v;
+    }
     return;
   }
   // sixteen threads a row: its largest magnitude, then the fp16 terms of q' 2^e (below 2^15)
   if (tid >= 256) return;
+  constexpr int DPT = D / 16;
   const int r = tid >> 4, k = tid & 15;
-  float top = 0.f;
+  float v[DPT], top = 0.f;
+  __builtin_memcpy(v, __builtin_assume_aligned(y + r * XS + DPT * k, DPT < 4 ? 4 * DPT : 16), 4 * DPT);
 #pragma unroll
-  for (int d = k; d < D; d += 16) top = fmaxf(top, fabsf(y[r * XS + d]));
+  for (int d = 0; d < DPT; ++d) top = fmaxf(top, fabsf(v[d]));
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 16));
   int qe;
@@ -738,24 +772,28 @@ __global__ __launch_bounds__(tree_rotate_threads(D)) void tree_rotate_kernel(Tre
   const float up = ldexpf(1.f, e);
   const int64_t row = unit * a.nrp + r0 + r;
   if (k == 0) a.qs[row] = ldexpf(a.scale, -(e + 8));
+  _Float16 h[DPT], l[DPT];
 #pragma unroll
-  for (int d = k; d < D; d += 16) {
-    const float v = y[r * XS + d] * up;
-    const _Float16 h = _Float16(v);
-    a.qh[row * D + d] = h;
-    if (a.exact) a.ql[row * D + d] = _Float16(v - float(h));
+  for (int d = 0; d < DPT; ++d) {
+    const float t = v[d] * up;
+    h[d] = _Float16(t);
+    l[d] = _Float16(t - float(h[d]));
   }
+  constexpr int AL = 2 * DPT < 16 ? 2 * DPT : 16;
+  __builtin_memcpy(__builtin_assume_aligned(a.qh + row * D + DPT * k, AL), h, 2 * DPT);
+  if (a.exact) __builtin_memcpy(__builtin_assume_aligned(a.ql + row * D + DPT * k, AL), l, 2 * DPT);
 }
 
 // R rows per work-group of 16 waves, 16 / R waves a row: the splits' partials merged (weights
 // 2^(m_s - max m)), divided by the sum, times Pi_V, cast. A row that saw no key is 0. The statistics
-// come a split to a lane, the accumulators a split to a load, eight of them in flight; the first of
+// come a split to a lane, the accumulators a split to a load, eight (R = 4) or four in flight; the first of
 // both, and Pi_V's operands, are asked for before anything is known of the sequence: what bounds
 // these few rows is one round trip after another.
 template <int D, int R>
 __global__ __launch_bounds__(1024) void tree_merge_kernel(TreeMergeArgs a) {
   constexpr int XS = D + 4, LD = D < 64 ? D : 64, VEC = D / LD;  // lanes a split, dims a lane
   constexpr int SUB = 64 / LD, PARTS = 16 / R * SUB;              // splits are taken in PARTS residue classes
+  constexpr int U = R == 4 ? 8 : 4;
   __shared__ __align__(16) float x[PARTS][R][XS];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rows = a.n_rep * a.T, blocks = (rows + R - 1) / R;
@@ -764,10 +802,10 @@ __global__ __launch_bounds__(1024) void tree_merge_kernel(TreeMergeArgs a) {
   const int r = wave % R, part = wave / R * SUB + lane / LD, d0 = VEC * (lane % LD);
   const int64_t first = unit * a.nsplit * a.nrp + min(blk * R + r, rows - 1);
   const auto stats = [&](int s) { return *reinterpret_cast<const float2*>(a.part_ml + 2 * (first + int64_t(min(s, a.nsplit - 1)) * a.nrp)); };
-  float v[8][VEC];
+  float v[U][VEC];
   const auto fetch = [&](int s0) {  // splits s0 + part, s0 + PARTS + part, ...
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < U; ++j) {
       const float* p = a.part_acc + (first + int64_t(min(s0 + PARTS * j + part, a.nsplit - 1)) * a.nrp) * D + d0;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) v[j][e] = p[e];
@@ -792,10 +830,10 @@ __global__ __launch_bounds__(1024) void tree_merge_kernel(TreeMergeArgs a) {
     const float w = own ? __builtin_amdgcn_exp2f(ml.x - M) : 0.f;  // split s0 + lane's; 0 for one that saw no key
     den = own ? fmaf(w, ml.y, den) : den;
     const int n = min(64, live - s0);
-    for (int i = 0; i < n; i += 8 * PARTS) {
+    for (int i = 0; i < n; i += U * PARTS) {
       if (s0 + i) fetch(s0 + i);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < U; ++j) {
         const int s = i + PARTS * j + part;
         const float ws = __shfl(w, s & 63, 64);
 #pragma unroll
