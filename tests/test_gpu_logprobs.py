@@ -159,3 +159,17 @@ def test_graph_replays_and_own_stream():
         want = _lp(x, t, top=6)
         for name in ("logprob", "entropy", "top_logprobs", "top_ids"):
             assert torch.equal(getattr(got, name), getattr(want, name))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N,V,top", [(1, 128256, 64), (3, 9001, 20), (1100, 4100, 7), (2, 70001, 1)])
+@pytest.mark.parametrize("order", ["rising", "falling", "sawtooth", "one_wave"])
+def test_alternatives_of_logits_in_an_order(dtype, N, V, top, order):
+    """Every logit of a rising row is the best so far; a falling row's are all in the first pieces;
+    a sawtooth repeats its values (equal logits, the lowest index first); a row whose best lie in
+    one piece, which one wave of the four reads."""
+    i = torch.arange(V, dtype=torch.float64)
+    x = {"rising": i / V * 20, "falling": -i / V * 20, "sawtooth": (i % 97) / 8,
+         "one_wave": torch.where((i >= V // 2) & (i < V // 2 + 100), 5 + (i % 13), -(i % 31) / 4)}[order]
+    x = x.to(dtype).expand(N, V).contiguous()
+    _check(x.to(DEV), (torch.arange(N) % V).to(DEV), top)

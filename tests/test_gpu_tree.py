@@ -328,3 +328,16 @@ def test_many_sequences_some_of_them_empty(columns):
     for splits in (None, 5):
         got = _pa().packed_tree_attention(q.to(DEV), d, 0.08, parents.to(DEV), num_splits=splits)
         _check(got, q, kv, parents, 0.08, torch.bfloat16, single=True)
+
+
+@pytest.mark.parametrize("bwk,bwv", [(4, 4), (8, 3)])
+@pytest.mark.parametrize("D", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("Hq,Hkv,T", [(6, 2, 33), (12, 1, 64)])
+def test_more_rows_than_a_block(D, bwk, bwv, Hq, Hkv, T):
+    """99 and 768 rows a kv head: whole row blocks, and ones whose last waves have none."""
+    q, kv, parents = _case(1900 + D + T + bwk, (T + 5, 0, 333), Hq, Hkv, D, T, bwk, bwv)
+    d, scale = to_device(kv, DEV), D ** -0.5
+    got = _pa().packed_tree_attention(q.to(DEV), d, scale, parents.to(DEV))
+    _check(got, q, kv, parents, scale, torch.float32)
+    one = _pa().packed_tree_attention(q.to(DEV), d, scale, parents.to(DEV), allow_tf32=True)
+    _check(one, q, kv, parents, scale, torch.float32, single=True)

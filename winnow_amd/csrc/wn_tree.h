@@ -11,24 +11,33 @@
 //                          r / n_rep, head r % n_rep of the group) as fp16, or as two
 //                          fp16 terms, with a power-of-two scale per row; and every
 //                          node's 64-bit word of visible nodes, from the parents;
-//   2. tree_scan_kernel    one work-group per (sequence, kv head, row block, split of the
-//                          tokens): online softmax over its chunks, an (acc, m, l)
-//                          partial per row;
+//   2. tree_scan_kernel    a work-group per (split of the batch's tokens, kv head, row block):
+//                          online softmax over its chunks, an (acc, m, l) partial per row
+//                          (tree_rows.hip holds the scan of long contexts);
 //   3. tree_merge_kernel   per row the max-stable merge of its splits, 1/l, Pi_V, cast.
 //
 // The scan, per chunk of 64 tokens (32 at head_dim 256): all threads turn the packed rows
 // into fp16 tiles in LDS, K as [token][dim] and V as [dim][token], each code looked up
-// once per work-group in a table of (high, low) fp16 terms of 2^8 c, one copy per bank;
-// then wave (rg, tg) takes row group rg and token group tg. Per 16 x 16 tile (lane
-// 16 g + c) scores have A = K (row c = token tile_row(t, c), k-slots = 8 dims) and B = q'
-// (column c = query row), so that a lane's score registers of tiles 2ks, 2ks + 1 are the
-// consecutive tokens 32 ks + 8 g .. + 7 of one row: as the value product's B operand P
-// never leaves the registers, and A is one 16-byte read of the V tile.
+// once per work-group in a table of (high, low) fp16 terms of 2^8 c, or, for 4-bit codes and
+// single terms, of a byte's two codes at once; then wave (rg, tg) takes row group rg and token
+// group tg. Per 16 x 16 tile (lane 16 g + c) scores have A = K (row c = token tile_row(t, c),
+// k-slots = 8 dims) and B = q' (column c = query row), so that a lane's score registers of tiles
+// 2ks, 2ks + 1 are the consecutive tokens 32 ks + 8 g .. + 7 of one row: as the value product's
+// B operand P never leaves the registers, and A is one 16-byte read of the V tile. Blocks of 16,
+// 32 or 64 rows and more per wave and work-group by how many rows a kv head has: a chunk is
+// decoded once for a whole block.
+//
+// What bounds it is instruction issue (decoding: six instructions a code by single lookups, three
+// by pairs; the softmax: thirteen a score) beside the matrix instructions, and, for few rows,
+// latency. Whole scans on a 256-CU device: 8 sequences of 500 to 6,000 tokens, 28 heads over 4,
+// 26 nodes, 4 bits, single terms: 41 us; 4 sequences of 15,000 to 20,000, 64 heads over 8, 64
+// nodes, 4 and 6 bits, two terms: 605 us, 0.73 PFLOP/s of fp16 products; one sequence of 300, 32
+// heads over 8, 8 nodes: 9.5 us, of which a chunk takes 2.
 //
 // Precision. EX = true: every factor is a sum of two fp16 terms (22 bits), and each product
 // the three larger of their four products (what is left out is below 2^-22 of a term):
 // fp32 accuracy for fp16 and fp32 results. EX = false: one fp16 term per factor (rounded to
-// nearest, 2^-12 of a factor at most, three bits finer than a bf16 result's own rounding),
+// nearest, off by 2^-11 of it at most, three bits finer than a bf16 result's own rounding),
 // a third of the matrix work. Sums, maxima and partials are fp32 either way.
 #pragma once
 

@@ -680,6 +680,8 @@ struct TreeProduct {
 __host__ __device__ constexpr int tree_rotate_threads(int D) { return 4 * D > 256 ? 4 * D : 256; }
 
 // q' of sixteen rows per work-group (rows past n_rep T: zero, up to a multiple of 32), and the nodes' words.
+// Products in fp32. Bound by latency and, with many tiles, by the instructions around 32 matrix
+// products: 5.5 us for 16 tiles, 14 us for 2,048 (64 heads, 64 nodes, 4 sequences: 12 MB moved).
 template <int D>
 __global__ __launch_bounds__(tree_rotate_threads(D)) void tree_rotate_kernel(TreeRotArgs a) {
   constexpr int XS = D + 4, NTHR = tree_rotate_threads(D);
@@ -788,7 +790,8 @@ __global__ __launch_bounds__(tree_rotate_threads(D)) void tree_rotate_kernel(Tre
 // 2^(m_s - max m)), divided by the sum, times Pi_V, cast. A row that saw no key is 0. The statistics
 // come a split to a lane, the accumulators a split to a load, eight (R = 4) or four in flight; the first of
 // both, and Pi_V's operands, are asked for before anything is known of the sequence: what bounds
-// these few rows is one round trip after another.
+// these few rows is one round trip after another: 6 us for 256 rows, 18 us for 16,384 of three
+// splits (two round trips and the product for each of 1,024 work-groups, of which 512 run at a time).
 template <int D, int R>
 __global__ __launch_bounds__(1024) void tree_merge_kernel(TreeMergeArgs a) {
   constexpr int XS = D + 4, LD = D < 64 ? D : 64, VEC = D / LD;  // lanes a split, dims a lane

@@ -6,6 +6,7 @@ likely alternatives. It scores what an engine generates (``Request.top_logprobs`
 drafted tokens of a speculative step. There is no host fallback."""
 from __future__ import annotations
 
+import functools
 from dataclasses import dataclass
 
 import torch
@@ -24,6 +25,11 @@ class TokenLogprobs:
     entropy: torch.Tensor               # fp32, in nats
     top_logprobs: torch.Tensor | None   # (..., top) fp32, the most likely first; None for top = 0
     top_ids: torch.Tensor | None        # (..., top) int64; equal logits by the lowest index
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(rows: int, vocab: int, top: int) -> int:
+    return int(_lib.lib().wn_token_logprobs_workspace_bytes(rows, vocab, top))
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, top: int = 0) -> TokenLogprobs:
@@ -50,7 +56,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
         if tokens.shape != rows or tokens.dtype not in (torch.int64, torch.int32) or tokens.device != logits.device:
             raise UnsupportedLayout(f"tokens must be {tuple(rows)} int64 on {logits.device}, got "
                                     f"{tuple(tokens.shape)} {tokens.dtype} on {tokens.device}")
-        tokens = tokens.to(torch.int64).contiguous()
+        if tokens.dtype != torch.int64 or not tokens.is_contiguous():
+            tokens = tokens.to(torch.int64).contiguous()
     N = rows.numel()
     dev = logits.device
     new = torch.empty((2 if tokens is not None else 1, *rows), dtype=torch.float32, device=dev)
@@ -62,7 +69,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
         return result
     st = logits.stride()
     outer, inner, n_inner = (st[0], st[1], rows[1]) if len(rows) == 2 else (0, st[0] if rows else 0, N)
-    need = int(_lib.lib().wn_token_logprobs_workspace_bytes(N, V, top))
+    need = _workspace_bytes(N, V, top)
     workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     with _lib.on(dev):
         _lib.call("wn_token_logprobs", _lib.ptr(logits), _lib.DTYPE_CODE[logits.dtype], outer, inner, n_inner,
