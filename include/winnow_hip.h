@@ -453,6 +453,13 @@ int wn_positions_in_range(const int32_t* start, int lengths, int n, const int32_
 /* 1 if every parents[b, i] is -1 or in 0 .. i - 1, else 0. Host memory. */
 int wn_parents_in_order(const int32_t* parents, int64_t parents_stride_b, int B, int T);
 
+/* The three host steps of a wn_tree_attention call at once, from host memory: 1 if the lengths' positions
+ * are in range (as wn_positions_in_range), the parents in order and plan[0 .. 2] holds wn_tree_plan's
+ * num_splits, span and parts for max_pages; else 0, and each step says what is wrong. */
+int wn_tree_prepare(const int32_t* lens, const int32_t* page_table, int64_t table_stride_b, int table_pages,
+                    const int32_t* parents, int64_t parents_stride_b, int B, int Hq, int Hkv, int T, int D, int S,
+                    int bw_k, int bw_v, int exact, int num_pages, int max_pages, int* plan);
+
 /* Keeps the accepted branch of a tree: for i < counts[b] (clipped to [0, A]) the row of node
  * path[b, i], position start_pos[b] + path[b, i], moves to position start_pos[b] + i, in every
  * layer and kv head, K and V, and lengths[b] = start_pos[b] + counts[b]. Every source is read

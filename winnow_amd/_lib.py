@@ -169,6 +169,8 @@ SIGNATURES = {
         _c_f, _c_i, _c_i, _c_i, _c_i,               # scale, exact, num_splits, span, parts
         _c_p, _c_p, _c_p]),                         # stream, ev_begin, ev_end
     "wn_positions_in_range": (_c_i, [_c_p, _c_i, _c_i, _c_p, _c_i64, _c_i, _c_i, _c_i, _c_i]),
+    "wn_tree_prepare": (_c_i, [_c_p, _c_p, _c_i64, _c_i, _c_p, _c_i64, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i,
+                               _c_i, ctypes.POINTER(_c_i)]),
     "wn_parents_in_order": (_c_i, [_c_p, _c_i64, _c_i, _c_i]),
     "wn_commit_kv": (_c_i, [
         _c_p, _c_i64, _c_i64, _c_i64, _c_i,         # k pages, strides (layer, page, head), row bytes
@@ -291,15 +293,16 @@ def on(device: torch.device):
     return _here if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
-def _host_int32(t: torch.Tensor) -> bool:
-    return t.dtype is torch.int32 and t.device.type == "cpu" and (t.shape[-1] <= 1 or t.stride(-1) == 1)
+def host_int32(t: torch.Tensor) -> bool:
+    """An int32 tensor in host memory with a contiguous last axis."""
+    return t.is_cpu and t.dtype is torch.int32 and (t.shape[-1] <= 1 or t.stride(-1) == 1)
 
 
 def positions_in_range(start: torch.Tensor, table: torch.Tensor, n: int | None, num_pages: int, page_size: int) -> bool:
     """Whether the loaded library finds positions start[b] .. start[b] + n - 1 (n None: 0 .. start[b] - 1)
     inside row b of the table and on pages of the pool (``wn_positions_in_range``, int32 host tensors).
     False also where it cannot say: the caller then looks for itself, and names the sequence."""
-    if _lib is None or table.dim() != 2 or start.shape != table.shape[:1] or not (_host_int32(start) and _host_int32(table)):
+    if _lib is None or table.dim() != 2 or start.shape != table.shape[:1] or not (host_int32(start) and host_int32(table)):
         return False
     B, width = table.shape
     return bool(_lib.wn_positions_in_range(start.data_ptr(), n is None, n or 0, table.data_ptr(), table.stride(0),
@@ -308,7 +311,7 @@ def positions_in_range(start: torch.Tensor, table: torch.Tensor, n: int | None, 
 
 def parents_in_order(parents: torch.Tensor) -> bool:
     """Whether the loaded library finds every parent -1 or an earlier node (``wn_parents_in_order``)."""
-    if _lib is None or parents.dim() != 2 or not _host_int32(parents):
+    if _lib is None or parents.dim() != 2 or not host_int32(parents):
         return False
     B, T = parents.shape
     return bool(_lib.wn_parents_in_order(parents.data_ptr(), parents.stride(0), B, T))
@@ -322,4 +325,4 @@ def stream_of(device: torch.device):
 
 
 def is_hip(t: torch.Tensor) -> bool:
-    return t.device.type == "cuda" and torch.version.hip is not None
+    return t.is_cuda and torch.version.hip is not None

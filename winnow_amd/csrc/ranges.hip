@@ -27,3 +27,11 @@ extern "C" int wn_parents_in_order(const int32_t* parents, int64_t parents_strid
     }
   return 1;
 }
+
+extern "C" int wn_tree_prepare(const int32_t* lens, const int32_t* page_table, int64_t table_stride_b, int table_pages,
+                               const int32_t* parents, int64_t parents_stride_b, int B, int Hq, int Hkv, int T, int D, int S,
+                               int bw_k, int bw_v, int exact, int num_pages, int max_pages, int* plan) {
+  return plan && wn_positions_in_range(lens, 1, 0, page_table, table_stride_b, B, table_pages, num_pages, S) &&
+         wn_parents_in_order(parents, parents_stride_b, B, T) &&
+         wn_tree_plan(B, Hq, Hkv, T, D, S, bw_k, bw_v, exact, max_pages, lens, plan, plan + 1, plan + 2) == 0;
+}

@@ -593,6 +593,23 @@ def tree_plan_for(q: torch.Tensor, kv: PackedKV, exact: bool, *, read_lens: bool
     return ns.value, span.value, parts.value
 
 
+def _tree_prepare(q: torch.Tensor, kv: PackedKV, parents: torch.Tensor | None, exact: bool):
+    """The range checks and the plan in one call where host mirrors hold all of it (``wn_tree_prepare``);
+    None where they do not, or something is out of range."""
+    lens, table = kv.seq_lens_host, kv.page_table_host
+    B, Hq, T, D = q.shape
+    if lens is None or table is None or parents is None or lens.shape != (B,) or table.dim() != 2 or table.shape[0] != B \
+            or parents.shape != (B, T) or not (_lib.host_int32(lens) and _lib.host_int32(table) and _lib.host_int32(parents)):
+        return None
+    P, Hkv, S, _ = kv.k_pages.shape
+    plan = (ctypes.c_int * 3)()
+    with _lib.on(q.device):
+        ok = _lib.lib().wn_tree_prepare(lens.data_ptr(), table.data_ptr(), table.stride(0), table.shape[1], parents.data_ptr(),
+                                        parents.stride(0), B, Hq, Hkv, T, D, S, kv.k_quant.bit_width, kv.v_quant.bit_width,
+                                        exact, P, kv.page_table.shape[1], plan)
+    return tuple(plan) if ok else None
+
+
 def packed_tree_attention(q: torch.Tensor, kv: PackedKV, scale: float, parents: torch.Tensor, *,
                           allow_tf32: bool = False, num_splits: int | None = None,
                           out_dtype: torch.dtype | None = None, workspace: torch.Tensor | None = None,
@@ -619,22 +636,27 @@ def packed_tree_attention(q: torch.Tensor, kv: PackedKV, scale: float, parents: 
     Raises ``UnsupportedLayout`` before any launch for what ``check_contract`` and
     ``check_tree`` reject; ``check_ranges`` covers lengths, page ids and parents, read from
     ``parents_host`` and the handle's host mirrors when given, else copied to the host."""
-    check_contract(q, kv, check_ranges=check_ranges)
+    check_contract(q, kv, check_ranges=False)
     check_tree(q, kv, parents)
-    if check_ranges:
-        check_parents(parents if parents_host is None else parents_host)
-        if parents_host is not None and parents_host.shape != parents.shape:
-            raise UnsupportedLayout(f"parents_host is {tuple(parents_host.shape)}, parents {tuple(parents.shape)}")
     B, Hq, T, D = q.shape
-    Hkv = kv.num_kv_heads
     out_dtype = out_dtype or q.dtype
     if out_dtype not in _lib.DTYPE_CODE:
         raise UnsupportedLayout(f"output dtype {out_dtype} is not supported")
     exact = tree_exact(q, out_dtype, allow_tf32)
+    plan = _tree_prepare(q, kv, parents_host, exact) if check_ranges else None
+    if check_ranges and plan is None:
+        check_contract(q, kv)
+        check_parents(parents if parents_host is None else parents_host)
+        if parents_host is not None and parents_host.shape != parents.shape:
+            raise UnsupportedLayout(f"parents_host is {tuple(parents_host.shape)}, parents {tuple(parents.shape)}")
+    Hkv = kv.num_kv_heads
     out = torch.empty(B, Hq, T, D, dtype=out_dtype, device=q.device)
     if B == 0:
         return out
-    ns, span, parts = (int(num_splits), 64, B * int(num_splits)) if num_splits else tree_plan_for(q, kv, exact, read_lens=check_ranges)
+    if num_splits:
+        ns, span, parts = int(num_splits), 64, B * int(num_splits)
+    else:
+        ns, span, parts = plan or tree_plan_for(q, kv, exact, read_lens=check_ranges)
     need = tree_workspace_bytes(B, Hq, Hkv, T, D, ns)
     if need < 0:
         raise UnsupportedLayout(f"bad tree sizes B={B} Hq={Hq} Hkv={Hkv} T={T} splits={ns}")

@@ -285,11 +285,14 @@ def append_kv(k: torch.Tensor, v: torch.Tensor | None, k_tq, v_tq,
     plan.launch(bound, timing_events)
 
 
+COMMIT_DTYPES = (torch.uint8, *pa.DENSE_PAGE_DTYPES)
+
+
 def _check_commit_side(name: str, pages: torch.Tensor, norms, lead) -> None:
     shape, st = pages.shape, pages.stride()
     if len(shape) not in (4, 5) or shape[:-1] != lead:
         raise pa.UnsupportedLayout(f"commit: {name} pages must be ([layers,] P, Hkv, S, row), got {tuple(shape)}")
-    if pages.dtype not in (torch.uint8, *pa.DENSE_PAGE_DTYPES) or (pages.dtype == torch.uint8) != (norms is not None):
+    if pages.dtype not in COMMIT_DTYPES or (pages.dtype == torch.uint8) != (norms is not None):
         raise pa.UnsupportedLayout(f"commit: {name} pages are uint8 with norms, or fp32/fp16/bf16 without")
     if st[-1] != 1 or st[-2] != shape[-1]:
         raise pa.UnsupportedLayout("commit: pages need contiguous (S, row) blocks")
