@@ -11,18 +11,21 @@ C ABI in ``include/winnow_hip.h`` (``libwinnow_hip.so``):
 
 Around them: ``cache.TQPackedCache`` (the contiguous packed cache, imported on its
 own: it pulls in transformers), ``packed_backend`` (the HF attention backend),
-``engine`` (continuous batching) and ``kernel.tq_dequant`` (fused dequantization).
+``engine`` (continuous batching), ``kernel.tq_dequant`` (fused dequantization) and, for
+speculative decoding, ``packed_attention.packed_tree_attention``, ``packed_backend.commit_kv``
+and ``logprobs.token_logprobs``.
 """
 from winnow_amd.packed_attention import (  # noqa: F401
     DenseKV, PackedKV, Quantizer, UnsupportedLayout, check_contract, default_scale,
-    packed_decode_attention,
+    packed_decode_attention, packed_tree_attention,
 )
+from winnow_amd.logprobs import TokenLogprobs, token_logprobs  # noqa: F401
 from winnow_amd.packing import SUPPORTED, pack, packed_bytes, unpack  # noqa: F401
 from winnow_amd.page_pool import PagePool, PageRef, PoolExhausted, StalePage  # noqa: F401
 from winnow_amd.quantizer import TurboQuantMSE, get_quantizer  # noqa: F401
 
 __all__ = [
     "DenseKV", "PackedKV", "Quantizer", "UnsupportedLayout", "check_contract", "default_scale",
-    "packed_decode_attention", "SUPPORTED", "pack", "packed_bytes", "unpack", "PagePool", "PageRef",
-    "PoolExhausted", "StalePage", "TurboQuantMSE", "get_quantizer",
+    "packed_decode_attention", "packed_tree_attention", "SUPPORTED", "pack", "packed_bytes", "unpack", "PagePool", "PageRef",
+    "PoolExhausted", "StalePage", "TokenLogprobs", "TurboQuantMSE", "get_quantizer", "token_logprobs",
 ]
