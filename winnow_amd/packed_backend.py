@@ -288,23 +288,29 @@ def append_kv(k: torch.Tensor, v: torch.Tensor | None, k_tq, v_tq,
 COMMIT_DTYPES = (torch.uint8, *pa.DENSE_PAGE_DTYPES)
 
 
-def _check_commit_side(name: str, pages: torch.Tensor, norms, lead) -> None:
-    shape, st = pages.shape, pages.stride()
+def _commit_side(name: str, pages: torch.Tensor, norms, lead) -> tuple:
+    """One side's operands of ``wn_commit_kv``, checked: the pages' address, layer, page and head
+    strides in bytes and bytes of a row; the norms' address and strides in elements."""
+    shape, st, dtype = pages.shape, pages.stride(), pages.dtype
     if len(shape) not in (4, 5) or shape[:-1] != lead:
         raise pa.UnsupportedLayout(f"commit: {name} pages must be ([layers,] P, Hkv, S, row), got {tuple(shape)}")
-    if pages.dtype not in COMMIT_DTYPES or (pages.dtype == torch.uint8) != (norms is not None):
+    if dtype not in COMMIT_DTYPES or (dtype == torch.uint8) != (norms is not None):
         raise pa.UnsupportedLayout(f"commit: {name} pages are uint8 with norms, or fp32/fp16/bf16 without")
-    if st[-1] != 1 or st[-2] != shape[-1]:
+    row = shape[-1]
+    if st[-1] != 1 or st[-2] != row:
         raise pa.UnsupportedLayout("commit: pages need contiguous (S, row) blocks")
-    nst = (1,)
+    layered, size = len(shape) == 5, dtype.itemsize
+    at, nst = (None, 0, 0, 0), (1,)
     if norms is not None:
         nst = norms.stride()
         if norms.dtype != torch.float16 or norms.shape != lead or nst[-1] != 1:
             raise pa.UnsupportedLayout(f"commit: {name} norms must be fp16 of the pages' leading shape, slots contiguous")
+        at = (norms.data_ptr(), nst[0] if layered else 0, nst[-3], nst[-2])
     if 0 in st or 0 in nst:  # an axis of one entry may have any stride
         for t in (pages, norms):
             if t is not None and any(n > 1 and s == 0 for n, s in zip(t.shape[:-1], t.stride())):
                 raise pa.UnsupportedLayout(f"commit: {name} is written in place and may not be expanded")
+    return (pages.data_ptr(), st[0] * size if layered else 0, st[-4] * size, st[-3] * size, row * size), at
 
 
 def commit_kv(k_pages: torch.Tensor, v_pages: torch.Tensor, k_norms: torch.Tensor | None,
@@ -329,8 +335,8 @@ def commit_kv(k_pages: torch.Tensor, v_pages: torch.Tensor, k_norms: torch.Tenso
     pages outside the pool, read as in ``append_kv``."""
     packed = k_pages.dtype == torch.uint8
     lead = k_pages.shape[:-1]
-    for name, pages, norms in (("K", k_pages, k_norms), ("V", v_pages, v_norms)):
-        _check_commit_side(name, pages, norms, lead)
+    k_at, kn_at = _commit_side("K", k_pages, k_norms, lead)
+    v_at, vn_at = _commit_side("V", v_pages, v_norms, lead)
     if v_pages.dtype != k_pages.dtype:
         raise pa.UnsupportedLayout(f"commit: K pages are {k_pages.dtype}, V pages {v_pages.dtype}")
     dev = k_pages.device
@@ -358,25 +364,10 @@ def commit_kv(k_pages: torch.Tensor, v_pages: torch.Tensor, k_norms: torch.Tenso
                             page_table_host if page_table_host is not None else page_table.cpu(), nodes, P, S)
     lengths = torch.empty(B, dtype=torch.int32, device=dev)
     with _lib.on(dev):
-        _lib.call("wn_commit_kv", *_commit_pages(k_pages), *_commit_pages(v_pages), *_commit_norms(k_norms),
-                  *_commit_norms(v_norms), _lib.ptr(page_table), page_table.stride(0), _lib.ptr(start_pos),
-                  _lib.ptr(path), path.stride(0), _lib.ptr(counts), _lib.ptr(lengths), layers, B, Hkv, S, A, nodes, P,
-                  width, _lib.stream_of(dev))
+        _lib.call("wn_commit_kv", *k_at, *v_at, *kn_at, *vn_at, page_table.data_ptr(), page_table.stride(0),
+                  start_pos.data_ptr(), path.data_ptr(), path.stride(0), counts.data_ptr(), lengths.data_ptr(),
+                  layers, B, Hkv, S, A, nodes, P, width, _lib.stream_of(dev))
     return lengths
-
-
-def _commit_pages(t: torch.Tensor) -> tuple:
-    """Address, layer, page and head strides in bytes, bytes of a row."""
-    size = t.element_size()
-    st = t.stride() if t.dim() == 5 else (0, *t.stride())
-    return _lib.ptr(t), st[0] * size, st[1] * size, st[2] * size, t.shape[-1] * size
-
-
-def _commit_norms(t: torch.Tensor | None) -> tuple:
-    if t is None:
-        return None, 0, 0, 0
-    st = t.stride() if t.dim() == 4 else (0, *t.stride())
-    return _lib.ptr(t), st[0], st[1], st[2]
 
 
 def _append_dense_rows(src: torch.Tensor, pages: torch.Tensor, meta: PageTable) -> None:
