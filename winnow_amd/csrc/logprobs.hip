@@ -24,9 +24,10 @@
 //   - later the waves publish their ceil(top / 4)-th best: again the least of the four;
 //   - where many lanes of a batch have a hit all the same (rising logits) it goes up to the
 //     top-th largest of the lanes' maxima before any is inserted.
-// 1,024 rows of 128,256 bf16: 46 us without alternatives (5.8 TB/s), 76 us with 20; 208 rows of
-// 50,257 fp16, one alternative: 13.6 us and 4 for the second launch; one row of 128,256 fp32, five:
-// 8.5 and 4, latency.
+// 1,024 rows of 128,256 bf16: 46 us without alternatives (5.8 TB/s; 37 us of them are the vector
+// instructions, nine an element with an exponential), 76 us with 20, whose insertions add to the
+// instructions; 208 rows of 50,257 fp16, one alternative: 13.6 us and 4 for the second launch; one
+// row of 128,256 fp32, five: 8.5 and 4, latency.
 #include <algorithm>
 
 #include "wn_common.h"
@@ -270,7 +271,7 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LpArgs a) {
       hit &= __ballot(live && lp_key(top, i) > list.last) & ~(hit & -hit);
     }
   };
-  uint32_t p = uint32_t(body + wave * STEP);
+  uint32_t p = uint32_t(body) + uint32_t(wave) * STEP;
   load(p);
   const int rank = (a.top + kLpWaves - 1) / kLpWaves;
   uint64_t told = 0;
