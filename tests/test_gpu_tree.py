@@ -341,3 +341,37 @@ def test_more_rows_than_a_block(D, bwk, bwv, Hq, Hkv, T):
     _check(got, q, kv, parents, scale, torch.float32)
     one = _pa().packed_tree_attention(q.to(DEV), d, scale, parents.to(DEV), allow_tf32=True)
     _check(one, q, kv, parents, scale, torch.float32, single=True)
+
+
+def test_a_workspace_that_is_no_buffer_is_refused():
+    pa = _pa()
+    q, kv, parents = _case(21, (50,), 8, 2, 128, 5, 4, 4)
+    d = to_device(kv, DEV)
+    need = pa.tree_workspace_bytes(1, 8, 2, 5, 128, 2)
+    one = torch.zeros(1, dtype=torch.uint8, device=DEV)
+    for ws in (one.expand(need), torch.zeros(2 * need, dtype=torch.uint8, device=DEV)[::2]):
+        with pytest.raises(pa.UnsupportedLayout, match="workspace"):
+            pa.packed_tree_attention(q.to(DEV), d, 0.1, parents.to(DEV), num_splits=2, workspace=ws)
+
+
+def test_host_mirrors_are_checked_and_need_not_be_int32():
+    """The mirrors in other types and strides, and out of range: as without them."""
+    pa = _pa()
+    q, kv, parents = _case(22, (50, 300), 8, 2, 128, 5, 4, 4)
+    d, dq, dp = to_device(kv, DEV), q.to(DEV), parents.to(DEV)
+    want = pa.packed_tree_attention(dq, d, 0.1, dp)
+    lens, table = kv.seq_lens.to(torch.int32), kv.page_table.to(torch.int32)
+    wide = torch.stack([table, table], -1).transpose(1, 2)[:, 0]
+    for h_lens, h_table, h_parents in ((lens, table, parents), (lens.long(), table.long(), parents.long()),
+                                       (lens, wide, parents.t().contiguous().t())):
+        d.seq_lens_host, d.page_table_host = h_lens, h_table
+        assert torch.equal(pa.packed_tree_attention(dq, d, 0.1, dp, parents_host=h_parents), want)
+    far, low = lens.clone(), table.clone()
+    far[1] = table.shape[1] * 16 + 1
+    low[0, 0] = -1
+    late = parents.clone()
+    late[1, 2] = 2
+    for h_lens, h_table, h_parents in ((far, table, parents), (lens, low, parents), (lens, table, late), (lens, table, parents[:1])):
+        d.seq_lens_host, d.page_table_host = h_lens, h_table
+        with pytest.raises(pa.UnsupportedLayout):
+            pa.packed_tree_attention(dq, d, 0.1, dp, parents_host=h_parents)

@@ -593,20 +593,21 @@ def tree_plan_for(q: torch.Tensor, kv: PackedKV, exact: bool, *, read_lens: bool
     return ns.value, span.value, parts.value
 
 
-def _tree_prepare(q: torch.Tensor, kv: PackedKV, parents: torch.Tensor | None, exact: bool):
+def _tree_prepare(kv: PackedKV, parents: torch.Tensor | None, sizes: tuple, exact: bool, device: torch.device):
     """The range checks and the plan in one call where host mirrors hold all of it (``wn_tree_prepare``);
-    None where they do not, or something is out of range."""
+    None where they do not, or something is out of range. sizes: B, Hq, Hkv, T, D, S, both widths."""
     lens, table = kv.seq_lens_host, kv.page_table_host
-    B, Hq, T, D = q.shape
-    if lens is None or table is None or parents is None or lens.shape != (B,) or table.dim() != 2 or table.shape[0] != B \
-            or parents.shape != (B, T) or not (_lib.host_int32(lens) and _lib.host_int32(table) and _lib.host_int32(parents)):
+    if lens is None or table is None or parents is None or not (lens.is_cpu and table.is_cpu and parents.is_cpu) \
+            or not lens.dtype == table.dtype == parents.dtype == torch.int32:
         return None
-    P, Hkv, S, _ = kv.k_pages.shape
+    B, T, shape, st, pst = sizes[0], sizes[3], table.shape, table.stride(), parents.stride()
+    if lens.shape != (B,) or len(shape) != 2 or shape[0] != B or parents.shape != (B, T) or not lens.is_contiguous() \
+            or (shape[1] > 1 and st[1] != 1) or (T > 1 and pst[1] != 1):
+        return None
     plan = (ctypes.c_int * 3)()
-    with _lib.on(q.device):
-        ok = _lib.lib().wn_tree_prepare(lens.data_ptr(), table.data_ptr(), table.stride(0), table.shape[1], parents.data_ptr(),
-                                        parents.stride(0), B, Hq, Hkv, T, D, S, kv.k_quant.bit_width, kv.v_quant.bit_width,
-                                        exact, P, kv.page_table.shape[1], plan)
+    with _lib.on(device):
+        ok = _lib.lib().wn_tree_prepare(lens.data_ptr(), table.data_ptr(), st[0], shape[1], parents.data_ptr(), pst[0],
+                                        *sizes, exact, kv.k_pages.shape[0], kv.page_table.shape[1], plan)
     return tuple(plan) if ok else None
 
 
@@ -643,13 +644,15 @@ def packed_tree_attention(q: torch.Tensor, kv: PackedKV, scale: float, parents: 
     if out_dtype not in _lib.DTYPE_CODE:
         raise UnsupportedLayout(f"output dtype {out_dtype} is not supported")
     exact = tree_exact(q, out_dtype, allow_tf32)
-    plan = _tree_prepare(q, kv, parents_host, exact) if check_ranges else None
+    kq, vq = kv.k_quant, kv.v_quant
+    P, Hkv, S, _ = kv.k_pages.shape
+    sizes = (B, Hq, Hkv, T, D, S, kq.bit_width, vq.bit_width)
+    plan = _tree_prepare(kv, parents_host, sizes, exact, q.device) if check_ranges else None
     if check_ranges and plan is None:
         check_contract(q, kv)
         check_parents(parents if parents_host is None else parents_host)
         if parents_host is not None and parents_host.shape != parents.shape:
             raise UnsupportedLayout(f"parents_host is {tuple(parents_host.shape)}, parents {tuple(parents.shape)}")
-    Hkv = kv.num_kv_heads
     out = torch.empty(B, Hq, T, D, dtype=out_dtype, device=q.device)
     if B == 0:
         return out
@@ -660,12 +663,15 @@ def packed_tree_attention(q: torch.Tensor, kv: PackedKV, scale: float, parents: 
     need = tree_workspace_bytes(B, Hq, Hkv, T, D, ns)
     if need < 0:
         raise UnsupportedLayout(f"bad tree sizes B={B} Hq={Hq} Hkv={Hkv} T={T} splits={ns}")
+    room = need
     if workspace is None:
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    elif workspace.numel() * workspace.element_size() < need or workspace.device != q.device:
-        raise UnsupportedLayout(f"workspace needs {need} bytes on {q.device}")
+    else:
+        room = workspace.numel() * workspace.element_size()
+        if room < need or workspace.device != q.device or not workspace.is_contiguous():
+            raise UnsupportedLayout(f"workspace needs {need} contiguous bytes on {q.device}")
     ev0, ev1 = timing_events or (None, None)
-    kq, vq, table = kv.k_quant, kv.v_quant, kv.page_table
+    table = kv.page_table
     kp, vp, kn, vn = kv.k_pages.stride(), kv.v_pages.stride(), kv.k_norms.stride(), kv.v_norms.stride()
     with _lib.on(q.device):
         _lib.call("wn_tree_attention", q.data_ptr(), _lib.DTYPE_CODE[q.dtype], *q.stride()[:3],
@@ -673,9 +679,8 @@ def packed_tree_attention(q: torch.Tensor, kv: PackedKV, scale: float, parents: 
                   kv.k_pages.data_ptr(), kp[0], kp[1], kv.v_pages.data_ptr(), vp[0], vp[1],
                   kv.k_norms.data_ptr(), kn[0], kn[1], kv.v_norms.data_ptr(), vn[0], vn[1],
                   table.data_ptr(), table.stride(0), kv.seq_lens.data_ptr(), parents.data_ptr(), parents.stride(0),
-                  out.data_ptr(), _lib.DTYPE_CODE[out_dtype], workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-                  B, Hq, Hkv, T, D, kv.page_size, kq.bit_width, vq.bit_width, kv.k_pages.shape[0],
-                  table.shape[1], float(scale), int(exact), ns, span, parts, _lib.stream_of(q.device), ev0, ev1)
+                  out.data_ptr(), _lib.DTYPE_CODE[out_dtype], workspace.data_ptr(), room,
+                  *sizes, P, table.shape[1], float(scale), int(exact), ns, span, parts, _lib.stream_of(q.device), ev0, ev1)
     return out
 
 
