@@ -34,11 +34,11 @@
 // nodes, 4 and 6 bits, two terms: 605 us, 0.73 PFLOP/s of fp16 products; one sequence of 300, 32
 // heads over 8, 8 nodes: 9.5 us, of which a chunk takes 2.
 //
-// Precision. EX = true: every factor is a sum of two fp16 terms (22 bits), and each product
-// the three larger of their four products (what is left out is below 2^-22 of a term):
-// fp32 accuracy for fp16 and fp32 results. EX = false: one fp16 term per factor (rounded to
-// nearest, off by 2^-11 of it at most, three bits finer than a bf16 result's own rounding),
-// a third of the matrix work. Sums, maxima and partials are fp32 either way.
+// Precision. EX = true, the callers' default for every type: every factor is a sum of two fp16
+// terms (22 bits), and each product the three larger of their four products (what is left out is
+// below 2^-22 of a term): fp32 accuracy. EX = false, where the caller allows TF32-class products:
+// one fp16 term per factor (rounded to nearest, off by 2^-11 of it at most, the bits of a TF32
+// factor), a third of the matrix work. Sums, maxima and partials are fp32 either way.
 #pragma once
 
 #include <cstdint>

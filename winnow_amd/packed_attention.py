@@ -569,13 +569,6 @@ def tree_workspace_bytes(batch: int, num_q_heads: int, num_kv_heads: int, nodes:
     return int(_lib.lib().wn_tree_workspace_bytes(batch, num_q_heads, num_kv_heads, nodes, head_dim, num_splits))
 
 
-def tree_exact(q: torch.Tensor, out_dtype: torch.dtype, allow_tf32: bool = False) -> bool:
-    """Whether ``packed_tree_attention`` takes two fp16 terms per factor (fp32 accuracy): unless
-    the result is bf16 of a bf16 query, whose own rounding is eight times coarser than a single
-    term's, or the caller allows TF32-class products."""
-    return not (allow_tf32 or q.dtype == out_dtype == torch.bfloat16)
-
-
 def tree_plan_for(q: torch.Tensor, kv: PackedKV, exact: bool, *, read_lens: bool = True) -> tuple[int, int, int]:
     """(num_splits, span, parts) of the tree attention for this query and handle (wn_tree_plan), from the
     lengths' host mirror, or, without one, a host copy (``read_lens``) or the width of the table."""
@@ -628,8 +621,8 @@ def packed_tree_attention(q: torch.Tensor, kv: PackedKV, scale: float, parents: 
 
     A chain (``parents[i] = i - 1``) is the causal mask of ``packed_prefill_attention``.
     Every head_dim, width pair, n_rep and page size of ``packed_decode_attention`` is
-    served. Products have fp32 accuracy, or, where the query and the result are bf16 or
-    ``allow_tf32`` is given, TF32-class accuracy (single fp16 operands, fp32 accumulation).
+    served. Products have fp32 accuracy whatever the query's type, or, where ``allow_tf32`` is
+    given, TF32-class accuracy (single fp16 operands, fp32 accumulation), as in the decode.
     ``num_splits`` replaces the library's split count, ``out_dtype`` the result's type,
     ``workspace`` is a caller-owned uint8 buffer of at least ``tree_workspace_bytes``,
     ``timing_events`` a pair of raw ``hipEvent_t`` handles recorded around the scan.
@@ -643,7 +636,7 @@ def packed_tree_attention(q: torch.Tensor, kv: PackedKV, scale: float, parents: 
     out_dtype = out_dtype or q.dtype
     if out_dtype not in _lib.DTYPE_CODE:
         raise UnsupportedLayout(f"output dtype {out_dtype} is not supported")
-    exact = tree_exact(q, out_dtype, allow_tf32)
+    exact = not allow_tf32
     kq, vq = kv.k_quant, kv.v_quant
     P, Hkv, S, _ = kv.k_pages.shape
     sizes = (B, Hq, Hkv, T, D, S, kq.bit_width, vq.bit_width)
