@@ -193,10 +193,6 @@ __global__ __launch_bounds__(64 * RG * TG, 2) void tree_scan_kernel(TreeArgs a) 
     tree_stage_table<C::NTHR>(a.cb_k, bwk, tabk, tid);
     tree_stage_table<C::NTHR>(a.cb_v, bwv, tabv, tid);
   }
-  if constexpr (D < G::DP) {  // the padded dims of the K tile stay zero
-    for (int i = tid; i < C::PL * G::KT / 4; i += C::NTHR) reinterpret_cast<uint32_t*>(lds + C::k_off)[i] = 0;
-  }
-
   // Unit (split of the batch, kv head), and its row block of ROWS. Work-groups go to the eight XCDs
   // in turn: a unit's row blocks, which read the same rows, share one, and units go round. A grid of
   // fewer units than there are (lengths that have grown since it was planned) goes over them again.
@@ -204,6 +200,16 @@ __global__ __launch_bounds__(64 * RG * TG, 2) void tree_scan_kernel(TreeArgs a) 
   for (int u = (int(blockIdx.x >> 3) / a.ncg) * 8 + int(blockIdx.x & 7);; u += step) {
     int b, s;
     if (!tree_split(a, lane, u / a.Hkv, &b, &s)) break;  // the whole work-group
+    if constexpr (D < G::DP) {
+      // the K tile's padded dims are zero, for each unit again: what the one before handed over at its
+      // end (below) lies in the tiles' place, and as fp16 it may be NaN, which the query's zeros keep
+      constexpr int PAD = (G::DP - D) / 2;  // words of a row
+      for (int i = tid; i < C::PL * G::CH * PAD; i += C::NTHR) {
+        const int row = i / PAD;
+        char* at = lds + C::k_off + row / G::CH * G::KT + row % G::CH * G::KROW;
+        reinterpret_cast<uint32_t*>(at + 2 * D)[i % PAD] = 0;
+      }
+    }
     const int kvh = u % a.Hkv;
     const int L = min(max(const_view(a.seq_lens)[b], 0), a.max_pages << a.log2S);
     const int span = tree_span(L, a.nsplit, a.span);
