@@ -403,9 +403,9 @@ int wn_dense_decode_attention(
 /* Splits of wn_tree_attention for this shape on the current device: splits of *span tokens (a
  * multiple of 64), *num_splits of them for the longest sequence and *parts in all, so that they
  * fill the device in few rounds. lens: B lengths in host memory (drafted tokens included), or NULL
- * (every sequence fills its table row). Any num_splits 1 .. 4096, span and parts >= 1 are valid for
- * any lengths: a sequence that num_splits spans do not cover takes longer ones, and work-groups
- * for fewer parts than there are take several. */
+ * (every sequence fills its table row). Any num_splits 1 .. 4096, any span that is a multiple of 64
+ * and any parts >= 1 are valid for any lengths: a sequence that num_splits spans do not cover takes
+ * longer ones, and work-groups for fewer parts than there are take several. */
 int wn_tree_plan(int B, int Hq, int Hkv, int T, int D, int S, int bw_k, int bw_v, int exact, int max_pages,
                  const int32_t* lens, int* num_splits, int* span, int* parts);
 

@@ -72,7 +72,7 @@ __global__ __launch_bounds__(64 * WPB) __attribute__((amdgpu_waves_per_eu(WPB / 
   const int hist = L - a.T;  // position of node 0
   const int span = tree_span(L, a.nsplit, a.span);
   {
-    const int t_lo = s * span, t_hi = min(L, t_lo + span), n = (t_hi - t_lo + 63) >> 6, col_hi = (t_hi - 1) >> a.log2S;
+    const int t_lo = s * span, t_hi = tree_end(L, span, s), n = (t_hi - t_lo + 63) >> 6, col_hi = (t_hi - 1) >> a.log2S;
     const int32_t* trow = a.table + int64_t(b) * a.tsb;
     const uint32_t last_page = uint32_t(a.num_pages - 1);
     auto tiles = [&](int c0) {

@@ -77,6 +77,14 @@ __host__ __device__ inline int tree_span(int L, int nsplit, int span) {
   return span > even ? span : even;
 }
 
+// Splits of a sequence of L, and where split s of them ends. A sequence may come as near to 2^31 as
+// 257 positions and a span too, so that their sum, or a whole last split, would pass it.
+__host__ __device__ inline int tree_count(int L, int span) { return L > 0 ? (L - 1) / span + 1 : 0; }
+__host__ __device__ inline int tree_end(int L, int span, int s) {
+  const int rest = L - s * span;
+  return rest < span ? L : s * span + span;
+}
+
 #ifdef __HIPCC__
 // Split j of the batch, its splits counted sequence after sequence: its sequence and place there.
 // False past the last one. Every lane of a wave takes part.
@@ -84,7 +92,7 @@ __device__ __forceinline__ bool tree_split(const TreeArgs& a, int lane, int j, i
   int before = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const int L = b0 + lane < a.B ? min(max(a.seq_lens[b0 + lane], 0), a.max_pages << a.log2S) : 0;
-    const int span = tree_span(L, a.nsplit, a.span), own = (L + span - 1) / span;
+    const int own = tree_count(L, tree_span(L, a.nsplit, a.span));
     int upto = own;  // of this lane's sequence and those before it
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {

@@ -213,7 +213,7 @@ __global__ __launch_bounds__(64 * RG * TG, 2) void tree_scan_kernel(TreeArgs a) 
     const int kvh = u % a.Hkv;
     const int L = min(max(const_view(a.seq_lens)[b], 0), a.max_pages << a.log2S);
     const int span = tree_span(L, a.nsplit, a.span);
-    const int ch_lo = s * (span / G::CH), ch_hi = (min(L, s * span + span) + G::CH - 1) / G::CH;
+    const int ch_lo = s * (span / G::CH), ch_hi = (tree_end(L, span, s) + G::CH - 1) / G::CH;
     const int hist = L - a.T;  // position of node 0
     const int rows = a.n_rep * a.T, r0 = cg * C::ROWS + rg * 16 * NCT;  // the wave's first row
     const int64_t row0 = (int64_t(b) * a.Hkv + kvh) * a.nrp + r0;
@@ -826,8 +826,8 @@ __global__ __launch_bounds__(1024) void tree_merge_kernel(TreeMergeArgs a) {
   pi.load(wave, lane, [&](int j, int kk) {
     return f32x4{a.pi_v[kk * D + j], a.pi_v[(kk + 1) * D + j], a.pi_v[(kk + 2) * D + j], a.pi_v[(kk + 3) * D + j]};
   });
-  const int L = min(max(a.seq_lens[unit / a.Hkv], 0), a.max_len), span = tree_span(L, a.nsplit, a.span);
-  const int live = (L + span - 1) / max(span, 1);  // splits that the sequence has: the others' partials are not its own
+  const int L = min(max(a.seq_lens[unit / a.Hkv], 0), a.max_len);
+  const int live = tree_count(L, tree_span(L, a.nsplit, a.span));  // splits that the sequence has: the others' partials are not its own
   float M = lane < live ? ml0.x : -INFINITY;
   for (int s = 64 + lane; s < live; s += 64) M = fmaxf(M, stats(s).x);
   M = wave_max(M);
