@@ -467,7 +467,10 @@ class PagedPackedCache:
         accepted nodes from a child of the last stored token down, each the next one's parent
         (empty: none). Their rows move to the positions right behind the history in one launch
         over every layer (``commit_kv``), the cache forgets the rest, and ``lengths`` are the
-        tokens kept. The next forward takes a new tree or none."""
+        tokens kept. The next forward takes a new tree or none.
+
+        A sequence whose pages have been released since the forward has nothing to keep: a path of
+        it raises ``StalePage`` before anything is moved (its pages may be another's by now)."""
         meta, pool = self.meta, self.pool
         if self.tree is None or meta is None or self.lengths != meta.seq_host.tolist():
             raise RuntimeError("commit follows a forward over a tree")
@@ -481,6 +484,7 @@ class PagedPackedCache:
                 if not 0 <= i < T or int(self.tree[b, i]) != parent:
                     raise ValueError(f"sequence {b}: {p} is not a branch of its tree from the root down")
                 parent = i
+        pool.still_held(self.owners, meta, [b for b, p in enumerate(paths) if p])
         A = max([1] + [len(p) for p in paths])
         host = torch.tensor([p + [0] * (A - len(p)) + [len(p)] for p in paths], dtype=torch.int32).reshape(B, A + 1)
         if B:

@@ -100,6 +100,8 @@ class PageTable:
     ``table_host`` (B, width) int32 (-1 padded), ``start_host`` (B,) the tokens stored
     before the forward, ``seq_host`` (B,) the lengths after it; ``table``, ``start``
     and ``seq`` are the device copies once ``to`` has run (the host ones until then).
+    ``gens`` (B, width) are the generations of the table's pages when it was made (None for
+    a table that the pool did not make).
     """
 
     table_host: torch.Tensor
@@ -109,6 +111,7 @@ class PageTable:
     table: torch.Tensor | None = None
     start: torch.Tensor | None = None
     seq: torch.Tensor | None = None
+    gens: np.ndarray | None = None
 
     def to(self, device) -> "PageTable":
         """Upload the three tensors with one copy (they are views of one int32 buffer)."""
@@ -295,8 +298,18 @@ class PagePool:
                 leases.append(lease)
             width = max([1] + [int(lz.pages.size) for lz in leases if lz is not None])
             table = np.full((len(leases), width), -1, np.int32)
+            gens = np.full(table.shape, -1, np.int64)
             for b, lz in enumerate(leases):
                 if lz is not None:
                     table[b, :lz.pages.size] = lz.pages
+                    gens[b, :lz.pages.size] = lz.gens
         start = torch.tensor(lengths, dtype=torch.int32)
-        return PageTable(torch.from_numpy(table), start, start + n_new, int(n_new))
+        return PageTable(torch.from_numpy(table), start, start + n_new, int(n_new), gens=gens)
+
+    def still_held(self, owners, meta: PageTable, rows) -> None:
+        """Raise ``StalePage`` unless each of the batch's ``rows`` still holds, under its owner and at
+        the generations of ``meta``, the pages that the forward over ``meta`` appended to."""
+        for b in rows:
+            lo, hi = int(meta.start_host[b]), int(meta.seq_host[b])
+            at = slice(lo // self.page_size, self.pages_for(hi))
+            self.validate(owners[b], [PageRef(int(p), int(g)) for p, g in zip(meta.table_host[b, at], meta.gens[b, at])])
