@@ -405,7 +405,9 @@ int wn_dense_decode_attention(
  * fill the device in few rounds. lens: B lengths in host memory (drafted tokens included), or NULL
  * (every sequence fills its table row). Any num_splits 1 .. 4096, any span that is a multiple of 64
  * and any parts >= 1 are valid for any lengths: a sequence that num_splits spans do not cover takes
- * longer ones, and work-groups for fewer parts than there are take several. */
+ * longer ones, and work-groups for fewer parts than there are take several. The plan is made for
+ * pages and norms that wn_prefill_attention would take, from base and strides; others, which the scan
+ * for long contexts cannot read, are served by the same plan. */
 int wn_tree_plan(int B, int Hq, int Hkv, int T, int D, int S, int bw_k, int bw_v, int exact, int max_pages,
                  const int32_t* lens, int* num_splits, int* span, int* parts);
 

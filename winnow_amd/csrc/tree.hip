@@ -25,21 +25,31 @@ TreeKernels pick_tree(int D, bool exact, int bw_k, int bw_v) {
   }
 }
 
-// Whether the row scan serves (head_dim 128, single-term products, 4 and 6-bit widths). `tokens`:
-// positions that the page table holds, over the batch and kv heads. A wave of it needs long splits
+// Whether the row scan serves (head_dim 128, single-term products, 4 and 6-bit widths, `wide`: rows and
+// norms laid out for its loads, see rows_wide). `tokens`: positions that the page table holds, over the
+// batch and kv heads (not the lengths: those of a captured call change between replays, and short
+// sequences behind a wide table pay what the figures for few tokens show). A wave of it needs long splits
 // (it starts with 128 KB of tables), and every 32 rows look codes up again, which the tile scan does
 // once per row block, by byte-pair tables if both sides have 4 bits. Whole calls, tile and row scan, us:
 //   4/4 bits, 32 rows:  256 k tokens 45 / 48, 512 k 60 / 56, 1 M 96 / 74
 //             64 rows:  256 k 59 / 60, 512 k 81 / 75, 1 M 122 / 101;  128 rows: 512 k 101 / 101
 //   4/6 bits, 32 rows:  64 k tokens 37 / 45, 128 k 46 / 43, 256 k 60 / 48, 1 M 148 / 79
 //             64 rows:  64 k 46 / 46, 128 k 62 / 53;  128 rows: 64 k 58 / 52, 1 M 277 / 184
-bool rows_serve(int D, bool exact, int bw_k, int bw_v, int64_t rows, int64_t tokens) {
-  if (D != 128 || exact || (bw_k != 4 && bw_k != 6) || (bw_v != 4 && bw_v != 6)) return false;
+bool rows_serve(int D, bool exact, bool wide, int bw_k, int bw_v, int64_t rows, int64_t tokens) {
+  if (D != 128 || exact || !wide || (bw_k != 4 && bw_k != 6) || (bw_v != 4 && bw_v != 6)) return false;
   return bw_k + bw_v == 8 ? rows <= 64 && tokens >= 524288 : std::max<int64_t>(rows, 32) * tokens >= 4194304;
 }
 
-TreeScan tree_variant(int D, bool exact, int bw_k, int bw_v, int64_t rows, int64_t tokens) {
-  if (rows_serve(D, exact, bw_k, bw_v, rows, tokens)) return tree_rows_scan(bw_k, bw_v);
+// The row scan reads K by 16 bytes (4 bits) or 8, and four norms at once.
+bool rows_wide(int bw_k, const void* k_pages, int64_t k_stride_p, int64_t k_stride_h, const void* k_norms, int64_t kn_stride_p,
+               int64_t kn_stride_h, const void* v_norms, int64_t vn_stride_p, int64_t vn_stride_h) {
+  const int k = bw_k == 4 ? 16 : 8;
+  return aligned(k_pages, k) && k_stride_p % k == 0 && k_stride_h % k == 0 && aligned(k_norms, 8) && aligned(v_norms, 8) &&
+         kn_stride_p % 4 == 0 && kn_stride_h % 4 == 0 && vn_stride_p % 4 == 0 && vn_stride_h % 4 == 0;
+}
+
+TreeScan tree_variant(int D, bool exact, bool wide, int bw_k, int bw_v, int64_t rows, int64_t tokens) {
+  if (rows_serve(D, exact, wide, bw_k, bw_v, rows, tokens)) return tree_rows_scan(bw_k, bw_v);
   return pick_tree(D, exact, bw_k, bw_v).scan[rows <= 32 ? 0 : rows <= 64 ? 1 : 2];
 }
 
@@ -108,7 +118,7 @@ extern "C" int wn_tree_plan(int B, int Hq, int Hkv, int T, int D, int S, int bw_
   WN_REQUIRE(is_pow2(S) && S >= 16 && valid_bw(bw_k) && valid_bw(bw_v), WN_E_UNSUPPORTED,
              "wn_tree_plan: (S=%d, bw_k=%d, bw_v=%d) not compiled", S, bw_k, bw_v);
   const int64_t rows = int64_t(Hq / Hkv) * T;
-  const TreeScan scan = tree_variant(D, exact != 0, bw_k, bw_v, rows, int64_t(B) * Hkv * max_pages * S);
+  const TreeScan scan = tree_variant(D, exact != 0, true, bw_k, bw_v, rows, int64_t(B) * Hkv * max_pages * S);
   const int groups = tree_slots(scan, tree_lds(scan, bw_k, bw_v));
   WN_REQUIRE(groups > 0, WN_E_LAUNCH, "wn_tree_plan: cannot query the device occupancy");
   const int64_t slots = groups * int64_t(std::max(1, scan.waves));
@@ -150,7 +160,7 @@ extern "C" int64_t wn_tree_workspace_bytes(int B, int Hq, int Hkv, int T, int D,
   if (!tree_shape(B, Hq, Hkv, T, D) || num_splits <= 0) return -1;
   // the most that any scan of this shape takes
   const int64_t rows = int64_t(Hq / Hkv) * T;
-  return tree_layout(B, Hkv, tree_nrp(tree_variant(D, false, 8, 8, rows, 0), rows), T, D, num_splits).total;
+  return tree_layout(B, Hkv, tree_nrp(tree_variant(D, false, false, 8, 8, rows, 0), rows), T, D, num_splits).total;
 }
 
 extern "C" int wn_tree_attention(
@@ -193,7 +203,8 @@ extern "C" int wn_tree_attention(
   const int n_rep = Hq / Hkv;
   const int64_t rows = int64_t(n_rep) * T;
   const TreeKernels k = pick_tree(D, exact != 0, bw_k, bw_v);
-  const TreeScan scan = tree_variant(D, exact != 0, bw_k, bw_v, rows, int64_t(B) * Hkv * max_pages * S);
+  const bool rows_ok = rows_wide(bw_k, k_pages, k_stride_p, k_stride_h, k_norms, kn_stride_p, kn_stride_h, v_norms, vn_stride_p, vn_stride_h);
+  const TreeScan scan = tree_variant(D, exact != 0, rows_ok, bw_k, bw_v, rows, int64_t(B) * Hkv * max_pages * S);
   const int nrp = tree_nrp(scan, rows), ncg = nrp / scan.rows;
   const TreeLayout lay = tree_layout(B, Hkv, nrp, T, D, num_splits);
   WN_REQUIRE(workspace && workspace_bytes >= lay.total && aligned(workspace, 256), WN_E_WORKSPACE,

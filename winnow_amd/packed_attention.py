@@ -438,14 +438,21 @@ def prefill_supported(q: torch.Tensor, kv: PackedKV) -> bool:
             return False
     if kv.page_table.stride(-1) != 1 or not kv.seq_lens.is_contiguous():
         return False
-    for n in (kv.k_norms, kv.v_norms):
-        if n.stride(-1) != 1 or n.data_ptr() % 8 or n.stride(0) % 4 or n.stride(1) % 4:
+    if kv.k_norms.stride(-1) != 1 or kv.v_norms.stride(-1) != 1:
+        return False
+    for pages in (kv.k_pages, kv.v_pages):
+        if pages.stride(-1) != 1 or pages.stride(-2) != pages.shape[-1] or pages.data_ptr() % 4 \
+                or pages.stride(0) % 4 or pages.stride(1) % 4:
             return False
-    for pages, align in ((kv.k_pages, 16 if kv.k_quant.bit_width == 4 else 8), (kv.v_pages, 4)):
-        if pages.stride(-1) != 1 or pages.stride(-2) != pages.shape[-1] or pages.data_ptr() % align \
-                or pages.stride(0) % align or pages.stride(1) % align:
-            return False
-    return True
+    return wide_rows(kv)
+
+
+def wide_rows(kv: PackedKV) -> bool:
+    """Whether the per-wave scans can read K rows by 16 bytes (4 bits) or 8, and four norms at once."""
+    align = 16 if kv.k_quant.bit_width == 4 else 8
+    k, kn, vn = kv.k_pages, kv.k_norms, kv.v_norms
+    return not (k.data_ptr() % align or k.stride(0) % align or k.stride(1) % align or kn.data_ptr() % 8 or vn.data_ptr() % 8
+                or kn.stride(0) % 4 or kn.stride(1) % 4 or vn.stride(0) % 4 or vn.stride(1) % 4)
 
 
 def prefill_plan_for(q: torch.Tensor, kv: PackedKV) -> int:
