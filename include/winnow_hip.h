@@ -469,7 +469,7 @@ int wn_tree_prepare(const int32_t* lens, const int32_t* page_table, int64_t tabl
  * at pages + layer * stride_l + page * stride_p + head * stride_h + slot * row (bytes); fp16
  * norms with strides in elements, or both null (an unquantized cache). A node outside
  * [0, nodes), a position outside the table or a page outside [0, num_pages) moves nothing.
- * 1 <= A <= nodes <= 64, S a power of two; lengths may not be start_pos. */
+ * layers >= 1, 1 <= A <= nodes <= 64, S a power of two; lengths may not be start_pos. */
 int wn_commit_kv(
     uint8_t* k_pages, int64_t k_stride_l, int64_t k_stride_p, int64_t k_stride_h, int k_row,
     uint8_t* v_pages, int64_t v_stride_l, int64_t v_stride_p, int64_t v_stride_h, int v_row,

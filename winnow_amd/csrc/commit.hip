@@ -133,11 +133,11 @@ extern "C" int wn_commit_kv(
     int layers, int B, int Hkv, int S, int A, int nodes, int num_pages, int max_pages, void* stream) {
   using namespace wn;
   clear_error();
-  WN_REQUIRE(layers >= 0 && B >= 0 && Hkv > 0 && k_row > 0 && v_row > 0 && num_pages > 0 && max_pages > 0, WN_E_INVALID,
+  WN_REQUIRE(layers > 0 && B >= 0 && Hkv > 0 && k_row > 0 && v_row > 0 && num_pages > 0 && max_pages > 0, WN_E_INVALID,
              "commit: bad sizes layers=%d B=%d Hkv=%d rows=%d/%d", layers, B, Hkv, k_row, v_row);
   WN_REQUIRE(A > 0 && nodes > 0 && A <= nodes && nodes <= 64, WN_E_INVALID, "commit: need 1 <= A <= nodes <= 64 (A=%d, nodes=%d)", A, nodes);
   WN_REQUIRE(is_pow2(S), WN_E_INVALID, "commit: page size %d is not a power of two", S);
-  if (layers == 0 || B == 0) return WN_OK;
+  if (B == 0) return WN_OK;
   WN_REQUIRE(k_pages && v_pages && !k_norms == !v_norms && page_table && start_pos && path && counts && lengths, WN_E_INVALID,
              "commit: null operand");
   WN_REQUIRE(lengths != start_pos, WN_E_INVALID, "commit: lengths may not be start_pos itself");

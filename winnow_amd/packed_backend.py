@@ -345,6 +345,8 @@ def commit_kv(k_pages: torch.Tensor, v_pages: torch.Tensor, k_norms: torch.Tenso
         raise pa.UnsupportedLayout("commit: every operand must be on one HIP device")
     layers = 1 if k_pages.dim() == 4 else k_pages.shape[0]
     P, Hkv, S = lead[-3:]
+    if 0 in (layers, P, Hkv, S):
+        raise pa.UnsupportedLayout(f"commit: pages {tuple(k_pages.shape)} have no rows")
     if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.stride(-1) != 1:
         raise pa.UnsupportedLayout("commit: page_table must be (B, max_pages) int32 with contiguous rows")
     B, width = page_table.shape
