@@ -650,9 +650,9 @@ def packed_tree_attention(q: torch.Tensor, kv: PackedKV, scale: float, parents: 
     plan = _tree_prepare(kv, parents_host, sizes, exact, q.device) if check_ranges else None
     if check_ranges and plan is None:
         check_contract(q, kv)
-        check_parents(parents if parents_host is None else parents_host)
         if parents_host is not None and parents_host.shape != parents.shape:
             raise UnsupportedLayout(f"parents_host is {tuple(parents_host.shape)}, parents {tuple(parents.shape)}")
+        check_parents(parents if parents_host is None else parents_host)
     out = torch.empty(B, Hq, T, D, dtype=out_dtype, device=q.device)
     if B == 0:
         return out
