@@ -12,7 +12,7 @@ from dataclasses import dataclass
 import torch
 
 from winnow_amd import _lib
-from winnow_amd.packed_attention import UnsupportedLayout
+from winnow_amd.packed_attention import UnsupportedLayout, values_only
 
 MAX_TOP = 64
 
@@ -39,14 +39,14 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
     Sums are fp32 whatever the logits' type. A logit of -inf has probability 0; a row with a
     NaN or +inf, or without a finite logit, gives NaN (its ``top_ids`` still lie in [0, V));
     a token outside [0, V) gives NaN for its row. Raises ``UnsupportedLayout`` before the
-    launch for tensors off the GPU, of other types or shapes, or that require a gradient."""
+    launch for tensors off the GPU, of other types or shapes, or where a gradient, a tangent or a
+    trace is asked for."""
     if not _lib.is_hip(logits):
         raise UnsupportedLayout("token_logprobs needs logits on a HIP device; there is no host fallback")
     if logits.dtype not in _lib.DTYPE_CODE or not 1 <= logits.dim() <= 3:
         raise UnsupportedLayout(f"logits must be (V,), (N, V) or (B, T, V) of fp32, fp16 or bf16, got "
                                 f"{tuple(logits.shape)} {logits.dtype}")
-    if logits.requires_grad and torch.is_grad_enabled():
-        raise UnsupportedLayout("token_logprobs has no gradient: call it under torch.no_grad() or detach the logits")
+    values_only("token_logprobs", logits)
     rows, V = logits.shape[:-1], logits.shape[-1]
     if not 1 <= V < 2 ** 31 or (V > 1 and logits.stride(-1) != 1):
         raise UnsupportedLayout(f"logits need a contiguous, non-empty last axis of fewer than 2^31, got {V}")

@@ -31,6 +31,7 @@ from dataclasses import dataclass
 
 import numpy as np
 import torch
+from torch.fx.experimental.proxy_tensor import get_proxy_mode
 
 from winnow_amd import _lib
 from winnow_amd.packing import packed_bytes
@@ -159,6 +160,20 @@ def pages_from_dense(k: torch.Tensor, v: torch.Tensor, seq_lens, k_tq, v_tq, pag
     return PackedKV(kp, kn, vp, vn, dtable, torch.tensor(lens, dtype=torch.int32, device=dev),
                     Quantizer.from_tq(k_tq), Quantizer.from_tq(v_tq), D,
                     seq_lens_host=torch.tensor(lens, dtype=torch.int32), page_table_host=table)
+
+
+def values_only(what: str, *operands: torch.Tensor) -> None:
+    """Refuse a call of the operator ``what`` from which more is asked than its values: a gradient or a
+    tangent of its operands, or a place in a trace (``torch.jit.trace``, ``make_fx``). A call into the
+    library shows in none of them: the result would silently have no derivative, and the trace would
+    hold an allocation in the operator's place."""
+    for t in operands:
+        if t.requires_grad and torch.is_grad_enabled():
+            raise UnsupportedLayout(f"{what} has no gradient: call it under torch.no_grad() or detach its operands")
+        if torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise UnsupportedLayout(f"{what} has no forward-mode derivative: call it on the primal")
+    if torch._C._get_tracing_state() is not None or get_proxy_mode() is not None:
+        raise UnsupportedLayout(f"{what} cannot be traced")
 
 
 def check_contract(q: torch.Tensor, kv: PackedKV, *, check_ranges: bool = True) -> None:
@@ -534,8 +549,7 @@ def check_tree(q: torch.Tensor, kv: PackedKV, parents: torch.Tensor) -> None:
                                 f"{kv.page_size} (a power of two >= 16)")
     if q.dtype not in _lib.DTYPE_CODE or q.stride(-1) != 1:
         raise UnsupportedLayout("q must be fp32/fp16/bf16 with a contiguous head_dim")
-    if q.requires_grad and torch.is_grad_enabled():
-        raise UnsupportedLayout("tree attention has no gradient: call it under torch.no_grad() or detach q")
+    values_only("tree attention", q)
     for pages, norms in ((kv.k_pages, kv.k_norms), (kv.v_pages, kv.v_norms)):
         st = pages.stride()
         if st[3] != 1 or st[2] != pages.shape[3]:

@@ -331,8 +331,9 @@ def commit_kv(k_pages: torch.Tensor, v_pages: torch.Tensor, k_norms: torch.Tenso
     before any is written, so the order of a path does not matter.
 
     Raises ``UnsupportedLayout`` before the launch for operands off the GPU or of the wrong
-    shape, and (``check_ranges``) where the nodes' positions lie outside a table row or its
+    shape, for pages that take part in a gradient, under a trace, and (``check_ranges``) where the nodes' positions lie outside a table row or its
     pages outside the pool, read as in ``append_kv``."""
+    pa.values_only("commit_kv", k_pages, v_pages)
     packed = k_pages.dtype == torch.uint8
     lead = k_pages.shape[:-1]
     k_at, kn_at = _commit_side("K", k_pages, k_norms, lead)
