@@ -215,6 +215,12 @@ class Engine:
         self._notify(req, kind="final", status=status, detail=req.detail)
         req.done.set()
 
+    def _fail(self, reqs: list[Request], exc: Exception) -> None:
+        """End requests with what a step raised, their pages behind one fence."""
+        fence = default_fence(self.device)
+        for r in reqs:
+            self._retire(r, "error", f"{type(exc).__name__}: {exc}", fence)
+
     def _expire(self) -> None:
         """End requests that were cancelled or are past their deadline."""
         now = self.clock()
@@ -307,7 +313,7 @@ class Engine:
             token = int(logits[0].argmax()) if last else -1
             score = self._scores([req], logits, [token])[0] if last else None
         except Exception as exc:  # noqa: BLE001 - reported on the request
-            self._retire(req, "error", f"{type(exc).__name__}: {exc}", default_fence(self.device))
+            self._fail([req], exc)
             return True
         if last:
             req.state = "decode"
@@ -324,12 +330,15 @@ class Engine:
         try:
             logits = self._forward(batch, [[r.generated[-1]] for r in batch])
             tokens = logits.argmax(-1).tolist()
-            scores = self._scores(batch, logits, tokens)
         except Exception as exc:  # noqa: BLE001 - reported on every request of the batch
-            fence = default_fence(self.device)
-            for r in batch:
-                self._retire(r, "error", f"{type(exc).__name__}: {exc}", fence)
+            self._fail(batch, exc)
             return True
+        try:
+            scores = self._scores(batch, logits, tokens)
+        except Exception as exc:  # noqa: BLE001 - reported on the requests that asked for scores
+            self._fail([r for r in batch if r.top_logprobs is not None], exc)
+            kept = [(r, t) for r, t in zip(batch, tokens) if r.top_logprobs is None]
+            batch, tokens, scores = [r for r, _ in kept], [t for _, t in kept], [None] * len(kept)
         now = self.clock()
         for r, t, score in zip(batch, tokens, scores):
             why = self._take_token(r, int(t), now, score)
