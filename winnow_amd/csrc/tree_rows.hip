@@ -14,22 +14,6 @@
 namespace wn {
 namespace {
 
-constexpr float kRowsRescale = 8.0f;  // a maximum moves when a score exceeds it by more
-constexpr int kRowsNoScale = -64;     // value scale before the first norm
-
-// g with x < 2^g for a finite fp16 x > 0, the least such.
-__device__ __forceinline__ int rows_exponent(uint32_t bits) {
-  return bits >> 10 ? int(bits >> 10) - 14 : 8 - __builtin_clz(bits);
-}
-
-// The largest of the four lanes 16 apart, in each of them.
-__device__ __forceinline__ float rows_max16(float x) {
-  const auto a = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
-  x = fmaxf(__builtin_bit_cast(float, uint32_t(a[0])), __builtin_bit_cast(float, uint32_t(a[1])));
-  const auto b = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
-  return fmaxf(__builtin_bit_cast(float, uint32_t(b[0])), __builtin_bit_cast(float, uint32_t(b[1])));
-}
-
 template <int NCT>
 __device__ __forceinline__ void rows_scale(PfState<NCT>& st, const float (&f)[NCT]) {
 #pragma unroll
@@ -66,7 +50,7 @@ __global__ __launch_bounds__(64 * WPB) __attribute__((amdgpu_waves_per_eu(WPB / 
     st.m[ct] = -INFINITY;
     st.l[ct] = 0.f;
   }
-  st.gs = kRowsNoScale;
+  st.gs = kTreeNoScale;
 
   const int L = min(max(const_view(a.seq_lens)[b], 0), a.max_pages << a.log2S);
   const int hist = L - a.T;  // position of node 0
@@ -145,7 +129,7 @@ __global__ __launch_bounds__(64 * WPB) __attribute__((amdgpu_waves_per_eu(WPB / 
           if (out) N.nk[k >> 1] &= ~(0xffffu << sh);
         }
       }
-      // value scale: every n_V < 2^(7 + gs), so 2^kRowsRescale n_V 2^-gs < 2^15 in fp16; it follows
+      // value scale: every n_V < 2^(7 + gs), so 2^kTreeRescale n_V 2^-gs < 2^15 in fp16; it follows
       // the norms' magnitude
       {
         u16x2 hi = __builtin_bit_cast(u16x2, N.nv[0] & 0x7fff7fffu);
@@ -155,8 +139,8 @@ __global__ __launch_bounds__(64 * WPB) __attribute__((amdgpu_waves_per_eu(WPB / 
         size = size < 0x7c00u ? size : 0;
         if (__any(f16_to_f32(uint16_t(size)) >= ldexpf(1.f, 7 + st.gs))) {  // wave-uniform, rare
           const uint32_t most = __builtin_bit_cast(uint16_t, _Float16(wave_max(f16_to_f32(uint16_t(size)))));
-          if (most && rows_exponent(most) - 7 > st.gs) {
-            const int to = rows_exponent(most) - 7;
+          if (most && tree_exponent(most) - 7 > st.gs) {
+            const int to = tree_exponent(most) - 7;
             float f[NCT];
 #pragma unroll
             for (int ct = 0; ct < NCT; ++ct) {
@@ -207,8 +191,8 @@ __global__ __launch_bounds__(64 * WPB) __attribute__((amdgpu_waves_per_eu(WPB / 
         for (int t = 0; t < 4; ++t)
 #pragma unroll
           for (int i = 0; i < 4; ++i) tops[ct] = fmaxf(tops[ct], d[ct][t][i]);
-        tops[ct] = rows_max16(tops[ct]) + gsf;
-        move[ct] = tops[ct] > kRowsRescale || (st.m[ct] == -INFINITY && tops[ct] > -INFINITY);
+        tops[ct] = tree_max16(tops[ct]) + gsf;
+        move[ct] = tops[ct] > kTreeRescale || (st.m[ct] == -INFINITY && tops[ct] > -INFINITY);
         any = any || move[ct];
       }
       if (__any(any)) {

@@ -85,7 +85,24 @@ __host__ __device__ inline int tree_end(int L, int span, int s) {
   return rest < span ? L : s * span + span;
 }
 
+// Of both scans:
+constexpr float kTreeRescale = 8.0f;  // a maximum moves when a score exceeds it by more
+constexpr int kTreeNoScale = -64;     // value scale before the first norm
+
 #ifdef __HIPCC__
+// g with x < 2^g for a non-negative finite fp16 x > 0, the least such.
+__device__ __forceinline__ int tree_exponent(uint32_t bits) {
+  return bits >> 10 ? int(bits >> 10) - 14 : 8 - __builtin_clz(bits);
+}
+
+// The largest of the four lanes 16 apart, in each of them.
+__device__ __forceinline__ float tree_max16(float x) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+  x = fmaxf(__builtin_bit_cast(float, uint32_t(a[0])), __builtin_bit_cast(float, uint32_t(a[1])));
+  const auto b = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+  return fmaxf(__builtin_bit_cast(float, uint32_t(b[0])), __builtin_bit_cast(float, uint32_t(b[1])));
+}
+
 // Split j of the batch, its splits counted sequence after sequence: its sequence and place there.
 // False past the last one. Every lane of a wave takes part.
 __device__ __forceinline__ bool tree_split(const TreeArgs& a, int lane, int j, int* b, int* s) {

@@ -11,9 +11,7 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr float kTreeCb = 256.0f;      // codebook values are scaled by 2^8
-constexpr float kTreeRescale = 8.0f;   // a maximum moves when a score exceeds it by more
-constexpr int kTreeNoScale = -64;      // value scale before the first norm
+constexpr float kTreeCb = 256.0f;  // codebook values are scaled by 2^8
 
 template <int D>
 struct TreeGeo {
@@ -139,19 +137,6 @@ __device__ __forceinline__ uint32_t tree_row_max(uint32_t x) {
   x = max(x, uint32_t(__builtin_amdgcn_mov_dpp(int(x), 0x124, 0xf, 0xf, true)));
   x = max(x, uint32_t(__builtin_amdgcn_mov_dpp(int(x), 0x122, 0xf, 0xf, true)));
   return max(x, uint32_t(__builtin_amdgcn_mov_dpp(int(x), 0x121, 0xf, 0xf, true)));
-}
-
-// g with x < 2^g for a non-negative finite fp16 x > 0, the least such.
-__device__ __forceinline__ int tree_exponent(uint32_t bits) {
-  return bits >> 10 ? int(bits >> 10) - 14 : 8 - __builtin_clz(bits);
-}
-
-// The largest of the four lanes 16 apart, in each of them.
-__device__ __forceinline__ float tree_max16(float x) {
-  const auto a = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
-  x = fmaxf(__builtin_bit_cast(float, uint32_t(a[0])), __builtin_bit_cast(float, uint32_t(a[1])));
-  const auto b = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
-  return fmaxf(__builtin_bit_cast(float, uint32_t(b[0])), __builtin_bit_cast(float, uint32_t(b[1])));
 }
 
 template <int D, bool EX, int NCT, int RG, int TG>
