@@ -9,8 +9,8 @@
 // flight at once (a full batch: 8,192 waves) and asks in three round trips: for the counts,
 // paths and starts, for both pages of every node, for rows and norms together. No load sits
 // behind a branch, where the compiler waits for each: 28 layers, 4 heads, 5 rows 3.2 us (16.7 with
-// the branches), 32 layers x 16 sequences x 8 heads, 12 rows 7.1 (19.6), x 24, 7 rows of 256 bytes
-// 9.1 (22.8). A row may be the target of one move and the
+// the branches), 32 layers x 16 sequences x 8 heads, 12 rows 6.7 (19.6), x 24, 7 rows of 256 bytes
+// 8.9 (22.8). A row may be the target of one move and the
 // source of another, so a wave reads every source of a block of columns before it writes;
 // blocks of columns are independent of each other.
 #include <algorithm>

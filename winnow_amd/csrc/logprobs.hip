@@ -25,7 +25,7 @@
 //   - where many lanes of a batch have a hit all the same (rising logits) it goes up to the
 //     top-th largest of the lanes' maxima before any is inserted.
 // 1,024 rows of 128,256 bf16: 46 us without alternatives (5.8 TB/s; 37 us of them are the vector
-// instructions, nine an element with an exponential), 76 us with 20, whose insertions add to the
+// instructions, nine an element with an exponential), 78 us with 20, whose insertions add to the
 // instructions; 208 rows of 50,257 fp16, one alternative: 13.6 us and 4 for the second launch; one
 // row of 128,256 fp32, five: 8.5 and 4, latency.
 #include <algorithm>

@@ -5,7 +5,7 @@
 // written to LDS and read back: 740 wave instructions per chunk of 32 rows (64 of them matrix
 // instructions, 128 table reads), where the tile kernel (wn_tree_kernels.h) spends 2,300 on 64 rows.
 // Two waves share a SIMD. What bounds it is instruction issue: 16 sequences of 32,768 tokens, 8 kv
-// heads, 64 rows, 4 bits: 255 us, 0.54 PFLOP/s (tile kernel: 388 us). 64 rows a wave (128
+// heads, 64 rows, 4 bits: 245 us, 0.56 PFLOP/s (tile kernel: 388 us). 64 rows a wave (128
 // accumulators, one wave per SIMD) took 318: a lookup then feeds four matrix instructions, but nothing
 // fills the waits.
 #include "wn_rows.h"

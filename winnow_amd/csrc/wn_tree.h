@@ -29,10 +29,12 @@
 //
 // What bounds it is instruction issue (decoding: six instructions a code by single lookups, three
 // by pairs; the softmax: thirteen a score) beside the matrix instructions, and, for few rows,
-// latency. Whole scans on a 256-CU device: 8 sequences of 500 to 6,000 tokens, 28 heads over 4,
-// 26 nodes, 4 bits, single terms: 41 us; 4 sequences of 15,000 to 20,000, 64 heads over 8, 64
-// nodes, 4 and 6 bits, two terms: 605 us, 0.73 PFLOP/s of fp16 products; one sequence of 300, 32
-// heads over 8, 8 nodes: 9.5 us, of which a chunk takes 2.
+// latency. Whole scans on a 256-CU device, medians of traces, two terms a factor and one: 8
+// sequences of 500 to 6,000 tokens, 28 heads over 4, 26 nodes, 4 bits: 68 us and 40; 16 of 32,768,
+// 32 heads over 8, 16 nodes, 4 bits: 520 to 650 us (twelve in a row lower the clock) and 245, with
+// two terms up to 0.8 PFLOP/s of fp16 products: of 520 us at 2.4 GHz the vector instructions fill
+// 45% and the products 31%; 4 of 15,000 to 20,000, 64 heads over 8, 64 nodes, 4 and 6 bits: 520 to 620 and 285; one of
+// 300, 32 heads over 8, 8 nodes: 12 and 10, of which a chunk takes 2.
 //
 // Precision. EX = true, the callers' default for every type: every factor is a sum of two fp16
 // terms (22 bits), and each product the three larger of their four products (what is left out is

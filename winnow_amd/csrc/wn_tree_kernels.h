@@ -883,7 +883,7 @@ TreeKernels tree_kernels() {
     k.scan[1] = tree_scan<D, EX, 2, 2, 2, W>();
     // More than 64 rows: blocks of 128, which decode a chunk once for all of them. With two terms a
     // factor decoding writes twice the bytes, and eight waves share it (64 query heads, 64 nodes, 4 and
-    // 6 bits: 605 us, two work-groups of four waves and 64 rows 710; a second set of tiles, to decode
+    // 6 bits, in traces: 605 us, two work-groups of four waves and 64 rows 710; a second set of tiles, to decode
     // ahead of the barrier, 600). With single terms four waves take 128 rows, and a second work-group
     // fills their waits (28 heads, 26 nodes: 41 us, eight waves 47).
     if constexpr (EX) k.scan[2] = tree_scan<D, EX, 2, 4, 2, W>();
