@@ -495,6 +495,24 @@ int wn_token_logprobs(const void* logits, int dtype, int64_t stride_outer, int64
                       int64_t* top_ids, int64_t N, int V, int top, void* workspace, int64_t workspace_bytes,
                       void* stream);
 
+/* ---- a step of a long conversation ---- */
+
+/* Penalties, biases and a mask applied to N rows of V logits (contiguous along V, row strides in
+ * elements) in one pass; out may be logits itself, with its stride. Per row, in fp32, rounded once:
+ *   history (N, H) int32, of which the first lengths[r] (null: H; clipped to [0, H]) count; a token
+ *     among them has x > 0 ? x / repetition : x * repetition; one that occurs c > 0 times from
+ *     prompt_lengths[r] (null: 0) on loses frequency * c + presence
+ *   bias_ids, bias (N, J): added in the order of the list, J <= 1024
+ *   allowed (N, ceil(V / 32)) words, stride in words: -inf where bit v % 32 of word v / 32 is 0
+ * repetition, presence, frequency: (N) fp32, or null for one value for all. Ids outside [0, V) are
+ * ignored. history, bias_ids and allowed may be null (H = 0, J = 0). H < 2^30, V < 2^31 - 65536. */
+int wn_adjust_logits(const void* logits, int dtype, int64_t stride, void* out, int64_t out_stride, int64_t N, int V,
+                     const int32_t* history, int64_t history_stride, int H, const int32_t* lengths,
+                     const int32_t* prompt_lengths, const float* repetition, const float* presence,
+                     const float* frequency, float repetition_all, float presence_all, float frequency_all,
+                     const int32_t* bias_ids, int64_t bias_ids_stride, const float* bias, int64_t bias_stride, int J,
+                     const uint32_t* allowed, int64_t allowed_stride, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -187,6 +187,12 @@ SIGNATURES = {
         _c_p, _c_p, _c_p, _c_p, _c_p,               # tokens, logprob, entropy, top_logprobs, top_ids
         _c_i64, _c_i, _c_i, _c_p, _c_i64,           # N, V, top, workspace, bytes
         _c_p]),
+    "wn_adjust_logits": (_c_i, [
+        _c_p, _c_i, _c_i64, _c_p, _c_i64, _c_i64, _c_i,   # logits, dtype, stride, out, stride, N, V
+        _c_p, _c_i64, _c_i, _c_p, _c_p,             # history, stride, H, lengths, prompt_lengths
+        _c_p, _c_p, _c_p, _c_f, _c_f, _c_f,         # repetition, presence, frequency: rows, all
+        _c_p, _c_i64, _c_p, _c_i64, _c_i,           # bias_ids, stride, bias, stride, J
+        _c_p, _c_i64, _c_p]),                       # allowed, stride, stream
 }
 
 # bench.py's measurement probes (include/winnow_probe.h): libwinnow_probe.so beside
