@@ -497,6 +497,31 @@ int wn_token_logprobs(const void* logits, int dtype, int64_t stride_outer, int64
 
 /* ---- a step of a long conversation ---- */
 
+/* wn_append_kv with the position rotation applied to K on the way, and to q beside it, in one launch.
+ *   cos, sin  (B, n, rot_dim), element strides s_b (0: one table for all) and s_n, rows contiguous,
+ *             type rot_dtype; rot_dim even, 2 .. D
+ *   q         (B, Hq, n, D) with element strides, last dim contiguous, type q_dtype; or null
+ *   q_out     (B, Hq, n, D) contiguous, type q_dtype, 16-byte aligned; may not be q
+ * Channel d < rot_dim / 2 becomes x_d cos_d - x_(d + rot_dim / 2) sin_d, d < rot_dim
+ * x_d cos_d + x_(d - rot_dim / 2) sin_d: exact products, the sum rounded once to fp32. K is quantized
+ * as that fp32 value, with wn_append_kv's codes and norms of it; q is rounded to its type. Other
+ * operands, preconditions and errors as wn_append_kv. B * Hq * n * D < 2^33. */
+int wn_append_rotated_kv(
+    const void* q, int64_t qs_b, int64_t qs_h, int64_t qs_n, int q_dtype, int Hq, void* q_out,
+    const void* cos, int64_t cs_b, int64_t cs_n, const void* sin, int64_t ss_b, int64_t ss_n, int rot_dtype, int rot_dim,
+    const void* k, int64_t ks_b, int64_t ks_h, int64_t ks_n,
+    const void* v, int64_t vs_b, int64_t vs_h, int64_t vs_n, int x_dtype,
+    const float* pi_k, const float* boundaries_k, int bw_k,
+    const float* pi_v, const float* boundaries_v, int bw_v,
+    const int32_t* page_table, int64_t table_stride_b,
+    const int32_t* start_pos,
+    uint8_t* k_pages, int64_t k_stride_p, int64_t k_stride_h,
+    uint8_t* v_pages, int64_t v_stride_p, int64_t v_stride_h,
+    uint16_t* k_norms, int64_t kn_stride_p, int64_t kn_stride_h,
+    uint16_t* v_norms, int64_t vn_stride_p, int64_t vn_stride_h,
+    int B, int Hkv, int n, int D, int S, int num_pages, int max_pages,
+    void* stream, void* ev_begin, void* ev_end);
+
 /* Penalties, biases and a mask applied to N rows of V logits (contiguous along V, row strides in
  * elements) in one pass; out may be logits itself, with its stride. Per row, in fp32, rounded once:
  *   history (N, H) int32, of which the first lengths[r] (null: H; clipped to [0, H]) count; a token

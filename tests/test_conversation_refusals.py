@@ -4,6 +4,7 @@ for HIP ones."""
 from __future__ import annotations
 
 import math
+import types
 
 import pytest
 import torch
@@ -96,3 +97,51 @@ def test_logits_c_abi():
         with pytest.raises(_lib.WinnowHipError, match=match):
             call(**kw)
     call(N=0, logits=None)
+
+
+# ------------------------------------------------------------------------ rotated append
+
+def _append(**kw):
+    """``append_rotated_kv`` on host tensors: the GPU's place is checked first."""
+    from winnow_amd.packed_backend import append_rotated_kv
+    tq = types.SimpleNamespace(Pi=torch.eye(64), boundaries=torch.zeros(15), centroids=torch.zeros(16), bit_width=4)
+    g = dict(q=torch.zeros(2, 4, 3, 64), k=torch.zeros(2, 2, 3, 64), v=torch.zeros(2, 2, 3, 64), cos=torch.zeros(2, 3, 64), sin=torch.zeros(2, 3, 64),
+             k_tq=tq, v_tq=tq, k_pages=torch.zeros(6, 2, 16, 32, dtype=torch.uint8), v_pages=torch.zeros(6, 2, 16, 32, dtype=torch.uint8),
+             k_norms=torch.zeros(6, 2, 16, dtype=torch.float16), v_norms=torch.zeros(6, 2, 16, dtype=torch.float16),
+             page_table=torch.tensor([[0, 1, -1], [2, 3, 4]], dtype=torch.int32), start_pos=torch.tensor([10, 30], dtype=torch.int32))
+    g.update(kw)
+    names = ("q", "k", "v", "cos", "sin", "k_tq", "v_tq", "k_pages", "v_pages", "k_norms", "v_norms", "page_table", "start_pos")
+    args = [g.pop(n) for n in names]
+    return append_rotated_kv(*args, **g)
+
+
+def test_append_needs_a_gpu():
+    with pytest.raises(pa.UnsupportedLayout, match="HIP device"):
+        _append()
+
+
+@pytest.mark.parametrize("name", ["q", "k", "v", "cos", "sin"])
+def test_append_has_no_gradient(name):
+    shape = (2, 3, 64) if name in ("cos", "sin") else (2, 4 if name == "q" else 2, 3, 64)
+    with pytest.raises(pa.UnsupportedLayout, match="no gradient"):
+        _append(**{name: torch.zeros(shape, requires_grad=True)})
+
+
+def test_append_c_abi():
+    """Nothing is launched for arguments outside the contract."""
+    x = torch.zeros(4096)
+    p = x.data_ptr()
+
+    def call(**kw):
+        a = dict(q=p, qb=0, qh=0, qn=0, qd=0, Hq=4, qo=p, cos=p, cb=0, cn=0, sin=p, sb=0, sn=0, rd=0, R=64, k=p, kb=0, kh=0, kn=0, v=p, vb=0, vh=0,
+                 vn=0, xd=0, pik=p, bk=p, bwk=4, piv=p, bv=p, bwv=4, table=p, ts=0, start=p, kp=p, kpp=0, kph=0, vp=p, vpp=0, vph=0, knp=p, knpp=0,
+                 knph=0, vnp=p, vnpp=0, vnph=0, B=1, Hkv=2, n=1, D=64, S=16, P=1, mp=1)
+        a.update(kw)
+        _lib.call("wn_append_rotated_kv", *a.values(), None, None, None)
+    for kw, match in ((dict(R=0), "rotated channels"), (dict(R=63), "rotated channels"), (dict(R=66), "rotated channels"), (dict(rd=3), "dtype"),
+                      (dict(qd=-1), "dtype"), (dict(Hq=0), "query heads"), (dict(cos=None), "null"), (dict(qo=None), "null"), (dict(cos=p + 2), "aligned"),
+                      (dict(qo=p + 8), "aligned"), (dict(B=2 ** 16, n=2 ** 16), "too many"), (dict(D=96), "head_dim"), (dict(k=None), "null"),
+                      (dict(v=None, pik=p + 4), "16-byte"), (dict(S=24), "power of two")):
+        with pytest.raises(_lib.WinnowHipError, match=match):
+            call(**kw)
+    call(n=0, k=None, cos=None)

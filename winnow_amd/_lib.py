@@ -82,6 +82,20 @@ SIGNATURES = {
         _c_p, _c_i64, _c_i64,
         _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i,
         _c_p, _c_p, _c_p]),                         # stream, ev_begin, ev_end
+    "wn_append_rotated_kv": (_c_i, [
+        _c_p, _c_i64, _c_i64, _c_i64, _c_i, _c_i, _c_p,   # q, strides, dtype, heads, rotated q
+        _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_i, _c_i,   # cos, strides, sin, strides, dtype, rotated channels
+        _c_p, _c_i64, _c_i64, _c_i64,
+        _c_p, _c_i64, _c_i64, _c_i64, _c_i,
+        _c_p, _c_p, _c_i,
+        _c_p, _c_p, _c_i,
+        _c_p, _c_i64, _c_p,
+        _c_p, _c_i64, _c_i64,
+        _c_p, _c_i64, _c_i64,
+        _c_p, _c_i64, _c_i64,
+        _c_p, _c_i64, _c_i64,
+        _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i,
+        _c_p, _c_p, _c_p]),                         # stream, ev_begin, ev_end
     "wn_quantize": (_c_i, [_c_p, _c_i, _c_i64, _c_i64, _c_p, _c_p, _c_i, _c_i, _c_p, _c_p, _c_p]),
     "wn_pack": (_c_i, [_c_p, _c_i64, _c_i, _c_i, _c_p, _c_p]),
     "wn_unpack": (_c_i, [_c_p, _c_i64, _c_i, _c_i, _c_p, _c_p]),

@@ -10,6 +10,9 @@
 // x / n is the correctly rounded fp32 quotient, so every code is the bucket of
 // the correctly rounded fp32 y; an fp32 GEMM elsewhere can differ from it only
 // when its own rounding error crosses a boundary.
+#include <algorithm>
+#include <type_traits>
+
 #include "wn_quant.h"
 
 namespace wn {
@@ -51,8 +54,13 @@ __device__ __forceinline__ uint8_t packed_byte(const uint8_t* codes, int k, int 
 //             (a lane's D/16 searches in lockstep).
 //   stores    D/8 threads per vector each pack eight codes (bw bytes) and store
 //             them; thread 0 of the vector stores its norm.
-template <int D>
-__global__ __launch_bounds__(kQBlock) void quantize_kernel(QuantArgs a) {
+// ROT (wn_append_rotated_kv): K's elements are rotated as they are loaded (side 0), and
+// work-groups past the sides rotate q.
+template <bool ROT>
+using AppendArgs = std::conditional_t<ROT, QuantRotArgs, QuantArgs>;
+
+template <int D, bool ROT>
+__global__ __launch_bounds__(kQBlock) void quantize_kernel(AppendArgs<ROT> a) {
   constexpr int EPT = D / 16;  // x elements per thread in the norm phase
   constexpr int KS = D / 4;    // K-steps of the rotation (4 input dims each)
   constexpr int TPW = D / 64;  // output tiles of sixteen dims per wave
@@ -65,6 +73,12 @@ __global__ __launch_bounds__(kQBlock) void quantize_kernel(QuantArgs a) {
   __shared__ int64_t rowoff[kVecPerBlock];  // byte offset of the vector's packed row (-1: skipped)
   __shared__ int64_t nrmoff[kVecPerBlock];  // element offset of its norm
 
+  if constexpr (ROT) {
+    if (blockIdx.y == gridDim.y - 1 && a.rot.q) {
+      rotate_queries<D, kQBlock>(a.rot, a.n, blockIdx.x, gridDim.x, threadIdx.x);
+      return;
+    }
+  }
   const QuantSide& sd = a.side[blockIdx.y];
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
   const int nb = (1 << sd.bw) - 1;
@@ -90,8 +104,20 @@ __global__ __launch_bounds__(kQBlock) void quantize_kernel(QuantArgs a) {
       const int h = int((v / a.n) % a.H);
       const int b = int(v / (int64_t(a.n) * a.H));
       const int64_t xo = b * sd.sb + h * sd.sh + i * sd.sn + EPT * part;
+      if constexpr (ROT) {
+        const QuantRotary& r = a.rot;
+        const int64_t co = b * r.csb + i * r.csn, so = b * r.ssb + i * r.ssn;
+        if (blockIdx.y == 0) {
 #pragma unroll
-      for (int k = 0; k < EPT; ++k) xv[k] = load_elem(sd.x, xo + k, a.x_dtype);
+          for (int k = 0; k < EPT; ++k) xv[k] = rotated_elem(r, sd.x, xo - EPT * part, a.x_dtype, co, so, EPT * part + k);
+        } else {
+#pragma unroll
+          for (int k = 0; k < EPT; ++k) xv[k] = load_elem(sd.x, xo + k, a.x_dtype);
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < EPT; ++k) xv[k] = load_elem(sd.x, xo + k, a.x_dtype);
+      }
     } else {
 #pragma unroll
       for (int k = 0; k < EPT; ++k) xv[k] = 0.f;
@@ -211,8 +237,8 @@ __global__ __launch_bounds__(kQBlock) void quantize_kernel(QuantArgs a) {
 // rows of Pi (each product exact, the sum in float64, rounded once to fp32),
 // bucketizes them into the LDS codes, and the store phase packs and scatters as
 // quantize_kernel does.
-template <int D>
-__global__ __launch_bounds__(kQBlock) void quantize_any_kernel(QuantArgs a) {
+template <int D, bool ROT>
+__global__ __launch_bounds__(kQBlock) void quantize_any_kernel(AppendArgs<ROT> a) {
   constexpr int TPV = D / 8;  // store threads per vector (eight codes each)
   __shared__ float bnd[255];
   __shared__ float xs[kVecPerBlock][D];
@@ -222,6 +248,12 @@ __global__ __launch_bounds__(kQBlock) void quantize_any_kernel(QuantArgs a) {
   __shared__ int64_t rowoff[kVecPerBlock];
   __shared__ int64_t nrmoff[kVecPerBlock];
 
+  if constexpr (ROT) {
+    if (blockIdx.y == gridDim.y - 1 && a.rot.q) {
+      rotate_queries<D, kQBlock>(a.rot, a.n, blockIdx.x, gridDim.x, threadIdx.x);
+      return;
+    }
+  }
   const QuantSide& sd = a.side[blockIdx.y];
   const int tid = threadIdx.x;
   const int nb = (1 << sd.bw) - 1;
@@ -237,7 +269,14 @@ __global__ __launch_bounds__(kQBlock) void quantize_any_kernel(QuantArgs a) {
       const int i = int(v % a.n);
       const int h = int((v / a.n) % a.H);
       const int b = int(v / (int64_t(a.n) * a.H));
-      x = load_elem(sd.x, b * sd.sb + h * sd.sh + i * sd.sn + dd, a.x_dtype);
+      const int64_t xo = b * sd.sb + h * sd.sh + i * sd.sn;
+      if constexpr (ROT) {
+        const QuantRotary& r = a.rot;
+        x = blockIdx.y == 0 ? rotated_elem(r, sd.x, xo, a.x_dtype, b * r.csb + i * r.csn, b * r.ssb + i * r.ssn, dd)
+                            : load_elem(sd.x, xo + dd, a.x_dtype);
+      } else {
+        x = load_elem(sd.x, xo + dd, a.x_dtype);
+      }
     }
     xs[vl][dd] = x;
   }
@@ -415,30 +454,42 @@ __global__ void unpack_kernel(const uint8_t* packed, int64_t rows, int D, int bw
 
 using namespace wn;
 
-static int launch_quantize(QuantArgs& a, int sides, int D, hipStream_t st, const char* what,
+// ROT: q, if there is any, takes one more row of the grid.
+template <bool ROT = false>
+static int launch_quantize(AppendArgs<ROT>& a, int sides, int D, hipStream_t st, const char* what,
                            void* ev_begin = nullptr, void* ev_end = nullptr) {
   if (a.total == 0) return WN_OK;
-  dim3 grid(unsigned((a.total + kVecPerBlock - 1) / kVecPerBlock), sides);
-  if (ev_begin) hipEventRecord(static_cast<hipEvent_t>(ev_begin), st);
-  if (quantize_tiles_ok(a, sides, D)) {
+  int64_t groups = (a.total + kVecPerBlock - 1) / kVecPerBlock;
+  bool q = false;
+  if constexpr (ROT) {
+    q = a.rot.q != nullptr;
+    if (q) groups = std::max<int64_t>(groups, std::min<int64_t>((int64_t(a.rot.B) * a.rot.Hq * a.n * (D / 8) + kQBlock - 1) / kQBlock, 2048));
+  }
+  dim3 grid(unsigned(groups), sides + q);
+  if (ev_begin) (void)hipEventRecord(static_cast<hipEvent_t>(ev_begin), st);
+  bool tiles = quantize_tiles_ok(a, sides, D);
+  if constexpr (ROT) tiles = tiles && a.rot.k_vec;
+  if (tiles) {
     const int rc = launch_quantize_tiles(a, sides, D, st);
     if (rc != WN_OK) {
       set_error("%s: cannot query the device", what);
       return rc;
     }
   } else switch (D) {
-    case 16: hipLaunchKernelGGL(quantize_any_kernel<16>, grid, dim3(kQBlock), 0, st, a); break;
-    case 32: hipLaunchKernelGGL(quantize_any_kernel<32>, grid, dim3(kQBlock), 0, st, a); break;
-    case 64: hipLaunchKernelGGL(quantize_kernel<64>, grid, dim3(kQBlock), 0, st, a); break;
-    case 128: hipLaunchKernelGGL(quantize_kernel<128>, grid, dim3(kQBlock), 0, st, a); break;
-    case 256: hipLaunchKernelGGL(quantize_any_kernel<256>, grid, dim3(kQBlock), 0, st, a); break;
+    case 16: hipLaunchKernelGGL(HIP_KERNEL_NAME(quantize_any_kernel<16, ROT>), grid, dim3(kQBlock), 0, st, a); break;
+    case 32: hipLaunchKernelGGL(HIP_KERNEL_NAME(quantize_any_kernel<32, ROT>), grid, dim3(kQBlock), 0, st, a); break;
+    case 64: hipLaunchKernelGGL(HIP_KERNEL_NAME(quantize_kernel<64, ROT>), grid, dim3(kQBlock), 0, st, a); break;
+    case 128: hipLaunchKernelGGL(HIP_KERNEL_NAME(quantize_kernel<128, ROT>), grid, dim3(kQBlock), 0, st, a); break;
+    case 256: hipLaunchKernelGGL(HIP_KERNEL_NAME(quantize_any_kernel<256, ROT>), grid, dim3(kQBlock), 0, st, a); break;
   }
-  if (ev_end) hipEventRecord(static_cast<hipEvent_t>(ev_end), st);
+  if (ev_end) (void)hipEventRecord(static_cast<hipEvent_t>(ev_end), st);
   return check_launch(what);
 }
 
-extern "C" int wn_append_kv(
-    const void* k, int64_t ks_b, int64_t ks_h, int64_t ks_n,
+// The checks and operands that wn_append_kv and wn_append_rotated_kv share. `done`: there is nothing
+// to write.
+static int append_args(
+    QuantArgs& a, bool* done, const void* k, int64_t ks_b, int64_t ks_h, int64_t ks_n,
     const void* v, int64_t vs_b, int64_t vs_h, int64_t vs_n, int x_dtype,
     const float* pi_k, const float* boundaries_k, int bw_k,
     const float* pi_v, const float* boundaries_v, int bw_v,
@@ -447,9 +498,7 @@ extern "C" int wn_append_kv(
     uint8_t* v_pages, int64_t v_stride_p, int64_t v_stride_h,
     uint16_t* k_norms, int64_t kn_stride_p, int64_t kn_stride_h,
     uint16_t* v_norms, int64_t vn_stride_p, int64_t vn_stride_h,
-    int B, int Hkv, int n, int D, int S, int num_pages, int max_pages,
-    void* stream, void* ev_begin, void* ev_end) {
-  clear_error();
+    int B, int Hkv, int n, int D, int S, int num_pages, int max_pages) {
   WN_REQUIRE(B >= 0 && Hkv > 0 && n >= 0 && num_pages >= 0 && max_pages >= 0, WN_E_INVALID,
              "append: bad sizes B=%d Hkv=%d n=%d", B, Hkv, n);
   WN_REQUIRE(valid_head_dim(D), WN_E_UNSUPPORTED, "append: head_dim %d not compiled (16, 32, 64, 128, 256)", D);
@@ -457,7 +506,8 @@ extern "C" int wn_append_kv(
   WN_REQUIRE(x_dtype >= WN_F32 && x_dtype <= WN_BF16, WN_E_INVALID, "append: dtype code %d", x_dtype);
   WN_REQUIRE(valid_bw(bw_k) && (!v || valid_bw(bw_v)), WN_E_INVALID, "append: bit widths %d/%d", bw_k,
              bw_v);
-  if (int64_t(B) * n == 0) return WN_OK;
+  *done = int64_t(B) * n == 0;
+  if (*done) return WN_OK;
   WN_REQUIRE(k && pi_k && boundaries_k && page_table && start_pos && k_pages && k_norms, WN_E_INVALID,
              "append: null operand");
   WN_REQUIRE(!v || (pi_v && boundaries_v && v_pages && v_norms), WN_E_INVALID, "append: null V operand");
@@ -466,7 +516,6 @@ extern "C" int wn_append_kv(
   WN_REQUIRE(aligned(k_pages, 8) && k_stride_p % 8 == 0 && k_stride_h % 8 == 0 &&
                  (!v || (aligned(v_pages, 8) && v_stride_p % 8 == 0 && v_stride_h % 8 == 0)),
              WN_E_INVALID, "append: pages need 8-byte aligned base and strides");
-  QuantArgs a{};
   a.side[0] = QuantSide{k, ks_b, ks_h, ks_n, pi_k, boundaries_k, bw_k, k_pages, k_stride_p, k_stride_h,
                         k_norms, kn_stride_p, kn_stride_h, nullptr, nullptr};
   if (v)
@@ -483,7 +532,69 @@ extern "C" int wn_append_kv(
   a.max_pages = max_pages;
   a.x_dtype = x_dtype;
   a.scatter = 1;
+  return WN_OK;
+}
+
+extern "C" int wn_append_kv(
+    const void* k, int64_t ks_b, int64_t ks_h, int64_t ks_n,
+    const void* v, int64_t vs_b, int64_t vs_h, int64_t vs_n, int x_dtype,
+    const float* pi_k, const float* boundaries_k, int bw_k,
+    const float* pi_v, const float* boundaries_v, int bw_v,
+    const int32_t* page_table, int64_t table_stride_b, const int32_t* start_pos,
+    uint8_t* k_pages, int64_t k_stride_p, int64_t k_stride_h,
+    uint8_t* v_pages, int64_t v_stride_p, int64_t v_stride_h,
+    uint16_t* k_norms, int64_t kn_stride_p, int64_t kn_stride_h,
+    uint16_t* v_norms, int64_t vn_stride_p, int64_t vn_stride_h,
+    int B, int Hkv, int n, int D, int S, int num_pages, int max_pages,
+    void* stream, void* ev_begin, void* ev_end) {
+  clear_error();
+  QuantArgs a{};
+  bool done = false;
+  const int rc = append_args(a, &done, k, ks_b, ks_h, ks_n, v, vs_b, vs_h, vs_n, x_dtype, pi_k, boundaries_k, bw_k, pi_v, boundaries_v, bw_v,
+                             page_table, table_stride_b, start_pos, k_pages, k_stride_p, k_stride_h, v_pages, v_stride_p, v_stride_h,
+                             k_norms, kn_stride_p, kn_stride_h, v_norms, vn_stride_p, vn_stride_h, B, Hkv, n, D, S, num_pages, max_pages);
+  if (rc != WN_OK || done) return rc;
   return launch_quantize(a, v ? 2 : 1, D, static_cast<hipStream_t>(stream), "wn_append_kv", ev_begin, ev_end);
+}
+
+extern "C" int wn_append_rotated_kv(
+    const void* q, int64_t qs_b, int64_t qs_h, int64_t qs_n, int q_dtype, int Hq, void* q_out,
+    const void* cos, int64_t cs_b, int64_t cs_n, const void* sin, int64_t ss_b, int64_t ss_n, int rot_dtype, int rot_dim,
+    const void* k, int64_t ks_b, int64_t ks_h, int64_t ks_n,
+    const void* v, int64_t vs_b, int64_t vs_h, int64_t vs_n, int x_dtype,
+    const float* pi_k, const float* boundaries_k, int bw_k,
+    const float* pi_v, const float* boundaries_v, int bw_v,
+    const int32_t* page_table, int64_t table_stride_b, const int32_t* start_pos,
+    uint8_t* k_pages, int64_t k_stride_p, int64_t k_stride_h,
+    uint8_t* v_pages, int64_t v_stride_p, int64_t v_stride_h,
+    uint16_t* k_norms, int64_t kn_stride_p, int64_t kn_stride_h,
+    uint16_t* v_norms, int64_t vn_stride_p, int64_t vn_stride_h,
+    int B, int Hkv, int n, int D, int S, int num_pages, int max_pages,
+    void* stream, void* ev_begin, void* ev_end) {
+  clear_error();
+  QuantRotArgs a{};
+  bool done = false;
+  const int rc = append_args(a, &done, k, ks_b, ks_h, ks_n, v, vs_b, vs_h, vs_n, x_dtype, pi_k, boundaries_k, bw_k, pi_v, boundaries_v, bw_v,
+                             page_table, table_stride_b, start_pos, k_pages, k_stride_p, k_stride_h, v_pages, v_stride_p, v_stride_h,
+                             k_norms, kn_stride_p, kn_stride_h, v_norms, vn_stride_p, vn_stride_h, B, Hkv, n, D, S, num_pages, max_pages);
+  if (rc != WN_OK) return rc;
+  WN_REQUIRE(rot_dim > 0 && rot_dim <= D && rot_dim % 2 == 0, WN_E_INVALID, "append: %d rotated channels of %d", rot_dim, D);
+  WN_REQUIRE(rot_dtype >= WN_F32 && rot_dtype <= WN_BF16 && (!q || (q_dtype >= WN_F32 && q_dtype <= WN_BF16)), WN_E_INVALID,
+             "append: dtype codes %d/%d", rot_dtype, q_dtype);
+  WN_REQUIRE(!q || Hq > 0, WN_E_INVALID, "append: %d query heads", Hq);
+  if (done) return WN_OK;
+  const int es = rot_dtype == WN_F32 ? 4 : 2, xs = x_dtype == WN_F32 ? 4 : 2, qes = q_dtype == WN_F32 ? 4 : 2;
+  WN_REQUIRE(cos && sin && (!q || q_out), WN_E_INVALID, "append: null operand");
+  WN_REQUIRE(aligned(cos, es) && aligned(sin, es) && (!q || (aligned(q, qes) && aligned(q_out, 16))), WN_E_INVALID,
+             "append: cos, sin and q aligned to their type, the rotated q to 16 bytes");
+  WN_REQUIRE(!q || int64_t(B) * Hq * n <= (INT32_MAX >> 1) / (D / 8), WN_E_INVALID, "append: %d x %d x %d rows of q are too many", B, Hq, n);
+  const auto by16 = [](const void* p, int size, int64_t a0, int64_t a1, int64_t a2) {
+    return aligned(p, 16) && a0 * size % 16 == 0 && a1 * size % 16 == 0 && a2 * size % 16 == 0;
+  };
+  const bool tables = rot_dim % 16 == 0 && by16(cos, es, cs_b, cs_n, 0) && by16(sin, es, ss_b, ss_n, 0);
+  a.rot = QuantRotary{cos, sin, cs_b, cs_n, ss_b, ss_n, q, qs_b, qs_h, qs_n, q_out, rot_dtype, rot_dim, q_dtype, Hq, B,
+                      q && tables && by16(q, qes, qs_b, qs_h, qs_n), tables && by16(k, xs, ks_b, ks_h, ks_n)};
+  return launch_quantize<true>(a, v ? 2 : 1, D, static_cast<hipStream_t>(stream), "wn_append_rotated_kv", ev_begin, ev_end);
 }
 
 extern "C" int wn_quantize(const void* x, int x_dtype, int64_t rows, int64_t row_stride, const float* pi,

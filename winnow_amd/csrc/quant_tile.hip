@@ -79,37 +79,6 @@ __device__ __forceinline__ uint32_t count_below(const float* bnd, int bw, float 
   return pos;
 }
 
-// Eight elements of a row of x, as they are stored.
-template <int DT>
-struct Raw8 {
-  uint4 w[DT == WN_F32 ? 2 : 1];
-};
-template <int DT>
-__device__ __forceinline__ Raw8<DT> load8(const void* x, int64_t i) {
-  Raw8<DT> r;
-  if constexpr (DT == WN_F32) {
-    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const float*>(x) + i);
-    r.w[0] = p[0];
-    r.w[1] = p[1];
-  } else {
-    r.w[0] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + i);
-  }
-  return r;
-}
-template <int DT>
-__device__ __forceinline__ float elem(const Raw8<DT>& r, int k) {
-  const uint4 a = r.w[DT == WN_F32 ? k >> 2 : 0];
-  if constexpr (DT == WN_F32) {
-    const int j = k & 3;
-    return __builtin_bit_cast(float, j == 0 ? a.x : j == 1 ? a.y : j == 2 ? a.z : a.w);
-  } else {
-    const int j = k >> 1;
-    const uint32_t w = j == 0 ? a.x : j == 1 ? a.y : j == 2 ? a.z : a.w;
-    if constexpr (DT == WN_BF16) return __builtin_bit_cast(float, k & 1 ? w & 0xffff0000u : w << 16);
-    else return f16_to_f32(uint16_t(k & 1 ? w >> 16 : w));
-  }
-}
-
 // float64 sum of squares of a lane's elements reduced over the four lanes of a vector,
 // in quantize_kernel's order: D/16 consecutive elements in turn, then the sixteen
 // partial sums by halves.
@@ -154,44 +123,59 @@ struct RowInfo {
   float n[2];    // the norms of the two groups (one group: the first)
 };
 
-template <int D>
+struct RotRowInfo : RowInfo {
+  int64_t cs, sn;  // element offsets of the token's cos and sin
+};
+
+template <int D, bool ROT = false>
 struct TileWave {
-  RowInfo row[kTileVecs];
+  std::conditional_t<ROT, RotRowInfo, RowInfo> row[kTileVecs];
   uint16_t list[kListMax];                   // vector D + dim
   __align__(8) uint8_t code[kTileVecs][D];     // code8()
 };
 
 // The eight codes of dims 8k .. 8k + 7 of row r (the eights of a row swapped about, so
 // that neither the MFMA layout's writes nor the row reads meet in a few banks).
-template <int D>
-__device__ __forceinline__ uint8_t* code8(TileWave<D>& w, int r, int k) {
+template <int D, bool ROT>
+__device__ __forceinline__ uint8_t* code8(TileWave<D, ROT>& w, int r, int k) {
   return w.code[r] + 8 * (k ^ ((r >> 1) & (D / 8 - 1)));
 }
 
-template <bool G2>
-using TileArgs = std::conditional_t<G2, QuantSplitArgs, QuantArgs>;
+template <bool G2, bool ROT = false>
+using TileArgs = std::conditional_t<ROT, QuantRotArgs, std::conditional_t<G2, QuantSplitArgs, QuantArgs>>;
 // The second group of a side that has one; else `none`.
 __device__ __forceinline__ const QuantGroup2& second_group(const QuantSplitSide& s, const QuantGroup2&) { return s.second; }
 __device__ __forceinline__ const QuantGroup2& second_group(const QuantSide&, const QuantGroup2& none) { return none; }
 
-template <int D, int DT, bool G2>
-__global__ __launch_bounds__(64 * tile_waves<G2>()) void quantize_tile_kernel(TileArgs<G2> a) {
-  constexpr int WV = tile_waves<G2>();
+// ROT (wn_append_rotated_kv): K's elements are rotated as they are loaded, from rows of type DT and
+// tables of type CT; both sides are then fp32 in the arithmetic (XT). The last row of the grid, if
+// there is a q, rotates it.
+template <int D, int DT, bool G2, bool ROT = false, int CT = WN_F32>
+__global__ __launch_bounds__(64 * tile_waves<G2>()) void quantize_tile_kernel(TileArgs<G2, ROT> a) {
+  static_assert(!(G2 && ROT), "one group of channels");
+  constexpr int WV = tile_waves<G2>(), XT = ROT ? WN_F32 : DT;
   constexpr int KS = D / 32;  // K-steps of 32 input dims
   constexpr int U = D / 32;   // eights of output dims per lane (two MFMA row tiles each)
   constexpr int NR = kTileVecs, NTHR = 64 * WV;
-  constexpr bool F32 = DT == WN_F32;
+  constexpr bool F32 = XT == WN_F32;
   constexpr int NG = G2 ? 2 : 1;
   __shared__ __align__(16) h8 ph[2 * U][KS][64], pl[2 * U][KS][64];
   __shared__ __align__(8) Cell cells[NG][kCells];
   __shared__ float bnd[NG][256];
   __shared__ float rowsq[D];
-  __shared__ TileWave<D> waves[WV];
+  __shared__ TileWave<D, ROT> waves[WV];
+
+  if constexpr (ROT) {
+    if (blockIdx.y == gridDim.y - 1 && a.rot.q) {
+      rotate_queries<D, NTHR>(a.rot, a.n, blockIdx.x, gridDim.x, threadIdx.x);
+      return;
+    }
+  }
 
   const auto& sd = a.side[blockIdx.y];
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
   const int wig = __builtin_amdgcn_readfirstlane(tid >> 6);
-  TileWave<D>& wv = waves[wig];
+  TileWave<D, ROT>& wv = waves[wig];
   const int bw = sd.bw;
   const QuantGroup2 none{};
   const QuantGroup2& s2 = second_group(sd, none);
@@ -270,14 +254,37 @@ __global__ __launch_bounds__(64 * tile_waves<G2>()) void quantize_tile_kernel(Ti
   }
   __syncthreads();  // the only block-wide barriers: waves run independently from here
 
+  // channels d .. d + 7 of the pass's row rr, whose elements start at xo
+  const auto fetch = [&](int rr, int64_t xo, int d) {
+    if constexpr (ROT) {
+      const RotRowInfo& o = wv.row[rr];
+      float y[8];
+      if (blockIdx.y == 0) {
+        rotated8<DT, CT>(a.rot, sd.x, xo, o.cs, o.sn, d, y);
+      } else {
+        const Raw8<DT> x = load8<DT>(sd.x, xo + d);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) y[k] = elem<DT>(x, k);
+      }
+      __builtin_amdgcn_sched_barrier(0);  // one eight's operands at a time: of all four they would spill
+      return __builtin_bit_cast(Raw8<XT>, y);
+    } else {
+      return load8<DT>(sd.x, xo + d);
+    }
+  };
+
   for (; pass < passes; pass += stride) {
     wave_lds_sync();  // the last pass's reads of the wave's LDS area are done
     if (lane < NR) {
       const int64_t vec = pass * NR + lane;
       const uint32_t vc = uint32_t(vec < a.total ? vec : a.total - 1);  // total < 2^31
       const uint32_t bh = vc / uint32_t(a.n), i = vc % uint32_t(a.n), b = bh / uint32_t(a.H), h = bh % uint32_t(a.H);
-      RowInfo& o = wv.row[lane];
+      auto& o = wv.row[lane];
       o.x = b * sd.sb + h * sd.sh + i * sd.sn;
+      if constexpr (ROT) {
+        o.cs = b * a.rot.csb + i * a.rot.csn;
+        o.sn = b * a.rot.ssb + i * a.rot.ssn;
+      }
       int64_t page = -1, norm = 0;
       if (vec < a.total) {
         if constexpr (G2) {
@@ -302,14 +309,14 @@ __global__ __launch_bounds__(64 * tile_waves<G2>()) void quantize_tile_kernel(Ti
     float r[NG], thr[NG];
     h8 xh[KS], xl[F32 ? KS : 1];
     {
-      Raw8<DT> x[KS];
-      const int64_t xo = wv.row[c].x + 8 * g;
+      Raw8<XT> x[KS];
+      const int64_t xo = wv.row[c].x;
 #pragma unroll
-      for (int s = 0; s < KS; ++s) x[s] = load8<DT>(sd.x, xo + 32 * s);
+      for (int s = 0; s < KS; ++s) x[s] = fetch(c, xo, 32 * s + 8 * g);
       float sc[NG];
 #pragma unroll
       for (int q = 0; q < NG; ++q) {
-        const float n = fmaxf(float(sqrt(sum_squares<DT, KS, G2>(x, q ? outl : ~outl))), 1e-10f);
+        const float n = fmaxf(float(sqrt(sum_squares<XT, KS, G2>(x, q ? outl : ~outl))), 1e-10f);
         if (g == 0) wv.row[c].n[q] = n;
         int e;
         frexpf(n, &e);
@@ -322,7 +329,7 @@ __global__ __launch_bounds__(64 * tile_waves<G2>()) void quantize_tile_kernel(Ti
       for (int s = 0; s < KS; ++s)
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const float z = elem<DT>(x[s], k) * (G2 && (outl >> (8 * s + k) & 1) ? sc[NG - 1] : sc[0]);
+          const float z = elem<XT>(x[s], k) * (G2 && (outl >> (8 * s + k) & 1) ? sc[NG - 1] : sc[0]);
           xh[s][k] = _Float16(z);
           if constexpr (F32) xl[s][k] = _Float16(z - float(xh[s][k]));
         }
@@ -382,7 +389,7 @@ __global__ __launch_bounds__(64 * tile_waves<G2>()) void quantize_tile_kernel(Ti
           }
         }
       }
-      *reinterpret_cast<uint2*>(code8<D>(wv, c, (D / 32) * g + u)) = make_uint2(word[0], word[1]);
+      *reinterpret_cast<uint2*>(code8(wv, c, (D / 32) * g + u)) = make_uint2(word[0], word[1]);
     }
     wave_lds_sync();  // codes, list, norms
     const bool all = flagged > kListMax;
@@ -394,12 +401,12 @@ __global__ __launch_bounds__(64 * tile_waves<G2>()) void quantize_tile_kernel(Ti
       const int q2 = G2 && dim >= split;  // the group
       const float n = wv.row[rr].n[q2], rn = 1.f / n;
       const bool divide = __any(!(n < 0x1p100f));  // wave-uniform
-      const int64_t xo = wv.row[rr].x + 8 * g;
+      const int64_t xo = wv.row[rr].x;
       const float* prow = sd.pi + dim * D + 8 * g;
       double sum = 0.0;
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-        const Raw8<DT> x = load8<DT>(sd.x, xo + 32 * s);
+        const Raw8<XT> x = fetch(rr, xo, 32 * s + 8 * g);
         const float4 p0 = *reinterpret_cast<const float4*>(prow + 32 * s);
         const float4 p1 = *reinterpret_cast<const float4*>(prow + 32 * s + 4);
         const float p[8] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
@@ -410,21 +417,21 @@ __global__ __launch_bounds__(64 * tile_waves<G2>()) void quantize_tile_kernel(Ti
         float z[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const float xv = elem<DT>(x, k), q = xv * rn;
+          const float xv = elem<XT>(x, k), q = xv * rn;
           z[k] = fmaf(fmaf(-q, n, xv), rn, q);
           if (G2 && int(outl >> (8 * s + k) & 1) != q2) z[k] = 0.f;
         }
         if (divide) {
           asm volatile("" ::: "memory");  // a branch: the divisions are not formed for a select
 #pragma unroll
-          for (int k = 0; k < 8; ++k) z[k] = G2 && int(outl >> (8 * s + k) & 1) != q2 ? 0.f : elem<DT>(x, k) / n;
+          for (int k = 0; k < 8; ++k) z[k] = G2 && int(outl >> (8 * s + k) & 1) != q2 ? 0.f : elem<XT>(x, k) / n;
         }
 #pragma unroll
         for (int k = 0; k < 8; ++k) sum = fma(double(z[k]), double(p[k]), sum);
       }
       sum += __shfl_xor(sum, 16, 64);
       sum += __shfl_xor(sum, 32, 64);
-      if (g == 0) code8<D>(wv, rr, dim >> 3)[dim & 7] = uint8_t(count_below(bnd[q2], q2 ? s2.bw : bw, float(sum)));
+      if (g == 0) code8(wv, rr, dim >> 3)[dim & 7] = uint8_t(count_below(bnd[q2], q2 ? s2.bw : bw, float(sum)));
     }
     wave_lds_sync();
     if constexpr (G2) {
@@ -438,7 +445,7 @@ __global__ __launch_bounds__(64 * tile_waves<G2>()) void quantize_tile_kernel(Ti
         uint32_t v = 0;
         for (int d = bit0 / w; first + d < end && d * w < bit0 + 8; ++d) {
           const int j = first + d, sh = d * w - bit0;
-          const uint32_t cd = code8<D>(wv, rr, j >> 3)[j & 7];
+          const uint32_t cd = code8(wv, rr, j >> 3)[j & 7];
           v |= sh >= 0 ? cd << sh : cd >> -sh;
         }
         if (q) s2.pages[row * nb2 + k - nb1] = uint8_t(v);
@@ -457,7 +464,7 @@ __global__ __launch_bounds__(64 * tile_waves<G2>()) void quantize_tile_kernel(Ti
       const int rr = it * RPI + lane / LPR, part = lane % LPR;
       const int64_t page = wv.row[rr].page;
       if (page < 0) continue;
-      const uint2 w = *reinterpret_cast<const uint2*>(code8<D>(wv, rr, part));
+      const uint2 w = *reinterpret_cast<const uint2*>(code8(wv, rr, part));
       if (!a.scatter) {
         *reinterpret_cast<uint2*>(sd.codes_out + page + 8 * part) = w;
         if (part == 0) sd.norms_out[wv.row[rr].norm] = wv.row[rr].n[0];
@@ -487,6 +494,19 @@ TileFn<G2> pick_tile(int dtype) {
   return dtype == WN_F32   ? quantize_tile_kernel<D, WN_F32, G2>
          : dtype == WN_F16 ? quantize_tile_kernel<D, WN_F16, G2>
                            : quantize_tile_kernel<D, WN_BF16, G2>;
+}
+
+template <int D, int DT>
+void (*pick_tile_rot(int rot_dtype))(QuantRotArgs) {
+  return rot_dtype == WN_F32   ? quantize_tile_kernel<D, DT, false, true, WN_F32>
+         : rot_dtype == WN_F16 ? quantize_tile_kernel<D, DT, false, true, WN_F16>
+                               : quantize_tile_kernel<D, DT, false, true, WN_BF16>;
+}
+template <int D>
+void (*pick_tile_rot(int dtype, int rot_dtype))(QuantRotArgs) {
+  return dtype == WN_F32   ? pick_tile_rot<D, WN_F32>(rot_dtype)
+         : dtype == WN_F16 ? pick_tile_rot<D, WN_F16>(rot_dtype)
+                           : pick_tile_rot<D, WN_BF16>(rot_dtype);
 }
 
 bool rows_aligned(const QuantSide& s, int es) {
@@ -523,6 +543,16 @@ static int launch_tiles(TileFn<G2> fn, const TileArgs<G2>& a, int sides, hipStre
 
 int launch_quantize_tiles(const QuantArgs& a, int sides, int D, hipStream_t st) {
   return launch_tiles<false>(D == 64 ? pick_tile<64, false>(a.x_dtype) : pick_tile<128, false>(a.x_dtype), a, sides, st);
+}
+
+// The rows of the grid (K, V, q) share the CUs.
+int launch_quantize_tiles(const QuantRotArgs& a, int sides, int D, hipStream_t st) {
+  const int cus = device_cus(), rows = sides + (a.rot.q != nullptr);
+  if (cus <= 0) return WN_E_LAUNCH;
+  const int64_t groups = std::min<int64_t>((a.total + kTileVecs - 1) / kTileVecs, std::max(1, cus / rows));
+  const auto fn = D == 64 ? pick_tile_rot<64>(a.x_dtype, a.rot.rot_dtype) : pick_tile_rot<128>(a.x_dtype, a.rot.rot_dtype);
+  hipLaunchKernelGGL(fn, dim3(unsigned(groups), rows), dim3(64 * tile_waves<false>()), 0, st, a);
+  return WN_OK;
 }
 
 bool quantize_split_ok(const QuantSplitArgs& a, int sides, int D) {

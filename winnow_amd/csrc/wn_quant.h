@@ -2,6 +2,8 @@
 // vectors per work-group, float64 rotation; quant_tile.hip: many vectors per wave).
 #pragma once
 
+#include <type_traits>
+
 #include "wn_common.h"
 
 namespace wn {
@@ -49,6 +51,130 @@ struct QuantSplitArgs : QuantArgsOf<QuantSplitSide> {
   int64_t cap;            // rows per (sequence, head)
 };
 
+// The position rotation of an append (wn_append_rotated_kv): K is rotated on its way into the
+// quantizer, and q beside it, by work-groups of its own.
+struct QuantRotary {
+  const void* cos;  // (B, n, R), a row per token, of rot_dtype
+  const void* sin;
+  int64_t csb, csn, ssb, ssn;  // element strides; of the batch 0 where it shares one table
+  const void* q;               // (B, Hq, n, D), or null
+  int64_t qsb, qsh, qsn;
+  void* q_out;                 // contiguous, q's type
+  int rot_dtype, R, q_dtype, Hq, B;
+  int q_vec;  // q, its output and the tables can be read by 16 bytes, eight channels and their partners at once
+  int k_vec;  // K and the tables can
+};
+
+struct QuantRotArgs : QuantArgs {
+  QuantRotary rot;
+};
+
+// Channel d of a rotated row, from the row's channels and its token's cos and sin:
+//   x_d cos_d - x_(d + R/2) sin_d   (d < R/2),   x_d cos_d + x_(d - R/2) sin_d   (d < R),   x_d
+// The products of fp32 values are exact in float64, so the sum is rounded once there and once to
+// fp32: the same bits whoever computes it.
+__device__ __forceinline__ float turn(float x, float partner, float c, float s) {
+  return float(fma(double(partner), double(s), double(x) * double(c)));
+}
+__device__ __forceinline__ float rotated_elem(const QuantRotary& r, const void* x, int64_t row, int x_dtype, int64_t co, int64_t so, int d) {
+  const float v = load_elem(x, row + d, x_dtype);
+  if (d >= r.R) return v;
+  const int half = r.R / 2;
+  const float p = load_elem(x, row + (d < half ? d + half : d - half), x_dtype);
+  return turn(v, d < half ? -p : p, load_elem(r.cos, co + d, r.rot_dtype), load_elem(r.sin, so + d, r.rot_dtype));
+}
+
+// Eight elements of a row as they are stored.
+template <int DT>
+struct Raw8 {
+  uint4 w[DT == WN_F32 ? 2 : 1];
+};
+template <int DT>
+__device__ __forceinline__ Raw8<DT> load8(const void* x, int64_t i) {
+  Raw8<DT> r;
+  if constexpr (DT == WN_F32) {
+    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const float*>(x) + i);
+    r.w[0] = p[0];
+    r.w[1] = p[1];
+  } else {
+    r.w[0] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + i);
+  }
+  return r;
+}
+template <int DT>
+__device__ __forceinline__ float elem(const Raw8<DT>& r, int k) {
+  const uint4 a = r.w[DT == WN_F32 ? k >> 2 : 0];
+  if constexpr (DT == WN_F32) {
+    const int j = k & 3;
+    return __builtin_bit_cast(float, j == 0 ? a.x : j == 1 ? a.y : j == 2 ? a.z : a.w);
+  } else {
+    const int j = k >> 1;
+    const uint32_t w = j == 0 ? a.x : j == 1 ? a.y : j == 2 ? a.z : a.w;
+    if constexpr (DT == WN_BF16) return __builtin_bit_cast(float, k & 1 ? w & 0xffff0000u : w << 16);
+    else return f16_to_f32(uint16_t(k & 1 ? w >> 16 : w));
+  }
+}
+
+// Channels d .. d + 7 of a rotated row (R and R / 2 multiples of 8: they and their partners are
+// eight in a row each). Of two 16-bit factors the products are exact in fp32 already, and the fused
+// sum there is the same value.
+template <int DT, int CT>
+__device__ __forceinline__ void rotated8(const QuantRotary& r, const void* x, int64_t row, int64_t co, int64_t so, int d, float (&y)[8]) {
+  const Raw8<DT> v = load8<DT>(x, row + d);
+  if (d >= r.R) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) y[k] = elem<DT>(v, k);
+    return;
+  }
+  const int half = r.R / 2;
+  const Raw8<DT> p = load8<DT>(x, row + (d < half ? d + half : d - half));
+  const Raw8<CT> c = load8<CT>(r.cos, co + d), s = load8<CT>(r.sin, so + d);
+  const uint32_t flip = d < half ? 0x80000000u : 0u;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const float q = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, elem<DT>(p, k)) ^ flip);
+    if constexpr (DT != WN_F32 && CT != WN_F32) y[k] = fmaf(q, elem<CT>(s, k), elem<DT>(v, k) * elem<CT>(c, k));
+    else y[k] = turn(elem<DT>(v, k), q, elem<CT>(c, k), elem<CT>(s, k));
+  }
+}
+
+// q's rows rotated, by the threads of `blocks` work-groups of NTHR. Rows are (b, h, i); eight
+// channels an item.
+template <int D, int NTHR>
+__device__ __forceinline__ void rotate_queries(const QuantRotary& r, int n, uint32_t block, uint32_t blocks, int tid) {
+  constexpr uint32_t EIGHTS = D / 8;
+  const uint32_t items = uint32_t(r.B) * uint32_t(r.Hq) * uint32_t(n) * EIGHTS;  // below 2^31 (the host's check)
+  for (uint32_t it = block * NTHR + tid; it < items; it += blocks * NTHR) {
+    const uint32_t row = it / EIGHTS, d = 8 * (it % EIGHTS), i = row % uint32_t(n), bh = row / uint32_t(n), h = bh % uint32_t(r.Hq),
+                   b = bh / uint32_t(r.Hq);
+    const int64_t qo = b * r.qsb + h * r.qsh + i * r.qsn, co = b * r.csb + i * r.csn, so = b * r.ssb + i * r.ssn;
+    const int64_t to = int64_t(row) * D + d;
+    float y[8];
+    if (r.q_vec) {
+      const auto by = [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        if (r.rot_dtype == WN_F32) rotated8<DT, WN_F32>(r, r.q, qo, co, so, d, y);
+        else if (r.rot_dtype == WN_BF16) rotated8<DT, WN_BF16>(r, r.q, qo, co, so, d, y);
+        else rotated8<DT, WN_F16>(r, r.q, qo, co, so, d, y);
+      };
+      if (r.q_dtype == WN_F32) by(std::integral_constant<int, WN_F32>{});
+      else if (r.q_dtype == WN_BF16) by(std::integral_constant<int, WN_BF16>{});
+      else by(std::integral_constant<int, WN_F16>{});
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) y[k] = rotated_elem(r, r.q, qo, r.q_dtype, co, so, d + k);
+    }
+    if (r.q_dtype == WN_F32) {  // the output is contiguous: rows of whole 16 bytes
+      __builtin_memcpy(__builtin_assume_aligned(static_cast<float*>(r.q_out) + to, 16), y, 32);
+    } else {
+      uint16_t o[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) o[k] = r.q_dtype == WN_BF16 ? f32_to_bf16(y[k]) : f32_to_f16(y[k]);
+      __builtin_memcpy(__builtin_assume_aligned(static_cast<uint16_t*>(r.q_out) + to, 16), o, 16);
+    }
+  }
+}
+
 // pos[k] = #{b < y[k]} over the 2^bw - 1 ascending boundaries (torch.bucketize,
 // right=False), for N values at once: the N binary searches advance in lockstep, so
 // each level issues N independent LDS reads instead of one dependent read per value.
@@ -86,6 +212,7 @@ __device__ __forceinline__ void store_packed8(uint8_t* p, uint64_t v, int bw) {
 // quant_tile.hip: whether its kernel serves these operands, and its launch (0: launched).
 bool quantize_tiles_ok(const QuantArgs& a, int sides, int D);
 int launch_quantize_tiles(const QuantArgs& a, int sides, int D, hipStream_t st);
+int launch_quantize_tiles(const QuantRotArgs& a, int sides, int D, hipStream_t st);
 // The same kernel with two groups of channels, rows of a contiguous cache (quant.hip's
 // wn_append_split).
 bool quantize_split_ok(const QuantSplitArgs& a, int sides, int D);

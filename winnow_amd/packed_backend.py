@@ -231,6 +231,59 @@ class AppendPlan:
                 _lib.call("wn_append_kv", *args, _lib.stream_of(self.device), ev0, ev1)
 
 
+    def bind_rotation(self, q: torch.Tensor | None, cos: torch.Tensor, sin: torch.Tensor, bound: tuple) -> tuple:
+        """Check what ``launch_rotated`` takes beside ``bind``'s operands."""
+        B, n, D = bound[4], bound[5], self.D
+        for name, t in (("cos", cos), ("sin", sin)):
+            if t.dim() != 3 or t.shape[0] not in (1, B) or t.shape[1] != n or t.dtype not in _lib.DTYPE_CODE \
+                    or not t.is_cuda or t.get_device() != self.dev_index:
+                raise pa.UnsupportedLayout(f"append: {name} must be ({B}, {n}, R) or (1, {n}, R) fp32/fp16/bf16 on {self.device}, "
+                                           f"got {tuple(t.shape)} {t.dtype} on {t.device}")
+        R = cos.shape[2]
+        if sin.shape != cos.shape or sin.dtype != cos.dtype or not 2 <= R <= D or R % 2:
+            raise pa.UnsupportedLayout(f"append: cos {tuple(cos.shape)} {cos.dtype} and sin {tuple(sin.shape)} {sin.dtype} must be alike and "
+                                       f"rotate an even number of the {D} channels")
+        if cos.stride(2) != 1 or sin.stride(2) != 1:
+            raise pa.UnsupportedLayout("append: cos and sin need contiguous rows")
+        if q is not None:
+            if not q.is_cuda or q.get_device() != self.dev_index:
+                raise pa.UnsupportedLayout("append: every operand must be on one HIP device")
+            if q.dim() != 4 or q.shape[0] != B or q.shape[1] < 1 or q.shape[2] != n or q.shape[3] != D or q.dtype not in _lib.DTYPE_CODE \
+                    or q.stride(3) != 1:
+                raise pa.UnsupportedLayout(f"append: q must be ({B}, Hq, {n}, {D}) fp32/fp16/bf16 with a contiguous head_dim, got "
+                                           f"{tuple(q.shape)} {q.dtype}")
+            if q.numel() >= 8 * (2 ** 30 - 1):
+                raise pa.UnsupportedLayout("append: q of 2^33 elements or more")
+        return q, cos, sin, R
+
+    def launch_rotated(self, bound: tuple, rotation: tuple, timing_events=None) -> torch.Tensor | None:
+        """``launch`` with K rotated on the way (``wn_append_rotated_kv``); returns the rotated q."""
+        k, v, page_table, start_pos, B, n = bound
+        q, cos, sin, R = rotation
+        out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        if B == 0 or n == 0:
+            return out
+        ks = k.stride()
+        if v is not None:
+            vs = v.stride()
+            vargs = (v.data_ptr(), vs[0], vs[1], vs[2])
+        else:
+            vargs = (None, 0, 0, 0)
+        if q is not None:
+            qs = q.stride()
+            qargs = (q.data_ptr(), qs[0], qs[1], qs[2], _lib.DTYPE_CODE[q.dtype], q.shape[1], out.data_ptr())
+        else:
+            qargs = (None, 0, 0, 0, 0, 0, None)
+        cs, ss, shared = cos.stride(), sin.stride(), cos.shape[0] == 1
+        ev0, ev1 = timing_events or (None, None)
+        with _lib.on(self.device):
+            _lib.call("wn_append_rotated_kv", *qargs, cos.data_ptr(), 0 if shared else cs[0], cs[1], sin.data_ptr(), 0 if shared else ss[0], ss[1],
+                      _lib.DTYPE_CODE[cos.dtype], R, k.data_ptr(), ks[0], ks[1], ks[2], *vargs, _lib.DTYPE_CODE[k.dtype], *self._quant,
+                      page_table.data_ptr(), page_table.stride(0), start_pos.data_ptr(), *self._store,
+                      B, self.Hkv, n, self.D, self.S, self.P, page_table.shape[1], _lib.stream_of(self.device), ev0, ev1)
+        return out
+
+
 # AppendPlans of the layers of live pools, built on a layer's first append and kept
 # with the pool tensors they were built on (a plan is rebuilt if those are replaced)
 _APPEND_PLANS: "weakref.WeakKeyDictionary[PagePool, dict]" = weakref.WeakKeyDictionary()
@@ -283,6 +336,44 @@ def append_kv(k: torch.Tensor, v: torch.Tensor | None, k_tq, v_tq,
         start = start_pos_host if start_pos_host is not None else start_pos.cpu()
         _positions_in_range(start, table, bound[5], plan.P, plan.S)
     plan.launch(bound, timing_events)
+
+
+def append_rotated_kv(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor | None, cos: torch.Tensor, sin: torch.Tensor, k_tq, v_tq,
+                      k_pages: torch.Tensor, v_pages: torch.Tensor | None,
+                      k_norms: torch.Tensor, v_norms: torch.Tensor | None,
+                      page_table: torch.Tensor, start_pos: torch.Tensor, *,
+                      page_table_host: torch.Tensor | None = None,
+                      start_pos_host: torch.Tensor | None = None,
+                      check_ranges: bool = True, timing_events=None) -> torch.Tensor | None:
+    """``append_kv`` of K (and V) as a model's projections leave them, with the position rotation
+    applied on the way, and q's beside it, in one launch (``wn_append_rotated_kv``).
+
+    ``cos`` and ``sin`` (B, n, R), or (1, n, R) for one table for all, fp32/fp16/bf16, are the new
+    tokens' as a rotary embedding gives them (the model's ``position_embeddings``). The first R
+    channels of K and of ``q`` (B, Hq, n, D) are rotated, channel d with channel d + R / 2:
+
+        x_d cos_d - x_(d + R/2) sin_d  (d < R/2),    x_d cos_d + x_(d - R/2) sin_d  (R/2 <= d < R)
+
+    Each product is exact and the sum is rounded once to fp32: the pages hold what ``append_kv``
+    writes for that fp32 K, bit for bit, and the returned q, (B, Hq, n, D) contiguous, is rounded
+    once more to its type (None without q). A model that rotates K itself rounds it to its own
+    type before it is quantized.
+
+    Raises as ``append_kv``, and for tables that do not fit; a gradient, a tangent or a trace is
+    refused."""
+    pa.values_only("append_rotated_kv", *(t for t in (q, k, v, cos, sin) if t is not None))
+    if v is not None and (v_pages is None or v_norms is None):
+        raise pa.UnsupportedLayout("append: V needs its pages and norms")
+    has_v = v is not None
+    plan = AppendPlan(k_tq, v_tq if has_v else None, k_pages, v_pages if has_v else None,
+                      k_norms, v_norms if has_v else None)
+    bound = plan.bind(k, v, page_table, start_pos)
+    rotation = plan.bind_rotation(q, cos, sin, bound)
+    if check_ranges:
+        table = page_table_host if page_table_host is not None else page_table.cpu()
+        start = start_pos_host if start_pos_host is not None else start_pos.cpu()
+        _positions_in_range(start, table, bound[5], plan.P, plan.S)
+    return plan.launch_rotated(bound, rotation, timing_events)
 
 
 COMMIT_DTYPES = (torch.uint8, *pa.DENSE_PAGE_DTYPES)
