@@ -522,6 +522,37 @@ int wn_append_rotated_kv(
     int B, int Hkv, int n, int D, int S, int num_pages, int max_pages,
     void* stream, void* ev_begin, void* ev_end);
 
+/* Attention over paged packed K/V under a sliding window with sinks, Q >= 1 queries per sequence, which
+ * are its last Q positions: the query at position p sees the positions j <= p with p - j < window
+ * or j < sinks; one that sees none (p < 0) gives 0.
+ *   q    (B, Hq, Q, D) with element strides, last dim contiguous, type q_dtype
+ *   out  (B, Hq, Q, D) contiguous, type out_dtype
+ * The algebra, pages, norms, table, rotations, `exact` and alignments are those of wn_tree_attention;
+ * n_rep * Q <= 2^20, S a power of two >= 16. Pages that no query of the call sees are not used: their
+ * ids may be any value. num_splits and span come from wn_window_plan; any num_splits 1 .. 4096 and
+ * any span that is a multiple of 64 are valid for any lengths. Lengths are taken as within [0,
+ * max_pages * S]; an id outside [0, num_pages) reads the last page (the Python layer refuses one that
+ * a query would see). ev_begin / ev_end (hipEvent_t or NULL) are recorded around the scan kernel. */
+int wn_window_plan(int B, int Hq, int Hkv, int Q, int D, int S, int bw_k, int bw_v, int exact, int max_pages, int window, int sinks,
+                   const int32_t* lens, int* num_splits, int* span);
+int64_t wn_window_workspace_bytes(int B, int Hq, int Hkv, int Q, int D, int num_splits);
+int wn_window_attention(
+    const void* q, int q_dtype, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_q,
+    const float* pi_k, const float* pi_v, const float* codebook_k, const float* codebook_v,
+    const uint8_t* k_pages, int64_t k_stride_p, int64_t k_stride_h,
+    const uint8_t* v_pages, int64_t v_stride_p, int64_t v_stride_h,
+    const uint16_t* k_norms, int64_t kn_stride_p, int64_t kn_stride_h,
+    const uint16_t* v_norms, int64_t vn_stride_p, int64_t vn_stride_h,
+    const int32_t* page_table, int64_t table_stride_b, const int32_t* seq_lens,
+    void* out, int out_dtype, void* workspace, int64_t workspace_bytes,
+    int B, int Hq, int Hkv, int Q, int D, int S, int bw_k, int bw_v, int num_pages, int max_pages,
+    int window, int sinks, float scale, int exact, int num_splits, int span, void* stream, void* ev_begin, void* ev_end);
+
+/* Host check of host memory, no launch: 1 if every length lies in [0, max_pages * S] and every page that
+ * a query of wn_window_attention sees in 0 .. num_pages - 1, else 0. */
+int wn_window_in_range(const int32_t* lens, const int32_t* page_table, int64_t table_stride_b, int B, int max_pages, int num_pages,
+                       int S, int Q, int window, int sinks);
+
 /* Penalties, biases and a mask applied to N rows of V logits (contiguous along V, row strides in
  * elements) in one pass; out may be logits itself, with its stride. Per row, in fp32, rounded once:
  *   history (N, H) int32, of which the first lengths[r] (null: H; clipped to [0, H]) count; a token

@@ -145,3 +145,96 @@ def test_append_c_abi():
         with pytest.raises(_lib.WinnowHipError, match=match):
             call(**kw)
     call(n=0, k=None, cos=None)
+
+
+# --------------------------------------------------------------------- windowed attention
+
+def _kv(D=64, P=6, Hkv=2, S=16, bw=4, B=2, lens=(20, 33)):
+    quant = pa.Quantizer(torch.eye(D), torch.linspace(-1, 1, 2 ** bw), bw)
+    pages, norms = torch.zeros(P, Hkv, S, D * bw // 8, dtype=torch.uint8), torch.ones(P, Hkv, S, dtype=torch.float16)
+    table = torch.tensor([[0, 1, -1], [2, 3, 4]], dtype=torch.int32)[:B]
+    return pa.PackedKV(pages, norms, pages.clone(), norms.clone(), table, torch.tensor(lens, dtype=torch.int32), quant, quant, D)
+
+
+def _window(q=None, kv=None, window=8, sinks=2, **kw):
+    return pa.packed_window_attention(torch.zeros(2, 4, 5, 64) if q is None else q, kv or _kv(), 0.1, window=window, sinks=sinks, **kw)
+
+
+def test_window_needs_a_gpu():
+    with pytest.raises(pa.UnsupportedLayout, match="HIP device"):
+        _window()
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(window=0), "at least 1"), (dict(window=-5), "at least 1"), (dict(sinks=-1), "at least"), (dict(window=2.5), "whole"), (dict(window=True), "whole"),
+    (dict(q=torch.zeros(2, 4, 0, 64)), "queries a sequence"), (dict(q=torch.zeros(2, 3, 5, 64)), "multiple"),
+    (dict(q=torch.zeros(1, 1, 1, 64).expand(2, 4, 2 ** 20, 64)), "queries a sequence"),
+    (dict(q=torch.zeros(2, 4, 64, 5).transpose(2, 3)), "contiguous head_dim"), (dict(q=torch.zeros(2, 4, 5, 64, dtype=torch.float64)), "fp32/fp16/bf16"),
+    (dict(q=torch.zeros(2, 4, 5, 64, requires_grad=True)), "no gradient"), (dict(out_dtype=torch.float64), "output dtype"),
+    (dict(q=torch.zeros(2, 4, 5, 8), kv=_kv(D=8)), "head_dim 8"), (dict(kv=_kv(S=24, lens=(3, 4))), "power of two"),
+    (dict(kv=_kv(lens=(20, 49))), "out of range"), (dict(kv=_kv(lens=(-1, 4))), "out of range")])
+def test_window_operands(as_hip, kw, match):
+    with pytest.raises(pa.UnsupportedLayout, match=match):
+        _window(**kw)
+
+
+def _in_range(lens, table, P, S, Q, window, sinks):
+    """Page by page, from the definition."""
+    for L, row in zip(lens.tolist(), table.tolist()):
+        if not 0 <= L <= len(row) * S:
+            return False
+        for j in range(L):
+            if any(j <= p and (p - j < window or j < sinks) for p in range(L - Q, L)) and not 0 <= row[j // S] < P:
+                return False
+    return True
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_window_ranges_are_those_in_view(monkeypatch, native):
+    """Random lengths, tables with ids out of range here and there, windows and sinks: a call is refused
+    exactly where a page in view is."""
+    lib = _lib.lib()
+    if not native:
+        monkeypatch.setattr(_lib, "_lib", None)
+    g = torch.Generator().manual_seed(3)
+    seen = set()
+    for _ in range(400):
+        r = lambda lo, hi: int(torch.randint(lo, hi, (1,), generator=g))  # noqa: E731
+        S, width, P, Q = 2 ** r(0, 4), r(1, 7), 5, r(1, 6)
+        lens = torch.randint(-1 if r(0, 9) == 0 else 0, width * S + (2 if r(0, 9) == 0 else 1), (2,), generator=g).int()
+        table = torch.randint(0, P, (2, width), generator=g).int()
+        if r(0, 3):
+            table[r(0, 2), r(0, width)] = (-1, P, 2 ** 31 - 1)[r(0, 3)]
+        window, sinks = r(1, 20), r(0, 9)
+        ok = _in_range(lens, table, P, S, Q, window, sinks)
+        seen.add(ok)
+        if native:
+            assert bool(lib.wn_window_in_range(lens.data_ptr(), table.data_ptr(), width, 2, width, P, S, Q, window, sinks)) == ok
+        if ok:
+            pa.check_window_ranges(lens, table, P, S, Q, window, sinks)
+        else:
+            with pytest.raises(pa.UnsupportedLayout):
+                pa.check_window_ranges(lens, table, P, S, Q, window, sinks)
+    assert seen == {True, False}
+
+
+def test_window_c_abi():
+    """Nothing is launched for arguments outside the contract."""
+    x = torch.zeros(4096)
+    p = x.data_ptr()
+
+    def call(**kw):
+        a = dict(q=p, qd=0, qb=0, qh=0, qq=0, pik=p, piv=p, cbk=p, cbv=p, kp=p, kpp=0, kph=0, vp=p, vpp=0, vph=0, knp=p, knpp=0, knph=0, vnp=p, vnpp=0,
+                 vnph=0, table=p, ts=0, lens=p, out=p, od=0, ws=None, wb=0, B=1, Hq=4, Hkv=2, Q=1, D=64, S=16, bwk=4, bwv=4, P=1, mp=4, window=8,
+                 sinks=0, scale=0.1, exact=1, ns=1, span=64)
+        a.update(kw)
+        _lib.call("wn_window_attention", *a.values(), None, None, None)
+    for kw, match in ((dict(window=0), "at least 1"), (dict(sinks=-1), "sinks"), (dict(Hq=3), "need"), (dict(Q=0), "need"), (dict(Q=2 ** 20), "need"),
+                      (dict(D=96), "need"), (dict(bwk=7), "widths"), (dict(S=8), "page size"), (dict(ns=0), "num_splits"), (dict(ns=4097), "num_splits"),
+                      (dict(span=32), "span"), (dict(mp=0), "max_pages"), (dict(mp=2 ** 30), "max_pages"), (dict(kp=p + 2), "4-byte"), (dict(kph=6), "4-byte"),
+                      (dict(vnpp=-1), "negative"), (dict(q=None), "null"), (dict(out=p + 1), "aligned"), (dict(), "workspace"), (dict(od=5), "dtype")):
+        with pytest.raises(_lib.WinnowHipError, match=match):
+            call(**kw)
+    call(B=0, q=None)
+    assert _lib.lib().wn_window_workspace_bytes(1, 3, 2, 1, 64, 1) == -1
+    assert _lib.lib().wn_window_workspace_bytes(1, 4, 2, 1, 64, 0) == -1

@@ -201,6 +201,22 @@ SIGNATURES = {
         _c_p, _c_p, _c_p, _c_p, _c_p,               # tokens, logprob, entropy, top_logprobs, top_ids
         _c_i64, _c_i, _c_i, _c_p, _c_i64,           # N, V, top, workspace, bytes
         _c_p]),
+    "wn_window_plan": (_c_i, [_c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_p,
+                              ctypes.POINTER(_c_i), ctypes.POINTER(_c_i)]),
+    "wn_window_workspace_bytes": (_c_i64, [_c_i, _c_i, _c_i, _c_i, _c_i, _c_i]),
+    "wn_window_attention": (_c_i, [
+        _c_p, _c_i, _c_i64, _c_i64, _c_i64,         # q, dtype, strides (b, h, q)
+        _c_p, _c_p, _c_p, _c_p,                     # pi_k, pi_v, codebooks
+        _c_p, _c_i64, _c_i64,                       # k pages
+        _c_p, _c_i64, _c_i64,                       # v pages
+        _c_p, _c_i64, _c_i64,                       # k norms
+        _c_p, _c_i64, _c_i64,                       # v norms
+        _c_p, _c_i64, _c_p,                         # table, stride, seq_lens
+        _c_p, _c_i, _c_p, _c_i64,                   # out, out dtype, workspace
+        _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i,   # B Hq Hkv Q D S bwk bwv num_pages max_pages
+        _c_i, _c_i, _c_f, _c_i, _c_i, _c_i,         # window, sinks, scale, exact, num_splits, span
+        _c_p, _c_p, _c_p]),                         # stream, ev_begin, ev_end
+    "wn_window_in_range": (_c_i, [_c_p, _c_p, _c_i64, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i]),
     "wn_adjust_logits": (_c_i, [
         _c_p, _c_i, _c_i64, _c_p, _c_i64, _c_i64, _c_i,   # logits, dtype, stride, out, stride, N, V
         _c_p, _c_i64, _c_i, _c_p, _c_p,             # history, stride, H, lengths, prompt_lengths
@@ -327,6 +343,16 @@ def positions_in_range(start: torch.Tensor, table: torch.Tensor, n: int | None, 
     B, width = table.shape
     return bool(_lib.wn_positions_in_range(start.data_ptr(), n is None, n or 0, table.data_ptr(), table.stride(0),
                                            B, width, num_pages, page_size))
+
+
+def window_in_range(lens: torch.Tensor, table: torch.Tensor, num_pages: int, page_size: int, queries: int, window: int, sinks: int) -> bool:
+    """Whether the loaded library finds every length and every page in view of the last ``queries``
+    positions in range (``wn_window_in_range``, int32 host tensors); False also where it cannot say."""
+    if _lib is None or table.dim() != 2 or lens.shape != table.shape[:1] or not (host_int32(lens) and host_int32(table)):
+        return False
+    B, width = table.shape
+    return bool(_lib.wn_window_in_range(lens.data_ptr(), table.data_ptr(), table.stride(0), B, width, num_pages, page_size,
+                                        queries, window, sinks))
 
 
 def parents_in_order(parents: torch.Tensor) -> bool:

@@ -18,6 +18,22 @@ extern "C" int wn_positions_in_range(const int32_t* start, int lengths, int n, c
   return 1;
 }
 
+extern "C" int wn_window_in_range(const int32_t* lens, const int32_t* page_table, int64_t table_stride_b, int B, int max_pages,
+                                  int num_pages, int S, int Q, int window, int sinks) {
+  if (!lens || !page_table || B < 0 || max_pages < 0 || S <= 0 || Q < 0 || window < 1 || sinks < 0) return 0;
+  for (int b = 0; b < B; ++b) {
+    const int64_t L = lens[b];
+    if (L < 0 || L > int64_t(max_pages) * S) return 0;
+    const int64_t lo = L - Q + 1 > window ? L - Q + 1 - window : 0, sink = sinks < L ? sinks : L;
+    const int32_t* row = page_table + b * table_stride_b;
+    for (int64_t c = 0; c * S < sink; ++c)
+      if (row[c] < 0 || row[c] >= num_pages) return 0;
+    for (int64_t c = lo / S; c * S < L; ++c)
+      if (row[c] < 0 || row[c] >= num_pages) return 0;
+  }
+  return 1;
+}
+
 extern "C" int wn_parents_in_order(const int32_t* parents, int64_t parents_stride_b, int B, int T) {
   if (!parents || B < 0 || T < 0) return 0;
   for (int b = 0; b < B; ++b)

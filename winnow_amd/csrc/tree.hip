@@ -1,18 +1,12 @@
 // Host side of the tree attention (wn_tree.h).
 #include <algorithm>
-#include <map>
-#include <mutex>
-#include <utility>
 
-#include "wn_tree.h"
+#include "wn_tree_host.h"
 
 namespace wn {
 namespace {
 
 constexpr int kTreeNodes = 64;
-// Tiles of 16 rows from which a work-group merges a whole one (4 rows each below: 16 tiles merged from
-// 10 splits took 7.7 us a tile to a work-group, 6.0 us in fours).
-constexpr int64_t kMergeTiles = 256;
 
 TreeKernels pick_tree(int D, bool exact, int bw_k, int bw_v) {
   switch (D) {
@@ -51,53 +45,6 @@ bool rows_wide(int bw_k, const void* k_pages, int64_t k_stride_p, int64_t k_stri
 TreeScan tree_variant(int D, bool exact, bool wide, int bw_k, int bw_v, int64_t rows, int64_t tokens) {
   if (rows_serve(D, exact, wide, bw_k, bw_v, rows, tokens)) return tree_rows_scan(bw_k, bw_v);
   return pick_tree(D, exact, bw_k, bw_v).scan[rows <= 32 ? 0 : rows <= 64 ? 1 : 2];
-}
-
-// Query rows per kv head, padded to whole work-groups.
-int tree_nrp(const TreeScan& s, int64_t rows) { return int((rows + s.rows - 1) / s.rows * s.rows); }
-
-int64_t align256(int64_t x) { return (x + 255) & ~int64_t(255); }
-
-struct TreeLayout {
-  int64_t qh, ql, qs, vis, acc, ml, total;
-};
-
-TreeLayout tree_layout(int B, int Hkv, int nrp, int T, int D, int num_splits) {
-  TreeLayout l;
-  const int64_t rows = int64_t(B) * Hkv * nrp;
-  l.qh = 0;
-  l.ql = l.qh + align256(rows * D * 2);
-  l.qs = l.ql + align256(rows * D * 2);
-  l.vis = l.qs + align256(rows * 4);
-  l.acc = l.vis + align256(int64_t(B) * T * 8);
-  l.ml = l.acc + align256(rows * num_splits * D * 4);
-  l.total = l.ml + align256(rows * num_splits * 2 * 4);
-  return l;
-}
-
-// Resident work-groups of a scan on the current device (0: the query failed), asked for
-// once per device, kernel and LDS size; the kernel is allowed that much LDS.
-int tree_slots(const TreeScan& s, int lds) {
-  static std::mutex mu;
-  static std::map<std::pair<std::pair<int, TreeScanFn>, int>, int> cache;
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess) return 0;
-  std::lock_guard<std::mutex> lock(mu);
-  auto it = cache.find({{dev, s.fn}, lds});
-  if (it != cache.end()) return it->second;
-  int per_cu = 0;
-  const void* f = reinterpret_cast<const void*>(s.fn);
-  if ((lds && hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != hipSuccess) ||
-      hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, f, s.threads, lds) != hipSuccess)
-    return 0;
-  const int n = per_cu * device_cus();
-  cache[{{dev, s.fn}, lds}] = n;
-  return n;
-}
-
-int tree_lds(const TreeScan& s, int bw_k, int bw_v) {
-  if (s.waves) return 0;  // static
-  return std::max(s.give, s.lds + (s.tables ? s.tables : tree_table_bytes(bw_k) + tree_table_bytes(bw_v)));
 }
 
 bool tree_shape(int B, int Hq, int Hkv, int T, int D) {

@@ -1,0 +1,231 @@
+// Attention over paged packed K/V under a sliding window with sinks, for gfx950: the Q queries of a
+// sequence are its last Q positions, and the one at position p sees the positions j <= p with
+// p - j < window or j < sinks,
+//   out = softmax(scale q . k_hat) v_hat,   k_hat = n_K (c_K Pi_K),   v_hat = n_V (c_V Pi_V).
+//
+// Host side. The kernels are the tree attention's (wn_tree.h, wn_tree_kernels.h), compiled for this
+// choice of keys: q' = q Pi_K^T once, a scan of the chunks that some query of a row block sees, split
+// where there are few blocks, and a merge with Pi_V. A row block's chunks are those of the sinks and
+// those from its first query's window to its last query (window_span): what lies between is not
+// read, so a call costs the window, not the context.
+#include "wn_tree_host.h"
+
+namespace wn {
+namespace {
+
+WindowKernels pick_window(int D, bool exact, int bw_k, int bw_v) {
+  switch (D) {
+    case 16: return window_kernels_16(exact, bw_k, bw_v);
+    case 32: return window_kernels_32(exact, bw_k, bw_v);
+    case 64: return window_kernels_64(exact, bw_k, bw_v);
+    case 128: return window_kernels_128(exact, bw_k, bw_v);
+    case 256: return window_kernels_256(exact, bw_k, bw_v);
+    default: return WindowKernels{};
+  }
+}
+
+int window_chunk(int D) { return D == 256 ? 32 : 64; }  // tokens of a scan's chunk
+
+int window_variant(int64_t rows) { return rows <= 32 ? 0 : rows <= 64 ? 1 : 2; }
+
+bool window_shape(int B, int Hq, int Hkv, int Q, int D) {
+  return B >= 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && Q > 0 && valid_head_dim(D) && int64_t(Hq / Hkv) * Q <= (1 << 20);
+}
+
+}  // namespace
+}  // namespace wn
+
+extern "C" int wn_window_plan(int B, int Hq, int Hkv, int Q, int D, int S, int bw_k, int bw_v, int exact, int max_pages, int window,
+                              int sinks, const int32_t* lens, int* num_splits, int* span) {
+  using namespace wn;
+  clear_error();
+  WN_REQUIRE(window_shape(B, Hq, Hkv, Q, D) && max_pages > 0 && int64_t(max_pages) * S <= INT32_MAX - 256 && window > 0 && sinks >= 0 &&
+                 num_splits && span,
+             WN_E_INVALID, "wn_window_plan: bad sizes B=%d Hq=%d Hkv=%d Q=%d D=%d max_pages=%d window=%d sinks=%d", B, Hq, Hkv, Q, D,
+             max_pages, window, sinks);
+  WN_REQUIRE(is_pow2(S) && S >= 16 && valid_bw(bw_k) && valid_bw(bw_v), WN_E_UNSUPPORTED,
+             "wn_window_plan: (S=%d, bw_k=%d, bw_v=%d) not compiled", S, bw_k, bw_v);
+  const int n_rep = Hq / Hkv, ch = window_chunk(D);
+  const int64_t rows = int64_t(n_rep) * Q;
+  const auto scan = pick_window(D, exact != 0, bw_k, bw_v).scan[window_variant(rows)];
+  const int64_t slots = tree_slots(scan, tree_lds(scan, bw_k, bw_v));
+  WN_REQUIRE(slots > 0, WN_E_LAUNCH, "wn_window_plan: cannot query the device occupancy");
+  const int blocks = tree_nrp(scan, rows) / scan.rows;
+  const int n = lens ? B : 1;
+  const int64_t each = (lens ? 1 : std::max(B, 1)) * int64_t(Hkv) * blocks;  // work-groups per entry of lens and split
+  // chunks of a sequence's last row block: the others have as many, or fewer
+  auto chunks = [&](int b) {
+    const int L = int(std::min<int64_t>(std::max(lens ? lens[b] : max_pages * S, 0), int64_t(max_pages) * S));
+    return int64_t(std::max(window_span(L, Q, n_rep, (blocks - 1) * scan.rows, scan.rows, ch, window, sinks, 1, ch).total, 1));
+  };
+  int64_t longest = 1;
+  for (int b = 0; b < n; ++b) longest = std::max(longest, chunks(b));
+  // For one to four rounds of the slots, the smallest split whose count over the batch fits; the least
+  // of rounds times (split and its fixed cost: tables, query, partials, about four chunks).
+  int64_t best = 0, best_cost = 0;
+  for (int64_t rounds = 1; rounds <= 4; ++rounds) {
+    int64_t lo = 1, hi = longest;
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) / 2;
+      int64_t count = 0;
+      for (int b = 0; b < n; ++b) count += (chunks(b) + mid - 1) / mid;
+      if (count * each <= rounds * slots) hi = mid;
+      else lo = mid + 1;
+    }
+    const int64_t cost = rounds * (lo + 4);
+    if (!best || cost < best_cost) {
+      best = lo;
+      best_cost = cost;
+    }
+  }
+  best = std::max(best, (longest + 255) / 256);
+  if (ch < 64) best = (best + 1) / 2 * 2;
+  *span = int(ch * best);
+  *num_splits = int((longest + best - 1) / best);
+  return WN_OK;
+}
+
+extern "C" int64_t wn_window_workspace_bytes(int B, int Hq, int Hkv, int Q, int D, int num_splits) {
+  using namespace wn;
+  if (!window_shape(B, Hq, Hkv, Q, D) || num_splits <= 0) return -1;
+  const int64_t rows = int64_t(Hq / Hkv) * Q;
+  const auto scan = pick_window(D, false, 8, 8).scan[window_variant(rows)];
+  return tree_layout(B, Hkv, tree_nrp(scan, rows), 0, D, num_splits).total;
+}
+
+extern "C" int wn_window_attention(
+    const void* q, int q_dtype, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_q,
+    const float* pi_k, const float* pi_v, const float* codebook_k, const float* codebook_v,
+    const uint8_t* k_pages, int64_t k_stride_p, int64_t k_stride_h,
+    const uint8_t* v_pages, int64_t v_stride_p, int64_t v_stride_h,
+    const uint16_t* k_norms, int64_t kn_stride_p, int64_t kn_stride_h,
+    const uint16_t* v_norms, int64_t vn_stride_p, int64_t vn_stride_h,
+    const int32_t* page_table, int64_t table_stride_b, const int32_t* seq_lens,
+    void* out, int out_dtype, void* workspace, int64_t workspace_bytes,
+    int B, int Hq, int Hkv, int Q, int D, int S, int bw_k, int bw_v, int num_pages, int max_pages,
+    int window, int sinks, float scale, int exact, int num_splits, int span, void* stream, void* ev_begin, void* ev_end) {
+  using namespace wn;
+  clear_error();
+  WN_REQUIRE(window_shape(B, Hq, Hkv, Q, D), WN_E_INVALID,
+             "window: need B>=0, Hq%%Hkv==0, Q>0, n_rep*Q<=2^20, D a power of two 16..256 (B=%d Hq=%d Hkv=%d Q=%d D=%d)", B, Hq, Hkv, Q, D);
+  WN_REQUIRE(valid_bw(bw_k) && valid_bw(bw_v), WN_E_UNSUPPORTED, "window: bit widths %d/%d not compiled", bw_k, bw_v);
+  WN_REQUIRE(is_pow2(S) && S >= 16, WN_E_INVALID, "window: page size %d is not a power of two >= 16", S);
+  WN_REQUIRE(q_dtype >= WN_F32 && q_dtype <= WN_BF16 && out_dtype >= WN_F32 && out_dtype <= WN_BF16, WN_E_INVALID,
+             "window: dtype codes %d/%d", q_dtype, out_dtype);
+  WN_REQUIRE(window > 0 && sinks >= 0, WN_E_INVALID, "window: window %d (at least 1), sinks %d", window, sinks);
+  WN_REQUIRE(num_splits > 0 && num_splits <= 4096 && span > 0 && span % 64 == 0, WN_E_INVALID, "window: num_splits %d, span %d",
+             num_splits, span);
+  WN_REQUIRE(num_pages > 0 && max_pages > 0 && int64_t(max_pages) * S <= INT32_MAX - 256, WN_E_INVALID,
+             "window: num_pages %d, max_pages %d", num_pages, max_pages);
+  if (B == 0) return WN_OK;
+  WN_REQUIRE(q && pi_k && pi_v && codebook_k && codebook_v && k_pages && v_pages && k_norms && v_norms && page_table && seq_lens && out,
+             WN_E_INVALID, "window: null operand");
+  WN_REQUIRE(aligned(k_pages, 4) && aligned(v_pages, 4) && k_stride_p % 4 == 0 && k_stride_h % 4 == 0 && v_stride_p % 4 == 0 &&
+                 v_stride_h % 4 == 0,
+             WN_E_INVALID, "window: pages need a 4-byte aligned base and strides");
+  WN_REQUIRE(k_stride_p >= 0 && v_stride_p >= 0 && k_stride_h >= 0 && v_stride_h >= 0 && kn_stride_p >= 0 && kn_stride_h >= 0 &&
+                 vn_stride_p >= 0 && vn_stride_h >= 0 && table_stride_b >= 0,
+             WN_E_INVALID, "window: negative stride");
+  WN_REQUIRE(aligned(pi_k, 16) && aligned(q, q_dtype == WN_F32 ? 4 : 2) && aligned(out, out_dtype == WN_F32 ? 4 : 2), WN_E_INVALID,
+             "window: Pi_K 16-byte aligned, q and out aligned to their type");
+  const int n_rep = Hq / Hkv;
+  const int64_t rows = int64_t(n_rep) * Q;
+  const WindowKernels k = pick_window(D, exact != 0, bw_k, bw_v);
+  const auto scan = k.scan[window_variant(rows)];
+  const int nrp = tree_nrp(scan, rows), ncg = nrp / scan.rows;
+  const TreeLayout lay = tree_layout(B, Hkv, nrp, 0, D, num_splits);
+  WN_REQUIRE(workspace && workspace_bytes >= lay.total && aligned(workspace, 256), WN_E_WORKSPACE,
+             "window: workspace needs %lld bytes, 256-aligned (got %lld)", (long long)lay.total, (long long)workspace_bytes);
+  // work-groups in eights: a unit's row blocks, which read much the same rows, on one XCD
+  const int64_t tiles = int64_t(B) * Hkv * (nrp / 16), groups = (int64_t(B) * num_splits * Hkv + 7) / 8 * 8 * ncg;
+  WN_REQUIRE(tiles < (int64_t(1) << 31) && groups < (int64_t(1) << 31), WN_E_INVALID, "window: grid too large");
+  const int lds = tree_lds(scan, bw_k, bw_v);
+  WN_REQUIRE(tree_slots(scan, lds) > 0, WN_E_LAUNCH, "window: cannot query the device occupancy");
+
+  char* ws = static_cast<char*>(workspace);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  TreeRotArgs ra{};
+  ra.q = q;
+  ra.qsb = q_stride_b;
+  ra.qsh = q_stride_h;
+  ra.qsq = q_stride_q;
+  ra.pi = pi_k;
+  ra.qh = reinterpret_cast<_Float16*>(ws + lay.qh);
+  ra.ql = reinterpret_cast<_Float16*>(ws + lay.ql);
+  ra.qs = reinterpret_cast<float*>(ws + lay.qs);
+  ra.scale = float(double(scale) * 1.4426950408889634);
+  ra.Hkv = Hkv;
+  ra.n_rep = n_rep;
+  ra.T = Q;
+  ra.nrp = nrp;
+  ra.q_dtype = q_dtype;
+  ra.exact = exact != 0;
+  const int per = q_dtype == WN_F32 ? 4 : 8;  // elements of 16 bytes
+  ra.vec = aligned(q, 16) && q_stride_b % per == 0 && q_stride_h % per == 0 && q_stride_q % per == 0;
+  hipLaunchKernelGGL(k.rotate, dim3(unsigned(tiles)), dim3(k.rotate_threads), 0, st, ra);
+
+  WindowArgs a{};
+  a.qh = ra.qh;
+  a.ql = ra.ql;
+  a.qs = ra.qs;
+  a.k_pages = k_pages;
+  a.v_pages = v_pages;
+  a.k_norms = k_norms;
+  a.v_norms = v_norms;
+  a.cb_k = codebook_k;
+  a.cb_v = codebook_v;
+  a.table = page_table;
+  a.seq_lens = seq_lens;
+  a.part_acc = reinterpret_cast<float*>(ws + lay.acc);
+  a.part_ml = reinterpret_cast<float*>(ws + lay.ml);
+  a.ksp = k_stride_p;
+  a.ksh = k_stride_h;
+  a.vsp = v_stride_p;
+  a.vsh = v_stride_h;
+  a.knp = kn_stride_p;
+  a.knh = kn_stride_h;
+  a.vnp = vn_stride_p;
+  a.vnh = vn_stride_h;
+  a.tsb = table_stride_b;
+  a.B = B;
+  a.Hkv = Hkv;
+  a.n_rep = n_rep;
+  a.T = Q;
+  a.nrp = nrp;
+  a.ncg = ncg;
+  a.nsplit = num_splits;
+  a.span = span;
+  a.log2S = ilog2(S);
+  a.max_pages = max_pages;
+  a.num_pages = num_pages;
+  a.bwk = bw_k;
+  a.bwv = bw_v;
+  a.window = window;
+  a.sinks = sinks;
+  if (ev_begin) (void)hipEventRecord(static_cast<hipEvent_t>(ev_begin), st);
+  hipLaunchKernelGGL(scan.fn, dim3(unsigned(groups)), dim3(scan.threads), lds, st, a);
+  if (ev_end) (void)hipEventRecord(static_cast<hipEvent_t>(ev_end), st);
+
+  WindowMergeArgs ma{};
+  ma.part_acc = a.part_acc;
+  ma.part_ml = a.part_ml;
+  ma.pi_v = pi_v;
+  ma.out = out;
+  ma.seq_lens = seq_lens;
+  ma.out_dtype = out_dtype;
+  ma.Hkv = Hkv;
+  ma.n_rep = n_rep;
+  ma.T = Q;
+  ma.nrp = nrp;
+  ma.nsplit = num_splits;
+  ma.span = span;
+  ma.max_len = max_pages * S;
+  ma.window = window;
+  ma.sinks = sinks;
+  ma.rows_block = scan.rows;
+  ma.chunk = window_chunk(D);
+  const int64_t wide = int64_t(B) * Hkv * ((rows + 15) / 16);
+  if (wide >= kMergeTiles) hipLaunchKernelGGL(k.merge[1], dim3(unsigned(wide)), dim3(1024), 0, st, ma);
+  else hipLaunchKernelGGL(k.merge[0], dim3(unsigned(int64_t(B) * Hkv * ((rows + 3) / 4))), dim3(1024), 0, st, ma);
+  return check_launch("wn_window_attention");
+}

@@ -195,20 +195,24 @@ using TreeScanFn = void (*)(TreeArgs);
 using TreeRotFn = void (*)(TreeRotArgs);
 using TreeMergeFn = void (*)(TreeMergeArgs);
 
-struct TreeScan {
-  TreeScanFn fn = nullptr;
+template <class Args>
+struct TreeScanOf {
+  void (*fn)(Args) = nullptr;
   int rows = 0, threads = 0;  // query rows and threads of a work-group
   int lds = 0, tables = 0;    // LDS bytes without the codebook tables; theirs (0: by the widths)
   int give = 0;               // LDS bytes that the hand-over at the end takes
   int waves = 0;              // > 0: the row scan, so many waves a work-group, each with its own rows
 };
+using TreeScan = TreeScanOf<TreeArgs>;
 
-struct TreeKernels {
-  TreeScan scan[3];  // for up to 32, up to 64 and more rows per kv head
+template <class Args, class MergeArgs>
+struct TreeKernelsOf {
+  TreeScanOf<Args> scan[3];  // for up to 32, up to 64 and more rows per kv head
   TreeRotFn rotate = nullptr;
   int rotate_threads = 0;
-  TreeMergeFn merge[2] = {};  // of four and of sixteen rows a work-group
+  void (*merge[2])(MergeArgs) = {};  // of four and of sixteen rows a work-group
 };
+using TreeKernels = TreeKernelsOf<TreeArgs, TreeMergeArgs>;
 
 // Bytes of one side's codebook table in LDS: 2^bw entries of (high, low), a copy per bank
 // (16 of 6-bit tables, 8 of 8-bit ones: their size).
@@ -223,5 +227,50 @@ TreeKernels tree_kernels_32(bool exact, int bw_k, int bw_v);
 TreeKernels tree_kernels_64(bool exact, int bw_k, int bw_v);
 TreeKernels tree_kernels_128(bool exact, int bw_k, int bw_v);
 TreeKernels tree_kernels_256(bool exact, int bw_k, int bw_v);
+
+// The windowed attention (window.hip): the same scan, rows and merge, with another choice of keys.
+// The T queries of a sequence are its last T positions; the one at position p sees the positions
+// j <= p with p - j < window or j < sinks.
+struct WindowArgs : TreeArgs {
+  int window, sinks;
+};
+
+struct WindowMergeArgs : TreeMergeArgs {
+  int window, sinks, rows_block, chunk;  // rows of a scan's work-group, tokens of its chunk
+};
+
+// The chunks that the queries of rows r0 .. r0 + rows - 1 of a (sequence, kv head) look at: those that
+// hold sinks, then those from the first query's window to the last query. `total` of them, counted as
+// if what lies between had been cut out: chunk c is the sequence's c < sink ? c : c + skip. Splits
+// take `span` of them each.
+struct WindowSpan {
+  int lo, hi;  // positions: first of the window, one past the last
+  int p_lo, p_hi;  // of the first and last query
+  int total, sink, skip, span;
+  __host__ __device__ int chunk(int c) const { return c < sink ? c : c + skip; }
+};
+__host__ __device__ inline WindowSpan window_span(int L, int T, int n_rep, int r0, int rows, int ch, int window, int sinks, int nsplit,
+                                                  int span) {
+  const auto lesser = [](int a, int b) { return a < b ? a : b; };
+  const auto greater = [](int a, int b) { return a > b ? a : b; };
+  WindowSpan w;
+  w.p_lo = L - T + r0 / n_rep;
+  w.p_hi = L - T + lesser(T - 1, (r0 + rows - 1) / n_rep);
+  w.hi = greater(w.p_hi + 1, 0);
+  w.lo = greater(greater(w.p_lo, 0) - window + 1, 0);
+  w.sink = (lesser(sinks, w.hi) + ch - 1) / ch;
+  w.skip = greater(w.lo / ch - w.sink, 0);
+  w.total = (w.hi + ch - 1) / ch - w.skip;
+  const int even = (w.total + nsplit - 1) / nsplit;
+  w.span = greater(span / ch, even);
+  return w;
+}
+
+using WindowKernels = TreeKernelsOf<WindowArgs, WindowMergeArgs>;
+WindowKernels window_kernels_16(bool exact, int bw_k, int bw_v);
+WindowKernels window_kernels_32(bool exact, int bw_k, int bw_v);
+WindowKernels window_kernels_64(bool exact, int bw_k, int bw_v);
+WindowKernels window_kernels_128(bool exact, int bw_k, int bw_v);
+WindowKernels window_kernels_256(bool exact, int bw_k, int bw_v);
 
 }  // namespace wn

@@ -1,6 +1,8 @@
 // The kernels of the tree attention (wn_tree.h), templates on the head dim.
 #pragma once
 
+#include <type_traits>
+
 #include "wn_tree.h"
 
 namespace wn {
@@ -159,8 +161,12 @@ struct TreeCfg {
   static_assert(NTW % 2 == 0 && tab_off % 16 == 0 && TG <= 2, "whole value K-steps");
 };
 
-template <int D, bool EX, int NCT, int RG, int TG, int W>
-__global__ __launch_bounds__(64 * RG * TG, 2) void tree_scan_kernel(TreeArgs a) {
+// Bits 0 .. x - 1 of 64.
+__device__ __forceinline__ uint64_t tree_below(int x) { return x <= 0 ? 0 : x >= 64 ? ~uint64_t(0) : (uint64_t(1) << x) - 1; }
+
+// WIN: the windowed attention; a work-group is one split of one row block of a (sequence, kv head).
+template <int D, bool EX, int NCT, int RG, int TG, int W, bool WIN = false>
+__global__ __launch_bounds__(64 * RG * TG, 2) void tree_scan_kernel(std::conditional_t<WIN, WindowArgs, TreeArgs> a) {
   using C = TreeCfg<D, EX, NCT, RG, TG>;
   using G = TreeGeo<D>;
   extern __shared__ __align__(16) char lds[];
@@ -169,6 +175,14 @@ __global__ __launch_bounds__(64 * RG * TG, 2) void tree_scan_kernel(TreeArgs a) 
   const int rg = wig % RG, tg = wig / RG;
   const int bwk = W ? W : a.bwk, bwv = W ? W : a.bwv;
   constexpr bool PAIR = W == 4 && !EX;
+  [[maybe_unused]] WindowSpan ws;
+  if constexpr (WIN) {
+    const int u = (int(blockIdx.x >> 3) / a.ncg) * 8 + int(blockIdx.x & 7), b = u / (a.nsplit * a.Hkv);
+    if (b >= a.B) return;  // the whole work-group, here and below
+    const int L = min(max(const_view(a.seq_lens)[b], 0), a.max_pages << a.log2S);
+    ws = window_span(L, a.T, a.n_rep, int(blockIdx.x >> 3) % a.ncg * C::ROWS, C::ROWS, G::CH, a.window, a.sinks, a.nsplit, a.span);
+    if (int64_t(u / a.Hkv % a.nsplit) * ws.span >= ws.total) return;
+  }
   char* tabk = lds + C::tab_off;
   char* tabv = tabk + (PAIR ? kPairBytes : tree_table_bytes(bwk));
   if constexpr (PAIR) {
@@ -184,7 +198,13 @@ __global__ __launch_bounds__(64 * RG * TG, 2) void tree_scan_kernel(TreeArgs a) 
   const int cg = int(blockIdx.x >> 3) % a.ncg, step = int(gridDim.x) / a.ncg;
   for (int u = (int(blockIdx.x >> 3) / a.ncg) * 8 + int(blockIdx.x & 7);; u += step) {
     int b, s;
-    if (!tree_split(a, lane, u / a.Hkv, &b, &s)) break;  // the whole work-group
+    if constexpr (WIN) {
+      b = u / (a.nsplit * a.Hkv);
+      s = u / a.Hkv % a.nsplit;
+      if (b >= a.B) break;  // the grid holds every unit once: the second turn ends here
+    } else if (!tree_split(a, lane, u / a.Hkv, &b, &s)) {
+      break;  // the whole work-group
+    }
     if constexpr (D < G::DP) {
       // the K tile's padded dims are zero, for each unit again: what the one before handed over at its
       // end (below) lies in the tiles' place, and as fp16 it may be NaN, which the query's zeros keep
@@ -197,8 +217,15 @@ __global__ __launch_bounds__(64 * RG * TG, 2) void tree_scan_kernel(TreeArgs a) 
     }
     const int kvh = u % a.Hkv;
     const int L = min(max(const_view(a.seq_lens)[b], 0), a.max_pages << a.log2S);
-    const int span = tree_span(L, a.nsplit, a.span);
-    const int ch_lo = s * (span / G::CH), ch_hi = (tree_end(L, span, s) + G::CH - 1) / G::CH;
+    int ch_lo, ch_hi;  // WIN: as ws counts them
+    if constexpr (WIN) {
+      ch_lo = s * ws.span;
+      ch_hi = min(ch_lo + ws.span, ws.total);
+    } else {
+      const int span = tree_span(L, a.nsplit, a.span);
+      ch_lo = s * (span / G::CH);
+      ch_hi = (tree_end(L, span, s) + G::CH - 1) / G::CH;
+    }
     const int hist = L - a.T;  // position of node 0
     const int rows = a.n_rep * a.T, r0 = cg * C::ROWS + rg * 16 * NCT;  // the wave's first row
     const int64_t row0 = (int64_t(b) * a.Hkv + kvh) * a.nrp + r0;
@@ -224,7 +251,9 @@ __global__ __launch_bounds__(64 * RG * TG, 2) void tree_scan_kernel(TreeArgs a) 
     }
 
     {
-      const int t_hi = min(G::CH * ch_hi, L), col_hi = (t_hi - 1) >> a.log2S, smask = (1 << a.log2S) - 1;
+      int t_hi = min(G::CH * ch_hi, L);
+      if constexpr (WIN) t_hi = ws.hi;
+      const int col_hi = (t_hi - 1) >> a.log2S, smask = (1 << a.log2S) - 1;
       const int32_t* trow = a.table + int64_t(b) * a.tsb;
       const uint32_t nbk = uint32_t(D * bwk / 8), nbv = uint32_t(D * bwv / 8), last_page = uint32_t(a.num_pages - 1);
       // The rows of each 16-token group of a chunk (S >= 16: they lie in one page). Tokens past the
@@ -364,7 +393,10 @@ __global__ __launch_bounds__(64 * RG * TG, 2) void tree_scan_kernel(TreeArgs a) 
         });
         if (C::NW <= G::NG || wig < G::NG) {
           // what lies past the sequence may hold anything
-          const uint32_t n = c0 + 16 * wig + c < t_hi ? nr[P] : 0, size = n & 0x7fffu;
+          bool own = c0 + 16 * wig + c < t_hi;
+          // nor may what no query of the block sees: its pages may be another's by now
+          if constexpr (WIN) own = own && (c0 + 16 * wig + c >= ws.lo || c0 + 16 * wig + c < a.sinks);
+          const uint32_t n = own ? nr[P] : 0, size = n & 0x7fffu;
           const uint32_t top = tree_row_max(size < 0x7c00u ? size : 0);  // of the finite ones
           if (lane < 32) reinterpret_cast<uint16_t*>(lds + C::n_off)[(lane >> 4) * G::CH + 16 * wig + c] = uint16_t(n);
           if (lane == 16) reinterpret_cast<uint32_t*>(lds + C::m_off)[wig] = top;
@@ -387,22 +419,29 @@ __global__ __launch_bounds__(64 * RG * TG, 2) void tree_scan_kernel(TreeArgs a) 
       };
       const int c_last = G::CH * (ch_hi - 1);
       auto next = [&](int c0) { return min(c0, c_last); };  // the last chunk again past the end
+      // position of chunk ch, the last one again past the end
+      auto at_chunk = [&](int ch) {
+        if constexpr (WIN) return G::CH * ws.chunk(min(ch, ch_hi - 1));
+        else return next(G::CH * ch);
+      };
       constexpr std::integral_constant<int, 0> even;
       constexpr std::integral_constant<int, AHEAD - 1> odd;
-      pages(page_ids(G::CH * ch_lo), G::CH * ch_lo);
+      const int c_first = WIN ? at_chunk(ch_lo) : G::CH * ch_lo;
+      pages(page_ids(c_first), c_first);
       load(even);
       if constexpr (AHEAD == 2) {
-        pages(page_ids(next(G::CH * (ch_lo + 1))), next(G::CH * (ch_lo + 1)));
+        pages(page_ids(at_chunk(ch_lo + 1)), at_chunk(ch_lo + 1));
         load(odd);
       }
-      uint32_t ids = page_ids(next(G::CH * (ch_lo + AHEAD)));
-      auto chunk = [&](auto set, int c0) {
+      uint32_t ids = page_ids(at_chunk(ch_lo + AHEAD));
+      auto chunk = [&](auto set, int ch) {
+        const int c0 = WIN ? at_chunk(ch) : G::CH * ch;
         __syncthreads();  // the last chunk's tiles are read (at first: the tables are staged)
         store(set, c0);
         // the page ids of the chunk after are asked for ahead of the rows: waiting for them next
         // time waits for no row
-        pages(ids, next(c0 + AHEAD * G::CH));
-        ids = page_ids(next(c0 + (AHEAD + 1) * G::CH));
+        pages(ids, at_chunk(ch + AHEAD));
+        ids = page_ids(at_chunk(ch + AHEAD + 1));
         load(set);
         __syncthreads();
         if (r0 >= rows) return;  // padding: the wave has only its part of the tiles to do
@@ -493,9 +532,15 @@ __global__ __launch_bounds__(64 * RG * TG, 2) void tree_scan_kernel(TreeArgs a) 
               int row = r0 + 16 * ct + c;
               asm volatile("" : "+v"(row));  // not ahead of the loop: once per split
               const int node = row / a.n_rep;
-              const uint64_t vis = node < a.T ? a.vis[int64_t(b) * a.T + node] : 0;
-              const int at = hist - c0;  // the tree's first position in the chunk (or before it)
-              const uint64_t word = at >= 0 ? (vis << at | ((uint64_t(1) << at) - 1)) : at > -64 ? vis >> -at : 0;
+              uint64_t word;
+              if constexpr (WIN) {
+                const int p = hist + node, from = max(max(p, 0) - a.window + 1, 0);
+                word = node < a.T ? tree_below(p - c0 + 1) & (~tree_below(from - c0) | tree_below(a.sinks - c0)) : 0;
+              } else {
+                const uint64_t vis = node < a.T ? a.vis[int64_t(b) * a.T + node] : 0;
+                const int at = hist - c0;  // the tree's first position in the chunk (or before it)
+                word = at >= 0 ? (vis << at | ((uint64_t(1) << at) - 1)) : at > -64 ? vis >> -at : 0;
+              }
 #pragma unroll
               for (int ks = 0; ks < KV; ++ks) seen[ks] = uint32_t(word >> (w0 + 32 * ks + 8 * g)) & 0xffu;
             }
@@ -512,7 +557,9 @@ __global__ __launch_bounds__(64 * RG * TG, 2) void tree_scan_kernel(TreeArgs a) 
               }
           }
         };
-        if (c0 + G::CH <= hist) scores(std::integral_constant<bool, false>{});
+        bool whole = c0 + G::CH <= hist;  // every row sees the chunk
+        if constexpr (WIN) whole = c0 + G::CH <= ws.p_lo + 1 && (c0 > ws.p_hi - a.window || c0 + G::CH <= a.sinks);
+        if (whole) scores(std::integral_constant<bool, false>{});
         else scores(std::integral_constant<bool, true>{});
         // a row's maximum moves when a score exceeds it by more than kTreeRescale, and on its first key
         bool move[NCT], any = false;
@@ -584,8 +631,8 @@ __global__ __launch_bounds__(64 * RG * TG, 2) void tree_scan_kernel(TreeArgs a) 
           }
       };
       for (int ch = ch_lo; ch < ch_hi; ch += AHEAD) {
-        chunk(even, G::CH * ch);
-        if (AHEAD == 2 && ch + 1 < ch_hi) chunk(odd, G::CH * (ch + 1));
+        chunk(even, ch);
+        if (AHEAD == 2 && ch + 1 < ch_hi) chunk(odd, ch + 1);
       }
     }
 
@@ -673,7 +720,8 @@ __host__ __device__ constexpr int tree_rotate_threads(int D) { return 4 * D > 25
 // q' of sixteen rows per work-group (rows past n_rep T: zero, up to a multiple of 32), and the nodes' words.
 // Products in fp32. Bound by latency and, with many tiles, by the instructions around 32 matrix
 // products: 5.5 us for 16 tiles, 14 us for 2,048 (64 heads, 64 nodes, 4 sequences: 12 MB moved).
-template <int D>
+// WIN: no nodes' words.
+template <int D, bool WIN = false>
 __global__ __launch_bounds__(tree_rotate_threads(D)) void tree_rotate_kernel(TreeRotArgs a) {
   constexpr int XS = D + 4, NTHR = tree_rotate_threads(D);
   __shared__ __align__(16) float x[16 * XS];
@@ -685,7 +733,7 @@ __global__ __launch_bounds__(tree_rotate_threads(D)) void tree_rotate_kernel(Tre
   const int r0 = 16 * int(blockIdx.x % tiles), kvh = int(unit % a.Hkv), rows = a.n_rep * a.T;
   const int64_t b = unit / a.Hkv;
   if (r0 >= (rows + 31) / 32 * 32) return;  // of no wave that computes
-  const bool words = kvh == 0 && r0 == 0;  // one work-group per sequence
+  const bool words = !WIN && kvh == 0 && r0 == 0;  // one work-group per sequence
   TreeProduct<D> pi;
   pi.load(wave, lane, [&](int j, int k) { return *reinterpret_cast<const f32x4*>(a.pi + j * D + k); });
   if (words && tid < 64) par[tid] = tid < a.T ? a.parents[b * a.psb + tid] : -1;
@@ -783,8 +831,8 @@ __global__ __launch_bounds__(tree_rotate_threads(D)) void tree_rotate_kernel(Tre
 // both, and Pi_V's operands, are asked for before anything is known of the sequence: what bounds
 // these few rows is one round trip after another: 6 us for 256 rows, 18 us for 16,384 of three
 // splits (two round trips and the product for each of 1,024 work-groups, of which 512 run at a time).
-template <int D, int R>
-__global__ __launch_bounds__(1024) void tree_merge_kernel(TreeMergeArgs a) {
+template <int D, int R, bool WIN = false>
+__global__ __launch_bounds__(1024) void tree_merge_kernel(std::conditional_t<WIN, WindowMergeArgs, TreeMergeArgs> a) {
   constexpr int XS = D + 4, LD = D < 64 ? D : 64, VEC = D / LD;  // lanes a split, dims a lane
   constexpr int SUB = 64 / LD, PARTS = 16 / R * SUB;              // splits are taken in PARTS residue classes
   constexpr int U = R == 4 ? 8 : 4;
@@ -812,7 +860,14 @@ __global__ __launch_bounds__(1024) void tree_merge_kernel(TreeMergeArgs a) {
     return f32x4{a.pi_v[kk * D + j], a.pi_v[(kk + 1) * D + j], a.pi_v[(kk + 2) * D + j], a.pi_v[(kk + 3) * D + j]};
   });
   const int L = min(max(a.seq_lens[unit / a.Hkv], 0), a.max_len);
-  const int live = tree_count(L, tree_span(L, a.nsplit, a.span));  // splits that the sequence has: the others' partials are not its own
+  int live;  // splits that the sequence has: the others' partials are not its own
+  if constexpr (WIN) {
+    const WindowSpan ws = window_span(L, a.T, a.n_rep, blk * R / a.rows_block * a.rows_block, a.rows_block, a.chunk, a.window, a.sinks,
+                                      a.nsplit, a.span);
+    live = ws.span ? (ws.total + ws.span - 1) / ws.span : 0;
+  } else {
+    live = tree_count(L, tree_span(L, a.nsplit, a.span));
+  }
   float M = lane < live ? ml0.x : -INFINITY;
   for (int s = 64 + lane; s < live; s += 64) M = fmaxf(M, stats(s).x);
   M = wave_max(M);
@@ -866,41 +921,46 @@ __global__ __launch_bounds__(1024) void tree_merge_kernel(TreeMergeArgs a) {
   }
 }
 
-template <int D, bool EX, int NCT, int RG, int TG, int W>
-TreeScan tree_scan() {
+template <bool WIN>
+using TreeArgsOf = std::conditional_t<WIN, WindowArgs, TreeArgs>;
+template <bool WIN>
+using TreeKernelSet = std::conditional_t<WIN, WindowKernels, TreeKernels>;
+
+template <int D, bool EX, int NCT, int RG, int TG, int W, bool WIN>
+TreeScanOf<TreeArgsOf<WIN>> tree_scan() {
   using C = TreeCfg<D, EX, NCT, RG, TG>;
-  return TreeScan{tree_scan_kernel<D, EX, NCT, RG, TG, W>, C::ROWS, C::NTHR, C::tab_off, W == 4 && !EX ? 2 * kPairBytes : 0, C::give, 0};
+  return {tree_scan_kernel<D, EX, NCT, RG, TG, W, WIN>, C::ROWS, C::NTHR, C::tab_off, W == 4 && !EX ? 2 * kPairBytes : 0, C::give, 0};
 }
 
-template <int D, bool EX, int W>
-TreeKernels tree_kernels() {
-  TreeKernels k;
+template <int D, bool EX, int W, bool WIN>
+TreeKernelSet<WIN> tree_kernels() {
+  TreeKernelSet<WIN> k;
   if constexpr (D == 256) {
     // 128 accumulator registers per 32 rows: sixteen rows a wave
-    k.scan[0] = k.scan[1] = k.scan[2] = tree_scan<D, EX, 1, 4, 1, W>();
+    k.scan[0] = k.scan[1] = k.scan[2] = tree_scan<D, EX, 1, 4, 1, W, WIN>();
   } else {
-    k.scan[0] = tree_scan<D, EX, 1, 2, 2, W>();
-    k.scan[1] = tree_scan<D, EX, 2, 2, 2, W>();
+    k.scan[0] = tree_scan<D, EX, 1, 2, 2, W, WIN>();
+    k.scan[1] = tree_scan<D, EX, 2, 2, 2, W, WIN>();
     // More than 64 rows: blocks of 128, which decode a chunk once for all of them. With two terms a
     // factor decoding writes twice the bytes, and eight waves share it (64 query heads, 64 nodes, 4 and
     // 6 bits, in traces: 605 us, two work-groups of four waves and 64 rows 710; a second set of tiles, to decode
     // ahead of the barrier, 600). With single terms four waves take 128 rows, and a second work-group
     // fills their waits (28 heads, 26 nodes: 41 us, eight waves 47).
-    if constexpr (EX) k.scan[2] = tree_scan<D, EX, 2, 4, 2, W>();
-    else k.scan[2] = tree_scan<D, EX, 2, 4, 1, W>();
+    if constexpr (EX) k.scan[2] = tree_scan<D, EX, 2, 4, 2, W, WIN>();
+    else k.scan[2] = tree_scan<D, EX, 2, 4, 1, W, WIN>();
   }
-  k.rotate = tree_rotate_kernel<D>;
-  k.merge[0] = tree_merge_kernel<D, 4>;
-  k.merge[1] = tree_merge_kernel<D, 16>;
+  k.rotate = tree_rotate_kernel<D, WIN>;
+  k.merge[0] = tree_merge_kernel<D, 4, WIN>;
+  k.merge[1] = tree_merge_kernel<D, 16, WIN>;
   k.rotate_threads = tree_rotate_threads(D);
   return k;
 }
 
 // Kernels for 4-bit K and V, the width that most caches take, and for any widths.
-template <int D>
-TreeKernels tree_kernels_for(bool exact, int bw_k, int bw_v) {
-  if (bw_k == 4 && bw_v == 4) return exact ? tree_kernels<D, true, 4>() : tree_kernels<D, false, 4>();
-  return exact ? tree_kernels<D, true, 0>() : tree_kernels<D, false, 0>();
+template <int D, bool WIN = false>
+TreeKernelSet<WIN> tree_kernels_for(bool exact, int bw_k, int bw_v) {
+  if (bw_k == 4 && bw_v == 4) return exact ? tree_kernels<D, true, 4, WIN>() : tree_kernels<D, false, 4, WIN>();
+  return exact ? tree_kernels<D, true, 0, WIN>() : tree_kernels<D, false, 0, WIN>();
 }
 
 }  // namespace

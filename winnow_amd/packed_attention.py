@@ -537,19 +537,17 @@ def packed_prefill_attention(q: torch.Tensor, kv: PackedKV, scale: float, *,
 TREE_NODES = 64      # drafted tokens per sequence: a node's visible nodes are one 64-bit word
 
 
-def check_tree(q: torch.Tensor, kv: PackedKV, parents: torch.Tensor) -> None:
-    """What ``packed_tree_attention`` needs beyond ``check_contract``."""
-    B, _, T, D = q.shape
-    if not 1 <= T <= TREE_NODES:
-        raise UnsupportedLayout(f"tree attention takes 1 to {TREE_NODES} drafted tokens, got {T}")
+def _check_scan(what: str, q: torch.Tensor, kv: PackedKV) -> None:
+    """What the tile scans (tree and windowed attention) need beyond ``check_contract``."""
+    D = q.shape[-1]
     if not _lib.is_hip(q):
-        raise UnsupportedLayout("tree attention needs tensors on a HIP device")
+        raise UnsupportedLayout(f"{what} needs tensors on a HIP device")
     if D not in SUPPORTED_HEAD_DIMS or not _pow2(kv.page_size):
-        raise UnsupportedLayout(f"tree attention: head_dim {D} (compiled: {SUPPORTED_HEAD_DIMS}), page size "
+        raise UnsupportedLayout(f"{what}: head_dim {D} (compiled: {SUPPORTED_HEAD_DIMS}), page size "
                                 f"{kv.page_size} (a power of two >= 16)")
     if q.dtype not in _lib.DTYPE_CODE or q.stride(-1) != 1:
         raise UnsupportedLayout("q must be fp32/fp16/bf16 with a contiguous head_dim")
-    values_only("tree attention", q)
+    values_only(what, q)
     for pages, norms in ((kv.k_pages, kv.k_norms), (kv.v_pages, kv.v_norms)):
         st = pages.stride()
         if st[3] != 1 or st[2] != pages.shape[3]:
@@ -568,6 +566,14 @@ def check_tree(q: torch.Tensor, kv: PackedKV, parents: torch.Tensor) -> None:
         raise UnsupportedLayout("page_table must hold 1 to 2^31 - 257 positions per sequence")
     if P < 1:
         raise UnsupportedLayout("the pool has no pages")
+
+
+def check_tree(q: torch.Tensor, kv: PackedKV, parents: torch.Tensor) -> None:
+    """What ``packed_tree_attention`` needs beyond ``check_contract``."""
+    B, _, T, _ = q.shape
+    if not 1 <= T <= TREE_NODES:
+        raise UnsupportedLayout(f"tree attention takes 1 to {TREE_NODES} drafted tokens, got {T}")
+    _check_scan("tree attention", q, kv)
     if parents.shape != (B, T) or parents.dtype != torch.int32 or parents.device != q.device \
             or (T > 1 and parents.stride(1) != 1):
         raise UnsupportedLayout(f"parents must be ({B}, {T}) int32 on {q.device} with contiguous rows")
@@ -695,6 +701,125 @@ def packed_tree_attention(q: torch.Tensor, kv: PackedKV, scale: float, parents: 
                   table.data_ptr(), table.stride(0), kv.seq_lens.data_ptr(), parents.data_ptr(), parents.stride(0),
                   out.data_ptr(), _lib.DTYPE_CODE[out_dtype], workspace.data_ptr(), room,
                   *sizes, P, table.shape[1], float(scale), int(exact), ns, span, parts, _lib.stream_of(q.device), ev0, ev1)
+    return out
+
+
+MAX_WINDOW_ROWS = 1 << 20      # queries of a kv head: n_rep * Q
+
+
+def check_window(window: int, sinks: int) -> tuple[int, int]:
+    """A window of at least one position and a count of sinks, as the C ABI takes them."""
+    if isinstance(window, bool) or isinstance(sinks, bool) or int(window) != window or int(sinks) != sinks or window < 1 or sinks < 0:
+        raise UnsupportedLayout(f"a window of {window} positions and {sinks} sinks (whole numbers, at least 1 and at least 0)")
+    return min(int(window), 2 ** 31 - 1), min(int(sinks), 2 ** 31 - 1)
+
+
+def check_window_ranges(seq_lens: torch.Tensor, page_table: torch.Tensor, num_pages: int, page_size: int, queries: int, window: int,
+                        sinks: int) -> None:
+    """Every length fits the table and every page that one of the last ``queries`` positions sees lies
+    in [0, num_pages). Reads host copies, natively for int32 mirrors."""
+    lens, table = seq_lens.detach().to("cpu"), page_table.detach().to("cpu")
+    if _lib.window_in_range(lens, table, num_pages, page_size, queries, window, sinks):
+        return
+    lens, table = lens.numpy().astype(np.int64), table.numpy()
+    width = table.shape[1]
+    if lens.size and (lens.min() < 0 or lens.max() > width * page_size):
+        raise UnsupportedLayout("seq_lens out of range for the page table")
+    col = np.arange(width)[None, :]
+    first = np.maximum(lens - queries - window + 1, 0)[:, None] // page_size
+    last = (lens[:, None] + page_size - 1) // page_size
+    seen = ((col >= first) & (col < last)) | (col * page_size < np.minimum(lens, sinks)[:, None])
+    bad = seen & ((table < 0) | (table >= num_pages))
+    if bad.any():
+        b = int(np.flatnonzero(bad.any(1))[0])
+        raise UnsupportedLayout(f"sequence {b} references a page outside [0, {num_pages})")
+
+
+@functools.lru_cache(maxsize=1024)
+def window_workspace_bytes(batch: int, num_q_heads: int, num_kv_heads: int, q_len: int, head_dim: int, num_splits: int) -> int:
+    return int(_lib.lib().wn_window_workspace_bytes(batch, num_q_heads, num_kv_heads, q_len, head_dim, num_splits))
+
+
+def window_plan_for(q: torch.Tensor, kv: PackedKV, window: int, sinks: int, exact: bool, *, read_lens: bool = True) -> tuple[int, int]:
+    """(num_splits, span) of the windowed attention for this query and handle (wn_window_plan), from the
+    lengths' host mirror, or, without one, a host copy (``read_lens``) or the width of the table."""
+    B, Hq, Q, D = q.shape
+    lens = kv.seq_lens_host
+    if lens is None and read_lens:
+        lens = kv.seq_lens.cpu()
+    if lens is not None and (lens.dtype != torch.int32 or lens.shape != (B,) or not lens.is_contiguous()):
+        lens = lens.to(torch.int32).reshape(B).contiguous()
+    ns, span = ctypes.c_int(0), ctypes.c_int(0)
+    with _lib.on(q.device):
+        _lib.call("wn_window_plan", B, Hq, kv.num_kv_heads, Q, D, kv.page_size, kv.k_quant.bit_width, kv.v_quant.bit_width, int(exact),
+                  kv.page_table.shape[1], window, sinks, _lib.ptr(lens), ctypes.byref(ns), ctypes.byref(span))
+    return ns.value, span.value
+
+
+def packed_window_attention(q: torch.Tensor, kv: PackedKV, scale: float, *, window: int, sinks: int = 0,
+                            allow_tf32: bool = False, num_splits: int | None = None,
+                            out_dtype: torch.dtype | None = None, workspace: torch.Tensor | None = None,
+                            check_ranges: bool = True, timing_events=None) -> torch.Tensor:
+    """Attention under a sliding window, with the first ``sinks`` positions in view throughout, over
+    packed pages: q (B, Hq, Q, D) -> (B, Hq, Q, D) in q.dtype (``wn_window_attention``).
+
+    The cache already holds the Q >= 1 queries' tokens, as after ``append_kv``: query i of a sequence of
+    length L is position p = L - Q + i. It sees the positions j <= p with p - j < ``window`` or
+    j < ``sinks``; a query with p < 0 sees none and gives 0. With a window of L or more it is the causal
+    mask of the decode and the prefill.
+
+    What no query sees is not read: a call costs the window, not the context, and page table entries
+    wholly outside may be -1 (their pages released). Every head_dim, width pair, n_rep and page
+    size of ``packed_decode_attention`` is served, Q up to 2^20 / n_rep. Products have fp32 accuracy
+    whatever the query's type, or, where ``allow_tf32`` is given, TF32-class accuracy (single fp16
+    operands, fp32 accumulation), as in the decode. ``num_splits`` replaces the library's split
+    count, ``out_dtype`` the result's type, ``workspace`` is a caller-owned uint8 buffer of at least
+    ``window_workspace_bytes``, ``timing_events`` a pair of raw ``hipEvent_t`` handles recorded
+    around the scan.
+
+    Raises ``UnsupportedLayout`` before any launch for what ``check_contract`` rejects, for layouts
+    that the scan does not read, for a gradient, a tangent or a trace; ``check_ranges`` covers lengths
+    and the ids of pages in view, read from the handle's host mirrors when given, else copied to the host."""
+    check_contract(q, kv, check_ranges=False)
+    window, sinks = check_window(window, sinks)
+    _check_scan("windowed attention", q, kv)
+    B, Hq, Q, D = q.shape
+    P, Hkv, S, _ = kv.k_pages.shape
+    if Q < 1 or Hq // Hkv * Q > MAX_WINDOW_ROWS:
+        raise UnsupportedLayout(f"windowed attention: {Q} queries a sequence, {Hq // Hkv} heads a kv head (1 to {MAX_WINDOW_ROWS} rows)")
+    out_dtype = out_dtype or q.dtype
+    if out_dtype not in _lib.DTYPE_CODE:
+        raise UnsupportedLayout(f"output dtype {out_dtype} is not supported")
+    if check_ranges:
+        check_window_ranges(kv.seq_lens if kv.seq_lens_host is None else kv.seq_lens_host,
+                            kv.page_table if kv.page_table_host is None else kv.page_table_host, P, S, Q, window, sinks)
+    exact = not allow_tf32
+    out = torch.empty(B, Hq, Q, D, dtype=out_dtype, device=q.device)
+    if B == 0:
+        return out
+    ns, span = (int(num_splits), 64) if num_splits else window_plan_for(q, kv, window, sinks, exact, read_lens=check_ranges)
+    need = window_workspace_bytes(B, Hq, Hkv, Q, D, ns)
+    if need < 0:
+        raise UnsupportedLayout(f"bad window sizes B={B} Hq={Hq} Hkv={Hkv} Q={Q} splits={ns}")
+    room = need
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    else:
+        room = workspace.numel() * workspace.element_size()
+        if room < need or workspace.device != q.device or not workspace.is_contiguous():
+            raise UnsupportedLayout(f"workspace needs {need} contiguous bytes on {q.device}")
+    ev0, ev1 = timing_events or (None, None)
+    kq, vq, table = kv.k_quant, kv.v_quant, kv.page_table
+    kp, vp, kn, vn = kv.k_pages.stride(), kv.v_pages.stride(), kv.k_norms.stride(), kv.v_norms.stride()
+    with _lib.on(q.device):
+        _lib.call("wn_window_attention", q.data_ptr(), _lib.DTYPE_CODE[q.dtype], *q.stride()[:3],
+                  kq.Pi.data_ptr(), vq.Pi.data_ptr(), kq.centroids.data_ptr(), vq.centroids.data_ptr(),
+                  kv.k_pages.data_ptr(), kp[0], kp[1], kv.v_pages.data_ptr(), vp[0], vp[1],
+                  kv.k_norms.data_ptr(), kn[0], kn[1], kv.v_norms.data_ptr(), vn[0], vn[1],
+                  table.data_ptr(), table.stride(0), kv.seq_lens.data_ptr(),
+                  out.data_ptr(), _lib.DTYPE_CODE[out_dtype], workspace.data_ptr(), room,
+                  B, Hq, Hkv, Q, D, S, kq.bit_width, vq.bit_width, P, table.shape[1], window, sinks, float(scale), int(exact), ns, span,
+                  _lib.stream_of(q.device), ev0, ev1)
     return out
 
 
