@@ -13,8 +13,14 @@ machine-readable ``reason``), ``Request``, ``EngineConfig``, and ``Engine`` with
 * decoding is greedy, so a request's tokens depend on its prompt alone and a batched
   run equals the request run by itself.
 
+What a request asks of its next token is applied to the step's logits before the choice
+(``logits.adjust_logits``): penalties for tokens that it holds already, biases, and a mask of the
+tokens that a grammar allows. ``EngineConfig.window`` and ``sinks`` limit what every request
+attends to, ``fuse_rotary`` moves the position rotation into the cache's append.
+
 A request that sets ``top_logprobs`` also gets a ``TokenScore`` per generated token (in
-``logprobs`` and in the token events), from ``logprobs.token_logprobs`` over the step's logits.
+``logprobs`` and in the token events), from ``logprobs.token_logprobs`` over the step's logits
+(the model's, before penalties, biases and masks).
 
 Structure (this module's own):
 
@@ -33,6 +39,7 @@ Structure (this module's own):
 from __future__ import annotations
 
 import itertools
+import math
 import threading
 import time
 from collections import deque
@@ -40,8 +47,9 @@ from dataclasses import dataclass, field
 
 import torch
 
+from winnow_amd.logits import MAX_BIASES, adjust_logits, mask_words, pack_allowed
 from winnow_amd.logprobs import MAX_TOP, token_logprobs
-from winnow_amd.packed_backend import PagedPackedCache
+from winnow_amd.packed_backend import PagedPackedCache, fuse_rotary
 from winnow_amd.page_pool import PoolExhausted, default_fence
 
 
@@ -87,6 +95,23 @@ class Request:
     # not in the reference: score each generated token, with so many alternatives (None: not)
     top_logprobs: int | None = None
     logprobs: list[TokenScore] = field(default_factory=list)
+    # not in the reference: what is asked of the next token (logits.adjust_logits). Repeated tokens of
+    # the prompt and the generated ones; presence and frequency of the generated ones
+    repetition_penalty: float = 1.0
+    presence_penalty: float = 0.0
+    frequency_penalty: float = 0.0
+    logit_bias: dict[int, float] = field(default_factory=dict)
+    # callable(request) before each token: the ids that may come next, a (vocab,) bool tensor, the int32
+    # words of one (logits.pack_allowed), or None for all
+    allowed_tokens: object = None
+
+    @property
+    def penalized(self) -> bool:
+        return self.repetition_penalty != 1 or self.presence_penalty != 0 or self.frequency_penalty != 0
+
+    @property
+    def steered(self) -> bool:
+        return self.penalized or bool(self.logit_bias) or self.allowed_tokens is not None
 
 
 @dataclass
@@ -100,6 +125,10 @@ class EngineConfig:
     max_new_tokens_cap: int = 512
     decode_backend: str = "auto"
     allow_tf32: bool = False       # TF32-class products in the packed decode operator
+    # not in the reference: attend to the last ``window`` positions and the first ``sinks`` only
+    window: int | None = None
+    sinks: int = 0
+    fuse_rotary: bool = False      # packed_backend.fuse_rotary on the model
 
 
 # Admission rules in the order they are checked: (reason, refused?, detail).
@@ -112,6 +141,11 @@ _RULES = (
      lambda e, r: f"must be 1..{e.cfg.max_new_tokens_cap}"),
     ("bad_top_logprobs", lambda e, r: r.top_logprobs is not None and not 0 <= r.top_logprobs <= MAX_TOP,
      lambda e, r: f"must be 0..{MAX_TOP}"),
+    ("bad_penalty", lambda e, r: not (math.isfinite(r.repetition_penalty) and r.repetition_penalty > 0
+                                      and math.isfinite(r.presence_penalty) and math.isfinite(r.frequency_penalty)),
+     lambda e, r: "penalties must be finite, the repetition's above 0"),
+    ("bad_logit_bias", lambda e, r: len(r.logit_bias) > MAX_BIASES or any(math.isnan(x) for x in r.logit_bias.values()),
+     lambda e, r: f"at most {MAX_BIASES} biases, none of them NaN"),
     ("exceeds_request_cap", lambda e, r: e._worst_pages(r) > e.pool.max_pages_per_request,
      lambda e, r: f"{e._worst_pages(r)} pages > {e.pool.max_pages_per_request}"),
 )
@@ -138,6 +172,10 @@ class Engine:
         self._live: dict[str, Request] = {}   # every request not yet done, by id
         self._mu = threading.Lock()           # waiting queue, id map, cancel flags
         self._sched = threading.Lock()        # one step at a time
+        self._history: torch.Tensor | None = None    # (max_batch, ...) int32: a row's tokens, of the request below
+        self._history_of: list[tuple[Request, int] | None] = [None] * self.cfg.max_batch    # ... and how many of them
+        if self.cfg.fuse_rotary:
+            fuse_rotary(model)
 
     def _worst_pages(self, req: Request) -> int:
         return self.pool.pages_for(len(req.prompt_ids) + req.max_new_tokens)
@@ -207,7 +245,8 @@ class Engine:
         req.detail = req.detail or detail
         req.finished_at = self.clock()
         if req in self._slots:
-            self._slots[self._slots.index(req)] = None
+            slot = self._slots.index(req)
+            self._slots[slot] = self._history_of[slot] = None
         self._admitted_at.pop(req.request_id, None)
         self.pool.release(req.request_id, fence)
         with self._mu:
@@ -263,7 +302,8 @@ class Engine:
         positions = start[:, None] + torch.arange(n, device=self.device)[None, :]
         cache = PagedPackedCache(self.pool, [r.request_id for r in reqs], [r.stored for r in reqs],
                                  k_quant=self.kq, v_quant=self.vq, head_dim=self.head_dim,
-                                 decode_backend=self.cfg.decode_backend, allow_tf32=self.cfg.allow_tf32)
+                                 decode_backend=self.cfg.decode_backend, allow_tf32=self.cfg.allow_tf32,
+                                 window=self.cfg.window, sinks=self.cfg.sinks if self.cfg.window is not None else 0)
         out = self.model(input_ids=ids, position_ids=positions, past_key_values=cache, use_cache=True,
                          logits_to_keep=1)
         for r, stored in zip(reqs, cache.lengths):
@@ -272,6 +312,92 @@ class Engine:
         if self.on_logits is not None:
             self.on_logits(reqs, logits)
         return logits
+
+    def _histories(self, reqs: list[Request], device) -> torch.Tensor:
+        """(len(reqs), H) int32 on the device: each request's prompt and generated tokens. Rows belong to the
+        batch slots; a step uploads what its requests gained since their last one."""
+        if self._history is None:
+            room = self.cfg.max_prompt_tokens + self.cfg.max_new_tokens_cap
+            self._history = torch.zeros(self.cfg.max_batch, room, dtype=torch.int32, device=device)
+        slots, at, new = [], [], []
+        for r in reqs:
+            slot = self._slots.index(r)
+            held = self._history_of[slot]
+            have = held[1] if held is not None and held[0] is r else 0
+            total = len(r.prompt_ids) + len(r.generated)
+            tokens = (r.prompt_ids[have:] if have < len(r.prompt_ids) else []) + r.generated[max(0, have - len(r.prompt_ids)):]
+            slots.append(slot)
+            at += [slot * self._history.shape[1] + k for k in range(have, total)]
+            new += tokens
+            self._history_of[slot] = (r, total)
+        if new:
+            host = torch.tensor([at, new], dtype=torch.int64).to(device)
+            self._history.view(-1).index_copy_(0, host[0], host[1].int())
+        longest = max(len(r.prompt_ids) + len(r.generated) for r in reqs)
+        return self._history[:, :longest].index_select(0, torch.tensor(slots, device=device))
+
+    def _allowed(self, reqs: list[Request], vocab: int) -> tuple[torch.Tensor | None, dict]:
+        """The words of the requests' masks on the host (None: no request has one), and what went wrong
+        for which request."""
+        words, bad = None, {}
+        for i, r in enumerate(reqs):
+            if r.allowed_tokens is None:
+                continue
+            try:
+                ok = r.allowed_tokens(r)
+                if ok is None:
+                    continue
+                if not isinstance(ok, torch.Tensor):
+                    ids = torch.tensor(sorted(int(t) for t in ok if 0 <= int(t) < vocab), dtype=torch.int64)
+                    ok = torch.zeros(vocab, dtype=torch.bool).index_fill_(0, ids, True)
+                ok = pack_allowed(ok.cpu()) if ok.dtype == torch.bool and ok.shape == (vocab,) else ok.cpu()
+                if ok.dtype != torch.int32 or ok.shape != (mask_words(vocab),):
+                    raise ValueError(f"allowed_tokens gave {tuple(ok.shape)} {ok.dtype}")
+            except Exception as exc:  # noqa: BLE001 - the caller's function: reported on its request
+                bad[r.request_id] = exc
+                continue
+            if words is None:
+                words = torch.full((len(reqs), mask_words(vocab)), -1, dtype=torch.int32)
+            words[i] = ok
+        return words, bad
+
+    def _choose(self, reqs: list[Request], logits: torch.Tensor) -> tuple[list[int], dict]:
+        """The next token of each request, greedily, from its logits with what it asks of them applied; and
+        what went wrong for which request (by id)."""
+        rows = [i for i, r in enumerate(reqs) if r.steered]
+        if not rows:
+            return logits.argmax(-1).tolist(), {}
+        asked, vocab, dev = [reqs[i] for i in rows], logits.shape[-1], logits.device
+        words, bad = self._allowed(asked, vocab)
+        try:
+            kw = {}
+            if any(r.penalized for r in asked):
+                kw["history"] = self._histories(asked, dev)
+                host = torch.tensor([[len(r.prompt_ids) + len(r.generated) for r in asked], [len(r.prompt_ids) for r in asked]], dtype=torch.int32).to(dev)
+                kw["lengths"], kw["prompt_lengths"] = host[0], host[1]
+                pen = torch.tensor([[r.repetition_penalty for r in asked], [r.presence_penalty for r in asked],
+                                    [r.frequency_penalty for r in asked]], dtype=torch.float32).to(dev)
+                kw["repetition"], kw["presence"], kw["frequency"] = pen[0], pen[1], pen[2]
+            J = max(len(r.logit_bias) for r in asked)
+            if J:
+                pad = [list(r.logit_bias.items()) + [(-1, 0.0)] * (J - len(r.logit_bias)) for r in asked]
+                kw["bias_ids"] = torch.tensor([[int(t) for t, _ in row] for row in pad], dtype=torch.int64).to(dev)
+                kw["bias"] = torch.tensor([[float(x) for _, x in row] for row in pad], dtype=torch.float32).to(dev)
+            if words is not None:
+                kw["allowed"] = words.to(dev)
+            at = torch.tensor(rows, device=dev)
+            some = adjust_logits(logits.index_select(0, at) if len(rows) < len(reqs) else logits, **kw)
+            best = some.argmax(-1)
+            found = some.gather(1, best[:, None])[:, 0]
+            tokens = logits.argmax(-1).index_copy(0, at, best).tolist()
+            for r, x in zip(asked, found.tolist()):
+                if x == -math.inf:
+                    bad.setdefault(r.request_id, ValueError("no token is allowed"))
+        except Exception as exc:  # noqa: BLE001 - reported on the requests that asked
+            for r in asked:
+                bad.setdefault(r.request_id, exc)
+            tokens = logits.argmax(-1).tolist()
+        return tokens, bad
 
     def _scores(self, reqs: list[Request], logits: torch.Tensor, tokens: list[int]) -> list[TokenScore | None]:
         """The score of each request's token where it asked for one, in one pass over the logits."""
@@ -310,8 +436,12 @@ class Engine:
         last = hi == len(req.prompt_ids)
         try:
             logits = self._forward([req], [req.prompt_ids[lo:hi]])
-            token = int(logits[0].argmax()) if last else -1
-            score = self._scores([req], logits, [token])[0] if last else None
+            token, score = -1, None
+            if last:
+                (token,), bad = self._choose([req], logits)
+                if bad:
+                    raise bad[req.request_id]
+                score = self._scores([req], logits, [token])[0]
         except Exception as exc:  # noqa: BLE001 - reported on the request
             self._fail([req], exc)
             return True
@@ -329,10 +459,18 @@ class Engine:
             return False
         try:
             logits = self._forward(batch, [[r.generated[-1]] for r in batch])
-            tokens = logits.argmax(-1).tolist()
+            tokens, bad = self._choose(batch, logits)
         except Exception as exc:  # noqa: BLE001 - reported on every request of the batch
             self._fail(batch, exc)
             return True
+        if bad:  # the others go on
+            for r in batch:
+                if r.request_id in bad:
+                    self._fail([r], bad[r.request_id])
+            keep = [i for i, r in enumerate(batch) if r.request_id not in bad]
+            if not keep:
+                return True
+            batch, tokens, logits = [batch[i] for i in keep], [tokens[i] for i in keep], logits[keep]
         try:
             scores = self._scores(batch, logits, tokens)
         except Exception as exc:  # noqa: BLE001 - reported on the requests that asked for scores

@@ -490,12 +490,22 @@ class PagedPackedCache:
     each of the n <= 64 tokens, (n,) for every sequence or (B, n), as a list or a host tensor
     (``packed_attention.packed_tree_attention``; ``tree_positions`` gives the model's position
     ids). The leases must cover the whole tree. ``commit`` then keeps the accepted branch.
+
+    ``window`` limits what the new tokens attend to: the last ``window`` positions up to their own and
+    the sequence's first ``sinks`` (``packed_attention.packed_window_attention``). Positions are
+    those of the whole sequence, and the cache keeps all of it.
     """
 
     def __init__(self, pool: PagePool, owners, lengths, *, k_quant, v_quant,
-                 head_dim: int, decode_backend: str = "auto", allow_tf32: bool = False, tree=None):
+                 head_dim: int, decode_backend: str = "auto", allow_tf32: bool = False, tree=None,
+                 window: int | None = None, sinks: int = 0):
         if len(owners) != len(lengths):
             raise ValueError("one length per owner")
+        if window is None and sinks:
+            raise ValueError("sinks stay in view beside a window: give one")
+        if window is not None and tree is not None:
+            raise ValueError("a tree of drafted tokens attends to the whole history: no window")
+        self.window, self.sinks = (None, 0) if window is None else pa.check_window(window, sinks)
         self.tree = None if tree is None else _tree_parents(tree, len(owners))
         self._tree_device: torch.Tensor | None = None
         self.pool = pool
@@ -526,14 +536,39 @@ class PagedPackedCache:
         self._tree_device = None if self.tree is None else self.tree.to(device)
         return self.meta
 
-    @torch.no_grad()
-    def update(self, key_states, value_states, layer_idx, *args, **kwargs):
-        B, Hkv, n, D = key_states.shape
+    def _meta_of(self, key_states, layer_idx) -> PageTable:
+        """The forward's page metadata, made by its first layer."""
+        B, _, n, _ = key_states.shape
         if B != len(self.owners):
             raise RuntimeError(f"batch {B} != {len(self.owners)} owners")
         if layer_idx == 0 or self.meta is None:
             self.begin(n, key_states.device)
+        return self.meta
+
+    def _packed_handle(self, layer_idx: int, D: int) -> pa.PackedKV:
         meta, pool = self.meta, self.pool
+        return pa.PackedKV(pool.k_pages[layer_idx], pool.k_norms[layer_idx],
+                           pool.v_pages[layer_idx], pool.v_norms[layer_idx],
+                           meta.table, meta.seq, pa.Quantizer.from_tq(self.kq),
+                           pa.Quantizer.from_tq(self.vq), D,
+                           seq_lens_host=meta.seq_host, page_table_host=meta.table_host)
+
+    def _appended(self, handle, layer_idx: int):
+        """The handle of a layer whose K and V are written, as the attention dispatcher takes it."""
+        handle.decode_backend = self.decode_backend
+        handle.allow_tf32 = self.allow_tf32
+        if self.tree is not None:
+            handle.tree, handle.tree_host = self._tree_device, self.tree
+        if self.window is not None:
+            handle.window, handle.sinks = self.window, self.sinks
+        if layer_idx == self.pool.num_layers - 1:
+            self.lengths = self.meta.seq_host.tolist()
+        return handle
+
+    @torch.no_grad()
+    def update(self, key_states, value_states, layer_idx, *args, **kwargs):
+        D = key_states.shape[-1]
+        meta, pool = self._meta_of(key_states, layer_idx), self.pool
         if pool.dense:
             _append_dense_rows(key_states, pool.k_pages[layer_idx], meta)
             _append_dense_rows(value_states, pool.v_pages[layer_idx], meta)
@@ -542,18 +577,22 @@ class PagedPackedCache:
         else:
             plan = _layer_append_plan(pool, layer_idx, self.kq, self.vq)
             plan.launch(plan.bind(key_states, value_states, meta.table, meta.start))  # ranges: begin()
-            handle = pa.PackedKV(pool.k_pages[layer_idx], pool.k_norms[layer_idx],
-                                 pool.v_pages[layer_idx], pool.v_norms[layer_idx],
-                                 meta.table, meta.seq, pa.Quantizer.from_tq(self.kq),
-                                 pa.Quantizer.from_tq(self.vq), D,
-                                 seq_lens_host=meta.seq_host, page_table_host=meta.table_host)
-        handle.decode_backend = self.decode_backend
-        handle.allow_tf32 = self.allow_tf32
-        if self.tree is not None:
-            handle.tree, handle.tree_host = self._tree_device, self.tree
-        if layer_idx == pool.num_layers - 1:
-            self.lengths = meta.seq_host.tolist()
+            handle = self._packed_handle(layer_idx, D)
+        handle = self._appended(handle, layer_idx)
         return handle, handle
+
+    def update_rotated(self, query_states, key_states, value_states, cos, sin, layer_idx: int):
+        """``update`` of a packed pool with q and K as the projections leave them: the position rotation
+        (``cos``, ``sin``, as in ``append_rotated_kv``) is applied on the way, in the append's one launch.
+        Returns the rotated q and the handle."""
+        if self.pool.dense:
+            raise pa.UnsupportedLayout("update_rotated writes packed pages")
+        pa.values_only("update_rotated", query_states, key_states, value_states, cos, sin)
+        meta = self._meta_of(key_states, layer_idx)
+        plan = _layer_append_plan(self.pool, layer_idx, self.kq, self.vq)
+        bound = plan.bind(key_states, value_states, meta.table, meta.start)             # ranges: begin()
+        q = plan.launch_rotated(bound, plan.bind_rotation(query_states, cos, sin, bound))
+        return q, self._appended(self._packed_handle(layer_idx, key_states.shape[-1]), layer_idx)
 
     @torch.no_grad()
     def commit(self, paths) -> list[int]:
@@ -728,10 +767,20 @@ def _offset_causal(lens: torch.Tensor, Q: int, Lmax: int, device):
     return mask[:, None].to(device), (last >= 0)[:, None, :, None].to(device)
 
 
-def _padded_sdpa(query, k, v, lens, scaling, tree=None):
+def _window_mask(lens: torch.Tensor, Q: int, Lmax: int, window: int, sinks: int, device):
+    """``_offset_causal`` within a window, the sinks in view throughout."""
+    p = (lens.to(torch.int64)[:, None] - Q + torch.arange(Q)[None, :])[:, :, None]              # (B, Q, 1)
+    j = torch.arange(Lmax)[None, None, :]
+    mask = (j <= p) & ((p - j < window) | (j < sinks))
+    return mask[:, None].to(device), (p >= 0)[:, None].to(device)
+
+
+def _padded_sdpa(query, k, v, lens, scaling, tree=None, window=None, sinks=0):
     """One SDPA call over histories padded to the longest; rows without a key are 0."""
     B, Hq, Q, _ = query.shape
-    if tree is None:
+    if window is not None:
+        mask, live = _window_mask(lens, Q, k.shape[2], window, sinks, query.device)
+    elif tree is None:
         mask, live = _offset_causal(lens, Q, k.shape[2], query.device)
     else:
         mask, live = _tree_mask(tree, lens, k.shape[2], query.device)
@@ -887,7 +936,7 @@ def _tree_mask(parents: torch.Tensor, lens: torch.Tensor, Lmax: int, device):
 def _dense_sdpa(query, kv: pa.DenseKV, scaling):
     """Gather every sequence's unquantized rows into one padded (B, Hkv, Lmax, D) pair with
     one indexed read per side, then one SDPA under the offset-causal mask
-    (packed_backend.py:229-246) or the handle's tree."""
+    (packed_backend.py:229-246), the handle's tree or its window."""
     B, Hq, Q, D = query.shape
     lens = _host_lens(kv).to(torch.int64)
     Lmax = int(lens.max()) if B else 0
@@ -901,7 +950,7 @@ def _dense_sdpa(query, kv: pa.DenseKV, scaling):
     slot = (t % S).to(query.device)[None, :].expand(B, Lmax)
     k = kv.k_pages[page, :, slot].permute(0, 2, 1, 3).to(query.dtype)         # (B, Hkv, Lmax, D)
     v = kv.v_pages[page, :, slot].permute(0, 2, 1, 3).to(query.dtype)
-    return _padded_sdpa(query, k, v, lens, scaling, getattr(kv, "tree_host", None))
+    return _padded_sdpa(query, k, v, lens, scaling, getattr(kv, "tree_host", None), getattr(kv, "window", None), getattr(kv, "sinks", 0))
 
 
 def _hip_packed(query, kv, scaling):
@@ -915,6 +964,10 @@ def _hip_dense(query, kv, scaling):
 def _hip_tree(query, kv, scaling):
     return pa.packed_tree_attention(query, kv, scaling, kv.tree, allow_tf32=getattr(kv, "allow_tf32", False),
                                     parents_host=kv.tree_host)
+
+
+def _hip_window(query, kv, scaling):
+    return pa.packed_window_attention(query, kv, scaling, window=kv.window, sinks=kv.sinks, allow_tf32=getattr(kv, "allow_tf32", False))
 
 
 def _hip_prefill(query, kv, scaling):
@@ -931,12 +984,20 @@ _ROUTES = {
     "prefill_dense_sdpa": _dense_sdpa,
     "tree_hip_packed": _hip_tree,
     "tree_dense_sdpa": _dense_sdpa,
+    "window_hip_packed": _hip_window,
+    "window_dense_sdpa": _dense_sdpa,
 }
 
 
 def _route(query, kv) -> str:
     if getattr(kv, "tree", None) is not None:
         return "tree_dense_sdpa" if isinstance(kv, pa.DenseKV) else "tree_hip_packed"
+    if getattr(kv, "window", None) is not None:
+        if isinstance(kv, pa.DenseKV):
+            return "window_dense_sdpa"
+        if getattr(kv, "decode_backend", "auto") == "reconstruct_sdpa":
+            raise ValueError("backend 'reconstruct_sdpa' attends to the whole history: no window")
+        return "window_hip_packed"
     if query.shape[2] > 1:
         if isinstance(kv, pa.DenseKV):
             return "prefill_dense_sdpa"
@@ -959,6 +1020,42 @@ def winnow_packed_attention(module, query, key, value, attention_mask, dropout: 
     route = _route(query, key)
     BACKEND_COUNTS[route] += 1
     return _ROUTES[route](query, key, scale).transpose(1, 2).contiguous(), None
+
+
+def _rotated_forward(attn):
+    """A Qwen2 attention module's forward whose rotation the cache's append applies: one launch writes
+    K and V and rotates q, in place of the rotation's elementary operations and an append. Calls that it
+    does not serve (no paged packed cache, another attention implementation, gradients, traces,
+    autocast to another type) go through the module's own forward."""
+    own = attn.forward
+
+    def forward(hidden_states, position_embeddings=None, attention_mask=None, past_key_values=None, **kwargs):
+        cache = past_key_values
+        if not isinstance(cache, PagedPackedCache) or cache.pool.dense or position_embeddings is None \
+                or attn.config._attn_implementation != ATTN_NAME or torch.is_grad_enabled() or not _plain(hidden_states):
+            return own(hidden_states=hidden_states, position_embeddings=position_embeddings, attention_mask=attention_mask,
+                       past_key_values=past_key_values, **kwargs)
+        shape = hidden_states.shape[:-1]
+        q, k, v = (proj(hidden_states).view(*shape, -1, attn.head_dim).transpose(1, 2) for proj in (attn.q_proj, attn.k_proj, attn.v_proj))
+        q, handle = cache.update_rotated(q, k, v, *position_embeddings, attn.layer_idx)
+        out, weights = winnow_packed_attention(attn, q, handle, handle, attention_mask, scaling=attn.scaling)
+        return attn.o_proj(out.reshape(*shape, -1)), weights
+    forward.own = own
+    return forward
+
+
+def fuse_rotary(model) -> int:
+    """Let the cache's append apply the position rotation in every attention layer of ``model``
+    (``append_rotated_kv``): K is then quantized from its fp32 rotation, not from one rounded to the
+    model's type. Returns the number of layers; a layer that has it already keeps it. Raises
+    ``UnsupportedModel`` for an architecture that this path does not serve."""
+    if _arch(model.config) not in SUPPORTED_ARCH:
+        raise UnsupportedModel(f"{_arch(model.config)} is not a supported architecture {SUPPORTED_ARCH}")
+    layers = [m for m in model.modules() if type(m).__name__ == "Qwen2Attention"]
+    for attn in layers:
+        if not hasattr(attn.forward, "own"):
+            attn.forward = _rotated_forward(attn)
+    return len(layers)
 
 
 def register() -> None:
