@@ -107,7 +107,9 @@ __global__ __launch_bounds__(kQBlock) void quantize_kernel(AppendArgs<ROT> a) {
       if constexpr (ROT) {
         const QuantRotary& r = a.rot;
         const int64_t co = b * r.csb + i * r.csn, so = b * r.ssb + i * r.ssn;
-        if (blockIdx.y == 0) {
+        if (EPT == 8 && blockIdx.y == 0 && r.k_vec) {
+          if constexpr (EPT == 8) rotated8_of(r, sd.x, a.x_dtype, xo - EPT * part, co, so, EPT * part, xv);
+        } else if (blockIdx.y == 0) {
 #pragma unroll
           for (int k = 0; k < EPT; ++k) xv[k] = rotated_elem(r, sd.x, xo - EPT * part, a.x_dtype, co, so, EPT * part + k);
         } else {

@@ -64,7 +64,10 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 template <bool G2>
 constexpr int tile_waves() { return G2 ? 8 : 16; }
 constexpr int kTileVecs = 16;    // vectors a wave takes per pass (an MFMA column tile)
-constexpr int kCells = 512;      // cells of the boundary grid
+// Cells of the boundary grid. A cell with two boundaries in reach sends every code there to float64: with ROT,
+// whose float64 path rotates again, a codebook of 8 bits whose levels crowd in the middle pays four times the cells.
+template <bool ROT>
+constexpr int tile_cells() { return ROT ? 2048 : 512; }
 constexpr int kListMax = 256;    // flagged pairs a wave lists; with more it recomputes the whole pass
 
 struct Cell {
@@ -155,6 +158,7 @@ __global__ __launch_bounds__(64 * tile_waves<G2>()) void quantize_tile_kernel(Ti
   static_assert(!(G2 && ROT), "one group of channels");
   constexpr int WV = tile_waves<G2>(), XT = ROT ? WN_F32 : DT;
   constexpr int KS = D / 32;  // K-steps of 32 input dims
+  constexpr int kCells = tile_cells<ROT>();
   constexpr int U = D / 32;   // eights of output dims per lane (two MFMA row tiles each)
   constexpr int NR = kTileVecs, NTHR = 64 * WV;
   constexpr bool F32 = XT == WN_F32;
@@ -165,14 +169,20 @@ __global__ __launch_bounds__(64 * tile_waves<G2>()) void quantize_tile_kernel(Ti
   __shared__ float rowsq[D];
   __shared__ TileWave<D, ROT> waves[WV];
 
-  if constexpr (ROT) {
-    if (blockIdx.y == gridDim.y - 1 && a.rot.q) {
-      rotate_queries<D, NTHR>(a.rot, a.n, blockIdx.x, gridDim.x, threadIdx.x);
+  // the work-group's side, and its place among the side's
+  int side = blockIdx.y;
+  uint32_t place = blockIdx.x, places = gridDim.x;
+  if constexpr (ROT) {  // dealt out by what each takes (launch_quantize_tiles)
+    side = place >= uint32_t(a.split[1]) ? 2 : place >= uint32_t(a.split[0]) ? 1 : 0;
+    if (side) place -= a.split[side - 1];
+    places = (side < 2 ? a.split[side] : places) - (side ? a.split[side - 1] : 0);
+    if (side == 2) {
+      rotate_queries<D, NTHR>(a.rot, a.n, place, places, threadIdx.x);
       return;
     }
   }
 
-  const auto& sd = a.side[blockIdx.y];
+  const auto& sd = a.side[side];
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
   const int wig = __builtin_amdgcn_readfirstlane(tid >> 6);
   TileWave<D, ROT>& wv = waves[wig];
@@ -190,8 +200,8 @@ __global__ __launch_bounds__(64 * tile_waves<G2>()) void quantize_tile_kernel(Ti
   }
   // passes are dealt to the work-groups in turn, so that a launch of few passes still
   // spreads over the CUs
-  const int64_t passes = (a.total + NR - 1) / NR, stride = int64_t(gridDim.x) * WV;
-  int64_t pass = int64_t(wig) * gridDim.x + blockIdx.x;
+  const int64_t passes = (a.total + NR - 1) / NR, stride = int64_t(places) * WV;
+  int64_t pass = int64_t(wig) * places + place;
 #pragma unroll
   for (int q = 0; q < NG; ++q)
     for (int i = tid; i < (1 << (q ? s2.bw : bw)) - 1; i += NTHR) bnd[q][i] = (q ? s2.bnd : sd.bnd)[i];
@@ -259,7 +269,7 @@ __global__ __launch_bounds__(64 * tile_waves<G2>()) void quantize_tile_kernel(Ti
     if constexpr (ROT) {
       const RotRowInfo& o = wv.row[rr];
       float y[8];
-      if (blockIdx.y == 0) {
+      if (side == 0) {
         rotated8<DT, CT>(a.rot, sd.x, xo, o.cs, o.sn, d, y);
       } else {
         const Raw8<DT> x = load8<DT>(sd.x, xo + d);
@@ -311,8 +321,29 @@ __global__ __launch_bounds__(64 * tile_waves<G2>()) void quantize_tile_kernel(Ti
     {
       Raw8<XT> x[KS];
       const int64_t xo = wv.row[c].x;
+      bool paired = false;  // whole heads rotated: a lane's eights hold each other's partners
+      if constexpr (ROT) {
+        paired = side == 0 && a.rot.R == D;
+        if (paired) {
+          Raw8<DT> raw[KS];
 #pragma unroll
-      for (int s = 0; s < KS; ++s) x[s] = fetch(c, xo, 32 * s + 8 * g);
+          for (int s = 0; s < KS; ++s) raw[s] = load8<DT>(sd.x, xo + 32 * s + 8 * g);
+#pragma unroll
+          for (int s = 0; s < KS / 2; ++s) {
+            float y0[8], y1[8];
+            const int64_t co = wv.row[c].cs + 32 * s + 8 * g, so = wv.row[c].sn + 32 * s + 8 * g;
+            rotated8_pair<DT, CT>(raw[s], raw[s + KS / 2], load8<CT>(a.rot.cos, co), load8<CT>(a.rot.sin, so), load8<CT>(a.rot.cos, co + D / 2),
+                                  load8<CT>(a.rot.sin, so + D / 2), y0, y1);
+            x[s] = __builtin_bit_cast(Raw8<XT>, y0);
+            x[s + KS / 2] = __builtin_bit_cast(Raw8<XT>, y1);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+      }
+      if (!paired) {
+#pragma unroll
+        for (int s = 0; s < KS; ++s) x[s] = fetch(c, xo, 32 * s + 8 * g);
+      }
       float sc[NG];
 #pragma unroll
       for (int q = 0; q < NG; ++q) {
@@ -545,13 +576,23 @@ int launch_quantize_tiles(const QuantArgs& a, int sides, int D, hipStream_t st) 
   return launch_tiles<false>(D == 64 ? pick_tile<64, false>(a.x_dtype) : pick_tile<128, false>(a.x_dtype), a, sides, st);
 }
 
-// The rows of the grid (K, V, q) share the CUs.
-int launch_quantize_tiles(const QuantRotArgs& a, int sides, int D, hipStream_t st) {
-  const int cus = device_cus(), rows = sides + (a.rot.q != nullptr);
+// One work-group a CU, as many of them for K, V and q as their work takes of it: a vector of K, rotated,
+// counts 6.5, one of V 5.2, a row of q 1, one in fp32 2.2. (The 65,528 vectors each and 262,112 rows of an 8,191-token prompt, 128
+// bf16 at 4 bits, on 256 CUs by shares of K, V and q, us: 107, 86 and 63: 58; 86, 86, 84: 64; 128, 64, 64: 63; 86, 64,
+// 106: 66; 128, 86, 42: 75. A wave's passes are whole, so neighbours of the best are not always near it.)
+int launch_quantize_tiles(const QuantRotArgs& args, int sides, int D, hipStream_t st) {
+  const int cus = device_cus();
   if (cus <= 0) return WN_E_LAUNCH;
-  const int64_t groups = std::min<int64_t>((a.total + kTileVecs - 1) / kTileVecs, std::max(1, cus / rows));
+  QuantRotArgs a = args;
+  const int64_t most = (a.total + kTileVecs - 1) / kTileVecs;  // passes of a side
+  const double k = 6.5 * double(a.total), v = sides > 1 ? 5.2 * double(a.total) : 0.0,
+               q = a.rot.q ? double(a.rot.B) * a.rot.Hq * a.n * (a.rot.q_dtype == WN_F32 ? 2.2 : 1.0) : 0.0, all = k + v + q;
+  const auto share = [&](double w) { return int(std::min<double>(double(most), std::max(1.0, w / all * cus + 0.5))); };
+  a.split[0] = share(k);
+  a.split[1] = a.split[0] + (sides > 1 ? share(v) : 0);
+  const int groups = a.split[1] + (a.rot.q ? std::max(1, cus - a.split[1]) : 0);
   const auto fn = D == 64 ? pick_tile_rot<64>(a.x_dtype, a.rot.rot_dtype) : pick_tile_rot<128>(a.x_dtype, a.rot.rot_dtype);
-  hipLaunchKernelGGL(fn, dim3(unsigned(groups), rows), dim3(64 * tile_waves<false>()), 0, st, a);
+  hipLaunchKernelGGL(fn, dim3(unsigned(groups)), dim3(64 * tile_waves<false>()), 0, st, a);
   return WN_OK;
 }
 

@@ -67,6 +67,7 @@ struct QuantRotary {
 
 struct QuantRotArgs : QuantArgs {
   QuantRotary rot;
+  int split[2];  // of the tile kernel: first work-group of V, and of q
 };
 
 // Channel d of a rotated row, from the row's channels and its token's cos and sin:
@@ -138,40 +139,118 @@ __device__ __forceinline__ void rotated8(const QuantRotary& r, const void* x, in
   }
 }
 
-// q's rows rotated, by the threads of `blocks` work-groups of NTHR. Rows are (b, h, i); eight
-// channels an item.
+// Channels d .. d + 7 (lo) and d + R / 2 .. d + R / 2 + 7 (hi) at once: each is the other's partner.
+template <int DT, int CT>
+__device__ __forceinline__ void rotated8_pair(const Raw8<DT>& lo, const Raw8<DT>& hi, const Raw8<CT>& c0, const Raw8<CT>& s0, const Raw8<CT>& c1,
+                                              const Raw8<CT>& s1, float (&y0)[8], float (&y1)[8]) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const float a = elem<DT>(lo, k), b = elem<DT>(hi, k);
+    if constexpr (DT != WN_F32 && CT != WN_F32) {
+      y0[k] = fmaf(-b, elem<CT>(s0, k), a * elem<CT>(c0, k));
+      y1[k] = fmaf(a, elem<CT>(s1, k), b * elem<CT>(c1, k));
+    } else {
+      y0[k] = turn(a, -b, elem<CT>(c0, k), elem<CT>(s0, k));
+      y1[k] = turn(b, a, elem<CT>(c1, k), elem<CT>(s1, k));
+    }
+  }
+}
+
+// Eight values as the rotated q's type, 16-byte aligned.
+template <int DT>
+__device__ __forceinline__ void store_rotated8(void* out, int64_t i, const float (&y)[8]) {
+  if constexpr (DT == WN_F32) {
+    __builtin_memcpy(__builtin_assume_aligned(static_cast<float*>(out) + i, 16), y, 32);
+  } else {
+    uint16_t o[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) o[k] = DT == WN_BF16 ? f32_to_bf16(y[k]) : f32_to_f16(y[k]);
+    __builtin_memcpy(__builtin_assume_aligned(static_cast<uint16_t*>(out) + i, 16), o, 16);
+  }
+}
+
+// q by 16 bytes: an item is sixteen channels of a token, eight and their partners or sixteen behind the
+// rotated ones, for HEADS heads, whose cos and sin are one; a head's rows are read and written once,
+// all in flight together.
+template <int D, int NTHR, int DT, int CT>
+__device__ __forceinline__ void rotate_heads(const QuantRotary& r, int n, uint32_t block, uint32_t blocks, int tid) {
+  constexpr int HEADS = DT == WN_F32 ? 2 : 4;
+  constexpr uint32_t PARTS = D / 16;
+  const uint32_t groups = (uint32_t(r.Hq) + HEADS - 1) / HEADS, items = uint32_t(r.B) * groups * uint32_t(n) * PARTS, turned = uint32_t(r.R) / 16;
+  for (uint32_t it = block * NTHR + tid; it < items; it += blocks * NTHR) {
+    const uint32_t row = it / PARTS, part = it % PARTS, i = row % uint32_t(n), bg = row / uint32_t(n), h0 = bg % groups * HEADS, b = bg / groups;
+    const bool turns = part < turned;
+    const uint32_t d = turns ? 8 * part : r.R + 16 * (part - turned), step = turns ? r.R / 2 : 8;
+    const int64_t qo = b * r.qsb + i * r.qsn + d;
+    Raw8<DT> lo[HEADS], hi[HEADS];
+#pragma unroll
+    for (int h = 0; h < HEADS; ++h) {
+      const int64_t at = qo + min(h0 + h, uint32_t(r.Hq) - 1) * r.qsh;  // past the last: it again
+      lo[h] = load8<DT>(r.q, at);
+      hi[h] = load8<DT>(r.q, at + step);
+    }
+    const uint32_t cd = turns ? d : 0;  // some row's: not used
+    const int64_t co = b * r.csb + i * r.csn + cd, so = b * r.ssb + i * r.ssn + cd;
+    const Raw8<CT> c0 = load8<CT>(r.cos, co), s0 = load8<CT>(r.sin, so), c1 = load8<CT>(r.cos, co + r.R / 2), s1 = load8<CT>(r.sin, so + r.R / 2);
+#pragma unroll
+    for (int h = 0; h < HEADS; ++h) {
+      if (h0 + h >= uint32_t(r.Hq)) break;
+      float y0[8], y1[8];
+      if (turns) {
+        rotated8_pair<DT, CT>(lo[h], hi[h], c0, s0, c1, s1, y0, y1);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          y0[k] = elem<DT>(lo[h], k);
+          y1[k] = elem<DT>(hi[h], k);
+        }
+      }
+      const int64_t to = ((int64_t(b) * r.Hq + h0 + h) * n + i) * D + d;
+      store_rotated8<DT>(r.q_out, to, y0);
+      store_rotated8<DT>(r.q_out, to + step, y1);
+    }
+  }
+}
+
+// f(x_dtype, type of the tables), as constants
+template <class F>
+__device__ __forceinline__ void rotary_types(const QuantRotary& r, int x_dtype, F&& f) {
+  const auto by = [&](auto dt) {
+    if (r.rot_dtype == WN_F32) f(dt, std::integral_constant<int, WN_F32>{});
+    else if (r.rot_dtype == WN_BF16) f(dt, std::integral_constant<int, WN_BF16>{});
+    else f(dt, std::integral_constant<int, WN_F16>{});
+  };
+  if (x_dtype == WN_F32) by(std::integral_constant<int, WN_F32>{});
+  else if (x_dtype == WN_BF16) by(std::integral_constant<int, WN_BF16>{});
+  else by(std::integral_constant<int, WN_F16>{});
+}
+
+// rotated8 of rows whose type is a run-time value.
+__device__ __forceinline__ void rotated8_of(const QuantRotary& r, const void* x, int x_dtype, int64_t row, int64_t co, int64_t so, int d, float (&y)[8]) {
+  rotary_types(r, x_dtype, [&](auto dt, auto ct) { rotated8<decltype(dt)::value, decltype(ct)::value>(r, x, row, co, so, d, y); });
+}
+
+// q's rows rotated, by the threads of `blocks` work-groups of NTHR: by rotate_heads, or eight channels of
+// a row (b, h, i) an item, element by element.
 template <int D, int NTHR>
 __device__ __forceinline__ void rotate_queries(const QuantRotary& r, int n, uint32_t block, uint32_t blocks, int tid) {
+  if (r.q_vec) {
+    rotary_types(r, r.q_dtype, [&](auto dt, auto ct) { rotate_heads<D, NTHR, decltype(dt)::value, decltype(ct)::value>(r, n, block, blocks, tid); });
+    return;
+  }
   constexpr uint32_t EIGHTS = D / 8;
-  const uint32_t items = uint32_t(r.B) * uint32_t(r.Hq) * uint32_t(n) * EIGHTS;  // below 2^31 (the host's check)
+  const uint32_t items = uint32_t(r.B) * uint32_t(r.Hq) * uint32_t(n) * EIGHTS;  // below 2^30 (the host's check)
   for (uint32_t it = block * NTHR + tid; it < items; it += blocks * NTHR) {
     const uint32_t row = it / EIGHTS, d = 8 * (it % EIGHTS), i = row % uint32_t(n), bh = row / uint32_t(n), h = bh % uint32_t(r.Hq),
                    b = bh / uint32_t(r.Hq);
     const int64_t qo = b * r.qsb + h * r.qsh + i * r.qsn, co = b * r.csb + i * r.csn, so = b * r.ssb + i * r.ssn;
     const int64_t to = int64_t(row) * D + d;
     float y[8];
-    if (r.q_vec) {
-      const auto by = [&](auto dt) {
-        constexpr int DT = decltype(dt)::value;
-        if (r.rot_dtype == WN_F32) rotated8<DT, WN_F32>(r, r.q, qo, co, so, d, y);
-        else if (r.rot_dtype == WN_BF16) rotated8<DT, WN_BF16>(r, r.q, qo, co, so, d, y);
-        else rotated8<DT, WN_F16>(r, r.q, qo, co, so, d, y);
-      };
-      if (r.q_dtype == WN_F32) by(std::integral_constant<int, WN_F32>{});
-      else if (r.q_dtype == WN_BF16) by(std::integral_constant<int, WN_BF16>{});
-      else by(std::integral_constant<int, WN_F16>{});
-    } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) y[k] = rotated_elem(r, r.q, qo, r.q_dtype, co, so, d + k);
-    }
-    if (r.q_dtype == WN_F32) {  // the output is contiguous: rows of whole 16 bytes
-      __builtin_memcpy(__builtin_assume_aligned(static_cast<float*>(r.q_out) + to, 16), y, 32);
-    } else {
-      uint16_t o[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) o[k] = r.q_dtype == WN_BF16 ? f32_to_bf16(y[k]) : f32_to_f16(y[k]);
-      __builtin_memcpy(__builtin_assume_aligned(static_cast<uint16_t*>(r.q_out) + to, 16), o, 16);
-    }
+    for (int k = 0; k < 8; ++k) y[k] = rotated_elem(r, r.q, qo, r.q_dtype, co, so, d + k);
+    if (r.q_dtype == WN_F32) store_rotated8<WN_F32>(r.q_out, to, y);
+    else if (r.q_dtype == WN_BF16) store_rotated8<WN_BF16>(r.q_out, to, y);
+    else store_rotated8<WN_F16>(r.q_out, to, y);
   }
 }
 
