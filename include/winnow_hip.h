@@ -530,12 +530,17 @@ int wn_append_rotated_kv(
  * The algebra, pages, norms, table, rotations, `exact` and alignments are those of wn_tree_attention;
  * n_rep * Q <= 2^20, S a power of two >= 16. Pages that no query of the call sees are not used: their
  * ids may be any value. num_splits and span come from wn_window_plan; any num_splits 1 .. 4096 and
- * any span that is a multiple of 64 are valid for any lengths. Lengths are taken as within [0,
+ * any span > 0 that is a multiple of 64 are valid for any lengths. span 0 is the row scan of one query
+ * at head_dim 128, num_splits waves of it (any number >= 1): the plan chooses it where `wide` says
+ * that pages and norms meet wn_decode_attention's alignments and stride limits, which the call
+ * requires (WN_E_INVALID otherwise). lens: B lengths in host memory, or NULL (every sequence fills
+ * its table row). Lengths are taken as within [0,
  * max_pages * S]; an id outside [0, num_pages) reads the last page (the Python layer refuses one that
  * a query would see). ev_begin / ev_end (hipEvent_t or NULL) are recorded around the scan kernel. */
-int wn_window_plan(int B, int Hq, int Hkv, int Q, int D, int S, int bw_k, int bw_v, int exact, int max_pages, int window, int sinks,
-                   const int32_t* lens, int* num_splits, int* span);
-int64_t wn_window_workspace_bytes(int B, int Hq, int Hkv, int Q, int D, int num_splits);
+int wn_window_plan(int B, int Hq, int Hkv, int Q, int D, int S, int bw_k, int bw_v, int exact, int wide, int max_pages, int window,
+                   int sinks, const int32_t* lens, int* num_splits, int* span);
+int64_t wn_window_workspace_bytes(int B, int Hq, int Hkv, int Q, int D, int S, int max_pages, int window, int sinks, int num_splits,
+                                  int span);
 int wn_window_attention(
     const void* q, int q_dtype, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_q,
     const float* pi_k, const float* pi_v, const float* codebook_k, const float* codebook_v,
@@ -552,6 +557,10 @@ int wn_window_attention(
  * a query of wn_window_attention sees in 0 .. num_pages - 1, else 0. */
 int wn_window_in_range(const int32_t* lens, const int32_t* page_table, int64_t table_stride_b, int B, int max_pages, int num_pages,
                        int S, int Q, int window, int sinks);
+/* wn_window_in_range and wn_window_plan of a call at once: 1 if the first holds and plan[0 .. 1] has num_splits and span, else 0. */
+int wn_window_prepare(const int32_t* lens, const int32_t* page_table, int64_t table_stride_b, int table_pages, int B, int Hq, int Hkv,
+                      int Q, int D, int S, int bw_k, int bw_v, int exact, int wide, int num_pages, int max_pages, int window, int sinks,
+                      int* plan);
 
 /* Penalties, biases and a mask applied to N rows of V logits (contiguous along V, row strides in
  * elements) in one pass; out may be logits itself, with its stride. Per row, in fp32, rounded once:

@@ -236,5 +236,8 @@ def test_window_c_abi():
         with pytest.raises(_lib.WinnowHipError, match=match):
             call(**kw)
     call(B=0, q=None)
-    assert _lib.lib().wn_window_workspace_bytes(1, 3, 2, 1, 64, 1) == -1
-    assert _lib.lib().wn_window_workspace_bytes(1, 4, 2, 1, 64, 0) == -1
+    size = _lib.lib().wn_window_workspace_bytes       # B, Hq, Hkv, Q, D, S, max_pages, window, sinks, num_splits, span
+    for bad in ((1, 3, 2, 1, 64, 16, 4, 8, 0, 1, 64), (1, 4, 2, 1, 64, 16, 4, 8, 0, 0, 64), (1, 4, 2, 1, 64, 16, 4, 0, 0, 1, 64),
+                (1, 4, 2, 2, 128, 16, 4, 8, 0, 8, 0), (1, 4, 2, 1, 64, 16, 4, 8, 0, 8, 0), (1, 4, 2, 1, 128, 24, 4, 8, 0, 8, 0)):
+        assert size(*bad) == -1
+    assert size(1, 4, 2, 1, 128, 16, 4, 8, 0, 8, 0) > 0 and size(1, 4, 2, 1, 64, 16, 4, 8, 0, 1, 64) > 0

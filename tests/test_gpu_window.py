@@ -112,7 +112,7 @@ def test_window_norm_ranges(factor, Q):
     _check(_run(q, kv, 0.05, 200, 4), q, kv, 0.05, 200, 4, torch.float32)
 
 
-@pytest.mark.parametrize("Q,S", [(1, 16), (1, 64), (12, 16), (12, 128), (100, 16)])
+@pytest.mark.parametrize("Q,S", [(1, 16), (1, 64), (1, 256), (12, 16), (12, 128), (100, 16)])
 @pytest.mark.parametrize("D,bw", [(128, 4), (64, 8)])
 def test_what_is_out_of_view_does_not_count(Q, S, D, bw):
     """Released pages (-1, ids of others, ids outside the pool), and NaN, infinities and the largest
@@ -154,6 +154,41 @@ def test_a_value_that_is_not_finite_reaches_the_rows_that_see_it(Q):
             assert not torch.isfinite(got[0, :, i]).any()
         else:
             assert torch.equal(got[0, :, i], clean[0, :, i])
+
+
+@pytest.mark.parametrize("Hq,Hkv,bwk,bwv", [(32, 8, 4, 4), (28, 4, 8, 8), (8, 8, 3, 3), (24, 2, 6, 4), (5, 1, 4, 8)])
+def test_row_scan_plans(Hq, Hkv, bwk, bwv):
+    """The row scan of one query over any number of waves: fewer than kv heads, one, many more than there
+    are chunks; ragged lengths, some empty or shorter than the sinks; and the tile scan beside it."""
+    lens = (0, 3, 64, 65, 700, 1, 1300)
+    q, kv = _case(60 + Hq + bwk, lens, Hq, Hkv, 128, 1, bwk, bwv)
+    dkv = to_device(kv, DEV)
+    for window, sinks in ((100, 4), (1, 0), (257, 33)):
+        for plan in ((1, 0), (3, 0), (Hkv, 0), (17 * Hkv, 0), (2048, 0), (2, 64), (1, 128)):
+            _check(_run(q, dkv, 0.09, window, sinks, plan=plan), q, kv, 0.09, window, sinks, torch.float32)
+    if bwk in (4, 6) and bwv in (4, 6):
+        _check(_run(q, dkv, 0.09, 100, 4, allow_tf32=True, plan=(40, 0)), q, kv, 0.09, 100, 4, torch.float32, single=True)
+
+
+def test_a_plan_that_the_layout_does_not_take():
+    """The row scan asks for the decode's alignments: refused where they are not met, or for other shapes."""
+    import dataclasses
+    from winnow_amd import _lib
+    pa = _pa()
+    q, kv = _case(3, (70, 300), 8, 2, 128, 1, 4, 4)
+    dkv = to_device(kv, DEV)
+    flat = torch.zeros(dkv.k_pages.numel() + 4, dtype=torch.uint8, device=DEV)
+    odd = dataclasses.replace(dkv, k_pages=flat[4:].view(dkv.k_pages.shape).copy_(dkv.k_pages))
+    assert pa.window_plan_for(q.to(DEV), dkv, 50, 4, True)[1] == 0 and pa.window_plan_for(q.to(DEV), odd, 50, 4, True)[1] > 0
+    with pytest.raises(_lib.WinnowHipError, match="row scan"):
+        _run(q, odd, 0.1, 50, 4, plan=(64, 0))
+    _check(_run(q, odd, 0.1, 50, 4), q, kv, 0.1, 50, 4, torch.float32)
+    q, kv = _case(4, (70, 300), 8, 2, 128, 2, 4, 4)
+    with pytest.raises(pa.UnsupportedLayout, match="sizes"):
+        _run(q, kv, 0.1, 50, 4, plan=(64, 0))
+    q, kv = _case(5, (70, 300), 8, 2, 64, 1, 4, 4)
+    with pytest.raises(pa.UnsupportedLayout, match="sizes"):
+        _run(q, kv, 0.1, 50, 4, plan=(64, 0))
 
 
 def test_a_wide_window_is_the_causal_mask():
@@ -206,7 +241,7 @@ def test_plans_workspaces_and_streams(Q):
     dkv, dq = to_device(kv, DEV), q.to(DEV)
     want = pa.packed_window_attention(dq, dkv, 0.1, window=300, sinks=4)
     _check(want, q, kv, 0.1, 300, 4, torch.float32)
-    need = pa.window_workspace_bytes(3, 8, 2, Q, 128, 7)
+    need = pa.window_workspace_bytes(3, 8, 2, Q, 128, 16, dkv.page_table.shape[1], 300, 4, 7, 64)
     ws = torch.full((need,), 255, dtype=torch.uint8, device=DEV)
     got = pa.packed_window_attention(dq, dkv, 0.1, window=300, sinks=4, num_splits=7, workspace=ws)
     _check(got, q, kv, 0.1, 300, 4, torch.float32)

@@ -201,9 +201,11 @@ SIGNATURES = {
         _c_p, _c_p, _c_p, _c_p, _c_p,               # tokens, logprob, entropy, top_logprobs, top_ids
         _c_i64, _c_i, _c_i, _c_p, _c_i64,           # N, V, top, workspace, bytes
         _c_p]),
-    "wn_window_plan": (_c_i, [_c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_p,
+    "wn_window_plan": (_c_i, [_c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_p,
                               ctypes.POINTER(_c_i), ctypes.POINTER(_c_i)]),
-    "wn_window_workspace_bytes": (_c_i64, [_c_i, _c_i, _c_i, _c_i, _c_i, _c_i]),
+    "wn_window_workspace_bytes": (_c_i64, [_c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i]),
+    "wn_window_prepare": (_c_i, [_c_p, _c_p, _c_i64, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i,
+                                 ctypes.POINTER(_c_i)]),
     "wn_window_attention": (_c_i, [
         _c_p, _c_i, _c_i64, _c_i64, _c_i64,         # q, dtype, strides (b, h, q)
         _c_p, _c_p, _c_p, _c_p,                     # pi_k, pi_v, codebooks

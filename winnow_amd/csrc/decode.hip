@@ -21,6 +21,7 @@
 #include <cstring>
 #include <map>
 #include <mutex>
+#include <type_traits>
 #include <utility>
 
 #include "wn_split.h"
@@ -40,14 +41,25 @@ struct RotArgs {
   int B, Hkv, n_rep, q_dtype;
 };
 
+// ... and of a windowed step: the pages in view, side by side.
+struct WindowRotArgs : RotArgs {
+  const int32_t* table;
+  int64_t tsb;
+  int32_t* view;      // (B, width) their ids
+  int32_t* view_len;  // (B)
+  int2* hole;         // (B)
+  int window, sinks, log2S, max_pages, num_pages, width;
+};
+
 // chunk_prefix[b] = sum over b' < b of ceil(L_b' / 64), b = 0..B (one 256-thread block).
-__device__ void chunk_prefix_block(const int32_t* seq_lens, int B, int32_t* prefix) {
+template <class Len>
+__device__ void chunk_prefix_block(Len&& len, int B, int32_t* prefix) {
   __shared__ int part[4];
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
   int carry = 0;
   for (int b0 = 0; b0 < B; b0 += 256) {
     const int b = b0 + tid;
-    const int n = b < B ? (seq_lens[b] + 63) >> 6 : 0;
+    const int n = b < B ? (len(b) + 63) >> 6 : 0;
     int x = n;  // inclusive wave scan
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -72,13 +84,32 @@ constexpr int rot_blocks(int D) { return D <= 128 ? 4 : D / 32; }
 // q_rot[b, kvh, h, j] = scale * sum_d q[b, kvh*n_rep + h, d] Pi_K[j, d] for output dims
 // j in block blockIdx.z of rot_blocks(D) (zero rows for h >= n_rep). The block's rows
 // of Pi_K are staged in LDS with a padded stride (thread j reads row j: banks j + d).
-template <int D, int NREP>
-__global__ __launch_bounds__(256) void rotate_q_kernel(RotArgs a) {
+template <int D, int NREP, bool WIN = false>
+__global__ __launch_bounds__(256) void rotate_q_kernel(std::conditional_t<WIN, WindowRotArgs, RotArgs> a) {
   constexpr int LDP = D + 1, JQ = D / rot_blocks(D);
   __shared__ float pis[JQ * LDP];
   __shared__ float qs[NREP][D];
   const int kvh = blockIdx.x, b = blockIdx.y, z = blockIdx.z, tid = threadIdx.x;
-  if (a.chunk_prefix && kvh == 0 && b == 0 && z == 0) chunk_prefix_block(a.seq_lens, a.B, a.chunk_prefix);
+  if constexpr (WIN) {
+    const auto view = [&](int i) {
+      return window_view(min(max(a.seq_lens[i], 0), a.max_pages << a.log2S), a.window, a.sinks, a.log2S);
+    };
+    if (kvh == 0 && b == 0 && z == 0) chunk_prefix_block([&](int i) { return view(i).len; }, a.B, a.chunk_prefix);
+    // a sequence's pages in view: by the z blocks of its first kv head in turn
+    if (kvh == 0) {
+      const WindowView v = view(b);
+      if (z == 0 && tid == 0) {
+        a.view_len[b] = v.len;
+        a.hole[b] = make_int2(v.hole_lo, v.hole_hi);
+      }
+      const int pages = (v.len + (1 << a.log2S) - 1) >> a.log2S;  // at most width (the host's count)
+      for (int c = 256 * z + tid; c < pages; c += 256 * int(gridDim.z))
+        // an id outside the pool reads the last page: only where the hole masks it (the caller's check)
+        a.view[int64_t(b) * a.width + c] = int32_t(min(uint32_t(a.table[b * a.tsb + (c < v.sink ? c : c + v.skip)]), uint32_t(a.num_pages - 1)));
+    }
+  } else {
+    if (a.chunk_prefix && kvh == 0 && b == 0 && z == 0) chunk_prefix_block([&](int i) { return a.seq_lens[i]; }, a.B, a.chunk_prefix);
+  }
   if (z == 0 && tid == 0) a.unit_meta[b * a.Hkv + kvh] = make_int2(0, 0);
   if (!a.pi_k) {  // no rotation (dense pages): q_rot = scale * q
     float* out = a.q_rot + (int64_t(b) * a.Hkv + kvh) * NREP * D + z * JQ;
@@ -709,6 +740,7 @@ int decode_attention(
   da.qrows = max(sk.nrep, 1);
   da.kvshift = sk.kvshift;
   da.kvdiv = sk.kvdiv;
+  da.hole = nullptr;
   // the row scan numbers its waves across work-groups of sk.wpb waves
   const int64_t waves = balanced ? int64_t(num_splits) : int64_t(num_splits) * Hkv_s * B;
   const dim3 grid = sk.rows ? dim3(unsigned((waves + sk.wpb - 1) / sk.wpb)) : dim3(num_splits, Hkv_s, B);
@@ -721,6 +753,144 @@ int decode_attention(
   return check_launch(tf32 ? "wn_decode_attention_tf32" : "wn_decode_attention");
 }
 }  // namespace
+
+// ---------------------------------------------------------------- a windowed step
+namespace wn {
+namespace {
+
+// Pages that a view may have: those of the sinks and, of the window, one more than whole ones.
+int window_width(int S, int max_pages, int window, int sinks) {
+  const int64_t n = (int64_t(sinks) + S - 1) / S + (int64_t(window) + S - 1) / S + 1;
+  return int(std::min<int64_t>(n, max_pages));
+}
+
+struct WindowLayout {
+  int64_t base, view, len, hole, total;
+};
+WindowLayout window_layout(int B, int Hq, int Hkv, int width, int num_splits) {
+  WindowLayout l;
+  l.base = 0;
+  l.view = align256(ws_layout(B, Hq, Hkv, 128, 0, num_splits).total);
+  l.len = l.view + align256(int64_t(B) * width * 4);
+  l.hole = l.len + align256(int64_t(B) * 4);
+  l.total = l.hole + align256(int64_t(B) * 8);
+  return l;
+}
+
+SplitKernel window_scan(int Hq, int Hkv, int bw_k, int bw_v, bool tf32) {
+  const int shift = row_shift(Hq / Hkv);
+  if (shift < 0) return SplitKernel{};
+  SplitKernel sk = pick_window_rows(bw_k, bw_v, (Hq / Hkv) >> shift, tf32);
+  sk.kvshift = shift;
+  sk.kvdiv = 1 << shift;
+  return sk;
+}
+
+}  // namespace
+
+int window_rows_waves(int Hq, int Hkv, int D, int bw_k, int bw_v, bool tf32) {
+  if (D != 128) return 0;
+  const SplitKernel sk = window_scan(Hq, Hkv, bw_k, bw_v, tf32);
+  return sk.fn ? resident_waves(sk) : 0;
+}
+
+// What the scan's loads and addresses ask of the layout, as wn_decode_attention does.
+bool window_rows_aligned(const WindowStep& s) {
+  const int nbk = 16 * s.bw_k, nbv = 16 * s.bw_v, align = nbk % 16 == 0 ? 16 : 8;
+  const int64_t lim = int64_t(1) << 31;
+  return aligned(s.k_pages, align) && s.ksp % align == 0 && s.ksh % align == 0 && aligned(s.v_pages, 8) && s.vsp % 8 == 0 &&
+         s.vsh % 8 == 0 && s.ksh >= int64_t(s.S) * nbk && s.vsh >= int64_t(s.S) * nbv && s.knp >= 0 && s.knp < lim && s.vnp >= 0 &&
+         s.vnp < lim && s.knh >= 0 && s.vnh >= 0 && int64_t(s.Hkv) * s.knh + s.S <= lim && int64_t(s.Hkv) * s.vnh + s.S <= lim &&
+         s.ksp >= 0 && s.ksp < 2 * lim && s.vsp >= 0 && s.vsp < 2 * lim && aligned(s.pi_v, 4);
+}
+
+int64_t window_rows_workspace(int B, int Hq, int Hkv, int S, int max_pages, int window, int sinks, int num_splits) {
+  return window_layout(B, Hq, Hkv, window_width(S, max_pages, window, sinks), num_splits).total;
+}
+
+int window_rows_attention(const WindowStep& s) {
+  const SplitKernel sk = window_scan(s.Hq, s.Hkv, s.bw_k, s.bw_v, s.tf32);
+  WN_REQUIRE(sk.fn && window_rows_aligned(s), WN_E_INVALID, "window: the row scan does not read this layout; ask wn_window_plan");
+  const int n_rep = s.Hq / s.Hkv, width = window_width(s.S, s.max_pages, s.window, s.sinks);
+  const WsLayout lay = ws_layout(s.B, s.Hq, s.Hkv, 128, 0, s.num_splits);
+  const WindowLayout wl = window_layout(s.B, s.Hq, s.Hkv, width, s.num_splits);
+  WN_REQUIRE(s.workspace && s.workspace_bytes >= wl.total && aligned(s.workspace, 256), WN_E_WORKSPACE,
+             "window: workspace needs %lld bytes, 256-aligned (got %lld)", (long long)wl.total, (long long)s.workspace_bytes);
+  char* ws = static_cast<char*>(s.workspace);
+  hipStream_t st = static_cast<hipStream_t>(s.stream);
+  const int Hkv_s = s.Hkv * sk.kvdiv, n_rep_s = n_rep / sk.kvdiv;
+  WindowRotArgs ra{};
+  ra.q = s.q;
+  ra.qsb = s.qsb;
+  ra.qsh = s.qsh;
+  ra.pi_k = s.pi_k;
+  ra.q_rot = reinterpret_cast<float*>(ws + lay.qrot);
+  ra.seq_lens = s.seq_lens;
+  ra.chunk_prefix = reinterpret_cast<int32_t*>(ws + lay.prefix);
+  ra.unit_meta = reinterpret_cast<int2*>(ws + lay.meta);
+  ra.scale = float(double(s.scale) * 1.4426950408889634);
+  ra.B = s.B;
+  ra.Hkv = Hkv_s;
+  ra.n_rep = n_rep_s;
+  ra.q_dtype = s.q_dtype;
+  ra.table = s.table;
+  ra.tsb = s.tsb;
+  ra.view = reinterpret_cast<int32_t*>(ws + wl.view);
+  ra.view_len = reinterpret_cast<int32_t*>(ws + wl.len);
+  ra.hole = reinterpret_cast<int2*>(ws + wl.hole);
+  ra.window = s.window;
+  ra.sinks = s.sinks;
+  ra.log2S = ilog2(s.S);
+  ra.max_pages = s.max_pages;
+  ra.num_pages = s.num_pages;
+  ra.width = width;
+  const dim3 rot(Hkv_s, s.B, rot_blocks(128));
+  if (sk.nrep == 4) hipLaunchKernelGGL(HIP_KERNEL_NAME(rotate_q_kernel<128, 4, true>), rot, dim3(256), 0, st, ra);
+  else hipLaunchKernelGGL(HIP_KERNEL_NAME(rotate_q_kernel<128, 8, true>), rot, dim3(256), 0, st, ra);
+
+  DecodeArgs da{};
+  da.q_rot = ra.q_rot;
+  da.k_pages = s.k_pages;
+  da.v_pages = s.v_pages;
+  da.k_norms = s.k_norms;
+  da.v_norms = s.v_norms;
+  da.cb_k = s.cb_k;
+  da.cb_v = s.cb_v;
+  da.table = ra.view;
+  da.seq_lens = ra.view_len;
+  da.part_acc = reinterpret_cast<float*>(ws + lay.acc);
+  da.part_ml = reinterpret_cast<float*>(ws + lay.ml);
+  da.ksp = s.ksp;
+  da.ksh = s.ksh;
+  da.vsp = s.vsp;
+  da.vsh = s.vsh;
+  da.knp = s.knp;
+  da.knh = s.knh;
+  da.vnp = s.vnp;
+  da.vnh = s.vnh;
+  da.tsb = width;
+  da.chunk_prefix = ra.chunk_prefix;
+  da.unit_meta = ra.unit_meta;
+  da.B = s.B;
+  da.Hkv = Hkv_s;
+  da.n_rep = n_rep_s;
+  da.log2S = ra.log2S;
+  da.num_splits = s.num_splits;
+  da.balanced = 1;
+  da.qrows = sk.nrep;
+  da.kvshift = sk.kvshift;
+  da.kvdiv = sk.kvdiv;
+  da.hole = ra.hole;
+  if (s.ev_begin) (void)hipEventRecord(static_cast<hipEvent_t>(s.ev_begin), st);
+  hipLaunchKernelGGL(sk.fn, dim3(unsigned((s.num_splits + sk.wpb - 1) / sk.wpb)), dim3(sk.block), 0, st, da);
+  if (s.ev_end) (void)hipEventRecord(static_cast<hipEvent_t>(s.ev_end), st);
+
+  MergeArgs ma{da.part_acc, da.part_ml, s.pi_v, ra.unit_meta, s.out, s.out_dtype, s.Hq, Hkv_s, n_rep_s, 1};
+  launch_merge(128, dim3(n_rep_s, Hkv_s, s.B), st, ma);
+  return check_launch("wn_window_attention");
+}
+
+}  // namespace wn
 
 #define WN_DECODE_PARAMS                                                                                       \
   const void *q, int q_dtype, int64_t q_stride_b, int64_t q_stride_h, const float *pi_k, const float *pi_v,    \

@@ -51,3 +51,10 @@ extern "C" int wn_tree_prepare(const int32_t* lens, const int32_t* page_table, i
          wn_parents_in_order(parents, parents_stride_b, B, T) &&
          wn_tree_plan(B, Hq, Hkv, T, D, S, bw_k, bw_v, exact, max_pages, lens, plan, plan + 1, plan + 2) == 0;
 }
+
+extern "C" int wn_window_prepare(const int32_t* lens, const int32_t* page_table, int64_t table_stride_b, int table_pages, int B, int Hq,
+                                 int Hkv, int Q, int D, int S, int bw_k, int bw_v, int exact, int wide, int num_pages, int max_pages,
+                                 int window, int sinks, int* plan) {
+  return plan && wn_window_in_range(lens, page_table, table_stride_b, B, table_pages, num_pages, S, Q, window, sinks) &&
+         wn_window_plan(B, Hq, Hkv, Q, D, S, bw_k, bw_v, exact, wide, max_pages, window, sinks, lens, plan, plan + 1) == 0;
+}

@@ -3,11 +3,19 @@
 // p - j < window or j < sinks,
 //   out = softmax(scale q . k_hat) v_hat,   k_hat = n_K (c_K Pi_K),   v_hat = n_V (c_V Pi_V).
 //
-// Host side. The kernels are the tree attention's (wn_tree.h, wn_tree_kernels.h), compiled for this
-// choice of keys: q' = q Pi_K^T once, a scan of the chunks that some query of a row block sees, split
-// where there are few blocks, and a merge with Pi_V. A row block's chunks are those of the sinks and
-// those from its first query's window to its last query (window_span): what lies between is not
-// read, so a call costs the window, not the context.
+// Host side. What lies between the sinks and the window is not read: a call costs the window, not the
+// context. Two scans:
+//
+// * the tree attention's (wn_tree.h, wn_tree_kernels.h), compiled for this choice of keys: q' = q Pi_K^T
+//   once, a scan of the chunks that some query of a row block sees (window_span), split where there are
+//   few blocks, and a merge with Pi_V. It serves every shape. 512 queries at a window of 4,096, 32 heads
+//   over 8, fp32 accuracy: 149 us of the call's 158, 0.7 PFLOP/s of fp16 products (three a factor).
+// * one query at head_dim 128: the decode's row scan (wn_decode_rows.h) over the pages in view, laid out
+//   side by side by the launch that rotates the query (window_view, decode.hip). Between the last sink
+//   and the window's first position lie fewer than two pages of it, which it masks. 32 sequences at a
+//   window of 8,192, 32 heads over 8, 4 bits: 75 us, 3.7 TB/s; a step of one user at 1,024: 20 us, three
+//   launches' latency.
+#include "wn_decode.h"
 #include "wn_tree_host.h"
 
 namespace wn {
@@ -35,8 +43,8 @@ bool window_shape(int B, int Hq, int Hkv, int Q, int D) {
 }  // namespace
 }  // namespace wn
 
-extern "C" int wn_window_plan(int B, int Hq, int Hkv, int Q, int D, int S, int bw_k, int bw_v, int exact, int max_pages, int window,
-                              int sinks, const int32_t* lens, int* num_splits, int* span) {
+extern "C" int wn_window_plan(int B, int Hq, int Hkv, int Q, int D, int S, int bw_k, int bw_v, int exact, int wide, int max_pages,
+                              int window, int sinks, const int32_t* lens, int* num_splits, int* span) {
   using namespace wn;
   clear_error();
   WN_REQUIRE(window_shape(B, Hq, Hkv, Q, D) && max_pages > 0 && int64_t(max_pages) * S <= INT32_MAX - 256 && window > 0 && sinks >= 0 &&
@@ -47,6 +55,17 @@ extern "C" int wn_window_plan(int B, int Hq, int Hkv, int Q, int D, int S, int b
              "wn_window_plan: (S=%d, bw_k=%d, bw_v=%d) not compiled", S, bw_k, bw_v);
   const int n_rep = Hq / Hkv, ch = window_chunk(D);
   const int64_t rows = int64_t(n_rep) * Q;
+  // One query at head_dim 128 takes the decode's row scan wherever that is compiled, whatever its size. Calls
+  // of 32 heads over 8 at 4 bits, us, row scan and tile scan: 1 sequence at 256 tokens in view 19.8 and 20.0, at
+  // 8,192 28 and 29; 8 at 1,024 23 and 30, at 4,096 29 and 51; 32 at 8,192 75 and 224.
+  if (Q == 1 && wide) {
+    const int waves = window_rows_waves(Hq, Hkv, D, bw_k, bw_v, exact == 0);
+    if (waves > 0) {
+      *num_splits = waves;
+      *span = 0;
+      return WN_OK;
+    }
+  }
   const auto scan = pick_window(D, exact != 0, bw_k, bw_v).scan[window_variant(rows)];
   const int64_t slots = tree_slots(scan, tree_lds(scan, bw_k, bw_v));
   WN_REQUIRE(slots > 0, WN_E_LAUNCH, "wn_window_plan: cannot query the device occupancy");
@@ -85,9 +104,11 @@ extern "C" int wn_window_plan(int B, int Hq, int Hkv, int Q, int D, int S, int b
   return WN_OK;
 }
 
-extern "C" int64_t wn_window_workspace_bytes(int B, int Hq, int Hkv, int Q, int D, int num_splits) {
+extern "C" int64_t wn_window_workspace_bytes(int B, int Hq, int Hkv, int Q, int D, int S, int max_pages, int window, int sinks,
+                                             int num_splits, int span) {
   using namespace wn;
-  if (!window_shape(B, Hq, Hkv, Q, D) || num_splits <= 0) return -1;
+  if (!window_shape(B, Hq, Hkv, Q, D) || !is_pow2(S) || max_pages <= 0 || window <= 0 || sinks < 0 || num_splits <= 0 || span < 0) return -1;
+  if (span == 0) return Q == 1 && D == 128 ? window_rows_workspace(B, Hq, Hkv, S, max_pages, window, sinks, num_splits) : -1;
   const int64_t rows = int64_t(Hq / Hkv) * Q;
   const auto scan = pick_window(D, false, 8, 8).scan[window_variant(rows)];
   return tree_layout(B, Hkv, tree_nrp(scan, rows), 0, D, num_splits).total;
@@ -113,8 +134,8 @@ extern "C" int wn_window_attention(
   WN_REQUIRE(q_dtype >= WN_F32 && q_dtype <= WN_BF16 && out_dtype >= WN_F32 && out_dtype <= WN_BF16, WN_E_INVALID,
              "window: dtype codes %d/%d", q_dtype, out_dtype);
   WN_REQUIRE(window > 0 && sinks >= 0, WN_E_INVALID, "window: window %d (at least 1), sinks %d", window, sinks);
-  WN_REQUIRE(num_splits > 0 && num_splits <= 4096 && span > 0 && span % 64 == 0, WN_E_INVALID, "window: num_splits %d, span %d",
-             num_splits, span);
+  WN_REQUIRE(span == 0 ? num_splits > 0 && Q == 1 && D == 128 : num_splits > 0 && num_splits <= 4096 && span > 0 && span % 64 == 0,
+             WN_E_INVALID, "window: num_splits %d, span %d", num_splits, span);
   WN_REQUIRE(num_pages > 0 && max_pages > 0 && int64_t(max_pages) * S <= INT32_MAX - 256, WN_E_INVALID,
              "window: num_pages %d, max_pages %d", num_pages, max_pages);
   if (B == 0) return WN_OK;
@@ -128,6 +149,12 @@ extern "C" int wn_window_attention(
              WN_E_INVALID, "window: negative stride");
   WN_REQUIRE(aligned(pi_k, 16) && aligned(q, q_dtype == WN_F32 ? 4 : 2) && aligned(out, out_dtype == WN_F32 ? 4 : 2), WN_E_INVALID,
              "window: Pi_K 16-byte aligned, q and out aligned to their type");
+  if (span == 0)
+    return window_rows_attention(WindowStep{q, q_dtype, q_stride_b, q_stride_h, pi_k, pi_v, codebook_k, codebook_v, k_pages, v_pages,
+                                            k_stride_p, k_stride_h, v_stride_p, v_stride_h, k_norms, v_norms, kn_stride_p, kn_stride_h,
+                                            vn_stride_p, vn_stride_h, page_table, table_stride_b, seq_lens, out, out_dtype, workspace,
+                                            workspace_bytes, B, Hq, Hkv, S, bw_k, bw_v, num_pages, max_pages, window, sinks, scale,
+                                            exact == 0, num_splits, stream, ev_begin, ev_end});
   const int n_rep = Hq / Hkv;
   const int64_t rows = int64_t(n_rep) * Q;
   const WindowKernels k = pick_window(D, exact != 0, bw_k, bw_v);

@@ -27,6 +27,7 @@ struct DecodeArgs {
   int qrows;     // rows of q_rot per kv head
   int kvshift;   // the pages of (virtual) kv head h are those of kv head h >> kvshift (row scans)
   int kvdiv;     // the same for the vector-ALU scan: kv head h / kvdiv
+  const int2* hole;  // windows: tokens [x, y) of each sequence that are masked
 };
 
 using SplitFn = void (*)(DecodeArgs);
@@ -59,6 +60,56 @@ SplitKernel pick_split_pair(int bw_k, int bw_v, int n_rep);
 // 4 and 6-bit K and V (alike or mixed) and up to eight query heads per kv head, or an
 // empty SplitKernel.
 SplitKernel pick_split_rows_tf(int bw_k, int bw_v, int n_rep);
+
+// The row scans of a windowed step (wn_window_attention, one query): as pick_split_rows, or with tf32
+// as pick_split_rows_tf where that is compiled, over the pages in view, with DecodeArgs::hole.
+SplitKernel pick_window_rows(int bw_k, int bw_v, int n_rep, bool tf32);
+
+// The pages in view of a single query, laid out side by side: the sinks' and the window's. Column c of them
+// is the sequence's column c < sink ? c : c + skip; `len` tokens in all, of which [hole.x, hole.y) are
+// behind the sinks and ahead of the window.
+struct WindowView {
+  int len, sink, skip, hole_lo, hole_hi;
+};
+__host__ __device__ inline WindowView window_view(int L, int window, int sinks, int log2S) {
+  WindowView v;
+  const int lo = L > window ? L - window : 0, own = sinks < L ? sinks : L, S = 1 << log2S;
+  v.sink = (own + S - 1) >> log2S;
+  v.skip = (lo >> log2S) > v.sink ? (lo >> log2S) - v.sink : 0;
+  v.len = L - (v.skip << log2S);
+  v.hole_lo = own;
+  v.hole_hi = lo - (v.skip << log2S);
+  return v;
+}
+
+// One windowed step on the row scans. Balanced plans: num_splits waves (window_rows_waves: those resident).
+struct WindowStep {
+  const void* q;
+  int q_dtype;
+  int64_t qsb, qsh;
+  const float *pi_k, *pi_v, *cb_k, *cb_v;
+  const uint8_t *k_pages, *v_pages;
+  int64_t ksp, ksh, vsp, vsh;
+  const uint16_t *k_norms, *v_norms;
+  int64_t knp, knh, vnp, vnh;
+  const int32_t* table;
+  int64_t tsb;
+  const int32_t* seq_lens;
+  void* out;
+  int out_dtype;
+  void* workspace;
+  int64_t workspace_bytes;
+  int B, Hq, Hkv, S, bw_k, bw_v, num_pages, max_pages, window, sinks;
+  float scale;
+  bool tf32;
+  int num_splits;
+  void *stream, *ev_begin, *ev_end;
+};
+// 0: the row scans do not serve this shape
+int window_rows_waves(int Hq, int Hkv, int D, int bw_k, int bw_v, bool tf32);
+bool window_rows_aligned(const WindowStep& s);
+int64_t window_rows_workspace(int B, int Hq, int Hkv, int S, int max_pages, int window, int sinks, int num_splits);
+int window_rows_attention(const WindowStep& s);
 
 // Dense-page scan (bf16 or fp16 pages of head_dim 64 or 128, up to 16 query heads
 // per kv head, page size >= 16) on the row scan's work plan, or an empty SplitKernel

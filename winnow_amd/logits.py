@@ -34,6 +34,8 @@ def pack_allowed(allowed: torch.Tensor) -> torch.Tensor:
 def _penalty(name: str, value, N: int, device: torch.device) -> tuple:
     """(tensor or None, scalar) of a penalty given as a number or one per row."""
     if not isinstance(value, torch.Tensor):
+        if type(value) is float and (value == 0.0 if name != "repetition" else value == 1.0):
+            return None, value
         value = float(value)
         if not math.isfinite(value) or (name == "repetition" and value <= 0):
             raise UnsupportedLayout(f"{name} must be finite{' and above 0' if name == 'repetition' else ''}, got {value}")
@@ -84,7 +86,7 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, 
     (N, V), dev = logits.shape, logits.device
     if not 1 <= V <= 2 ** 31 - 1 - 65536 or (V > 1 and logits.stride(1) != 1):
         raise UnsupportedLayout(f"logits need a contiguous, non-empty last axis of fewer than 2^31 - 65536, got {V}")
-    values_only("adjust_logits", *(t for t in (logits, bias, repetition, presence, frequency, out) if isinstance(t, torch.Tensor)))
+    values_only("adjust_logits", *[t for t in (logits, bias, repetition, presence, frequency, out) if isinstance(t, torch.Tensor)])
     if history is None and (lengths is not None or prompt_lengths is not None):
         raise UnsupportedLayout("lengths and prompt_lengths are those of a history")
     H = 0
@@ -93,9 +95,12 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, 
             raise UnsupportedLayout(f"history must be ({N}, H), H <= {MAX_HISTORY}, got {tuple(history.shape)}")
         H = history.shape[1]
         history = _whole("history", history, (N, H), dev)
-        lengths, prompt_lengths = (None if t is None else _whole(name, t, (N,), dev).contiguous()
-                                   for name, t in (("lengths", lengths), ("prompt_lengths", prompt_lengths)))
-    rep, pres, freq = (_penalty(name, t, N, dev) for name, t in (("repetition", repetition), ("presence", presence), ("frequency", frequency)))
+        if lengths is not None:
+            lengths = _whole("lengths", lengths, (N,), dev)
+        if prompt_lengths is not None:
+            prompt_lengths = _whole("prompt_lengths", prompt_lengths, (N,), dev)
+    rep = _penalty("repetition", repetition, N, dev)
+    pres, freq = _penalty("presence", presence, N, dev), _penalty("frequency", frequency, N, dev)
     if (bias is None) != (bias_ids is None):
         raise UnsupportedLayout("bias and bias_ids come together")
     J = 0
@@ -105,7 +110,7 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, 
         J = bias.shape[1]
         bias_ids = _whole("bias_ids", bias_ids, (N, J), dev)
         bias = bias if J <= 1 or bias.stride(1) == 1 else bias.contiguous()
-    words = mask_words(V)
+    words = (V + 31) // 32
     if allowed is not None and (allowed.shape != (N, words) or allowed.dtype != torch.int32 or allowed.device != dev
                                 or (words > 1 and allowed.stride(1) != 1)):
         raise UnsupportedLayout(f"allowed must be ({N}, {words}) int32 on {dev} with contiguous rows, got "

@@ -31,6 +31,7 @@ from dataclasses import dataclass
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 from torch.fx.experimental.proxy_tensor import get_proxy_mode
 
 from winnow_amd import _lib
@@ -167,11 +168,14 @@ def values_only(what: str, *operands: torch.Tensor) -> None:
     tangent of its operands, or a place in a trace (``torch.jit.trace``, ``make_fx``). A call into the
     library shows in none of them: the result would silently have no derivative, and the trace would
     hold an allocation in the operator's place."""
-    for t in operands:
-        if t.requires_grad and torch.is_grad_enabled():
-            raise UnsupportedLayout(f"{what} has no gradient: call it under torch.no_grad() or detach its operands")
-        if torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
-            raise UnsupportedLayout(f"{what} has no forward-mode derivative: call it on the primal")
+    if torch.is_grad_enabled():
+        for t in operands:
+            if t.requires_grad:
+                raise UnsupportedLayout(f"{what} has no gradient: call it under torch.no_grad() or detach its operands")
+    if forward_ad._current_level >= 0:  # a tensor has a tangent within a level only
+        for t in operands:
+            if forward_ad.unpack_dual(t).tangent is not None:
+                raise UnsupportedLayout(f"{what} has no forward-mode derivative: call it on the primal")
     if torch._C._get_tracing_state() is not None or get_proxy_mode() is not None:
         raise UnsupportedLayout(f"{what} cannot be traced")
 
@@ -709,6 +713,8 @@ MAX_WINDOW_ROWS = 1 << 20      # queries of a kv head: n_rep * Q
 
 def check_window(window: int, sinks: int) -> tuple[int, int]:
     """A window of at least one position and a count of sinks, as the C ABI takes them."""
+    if type(window) is int and type(sinks) is int and 0 < window < 2 ** 31 and 0 <= sinks < 2 ** 31:
+        return window, sinks
     if isinstance(window, bool) or isinstance(sinks, bool) or int(window) != window or int(sinks) != sinks or window < 1 or sinks < 0:
         raise UnsupportedLayout(f"a window of {window} positions and {sinks} sinks (whole numbers, at least 1 and at least 0)")
     return min(int(window), 2 ** 31 - 1), min(int(sinks), 2 ** 31 - 1)
@@ -718,10 +724,13 @@ def check_window_ranges(seq_lens: torch.Tensor, page_table: torch.Tensor, num_pa
                         sinks: int) -> None:
     """Every length fits the table and every page that one of the last ``queries`` positions sees lies
     in [0, num_pages). Reads host copies, natively for int32 mirrors."""
-    lens, table = seq_lens.detach().to("cpu"), page_table.detach().to("cpu")
-    if _lib.window_in_range(lens, table, num_pages, page_size, queries, window, sinks):
+    if not seq_lens.is_cpu:
+        seq_lens = seq_lens.cpu()
+    if not page_table.is_cpu:
+        page_table = page_table.cpu()
+    if _lib.window_in_range(seq_lens, page_table, num_pages, page_size, queries, window, sinks):
         return
-    lens, table = lens.numpy().astype(np.int64), table.numpy()
+    lens, table = seq_lens.detach().numpy().astype(np.int64), page_table.detach().numpy()
     width = table.shape[1]
     if lens.size and (lens.min() < 0 or lens.max() > width * page_size):
         raise UnsupportedLayout("seq_lens out of range for the page table")
@@ -736,8 +745,23 @@ def check_window_ranges(seq_lens: torch.Tensor, page_table: torch.Tensor, num_pa
 
 
 @functools.lru_cache(maxsize=1024)
-def window_workspace_bytes(batch: int, num_q_heads: int, num_kv_heads: int, q_len: int, head_dim: int, num_splits: int) -> int:
-    return int(_lib.lib().wn_window_workspace_bytes(batch, num_q_heads, num_kv_heads, q_len, head_dim, num_splits))
+def window_workspace_bytes(batch: int, num_q_heads: int, num_kv_heads: int, q_len: int, head_dim: int, page_size: int, max_pages: int,
+                           window: int, sinks: int, num_splits: int, span: int) -> int:
+    return int(_lib.lib().wn_window_workspace_bytes(batch, num_q_heads, num_kv_heads, q_len, head_dim, page_size, max_pages, window, sinks,
+                                                    num_splits, span))
+
+
+def _decode_rows(kv: PackedKV) -> bool:
+    """Whether pages and norms meet the alignments and limits of the decode's row scans."""
+    for pages in (kv.k_pages, kv.v_pages):
+        st, align = pages.stride(), 16 if pages.shape[3] % 16 == 0 and pages is kv.k_pages else 8
+        if pages.data_ptr() % align or st[0] % align or st[1] % align or not 0 <= st[0] < 2 ** 32 or st[1] < pages.shape[2] * pages.shape[3]:
+            return False
+    for norms in (kv.k_norms, kv.v_norms):
+        st = norms.stride()
+        if not (0 <= st[0] < 2 ** 31 and 0 <= st[1] and norms.shape[1] * st[1] + norms.shape[2] <= 2 ** 31):
+            return False
+    return True
 
 
 def window_plan_for(q: torch.Tensor, kv: PackedKV, window: int, sinks: int, exact: bool, *, read_lens: bool = True) -> tuple[int, int]:
@@ -749,17 +773,33 @@ def window_plan_for(q: torch.Tensor, kv: PackedKV, window: int, sinks: int, exac
         lens = kv.seq_lens.cpu()
     if lens is not None and (lens.dtype != torch.int32 or lens.shape != (B,) or not lens.is_contiguous()):
         lens = lens.to(torch.int32).reshape(B).contiguous()
-    ns, span = ctypes.c_int(0), ctypes.c_int(0)
+    plan = (ctypes.c_int * 2)()
     with _lib.on(q.device):
         _lib.call("wn_window_plan", B, Hq, kv.num_kv_heads, Q, D, kv.page_size, kv.k_quant.bit_width, kv.v_quant.bit_width, int(exact),
-                  kv.page_table.shape[1], window, sinks, _lib.ptr(lens), ctypes.byref(ns), ctypes.byref(span))
-    return ns.value, span.value
+                  _decode_rows(kv), kv.page_table.shape[1], window, sinks, _lib.ptr(lens), plan, ctypes.cast(ctypes.byref(plan, 4), ctypes.POINTER(ctypes.c_int)))
+    return plan[0], plan[1]
+
+
+def _window_prepare(kv: PackedKV, sizes: tuple, exact: bool, wide: bool, window: int, sinks: int, device: torch.device):
+    """The range check and the plan in one call where host mirrors hold all of it (``wn_window_prepare``);
+    None where they do not, or something is out of range. sizes: B, Hq, Hkv, Q, D, S, both widths."""
+    lens, table = kv.seq_lens_host, kv.page_table_host
+    if lens is None or table is None or not (lens.is_cpu and table.is_cpu) or not lens.dtype == table.dtype == torch.int32:
+        return None
+    shape, st = table.shape, table.stride()
+    if lens.shape != (sizes[0],) or len(shape) != 2 or shape[0] != sizes[0] or not lens.is_contiguous() or (shape[1] > 1 and st[1] != 1):
+        return None
+    plan = (ctypes.c_int * 2)()
+    with _lib.on(device):
+        ok = _lib.lib().wn_window_prepare(lens.data_ptr(), table.data_ptr(), st[0], shape[1], *sizes, exact, wide, kv.k_pages.shape[0],
+                                          kv.page_table.shape[1], window, sinks, plan)
+    return tuple(plan) if ok else None
 
 
 def packed_window_attention(q: torch.Tensor, kv: PackedKV, scale: float, *, window: int, sinks: int = 0,
                             allow_tf32: bool = False, num_splits: int | None = None,
                             out_dtype: torch.dtype | None = None, workspace: torch.Tensor | None = None,
-                            check_ranges: bool = True, timing_events=None) -> torch.Tensor:
+                            check_ranges: bool = True, timing_events=None, plan: tuple[int, int] | None = None) -> torch.Tensor:
     """Attention under a sliding window, with the first ``sinks`` positions in view throughout, over
     packed pages: q (B, Hq, Q, D) -> (B, Hq, Q, D) in q.dtype (``wn_window_attention``).
 
@@ -772,10 +812,11 @@ def packed_window_attention(q: torch.Tensor, kv: PackedKV, scale: float, *, wind
     wholly outside may be -1 (their pages released). Every head_dim, width pair, n_rep and page
     size of ``packed_decode_attention`` is served, Q up to 2^20 / n_rep. Products have fp32 accuracy
     whatever the query's type, or, where ``allow_tf32`` is given, TF32-class accuracy (single fp16
-    operands, fp32 accumulation), as in the decode. ``num_splits`` replaces the library's split
-    count, ``out_dtype`` the result's type, ``workspace`` is a caller-owned uint8 buffer of at least
-    ``window_workspace_bytes``, ``timing_events`` a pair of raw ``hipEvent_t`` handles recorded
-    around the scan.
+    operands, fp32 accumulation), as in the decode. ``num_splits`` asks for so many splits of the
+    tile scan, ``plan`` = ``(num_splits, span)`` replaces the library's plan (``window_plan_for``; span 0
+    is the row scan of one query at head_dim 128, over ``num_splits`` waves), ``out_dtype`` the result's
+    type, ``workspace`` is a caller-owned uint8 buffer of at least ``window_workspace_bytes``,
+    ``timing_events`` a pair of raw ``hipEvent_t`` handles recorded around the scan.
 
     Raises ``UnsupportedLayout`` before any launch for what ``check_contract`` rejects, for layouts
     that the scan does not read, for a gradient, a tangent or a trace; ``check_ranges`` covers lengths
@@ -790,15 +831,22 @@ def packed_window_attention(q: torch.Tensor, kv: PackedKV, scale: float, *, wind
     out_dtype = out_dtype or q.dtype
     if out_dtype not in _lib.DTYPE_CODE:
         raise UnsupportedLayout(f"output dtype {out_dtype} is not supported")
-    if check_ranges:
+    exact, kq, vq, table = not allow_tf32, kv.k_quant, kv.v_quant, kv.page_table
+    sizes = (B, Hq, Hkv, Q, D, S, kq.bit_width, vq.bit_width)
+    made = _window_prepare(kv, sizes, exact, Q == 1 and _decode_rows(kv), window, sinks, q.device) if check_ranges and B else None
+    if check_ranges and made is None:
         check_window_ranges(kv.seq_lens if kv.seq_lens_host is None else kv.seq_lens_host,
-                            kv.page_table if kv.page_table_host is None else kv.page_table_host, P, S, Q, window, sinks)
-    exact = not allow_tf32
+                            table if kv.page_table_host is None else kv.page_table_host, P, S, Q, window, sinks)
     out = torch.empty(B, Hq, Q, D, dtype=out_dtype, device=q.device)
     if B == 0:
         return out
-    ns, span = (int(num_splits), 64) if num_splits else window_plan_for(q, kv, window, sinks, exact, read_lens=check_ranges)
-    need = window_workspace_bytes(B, Hq, Hkv, Q, D, ns)
+    if plan is not None:
+        ns, span = plan
+    elif num_splits:
+        ns, span = int(num_splits), 64
+    else:
+        ns, span = made or window_plan_for(q, kv, window, sinks, exact, read_lens=check_ranges)
+    need = window_workspace_bytes(B, Hq, Hkv, Q, D, S, table.shape[1], window, sinks, ns, span)
     if need < 0:
         raise UnsupportedLayout(f"bad window sizes B={B} Hq={Hq} Hkv={Hkv} Q={Q} splits={ns}")
     room = need
@@ -809,7 +857,6 @@ def packed_window_attention(q: torch.Tensor, kv: PackedKV, scale: float, *, wind
         if room < need or workspace.device != q.device or not workspace.is_contiguous():
             raise UnsupportedLayout(f"workspace needs {need} contiguous bytes on {q.device}")
     ev0, ev1 = timing_events or (None, None)
-    kq, vq, table = kv.k_quant, kv.v_quant, kv.page_table
     kp, vp, kn, vn = kv.k_pages.stride(), kv.v_pages.stride(), kv.k_norms.stride(), kv.v_norms.stride()
     with _lib.on(q.device):
         _lib.call("wn_window_attention", q.data_ptr(), _lib.DTYPE_CODE[q.dtype], *q.stride()[:3],
@@ -818,7 +865,7 @@ def packed_window_attention(q: torch.Tensor, kv: PackedKV, scale: float, *, wind
                   kv.k_norms.data_ptr(), kn[0], kn[1], kv.v_norms.data_ptr(), vn[0], vn[1],
                   table.data_ptr(), table.stride(0), kv.seq_lens.data_ptr(),
                   out.data_ptr(), _lib.DTYPE_CODE[out_dtype], workspace.data_ptr(), room,
-                  B, Hq, Hkv, Q, D, S, kq.bit_width, vq.bit_width, P, table.shape[1], window, sinks, float(scale), int(exact), ns, span,
+                  *sizes, P, table.shape[1], window, sinks, float(scale), int(exact), ns, span,
                   _lib.stream_of(q.device), ev0, ev1)
     return out
 

@@ -142,41 +142,36 @@ class AppendPlan:
 
     def __init__(self, k_tq, v_tq, k_pages: torch.Tensor, v_pages: torch.Tensor | None,
                  k_norms: torch.Tensor, v_norms: torch.Tensor | None):
-        self.has_v = v_pages is not None or v_norms is not None or v_tq is not None
-        ops = [k_pages, k_norms] + ([v_pages, v_norms] if self.has_v else [])
-        if any(t is None for t in ops) or (self.has_v and v_tq is None):
+        self.has_v = has_v = v_pages is not None or v_norms is not None or v_tq is not None
+        if k_pages is None or k_norms is None or (has_v and (v_pages is None or v_norms is None or v_tq is None)):
             raise pa.UnsupportedLayout("append: V needs its pages and norms")
-        if not all(_lib.is_hip(t) for t in ops) or len({t.device for t in ops}) != 1:
+        self.device = dev = k_pages.device
+        if not _lib.is_hip(k_pages) or k_norms.device != dev or (has_v and (v_pages.device != dev or v_norms.device != dev)):
             raise pa.UnsupportedLayout("append: every operand must be on one HIP device")
-        if k_pages.dim() != 4:
-            raise pa.UnsupportedLayout(f"append: pages must be (P, Hkv, S, NB), got {tuple(k_pages.shape)}")
-        self.device = k_pages.device
+        lead = k_pages.shape
+        if len(lead) != 4:
+            raise pa.UnsupportedLayout(f"append: pages must be (P, Hkv, S, NB), got {tuple(lead)}")
         self.dev_index = k_pages.get_device()
-        self.P, self.Hkv, self.S = k_pages.shape[0], k_pages.shape[1], k_pages.shape[2]
+        self.P, self.Hkv, self.S = P, Hkv, S = lead[0], lead[1], lead[2]
         self.D = D = k_tq.Pi.shape[-1]
-        P, Hkv, S = self.P, self.Hkv, self.S
-        sides = [(k_pages, k_norms, k_tq)] + ([(v_pages, v_norms, v_tq)] if self.has_v else [])
-        for pages, norms, tq in sides:
-            nb = packed_bytes(D, tq.bit_width)
-            if pages.dtype != torch.uint8 or pages.shape != (P, Hkv, S, nb) or pages.stride(-1) != 1 \
-                    or pages.stride(-2) != nb:
+        strides = []
+        for pages, norms, tq in ((k_pages, k_norms, k_tq), (v_pages, v_norms, v_tq))[:2 if has_v else 1]:
+            nb, st, nst = packed_bytes(D, tq.bit_width), pages.stride(), norms.stride()
+            if pages.dtype != torch.uint8 or pages.shape != (P, Hkv, S, nb) or st[3] != 1 or st[2] != nb:
                 raise pa.UnsupportedLayout(f"append: pages must be (P={P}, Hkv={Hkv}, S={S}, NB={nb}) uint8 "
                                            f"with contiguous rows, got {tuple(pages.shape)}")
-            if norms.dtype != torch.float16 or norms.shape != (P, Hkv, S) or norms.stride(-1) != 1:
+            if norms.dtype != torch.float16 or norms.shape != (P, Hkv, S) or nst[2] != 1:
                 raise pa.UnsupportedLayout("append: norms must be (P, Hkv, S) fp16 with a contiguous slot axis")
-            if tq.Pi.shape != (D, D) or tq.Pi.device != self.device or tq.boundaries.numel() != 2 ** tq.bit_width - 1:
+            if tq.Pi.shape != (D, D) or tq.Pi.device != dev or tq.boundaries.numel() != 2 ** tq.bit_width - 1:
                 raise pa.UnsupportedLayout("append: quantizer does not match head_dim or device")
+            strides.append((st, nst))
+        (ks, kns), (vs, vns) = strides[0], strides[-1]
         self._keep = (k_tq, v_tq, k_pages, v_pages, k_norms, v_norms)   # the pointers below stay valid
         # the C arguments of these operands, as plain integers (None: no V side)
         self._quant = (k_tq.Pi.data_ptr(), k_tq.boundaries.data_ptr(), k_tq.bit_width,
-                       *((v_tq.Pi.data_ptr(), v_tq.boundaries.data_ptr(), v_tq.bit_width) if self.has_v
-                         else (None, None, 0)))
-        self._store = (k_pages.data_ptr(), k_pages.stride(0), k_pages.stride(1),
-                       *((v_pages.data_ptr(), v_pages.stride(0), v_pages.stride(1)) if self.has_v
-                         else (None, 0, 0)),
-                       k_norms.data_ptr(), k_norms.stride(0), k_norms.stride(1),
-                       *((v_norms.data_ptr(), v_norms.stride(0), v_norms.stride(1)) if self.has_v
-                         else (None, 0, 0)))
+                       *((v_tq.Pi.data_ptr(), v_tq.boundaries.data_ptr(), v_tq.bit_width) if has_v else (None, None, 0)))
+        self._store = (k_pages.data_ptr(), ks[0], ks[1], *((v_pages.data_ptr(), vs[0], vs[1]) if has_v else (None, 0, 0)),
+                       k_norms.data_ptr(), kns[0], kns[1], *((v_norms.data_ptr(), vns[0], vns[1]) if has_v else (None, 0, 0)))
 
     def bind(self, k: torch.Tensor, v: torch.Tensor | None, page_table: torch.Tensor,
              start_pos: torch.Tensor) -> tuple:
@@ -232,54 +227,47 @@ class AppendPlan:
 
 
     def bind_rotation(self, q: torch.Tensor | None, cos: torch.Tensor, sin: torch.Tensor, bound: tuple) -> tuple:
-        """Check what ``launch_rotated`` takes beside ``bind``'s operands."""
-        B, n, D = bound[4], bound[5], self.D
+        """Check what ``launch_rotated`` takes beside ``bind``'s operands; returns its C arguments for q (but
+        for the rotated one) and for the tables."""
+        B, n, D, code = bound[4], bound[5], self.D, _lib.DTYPE_CODE
+        shape, ct, cs, ss = cos.shape, cos.dtype, cos.stride(), sin.stride()
         for name, t in (("cos", cos), ("sin", sin)):
-            if t.dim() != 3 or t.shape[0] not in (1, B) or t.shape[1] != n or t.dtype not in _lib.DTYPE_CODE \
-                    or not t.is_cuda or t.get_device() != self.dev_index:
+            if len(shape) != 3 or shape[0] not in (1, B) or shape[1] != n or ct not in code or not t.is_cuda or t.get_device() != self.dev_index:
                 raise pa.UnsupportedLayout(f"append: {name} must be ({B}, {n}, R) or (1, {n}, R) fp32/fp16/bf16 on {self.device}, "
                                            f"got {tuple(t.shape)} {t.dtype} on {t.device}")
-        R = cos.shape[2]
-        if sin.shape != cos.shape or sin.dtype != cos.dtype or not 2 <= R <= D or R % 2:
-            raise pa.UnsupportedLayout(f"append: cos {tuple(cos.shape)} {cos.dtype} and sin {tuple(sin.shape)} {sin.dtype} must be alike and "
+        R = shape[2]
+        if sin.shape != shape or sin.dtype != ct or not 2 <= R <= D or R % 2:
+            raise pa.UnsupportedLayout(f"append: cos {tuple(shape)} {ct} and sin {tuple(sin.shape)} {sin.dtype} must be alike and "
                                        f"rotate an even number of the {D} channels")
-        if cos.stride(2) != 1 or sin.stride(2) != 1:
+        if cs[2] != 1 or ss[2] != 1:
             raise pa.UnsupportedLayout("append: cos and sin need contiguous rows")
+        qargs = (None, 0, 0, 0, 0, 0)
         if q is not None:
             if not q.is_cuda or q.get_device() != self.dev_index:
                 raise pa.UnsupportedLayout("append: every operand must be on one HIP device")
-            if q.dim() != 4 or q.shape[0] != B or q.shape[1] < 1 or q.shape[2] != n or q.shape[3] != D or q.dtype not in _lib.DTYPE_CODE \
-                    or q.stride(3) != 1:
+            qshape, qs = q.shape, q.stride()
+            if len(qshape) != 4 or qshape[0] != B or qshape[1] < 1 or qshape[2] != n or qshape[3] != D or q.dtype not in code or qs[3] != 1:
                 raise pa.UnsupportedLayout(f"append: q must be ({B}, Hq, {n}, {D}) fp32/fp16/bf16 with a contiguous head_dim, got "
-                                           f"{tuple(q.shape)} {q.dtype}")
+                                           f"{tuple(qshape)} {q.dtype}")
             if q.numel() >= 8 * (2 ** 30 - 1):
                 raise pa.UnsupportedLayout("append: q of 2^33 elements or more")
-        return q, cos, sin, R
+            qargs = (q.data_ptr(), qs[0], qs[1], qs[2], code[q.dtype], qshape[1])
+        own = shape[0] != 1  # a table a sequence
+        return q, qargs, (cos.data_ptr(), cs[0] if own else 0, cs[1], sin.data_ptr(), ss[0] if own else 0, ss[1], code[ct], R), (cos, sin)
 
     def launch_rotated(self, bound: tuple, rotation: tuple, timing_events=None) -> torch.Tensor | None:
         """``launch`` with K rotated on the way (``wn_append_rotated_kv``); returns the rotated q."""
         k, v, page_table, start_pos, B, n = bound
-        q, cos, sin, R = rotation
-        out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        q, qargs, tables, _ = rotation
+        out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=self.device)
         if B == 0 or n == 0:
             return out
-        ks = k.stride()
-        if v is not None:
-            vs = v.stride()
-            vargs = (v.data_ptr(), vs[0], vs[1], vs[2])
-        else:
-            vargs = (None, 0, 0, 0)
-        if q is not None:
-            qs = q.stride()
-            qargs = (q.data_ptr(), qs[0], qs[1], qs[2], _lib.DTYPE_CODE[q.dtype], q.shape[1], out.data_ptr())
-        else:
-            qargs = (None, 0, 0, 0, 0, 0, None)
-        cs, ss, shared = cos.stride(), sin.stride(), cos.shape[0] == 1
+        ks, vs = k.stride(), (0, 0, 0) if v is None else v.stride()
         ev0, ev1 = timing_events or (None, None)
         with _lib.on(self.device):
-            _lib.call("wn_append_rotated_kv", *qargs, cos.data_ptr(), 0 if shared else cs[0], cs[1], sin.data_ptr(), 0 if shared else ss[0], ss[1],
-                      _lib.DTYPE_CODE[cos.dtype], R, k.data_ptr(), ks[0], ks[1], ks[2], *vargs, _lib.DTYPE_CODE[k.dtype], *self._quant,
-                      page_table.data_ptr(), page_table.stride(0), start_pos.data_ptr(), *self._store,
+            _lib.call("wn_append_rotated_kv", *qargs, None if out is None else out.data_ptr(), *tables,
+                      k.data_ptr(), ks[0], ks[1], ks[2], None if v is None else v.data_ptr(), vs[0], vs[1], vs[2], _lib.DTYPE_CODE[k.dtype],
+                      *self._quant, page_table.data_ptr(), page_table.stride(0), start_pos.data_ptr(), *self._store,
                       B, self.Hkv, n, self.D, self.S, self.P, page_table.shape[1], _lib.stream_of(self.device), ev0, ev1)
         return out
 
@@ -361,7 +349,10 @@ def append_rotated_kv(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor |
 
     Raises as ``append_kv``, and for tables that do not fit; a gradient, a tangent or a trace is
     refused."""
-    pa.values_only("append_rotated_kv", *(t for t in (q, k, v, cos, sin) if t is not None))
+    if q is None or v is None:
+        pa.values_only("append_rotated_kv", *(t for t in (q, k, v, cos, sin) if t is not None))
+    else:
+        pa.values_only("append_rotated_kv", q, k, v, cos, sin)
     if v is not None and (v_pages is None or v_norms is None):
         raise pa.UnsupportedLayout("append: V needs its pages and norms")
     has_v = v is not None
