@@ -241,3 +241,17 @@ def test_window_c_abi():
                 (1, 4, 2, 2, 128, 16, 4, 8, 0, 8, 0), (1, 4, 2, 1, 64, 16, 4, 8, 0, 8, 0), (1, 4, 2, 1, 128, 24, 4, 8, 0, 8, 0)):
         assert size(*bad) == -1
     assert size(1, 4, 2, 1, 128, 16, 4, 8, 0, 8, 0) > 0 and size(1, 4, 2, 1, 64, 16, 4, 8, 0, 1, 64) > 0
+
+
+@pytest.mark.parametrize("call", [lambda x: adjust_logits(x.reshape(-1, 64)), lambda x: _append(q=x), lambda x: _window(q=x[:, :, :1].expand(2, 4, 5, 64))],
+                         ids=["logits", "append", "window"])
+def test_tangents_and_traces(as_hip, call):
+    """A forward-mode derivative and a place in a trace are refused, on tensors that pass else."""
+    import torch.autograd.forward_ad as fwd
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x = torch.randn(2, 4, 3, 64)
+    with fwd.dual_level():
+        with pytest.raises(pa.UnsupportedLayout, match="forward-mode"):
+            call(fwd.make_dual(x, torch.ones_like(x)))
+    with pytest.raises(pa.UnsupportedLayout, match="traced"):
+        make_fx(lambda t: call(t))(x)

@@ -152,3 +152,10 @@ def test_refusals():
         with pytest.raises(Refused) as err:
             e.submit(Request("r", [1], 3, **kw))
         assert err.value.reason == why
+
+
+def test_sinks_without_a_window():
+    pool = PagePool(num_layers=1, num_pages=4, num_kv_heads=1, page_size=16, nb_k=64, nb_v=64)
+    with pytest.raises(ValueError, match="window"):
+        Engine(_Model(), pool, None, None, 128, config=EngineConfig(sinks=4))
+    assert Request("r", [1], 2, logit_bias=None).logit_bias == {}

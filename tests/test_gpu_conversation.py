@@ -150,6 +150,21 @@ def test_the_rotation_in_the_append(model, monkeypatch):
     assert len(calls) == n and cache.lengths == [4]
 
 
+def test_a_copy_of_a_fused_model_has_its_own_weights(model):
+    import copy
+    from winnow_amd import packed_backend as pb
+    pb.fuse_rotary(model)
+    other = copy.deepcopy(model)
+    with torch.no_grad():
+        for m in other.modules():
+            if isinstance(m, torch.nn.Linear) and m.weight.shape[0] == 512 and m.bias is not None:
+                m.weight.mul_(0.5)
+    _, a, _ = _generate(model, _prompts(1), 2)
+    _, b, _ = _generate(other, _prompts(1), 2)
+    _, again, _ = _generate(model, _prompts(1), 2)
+    assert torch.equal(a, again) and not torch.equal(a, b)
+
+
 def test_fuse_rotary_refuses_other_models(model):
     from winnow_amd import packed_backend as pb
     model.config.architectures = ["OtherForCausalLM"]
@@ -236,5 +251,8 @@ def test_caches_that_are_refused(model):
                      (dict(window=4, tree=[-1, 0]), ValueError)):
         with pytest.raises(err):
             pb.PagedPackedCache(pool, ["a"], [0], **kw, **bad)
+    for backend in ("reconstruct_sdpa", "hip_dense", "nonsense"):
+        with pytest.raises(ValueError, match="no window"):
+            _generate(model, _prompts(1), 2, window=8, decode_backend=backend)
     with pytest.raises(ValueError, match="no window"):
-        _generate(model, _prompts(1), 2, window=8, decode_backend="reconstruct_sdpa")
+        _generate(model, _prompts(1), 2, window=8, dense=True, decode_backend="hip_dense")

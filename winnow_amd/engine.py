@@ -105,6 +105,9 @@ class Request:
     # words of one (logits.pack_allowed), or None for all
     allowed_tokens: object = None
 
+    def __post_init__(self):
+        self.logit_bias = {} if self.logit_bias is None else self.logit_bias
+
     @property
     def penalized(self) -> bool:
         return self.repetition_penalty != 1 or self.presence_penalty != 0 or self.frequency_penalty != 0
@@ -160,6 +163,8 @@ class Engine:
         self.kq, self.vq, self.head_dim = k_quant, v_quant, head_dim
         self.eos = frozenset(int(t) for t in eos_ids)
         self.cfg = config or EngineConfig()
+        if self.cfg.window is None and self.cfg.sinks:
+            raise ValueError("sinks stay in view beside a window: give one")
         self.clock = clock
         self.device = next(model.parameters()).device
         self.closed = False
@@ -303,7 +308,7 @@ class Engine:
         cache = PagedPackedCache(self.pool, [r.request_id for r in reqs], [r.stored for r in reqs],
                                  k_quant=self.kq, v_quant=self.vq, head_dim=self.head_dim,
                                  decode_backend=self.cfg.decode_backend, allow_tf32=self.cfg.allow_tf32,
-                                 window=self.cfg.window, sinks=self.cfg.sinks if self.cfg.window is not None else 0)
+                                 window=self.cfg.window, sinks=self.cfg.sinks)
         out = self.model(input_ids=ids, position_ids=positions, past_key_values=cache, use_cache=True,
                          logits_to_keep=1)
         for r, stored in zip(reqs, cache.lengths):

@@ -572,6 +572,45 @@ def _check_scan(what: str, q: torch.Tensor, kv: PackedKV) -> None:
         raise UnsupportedLayout("the pool has no pages")
 
 
+def _scan_arguments(q: torch.Tensor, kv: PackedKV):
+    """((the C ABI's arguments of q, from its strides to the lengths, for the tile scans), whether the decode's
+    row scans read the layout too), for operands that ``check_contract`` (but for the ranges) and
+    ``_check_scan`` accept; None for others, and each of the two says what is wrong. Every attribute is
+    asked for once: the two checks one after the other take twice the host time."""
+    kq, vq, k, v, kn, vn, table, lens = kv.k_quant, kv.v_quant, kv.k_pages, kv.v_pages, kv.k_norms, kv.v_norms, kv.page_table, kv.seq_lens
+    pk, pv, ck, cv = kq.Pi, vq.Pi, kq.centroids, vq.centroids
+    shape, lead, dev = q.shape, k.shape, q.device
+    if len(shape) != 4 or len(lead) != 4 or len(v.shape) != 4 or not _lib.is_hip(q):
+        return None
+    B, Hq, _, D = shape
+    P, Hkv, S, nbk = lead
+    bk, bv, nbv, three = kq.bit_width, vq.bit_width, v.shape[-1], lead[:3]
+    if D != kv.head_dim or D not in SUPPORTED_HEAD_DIMS or q.dtype not in _lib.DTYPE_CODE or Hkv < 1 or Hq % Hkv or S < 16 or S & (S - 1) or P < 1 \
+            or 8 * nbk != D * bk or 8 * nbv != D * bv or v.shape[:3] != three or kn.shape != three or vn.shape != three:
+        return None
+    if pk.shape != (D, D) or pv.shape != (D, D) or ck.numel() != 1 << bk or cv.numel() != 1 << bv or lens.shape != (B,) or len(table.shape) != 2 \
+            or table.shape[0] != B or not 1 <= table.shape[1] <= (2 ** 31 - 257) // S:
+        return None
+    if not (k.dtype is v.dtype is torch.uint8 and kn.dtype is vn.dtype is torch.float16 and table.dtype is lens.dtype is torch.int32
+            and pk.dtype is pv.dtype is ck.dtype is cv.dtype is torch.float32):
+        return None
+    if k.device != dev or v.device != dev or kn.device != dev or vn.device != dev or table.device != dev or lens.device != dev or pk.device != dev \
+            or pv.device != dev or ck.device != dev or cv.device != dev:
+        return None
+    qs, ks, vs, kns, vns, ts = q.stride(), k.stride(), v.stride(), kn.stride(), vn.stride(), table.stride()
+    ka, va, pa = k.data_ptr(), v.data_ptr(), pk.data_ptr()
+    if qs[3] != 1 or ks[3] != 1 or vs[3] != 1 or ks[2] != nbk or vs[2] != nbv or kns[2] != 1 or vns[2] != 1 or ts[1] != 1 \
+            or (ka | ks[0] | ks[1] | va | vs[0] | vs[1]) & 3 or (pa | pv.data_ptr()) & 15 \
+            or not (pk.is_contiguous() and pv.is_contiguous() and ck.is_contiguous() and cv.is_contiguous() and lens.is_contiguous()):
+        return None
+    rows = not ((ka | ks[0] | ks[1]) & (15 if nbk % 16 == 0 else 7) or (va | vs[0] | vs[1]) & 7) and 0 <= ks[0] < 2 ** 32 and 0 <= vs[0] < 2 ** 32 \
+        and ks[1] >= S * nbk and vs[1] >= S * nbv and 0 <= kns[0] < 2 ** 31 and 0 <= vns[0] < 2 ** 31 and kns[1] >= 0 and vns[1] >= 0 \
+        and Hkv * kns[1] + S <= 2 ** 31 and Hkv * vns[1] + S <= 2 ** 31
+    return (q.data_ptr(), _lib.DTYPE_CODE[q.dtype], qs[0], qs[1], qs[2], pa, pv.data_ptr(), ck.data_ptr(), cv.data_ptr(),
+            ka, ks[0], ks[1], va, vs[0], vs[1], kn.data_ptr(), kns[0], kns[1], vn.data_ptr(), vns[0], vns[1],
+            table.data_ptr(), ts[0], lens.data_ptr()), rows
+
+
 def check_tree(q: torch.Tensor, kv: PackedKV, parents: torch.Tensor) -> None:
     """What ``packed_tree_attention`` needs beyond ``check_contract``."""
     B, _, T, _ = q.shape
@@ -751,20 +790,8 @@ def window_workspace_bytes(batch: int, num_q_heads: int, num_kv_heads: int, q_le
                                                     num_splits, span))
 
 
-def _decode_rows(kv: PackedKV) -> bool:
-    """Whether pages and norms meet the alignments and limits of the decode's row scans."""
-    for pages in (kv.k_pages, kv.v_pages):
-        st, align = pages.stride(), 16 if pages.shape[3] % 16 == 0 and pages is kv.k_pages else 8
-        if pages.data_ptr() % align or st[0] % align or st[1] % align or not 0 <= st[0] < 2 ** 32 or st[1] < pages.shape[2] * pages.shape[3]:
-            return False
-    for norms in (kv.k_norms, kv.v_norms):
-        st = norms.stride()
-        if not (0 <= st[0] < 2 ** 31 and 0 <= st[1] and norms.shape[1] * st[1] + norms.shape[2] <= 2 ** 31):
-            return False
-    return True
-
-
-def window_plan_for(q: torch.Tensor, kv: PackedKV, window: int, sinks: int, exact: bool, *, read_lens: bool = True) -> tuple[int, int]:
+def window_plan_for(q: torch.Tensor, kv: PackedKV, window: int, sinks: int, exact: bool, *, read_lens: bool = True,
+                    wide: bool | None = None) -> tuple[int, int]:
     """(num_splits, span) of the windowed attention for this query and handle (wn_window_plan), from the
     lengths' host mirror, or, without one, a host copy (``read_lens``) or the width of the table."""
     B, Hq, Q, D = q.shape
@@ -773,10 +800,13 @@ def window_plan_for(q: torch.Tensor, kv: PackedKV, window: int, sinks: int, exac
         lens = kv.seq_lens.cpu()
     if lens is not None and (lens.dtype != torch.int32 or lens.shape != (B,) or not lens.is_contiguous()):
         lens = lens.to(torch.int32).reshape(B).contiguous()
+    if wide is None:
+        made = _scan_arguments(q, kv)
+        wide = made is not None and made[1]
     plan = (ctypes.c_int * 2)()
     with _lib.on(q.device):
         _lib.call("wn_window_plan", B, Hq, kv.num_kv_heads, Q, D, kv.page_size, kv.k_quant.bit_width, kv.v_quant.bit_width, int(exact),
-                  _decode_rows(kv), kv.page_table.shape[1], window, sinks, _lib.ptr(lens), plan, ctypes.cast(ctypes.byref(plan, 4), ctypes.POINTER(ctypes.c_int)))
+                  wide, kv.page_table.shape[1], window, sinks, _lib.ptr(lens), plan, ctypes.cast(ctypes.byref(plan, 4), ctypes.POINTER(ctypes.c_int)))
     return plan[0], plan[1]
 
 
@@ -821,9 +851,14 @@ def packed_window_attention(q: torch.Tensor, kv: PackedKV, scale: float, *, wind
     Raises ``UnsupportedLayout`` before any launch for what ``check_contract`` rejects, for layouts
     that the scan does not read, for a gradient, a tangent or a trace; ``check_ranges`` covers lengths
     and the ids of pages in view, read from the handle's host mirrors when given, else copied to the host."""
-    check_contract(q, kv, check_ranges=False)
     window, sinks = check_window(window, sinks)
-    _check_scan("windowed attention", q, kv)
+    operands = _scan_arguments(q, kv)
+    if operands is None:
+        check_contract(q, kv, check_ranges=False)
+        _check_scan("windowed attention", q, kv)
+        raise UnsupportedLayout("windowed attention: unsupported layout")
+    values_only("windowed attention", q)
+    operands, wide = operands
     B, Hq, Q, D = q.shape
     P, Hkv, S, _ = kv.k_pages.shape
     if Q < 1 or Hq // Hkv * Q > MAX_WINDOW_ROWS:
@@ -833,7 +868,7 @@ def packed_window_attention(q: torch.Tensor, kv: PackedKV, scale: float, *, wind
         raise UnsupportedLayout(f"output dtype {out_dtype} is not supported")
     exact, kq, vq, table = not allow_tf32, kv.k_quant, kv.v_quant, kv.page_table
     sizes = (B, Hq, Hkv, Q, D, S, kq.bit_width, vq.bit_width)
-    made = _window_prepare(kv, sizes, exact, Q == 1 and _decode_rows(kv), window, sinks, q.device) if check_ranges and B else None
+    made = _window_prepare(kv, sizes, exact, wide, window, sinks, q.device) if check_ranges and B else None
     if check_ranges and made is None:
         check_window_ranges(kv.seq_lens if kv.seq_lens_host is None else kv.seq_lens_host,
                             table if kv.page_table_host is None else kv.page_table_host, P, S, Q, window, sinks)
@@ -845,7 +880,7 @@ def packed_window_attention(q: torch.Tensor, kv: PackedKV, scale: float, *, wind
     elif num_splits:
         ns, span = int(num_splits), 64
     else:
-        ns, span = made or window_plan_for(q, kv, window, sinks, exact, read_lens=check_ranges)
+        ns, span = made or window_plan_for(q, kv, window, sinks, exact, read_lens=check_ranges, wide=wide)
     need = window_workspace_bytes(B, Hq, Hkv, Q, D, S, table.shape[1], window, sinks, ns, span)
     if need < 0:
         raise UnsupportedLayout(f"bad window sizes B={B} Hq={Hq} Hkv={Hkv} Q={Q} splits={ns}")
@@ -857,16 +892,9 @@ def packed_window_attention(q: torch.Tensor, kv: PackedKV, scale: float, *, wind
         if room < need or workspace.device != q.device or not workspace.is_contiguous():
             raise UnsupportedLayout(f"workspace needs {need} contiguous bytes on {q.device}")
     ev0, ev1 = timing_events or (None, None)
-    kp, vp, kn, vn = kv.k_pages.stride(), kv.v_pages.stride(), kv.k_norms.stride(), kv.v_norms.stride()
     with _lib.on(q.device):
-        _lib.call("wn_window_attention", q.data_ptr(), _lib.DTYPE_CODE[q.dtype], *q.stride()[:3],
-                  kq.Pi.data_ptr(), vq.Pi.data_ptr(), kq.centroids.data_ptr(), vq.centroids.data_ptr(),
-                  kv.k_pages.data_ptr(), kp[0], kp[1], kv.v_pages.data_ptr(), vp[0], vp[1],
-                  kv.k_norms.data_ptr(), kn[0], kn[1], kv.v_norms.data_ptr(), vn[0], vn[1],
-                  table.data_ptr(), table.stride(0), kv.seq_lens.data_ptr(),
-                  out.data_ptr(), _lib.DTYPE_CODE[out_dtype], workspace.data_ptr(), room,
-                  *sizes, P, table.shape[1], window, sinks, float(scale), int(exact), ns, span,
-                  _lib.stream_of(q.device), ev0, ev1)
+        _lib.call("wn_window_attention", *operands, out.data_ptr(), _lib.DTYPE_CODE[out_dtype], workspace.data_ptr(), room,
+                  *sizes, P, table.shape[1], window, sinks, float(scale), exact, ns, span, _lib.stream_of(q.device), ev0, ev1)
     return out
 
 

@@ -984,11 +984,10 @@ def _route(query, kv) -> str:
     if getattr(kv, "tree", None) is not None:
         return "tree_dense_sdpa" if isinstance(kv, pa.DenseKV) else "tree_hip_packed"
     if getattr(kv, "window", None) is not None:
-        if isinstance(kv, pa.DenseKV):
-            return "window_dense_sdpa"
-        if getattr(kv, "decode_backend", "auto") == "reconstruct_sdpa":
-            raise ValueError("backend 'reconstruct_sdpa' attends to the whole history: no window")
-        return "window_hip_packed"
+        dense, requested = isinstance(kv, pa.DenseKV), getattr(kv, "decode_backend", "auto")
+        if requested not in (("auto", "dense_sdpa") if dense else ("auto", "triton_packed", "hip_packed")):
+            raise ValueError(f"backend {requested!r} attends to the whole history: no window")
+        return "window_dense_sdpa" if dense else "window_hip_packed"
     if query.shape[2] > 1:
         if isinstance(kv, pa.DenseKV):
             return "prefill_dense_sdpa"
@@ -1013,26 +1012,32 @@ def winnow_packed_attention(module, query, key, value, attention_mask, dropout: 
     return _ROUTES[route](query, key, scale).transpose(1, 2).contiguous(), None
 
 
-def _rotated_forward(attn):
-    """A Qwen2 attention module's forward whose rotation the cache's append applies: one launch writes
-    K and V and rotates q, in place of the rotation's elementary operations and an append. Calls that it
-    does not serve (no paged packed cache, another attention implementation, gradients, traces,
-    autocast to another type) go through the module's own forward."""
-    own = attn.forward
+_ROTATED: dict[type, type] = {}
 
-    def forward(hidden_states, position_embeddings=None, attention_mask=None, past_key_values=None, **kwargs):
+
+def _rotated_class(base: type) -> type:
+    """The class of a Qwen2 attention module whose rotation the cache's append applies: one launch writes K and
+    V and rotates q, in place of the rotation's elementary operations and an append. Calls that it does
+    not serve (no paged packed cache, another attention implementation, gradients, traces, autocast to
+    another type) go through the base's forward. A class, and no function set on the module: a copy
+    of the model then runs with its own weights."""
+    if base in _ROTATED:
+        return _ROTATED[base]
+
+    def forward(self, hidden_states, position_embeddings=None, attention_mask=None, past_key_values=None, **kwargs):
         cache = past_key_values
         if not isinstance(cache, PagedPackedCache) or cache.pool.dense or position_embeddings is None \
-                or attn.config._attn_implementation != ATTN_NAME or torch.is_grad_enabled() or not _plain(hidden_states):
-            return own(hidden_states=hidden_states, position_embeddings=position_embeddings, attention_mask=attention_mask,
-                       past_key_values=past_key_values, **kwargs)
+                or self.config._attn_implementation != ATTN_NAME or torch.is_grad_enabled() or not _plain(hidden_states):
+            return base.forward(self, hidden_states=hidden_states, position_embeddings=position_embeddings, attention_mask=attention_mask,
+                                past_key_values=past_key_values, **kwargs)
         shape = hidden_states.shape[:-1]
-        q, k, v = (proj(hidden_states).view(*shape, -1, attn.head_dim).transpose(1, 2) for proj in (attn.q_proj, attn.k_proj, attn.v_proj))
-        q, handle = cache.update_rotated(q, k, v, *position_embeddings, attn.layer_idx)
-        out, weights = winnow_packed_attention(attn, q, handle, handle, attention_mask, scaling=attn.scaling)
-        return attn.o_proj(out.reshape(*shape, -1)), weights
-    forward.own = own
-    return forward
+        q, k, v = (proj(hidden_states).view(*shape, -1, self.head_dim).transpose(1, 2) for proj in (self.q_proj, self.k_proj, self.v_proj))
+        q, handle = cache.update_rotated(q, k, v, *position_embeddings, self.layer_idx)
+        out, weights = winnow_packed_attention(self, q, handle, handle, attention_mask, scaling=self.scaling)
+        return self.o_proj(out.reshape(*shape, -1)), weights
+
+    _ROTATED[base] = type("Rotated" + base.__name__, (base,), {"forward": forward, "__module__": __name__})
+    return _ROTATED[base]
 
 
 def fuse_rotary(model) -> int:
@@ -1042,11 +1047,12 @@ def fuse_rotary(model) -> int:
     ``UnsupportedModel`` for an architecture that this path does not serve."""
     if _arch(model.config) not in SUPPORTED_ARCH:
         raise UnsupportedModel(f"{_arch(model.config)} is not a supported architecture {SUPPORTED_ARCH}")
-    layers = [m for m in model.modules() if type(m).__name__ == "Qwen2Attention"]
-    for attn in layers:
-        if not hasattr(attn.forward, "own"):
-            attn.forward = _rotated_forward(attn)
-    return len(layers)
+    count = 0
+    for m in model.modules():
+        if type(m).__name__ == "Qwen2Attention":
+            m.__class__ = _rotated_class(type(m))
+        count += type(m) in _ROTATED.values()
+    return count
 
 
 def register() -> None:
