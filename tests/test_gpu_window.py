@@ -284,3 +284,15 @@ def test_a_long_prompt_chunk():
     for window, sinks in ((64, 4), (500, 0), (900, 33)):
         _check(_run(q, kv, 0.09, window, sinks), q, kv, 0.09, window, sinks, torch.float32)
         _check(_run(q, kv, 0.09, window, sinks, allow_tf32=True), q, kv, 0.09, window, sinks, torch.float32, single=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("D,Hq,Hkv,Q,splits", [(128, 32, 8, 70, None), (64, 6, 2, 500, 3), (32, 10, 2, 171, None), (16, 8, 8, 99, 17),
+                                               (256, 8, 4, 133, 2)])
+def test_window_many_rows(D, Hq, Hkv, Q, splits, dtype):
+    """Rows whose merge has more tiles of sixteen than the device's work-groups that stay, or fewer;
+    sequences of nothing and of fewer positions than queries between long ones."""
+    lens = (Q + 40, 0, 300 + Q, Q // 3, Q, 90 + Q, 1, 2 * Q, Q + 7, Q + 129, Q, 64 + Q) * (3 if D == 128 else 1)
+    q, kv = _case(60 + D, lens, Hq, Hkv, D, Q, 4, 4, dtype=dtype)
+    for window, sinks in ((100, 4), (33, 0)):
+        _check(_run(q, kv, D ** -0.5, window, sinks, num_splits=splits), q, kv, D ** -0.5, window, sinks, dtype)

@@ -237,7 +237,11 @@ struct WindowArgs : TreeArgs {
 
 struct WindowMergeArgs : TreeMergeArgs {
   int window, sinks, rows_block, chunk;  // rows of a scan's work-group, tokens of its chunk
+  int tiles;  // of sixteen rows of a unit, over all of them
 };
+
+// Of window_merge_kernel: a wave per 16 columns, four at least.
+__host__ __device__ constexpr int window_merge_threads(int D) { return 4 * D > 256 ? 4 * D : 256; }
 
 // The chunks that the queries of rows r0 .. r0 + rows - 1 of a (sequence, kv head) look at: those that
 // hold sinks, then those from the first query's window to the last query. `total` of them, counted as

@@ -951,7 +951,7 @@ TreeKernelSet<WIN> tree_kernels() {
   }
   k.rotate = tree_rotate_kernel<D, WIN>;
   k.merge[0] = tree_merge_kernel<D, 4, WIN>;
-  k.merge[1] = tree_merge_kernel<D, 16, WIN>;
+  if constexpr (!WIN) k.merge[1] = tree_merge_kernel<D, 16, WIN>;
   k.rotate_threads = tree_rotate_threads(D);
   return k;
 }

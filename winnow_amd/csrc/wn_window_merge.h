@@ -1,0 +1,85 @@
+// Merge of the windowed attention's partials where there are many rows (prompt chunks): work-groups
+// that stay, each with its part of the rotation in registers, take tile after tile of sixteen rows, the
+// next tile's partials on their way while one is multiplied. A work-group per tile (tree_merge_kernel)
+// reads the 4 D^2 bytes of the rotation again for each. us in traces, head_dim 128, by tiles, a
+// work-group a tile and this: 512 10.2 and 8.5, 1,024 18.5 and 13.8, 4,000 64 and 40; head_dim 64 and
+// 4,000 47 and 17; head_dim 256 and 500 23.6 and 21.6. The bytes of 4,000 tiles (partials read, a bf16
+// result written) take 10 us at 4.8 TB/s; what is left is the tile's chain of load, barrier and products.
+#pragma once
+
+#include "wn_tree_kernels.h"
+
+namespace wn {
+namespace {
+
+// A lane takes EPT elements of one row, its splits one after the other.
+template <int D>
+__global__ __launch_bounds__(window_merge_threads(D)) void window_merge_kernel(WindowMergeArgs a) {
+  constexpr int XS = D + 4, EPT = 16 * D / window_merge_threads(D);
+  __shared__ __align__(16) float x[2][16 * XS];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, rows = a.n_rep * a.T, blocks = (rows + 15) / 16, Hq = a.Hkv * a.n_rep;
+  TreeProduct<D> pi;
+  if (wave < D / 16)
+    pi.load(wave, lane, [&](int j, int k) {
+      return f32x4{a.pi_v[k * D + j], a.pi_v[(k + 1) * D + j], a.pi_v[(k + 2) * D + j], a.pi_v[(k + 3) * D + j]};
+    });
+  const int rr = tid * EPT / D, d0 = tid * EPT % D;
+  float v[EPT];
+  float2 ml;
+  const auto fetch = [&](int64_t row) {
+    ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * row);
+    __builtin_memcpy(v, __builtin_assume_aligned(a.part_acc + row * D + d0, 4 * EPT), 4 * EPT);
+  };
+  // The row of a tile in its unit's first split (past the last row: that again).
+  const auto first = [&](int tile) {
+    return int64_t(tile / blocks) * a.nsplit * a.nrp + min(16 * (tile % blocks) + rr, rows - 1);
+  };
+  fetch(first(blockIdx.x));
+  for (int tile = blockIdx.x, buf = 0; tile < a.tiles; tile += gridDim.x, buf ^= 1) {
+    const int unit = tile / blocks, blk = tile % blocks, b = unit / a.Hkv;
+    const int L = min(max(a.seq_lens[b], 0), a.max_len);
+    const WindowSpan ws = window_span(L, a.T, a.n_rep, 16 * blk / a.rows_block * a.rows_block, a.rows_block, a.chunk, a.window, a.sinks,
+                                      a.nsplit, a.span);
+    const int live = ws.span ? (ws.total + ws.span - 1) / ws.span : 0;
+    float M = -INFINITY, den = 0.f, num[EPT] = {};
+    for (int s = 0; s < live; ++s) {
+      if (s) fetch(first(tile) + int64_t(s) * a.nrp);
+      if (ml.x == -INFINITY) continue;  // a split that saw no key
+      const float up = fmaxf(M, ml.x), old = __builtin_amdgcn_exp2f(M - up), w = __builtin_amdgcn_exp2f(ml.x - up);
+      den = den * old + w * ml.y;
+#pragma unroll
+      for (int e = 0; e < EPT; ++e) num[e] = num[e] * old + w * v[e];
+      M = up;
+    }
+    const float inv = den != 0.f ? 1.f / den : 0.f;
+#pragma unroll
+    for (int e = 0; e < EPT; ++e) x[buf][rr * XS + d0 + e] = num[e] * inv;
+    __syncthreads();  // x[buf]; its last readers are a barrier behind
+    if (tile + int(gridDim.x) < a.tiles) fetch(first(tile + gridDim.x));
+    const int g = lane >> 4, c = lane & 15, row = 16 * blk + c;
+    if (wave < D / 16) {
+      const f32x4 y = pi.run(x[buf] + c * XS, lane);
+      if (row < rows) {
+        const int64_t o = ((int64_t(b) * Hq + unit % a.Hkv * a.n_rep + row % a.n_rep) * a.T + row / a.n_rep) * D + 16 * wave + 4 * g;
+        if (a.out_dtype == WN_F32) {
+          __builtin_memcpy(static_cast<float*>(a.out) + o, &y, 16);
+        } else {
+          uint16_t h[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) h[i] = a.out_dtype == WN_BF16 ? f32_to_bf16(y[i]) : f32_to_f16(y[i]);
+          __builtin_memcpy(static_cast<uint16_t*>(a.out) + o, h, 8);
+        }
+      }
+    }
+  }
+}
+
+template <int D>
+WindowKernels window_kernels_for(bool exact, int bw_k, int bw_v) {
+  WindowKernels k = tree_kernels_for<D, true>(exact, bw_k, bw_v);
+  k.merge[1] = window_merge_kernel<D>;
+  return k;
+}
+
+}  // namespace
+}  // namespace wn
