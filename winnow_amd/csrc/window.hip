@@ -255,7 +255,9 @@ extern "C" int wn_window_attention(
   ma.tiles = int(wide);
   const int threads = window_merge_threads(D);
   const int64_t stay = int64_t(std::max(1, device_cus())) * (1024 / threads);  // 1,024 threads a compute unit
-  if (wide >= kMergeTiles) hipLaunchKernelGGL(k.merge[1], dim3(unsigned(std::min(wide, stay))), dim3(threads), 0, st, ma);
+  // few splits, or many rows: wn_window_merge.h has both sides
+  if (num_splits <= 8 || wide >= 128)
+    hipLaunchKernelGGL(k.merge[1], dim3(unsigned(std::min(wide, stay))), dim3(threads), 0, st, ma);
   else hipLaunchKernelGGL(k.merge[0], dim3(unsigned(int64_t(B) * Hkv * ((rows + 3) / 4))), dim3(1024), 0, st, ma);
   return check_launch("wn_window_attention");
 }

@@ -1,10 +1,16 @@
-// Merge of the windowed attention's partials where there are many rows (prompt chunks): work-groups
-// that stay, each with its part of the rotation in registers, take tile after tile of sixteen rows, the
-// next tile's partials on their way while one is multiplied. A work-group per tile (tree_merge_kernel)
-// reads the 4 D^2 bytes of the rotation again for each. us in traces, head_dim 128, by tiles, a
-// work-group a tile and this: 512 10.2 and 8.5, 1,024 18.5 and 13.8, 4,000 64 and 40; head_dim 64 and
-// 4,000 47 and 17; head_dim 256 and 500 23.6 and 21.6. The bytes of 4,000 tiles (partials read, a bf16
-// result written) take 10 us at 4.8 TB/s; what is left is the tile's chain of load, barrier and products.
+// Merge of the windowed attention's partials by work-groups that stay: each keeps its part of the
+// rotation in registers and takes tile after tile of sixteen rows, the next tile's partials on their way
+// while one is multiplied. tree_merge_kernel<D, 4> reads the 4 D^2 bytes of the rotation once for every four rows, but
+// joins the splits of a row by a whole wave. us in traces, it and this, by head_dim, tiles and splits:
+//   128    8 tiles   2 splits  6.4   4.8     8 splits  6.1   5.3     32 splits  6.0   9.4
+//   128  128 tiles   2 splits 12.5   5.1     8 splits 12.6   6.1     32 splits 14.6  12.8
+//   128  384 tiles   2 splits 34     8.0     8 splits 34    10.4     32 splits 37    26
+//    64  128 tiles   2 splits  8.8   4.7     8 splits  8.2   4.0     32 splits  8.4   8.4
+//   256  128 tiles   2 splits 22    11       8 splits 24    14       32 splits 27    26
+// Against sixteen rows a work-group (tree_merge_kernel<D, 16>), head_dim 128, one or two splits: 512 tiles
+// 10.2 and 8.5, 1,024 18.5 and 13.8, 4,000 64 and 40; head_dim 64 and 4,000 47 and 17. The bytes of
+// 4,000 tiles (partials read, a bf16 result written) take 10 us at 4.8 TB/s; what is left is the tile's
+// chain of load, barrier and products.
 #pragma once
 
 #include "wn_tree_kernels.h"
@@ -16,6 +22,7 @@ namespace {
 template <int D>
 __global__ __launch_bounds__(window_merge_threads(D)) void window_merge_kernel(WindowMergeArgs a) {
   constexpr int XS = D + 4, EPT = 16 * D / window_merge_threads(D);
+  constexpr int U = D == 256 ? 1 : 8;  // splits loaded at once (at 256 the rotation takes half of the 128 registers)
   __shared__ __align__(16) float x[2][16 * XS];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, rows = a.n_rep * a.T, blocks = (rows + 15) / 16, Hq = a.Hkv * a.n_rep;
   TreeProduct<D> pi;
@@ -24,17 +31,20 @@ __global__ __launch_bounds__(window_merge_threads(D)) void window_merge_kernel(W
       return f32x4{a.pi_v[k * D + j], a.pi_v[(k + 1) * D + j], a.pi_v[(k + 2) * D + j], a.pi_v[(k + 3) * D + j]};
     });
   const int rr = tid * EPT / D, d0 = tid * EPT % D;
-  float v[EPT];
-  float2 ml;
-  const auto fetch = [&](int64_t row) {
-    ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * row);
-    __builtin_memcpy(v, __builtin_assume_aligned(a.part_acc + row * D + d0, 4 * EPT), 4 * EPT);
+  float v[U][EPT];
+  float2 ml[U];
+  // A tile's row (past the last row: that again) in U splits from s.
+  const auto fetch = [&](int tile, int s) {
+    const int64_t row = (int64_t(tile / blocks) * a.nsplit + s) * a.nrp + min(16 * (tile % blocks) + rr, rows - 1);
+    const float* acc = a.part_acc + row * D + d0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (s + u >= a.nsplit) break;
+      ml[u] = *reinterpret_cast<const float2*>(a.part_ml + 2 * (row + int64_t(u) * a.nrp));
+      __builtin_memcpy(v[u], __builtin_assume_aligned(acc + int64_t(u) * a.nrp * D, 4 * EPT), 4 * EPT);
+    }
   };
-  // The row of a tile in its unit's first split (past the last row: that again).
-  const auto first = [&](int tile) {
-    return int64_t(tile / blocks) * a.nsplit * a.nrp + min(16 * (tile % blocks) + rr, rows - 1);
-  };
-  fetch(first(blockIdx.x));
+  fetch(blockIdx.x, 0);
   for (int tile = blockIdx.x, buf = 0; tile < a.tiles; tile += gridDim.x, buf ^= 1) {
     const int unit = tile / blocks, blk = tile % blocks, b = unit / a.Hkv;
     const int L = min(max(a.seq_lens[b], 0), a.max_len);
@@ -42,20 +52,24 @@ __global__ __launch_bounds__(window_merge_threads(D)) void window_merge_kernel(W
                                       a.nsplit, a.span);
     const int live = ws.span ? (ws.total + ws.span - 1) / ws.span : 0;
     float M = -INFINITY, den = 0.f, num[EPT] = {};
-    for (int s = 0; s < live; ++s) {
-      if (s) fetch(first(tile) + int64_t(s) * a.nrp);
-      if (ml.x == -INFINITY) continue;  // a split that saw no key
-      const float up = fmaxf(M, ml.x), old = __builtin_amdgcn_exp2f(M - up), w = __builtin_amdgcn_exp2f(ml.x - up);
-      den = den * old + w * ml.y;
+    for (int s = 0; s < live; s += U) {
+      if (s) fetch(tile, s);
 #pragma unroll
-      for (int e = 0; e < EPT; ++e) num[e] = num[e] * old + w * v[e];
-      M = up;
+      for (int u = 0; u < U; ++u) {
+        if (s + u >= live) break;
+        if (ml[u].x == -INFINITY) continue;  // a split that saw no key
+        const float up = fmaxf(M, ml[u].x), old = __builtin_amdgcn_exp2f(M - up), w = __builtin_amdgcn_exp2f(ml[u].x - up);
+        den = den * old + w * ml[u].y;
+#pragma unroll
+        for (int e = 0; e < EPT; ++e) num[e] = num[e] * old + w * v[u][e];
+        M = up;
+      }
     }
     const float inv = den != 0.f ? 1.f / den : 0.f;
 #pragma unroll
     for (int e = 0; e < EPT; ++e) x[buf][rr * XS + d0 + e] = num[e] * inv;
     __syncthreads();  // x[buf]; its last readers are a barrier behind
-    if (tile + int(gridDim.x) < a.tiles) fetch(first(tile + gridDim.x));
+    if (tile + int(gridDim.x) < a.tiles) fetch(tile + gridDim.x, 0);
     const int g = lane >> 4, c = lane & 15, row = 16 * blk + c;
     if (wave < D / 16) {
       const f32x4 y = pi.run(x[buf] + c * XS, lane);
