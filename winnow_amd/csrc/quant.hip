@@ -4,8 +4,8 @@
 // quantize (turboquant_kv/cache.py:108-115):
 //   n = max(||x||_2, 1e-10);  y = (x / n) Pi^T;  code = #{boundaries < y}
 // A work-group quantizes sixteen vectors (quantize_kernel on the float64 matrix
-// cores at head_dim 64 and 128, quantize_any_kernel on the vector ALU at 16, 32 and
-// 256); many vectors at 64 and 128 run on quant_tile.hip, with the same codes. The squared norm and the rotation are
+// cores at head_dim 64 and 128, with K's rotation at 256 too; quantize_any_kernel on the vector ALU at
+// the others); many vectors at 64 and 128 run on quant_tile.hip, with the same codes. The squared norm and the rotation are
 // accumulated in float64 from exact fp32 inputs and rounded once to fp32, and
 // x / n is the correctly rounded fp32 quotient, so every code is the bucket of
 // the correctly rounded fp32 y; an fp32 GEMM elsewhere can differ from it only
@@ -36,7 +36,7 @@ __device__ __forceinline__ uint8_t packed_byte(const uint8_t* codes, int k, int 
 // A work-group quantizes sixteen vectors (sixteen per work-group keep even a
 // 4096-vector append spread over the whole GPU), in phases that each run over all
 // sixteen at once, so a small append costs a few round trips, not one per vector:
-//   loads     sixteen threads per vector for x (D/16 consecutive elements each),
+//   loads     sixteen threads per vector for x (D/16 consecutive elements each; thirty-two at head_dim 256),
 //             then the rows of Pi this wave's rotation needs (B operands, from L2 with
 //             16-byte loads: Pi is not staged in LDS); in scatter mode threads 0-15
 //             look up the start position, later the page, of vector tid.
@@ -59,11 +59,16 @@ __device__ __forceinline__ uint8_t packed_byte(const uint8_t* codes, int k, int 
 template <bool ROT>
 using AppendArgs = std::conditional_t<ROT, QuantRotArgs, QuantArgs>;
 
+// Threads of quantize_kernel: at head_dim 256 a wave keeps 32 rows of Pi, as at 128.
+constexpr int quantize_threads(int D) { return D > 128 ? 2 * kQBlock : kQBlock; }
+
 template <int D, bool ROT>
-__global__ __launch_bounds__(kQBlock) void quantize_kernel(AppendArgs<ROT> a) {
-  constexpr int EPT = D / 16;  // x elements per thread in the norm phase
-  constexpr int KS = D / 4;    // K-steps of the rotation (4 input dims each)
-  constexpr int TPW = D / 64;  // output tiles of sixteen dims per wave
+__global__ __launch_bounds__(quantize_threads(D)) void quantize_kernel(AppendArgs<ROT> a) {
+  constexpr int NT = quantize_threads(D), VT = NT / 16;  // threads per vector in the norm phase
+  constexpr int EPT = D / VT;   // x elements of each
+  constexpr int KS = D / 4;     // K-steps of the rotation (4 input dims each)
+  constexpr int OW = 64 * D / NT;  // output dims of a wave
+  constexpr int TPW = OW / 16;  // in tiles of sixteen
   constexpr int TPV = D / 8;   // threads per vector in the store phase
   typedef double f64x4 __attribute__((ext_vector_type(4)));
   __shared__ float bnd[255];
@@ -75,7 +80,7 @@ __global__ __launch_bounds__(kQBlock) void quantize_kernel(AppendArgs<ROT> a) {
 
   if constexpr (ROT) {
     if (blockIdx.y == gridDim.y - 1 && a.rot.q) {
-      rotate_queries<D, kQBlock>(a.rot, a.n, blockIdx.x, gridDim.x, threadIdx.x);
+      rotate_queries<D, NT>(a.rot, a.n, blockIdx.x, gridDim.x, threadIdx.x);
       return;
     }
   }
@@ -91,12 +96,12 @@ __global__ __launch_bounds__(kQBlock) void quantize_kernel(AppendArgs<ROT> a) {
   int dst_pos = 0;
   if (dst_thread && a.scatter)
     dst_pos = a.start_pos[int((v0 + tid) / (int64_t(a.n) * a.H))] + int((v0 + tid) % a.n);
-  for (int i = tid; i < nb; i += kQBlock) bnd[i] = sd.bnd[i];
+  for (int i = tid; i < nb; i += NT) bnd[i] = sd.bnd[i];
 
   float4 pb[TPW][KS / 4];  // B operands: rows of Pi (from L2, not staged in LDS)
-  // norms: vector tid / 16, elements EPT * (tid % 16) ..
+  // norms: vector tid / VT, elements EPT * (tid % VT) ..
   {
-    const int vl = tid >> 4, part = tid & 15;
+    const int vl = tid / VT, part = tid % VT;
     const int64_t v = v0 + vl;
     float xv[EPT];
     if (v < a.total) {
@@ -128,7 +133,7 @@ __global__ __launch_bounds__(kQBlock) void quantize_kernel(AppendArgs<ROT> a) {
     // order, so the norms wait only for x and Pi arrives during them
 #pragma unroll
     for (int j = 0; j < TPW; ++j) {
-      const float4* row = reinterpret_cast<const float4*>(sd.pi + int64_t(w * KS + 16 * j + (lane & 15)) * D +
+      const float4* row = reinterpret_cast<const float4*>(sd.pi + int64_t(w * OW + 16 * j + (lane & 15)) * D +
                                                           KS * (lane >> 4));
 #pragma unroll
       for (int q = 0; q < KS / 4; ++q) pb[j][q] = row[q];
@@ -137,7 +142,7 @@ __global__ __launch_bounds__(kQBlock) void quantize_kernel(AppendArgs<ROT> a) {
 #pragma unroll
     for (int k = 0; k < EPT; ++k) ss = fma(double(xv[k]), double(xv[k]), ss);
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 16);
+    for (int o = VT / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, VT);
     const float n = fmaxf(float(sqrt(ss)), 1e-10f);
 #pragma unroll
     for (int k = 0; k < EPT; ++k) xs[vl][EPT * part + k] = float(double(xv[k]) / double(n));
@@ -185,7 +190,7 @@ __global__ __launch_bounds__(kQBlock) void quantize_kernel(AppendArgs<ROT> a) {
 #pragma unroll
     for (int j = 0; j < TPW; ++j)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) cs[(lane >> 4) + 4 * i][w * KS + 16 * j + (lane & 15)] = uint8_t(code[4 * j + i]);
+      for (int i = 0; i < 4; ++i) cs[(lane >> 4) + 4 * i][w * OW + 16 * j + (lane & 15)] = uint8_t(code[4 * j + i]);
   }
   if (tid < kVecPerBlock) {
     // byte offset of the vector's packed row and element offset of its norm; -1: the
@@ -482,7 +487,12 @@ static int launch_quantize(AppendArgs<ROT>& a, int sides, int D, hipStream_t st,
     case 32: hipLaunchKernelGGL(HIP_KERNEL_NAME(quantize_any_kernel<32, ROT>), grid, dim3(kQBlock), 0, st, a); break;
     case 64: hipLaunchKernelGGL(HIP_KERNEL_NAME(quantize_kernel<64, ROT>), grid, dim3(kQBlock), 0, st, a); break;
     case 128: hipLaunchKernelGGL(HIP_KERNEL_NAME(quantize_kernel<128, ROT>), grid, dim3(kQBlock), 0, st, a); break;
-    case 256: hipLaunchKernelGGL(HIP_KERNEL_NAME(quantize_any_kernel<256, ROT>), grid, dim3(kQBlock), 0, st, a); break;
+    case 256:
+      // one token of two sequences, 8 heads, on the matrix cores 20 us and on the vector ALU 45; 2,000
+      // tokens 163 and 248 (without q and the rotation)
+      if constexpr (ROT) hipLaunchKernelGGL(HIP_KERNEL_NAME(quantize_kernel<256, true>), grid, dim3(quantize_threads(256)), 0, st, a);
+      else hipLaunchKernelGGL(HIP_KERNEL_NAME(quantize_any_kernel<256, false>), grid, dim3(kQBlock), 0, st, a);
+      break;
   }
   if (ev_end) (void)hipEventRecord(static_cast<hipEvent_t>(ev_end), st);
   return check_launch(what);
