@@ -45,7 +45,8 @@ __device__ __forceinline__ uint8_t packed_byte(const uint8_t* codes, int k, int 
 //   rotation  y = (x / n) Pi^T on the float64 matrix cores (v_mfma_f64_16x16x4f64:
 //             products of fp32 values are exact in float64 and the sums stay in
 //             float64), rows = the sixteen vectors, columns = output dims: wave w
-//             forms output dims [D/4 w, D/4 (w+1)), D/64 tiles of sixteen. K-step
+//             forms output dims [D/4 w, D/4 (w+1)), D/64 tiles of sixteen (eight waves at
+//             head_dim 256: D/8 dims each). K-step
 //             s, slot k (= lane / 16) is input dim (D/4) k + s, so a lane's A
 //             operands are D/4 consecutive floats of one xs row and its B operands
 //             D/4 consecutive floats of one row of Pi. Output lane l, register i of a

@@ -34,7 +34,16 @@ WindowKernels pick_window(int D, bool exact, int bw_k, int bw_v) {
 
 int window_chunk(int D) { return D == 256 ? 32 : 64; }  // tokens of a scan's chunk
 
-int window_variant(int64_t rows) { return rows <= 32 ? 0 : rows <= 64 ? 1 : 2; }
+// The tile scan for so many rows per kv head and (sequence, kv head) pairs. Blocks of 256 rows decode a
+// chunk for twice the rows of blocks of 128, in 1.7 times the time (7.6 and 4.5 us a chunk): where that
+// many fewer serve, and there are enough of them to go round. Calls of 32 heads over 8, 4 bits, us, 128 and
+// 256 rows: 2,048 rows at a window of 4,096 175 and 155, 8,000 rows 241 and 205, 192 rows of 8 sequences 162
+// and 140, of one 53 and 55; 384 rows 60 and 64; 512 68 and 66; 336 rows, 4 kv heads 49 and 57.
+int window_variant(int64_t rows, int64_t pairs) {
+  if (rows <= 64) return rows <= 32 ? 0 : 1;
+  const int64_t small = (rows + 127) / 128, large = (rows + 255) / 256;
+  return 17 * large <= 10 * small && pairs * small >= 32 ? 3 : 2;
+}
 
 bool window_shape(int B, int Hq, int Hkv, int Q, int D) {
   return B >= 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && Q > 0 && valid_head_dim(D) && int64_t(Hq / Hkv) * Q <= (1 << 20);
@@ -66,7 +75,7 @@ extern "C" int wn_window_plan(int B, int Hq, int Hkv, int Q, int D, int S, int b
       return WN_OK;
     }
   }
-  const auto scan = pick_window(D, exact != 0, bw_k, bw_v).scan[window_variant(rows)];
+  const auto scan = pick_window(D, exact != 0, bw_k, bw_v).scan[window_variant(rows, int64_t(B) * Hkv)];
   const int64_t slots = tree_slots(scan, tree_lds(scan, bw_k, bw_v));
   WN_REQUIRE(slots > 0, WN_E_LAUNCH, "wn_window_plan: cannot query the device occupancy");
   const int blocks = tree_nrp(scan, rows) / scan.rows;
@@ -110,7 +119,7 @@ extern "C" int64_t wn_window_workspace_bytes(int B, int Hq, int Hkv, int Q, int 
   if (!window_shape(B, Hq, Hkv, Q, D) || !is_pow2(S) || max_pages <= 0 || window <= 0 || sinks < 0 || num_splits <= 0 || span < 0) return -1;
   if (span == 0) return Q == 1 && D == 128 ? window_rows_workspace(B, Hq, Hkv, S, max_pages, window, sinks, num_splits) : -1;
   const int64_t rows = int64_t(Hq / Hkv) * Q;
-  const auto scan = pick_window(D, false, 8, 8).scan[window_variant(rows)];
+  const auto scan = pick_window(D, false, 8, 8).scan[window_variant(rows, int64_t(B) * Hkv)];
   return tree_layout(B, Hkv, tree_nrp(scan, rows), 0, D, num_splits).total;
 }
 
@@ -158,7 +167,7 @@ extern "C" int wn_window_attention(
   const int n_rep = Hq / Hkv;
   const int64_t rows = int64_t(n_rep) * Q;
   const WindowKernels k = pick_window(D, exact != 0, bw_k, bw_v);
-  const auto scan = k.scan[window_variant(rows)];
+  const auto scan = k.scan[window_variant(rows, int64_t(B) * Hkv)];
   const int nrp = tree_nrp(scan, rows), ncg = nrp / scan.rows;
   const TreeLayout lay = tree_layout(B, Hkv, nrp, 0, D, num_splits);
   WN_REQUIRE(workspace && workspace_bytes >= lay.total && aligned(workspace, 256), WN_E_WORKSPACE,

@@ -207,7 +207,7 @@ using TreeScan = TreeScanOf<TreeArgs>;
 
 template <class Args, class MergeArgs>
 struct TreeKernelsOf {
-  TreeScanOf<Args> scan[3];  // for up to 32, up to 64 and more rows per kv head
+  TreeScanOf<Args> scan[4];  // for up to 32, up to 64, more rows per kv head; the windowed attention's for many
   TreeRotFn rotate = nullptr;
   int rotate_threads = 0;
   void (*merge[2])(MergeArgs) = {};  // of four and of sixteen rows a work-group

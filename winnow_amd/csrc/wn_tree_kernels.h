@@ -446,18 +446,22 @@ __global__ __launch_bounds__(64 * RG * TG, 2) void tree_scan_kernel(std::conditi
         __syncthreads();
         if (r0 >= rows) return;  // padding: the wave has only its part of the tiles to do
 
-        // scores of the wave's tokens: register i of tile t is token w0 + tree_tok(t, 4 g + i)
-        f32x4 d[NCT][C::NTW];
+        // a wave that takes the whole chunk for 32 rows does so in halves, for their registers
+        constexpr int HV = WIN && RG == 8 ? C::NTW / 2 : 1, NT = C::NTW / HV;
 #pragma unroll
-        for (int t = 0; t < C::NTW; ++t)
+        for (int hf = 0; hf < HV; ++hf) {
+        // scores of the wave's tokens: register i of tile t is token w0 + tree_tok(t, 4 g + i)
+        f32x4 d[NCT][NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int ct = 0; ct < NCT; ++ct) d[ct][t] = f32x4{0.f, 0.f, 0.f, 0.f};
         // two tiles at a time, so that an accumulator's next product is 2 NCT instructions off
 #pragma unroll
-        for (int t0 = 0; t0 < C::NTW; t0 += 2)
+        for (int t0 = 0; t0 < NT; t0 += 2)
 #pragma unroll
           for (int k = 0; k < G::KS; ++k) {
-            const char* kp[2] = {lds + k_addr(t0, k), lds + k_addr(t0 + 1, k)};
+            const char* kp[2] = {lds + k_addr(NT * hf + t0, k), lds + k_addr(NT * hf + t0 + 1, k)};
             h8 kh[2], kl[2];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
@@ -480,7 +484,7 @@ __global__ __launch_bounds__(64 * RG * TG, 2) void tree_scan_kernel(std::conditi
         __builtin_amdgcn_sched_barrier(0);
         // value scale: every n_V < 2^(7 + gs), so 2^kTreeRescale n_V 2^-gs < 2^15 in fp16; it
         // follows the norms' magnitude (n_V = 2^-20 keeps its bits)
-        constexpr int KV = C::NTW / 2;
+        constexpr int KV = NT / 2;
         {
           const uint32_t* gm = reinterpret_cast<const uint32_t*>(lds + C::m_off);
           uint32_t top = gm[0];
@@ -503,7 +507,7 @@ __global__ __launch_bounds__(64 * RG * TG, 2) void tree_scan_kernel(std::conditi
         h8 nk[KV], nv[KV];
 #pragma unroll
         for (int ks = 0; ks < KV; ++ks) {
-          const uint16_t* np = reinterpret_cast<const uint16_t*>(lds + C::n_off) + w0 + 32 * ks + 8 * g;
+          const uint16_t* np = reinterpret_cast<const uint16_t*>(lds + C::n_off) + w0 + 32 * (KV * hf + ks) + 8 * g;
           nk[ks] = *reinterpret_cast<const h8*>(np);
           nv[ks] = *reinterpret_cast<const h8*>(np + G::CH);
         }
@@ -542,7 +546,7 @@ __global__ __launch_bounds__(64 * RG * TG, 2) void tree_scan_kernel(std::conditi
                 word = at >= 0 ? (vis << at | ((uint64_t(1) << at) - 1)) : at > -64 ? vis >> -at : 0;
               }
 #pragma unroll
-              for (int ks = 0; ks < KV; ++ks) seen[ks] = uint32_t(word >> (w0 + 32 * ks + 8 * g)) & 0xffu;
+              for (int ks = 0; ks < KV; ++ks) seen[ks] = uint32_t(word >> (w0 + 32 * (KV * hf + ks) + 8 * g)) & 0xffu;
             }
             const float m0 = (m[ct] == -INFINITY ? 0.f : m[ct]) + gsf;
             top[ct] = -INFINITY;
@@ -612,7 +616,7 @@ __global__ __launch_bounds__(64 * RG * TG, 2) void tree_scan_kernel(std::conditi
             h8 vh[MP], vl[MP];
 #pragma unroll
             for (int i = 0; i < MP; ++i) {
-              const char* vp = lds + v_addr(m0 + i, ks);
+              const char* vp = lds + v_addr(m0 + i, KV * hf + ks);
               vh[i] = *reinterpret_cast<const h8*>(vp);
               if constexpr (EX) vl[i] = *reinterpret_cast<const h8*>(vp + G::VT);
             }
@@ -629,6 +633,7 @@ __global__ __launch_bounds__(64 * RG * TG, 2) void tree_scan_kernel(std::conditi
               products(vh, pl);
             }
           }
+        }
       };
       for (int ch = ch_lo; ch < ch_hi; ch += AHEAD) {
         chunk(even, ch);
@@ -937,7 +942,7 @@ TreeKernelSet<WIN> tree_kernels() {
   TreeKernelSet<WIN> k;
   if constexpr (D == 256) {
     // 128 accumulator registers per 32 rows: sixteen rows a wave
-    k.scan[0] = k.scan[1] = k.scan[2] = tree_scan<D, EX, 1, 4, 1, W, WIN>();
+    k.scan[0] = k.scan[1] = k.scan[2] = k.scan[3] = tree_scan<D, EX, 1, 4, 1, W, WIN>();
   } else {
     k.scan[0] = tree_scan<D, EX, 1, 2, 2, W, WIN>();
     k.scan[1] = tree_scan<D, EX, 2, 2, 2, W, WIN>();
@@ -948,6 +953,7 @@ TreeKernelSet<WIN> tree_kernels() {
     // fills their waits (28 heads, 26 nodes: 41 us, eight waves 47).
     if constexpr (EX) k.scan[2] = tree_scan<D, EX, 2, 4, 2, W, WIN>();
     else k.scan[2] = tree_scan<D, EX, 2, 4, 1, W, WIN>();
+    if constexpr (WIN) k.scan[3] = tree_scan<D, EX, 2, 8, 1, W, WIN>();
   }
   k.rotate = tree_rotate_kernel<D, WIN>;
   k.merge[0] = tree_merge_kernel<D, 4, WIN>;
