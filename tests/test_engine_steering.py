@@ -159,3 +159,10 @@ def test_sinks_without_a_window():
     with pytest.raises(ValueError, match="window"):
         Engine(_Model(), pool, None, None, 128, config=EngineConfig(sinks=4))
     assert Request("r", [1], 2, logit_bias=None).logit_bias == {}
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (-3, 0), (2.5, 0), (8, -1)])
+def test_a_window_that_is_none(window, sinks):
+    pool = PagePool(num_layers=1, num_pages=4, num_kv_heads=1, page_size=16, nb_k=64, nb_v=64)
+    with pytest.raises(ValueError, match="at least"):
+        Engine(_Model(), pool, None, None, 128, config=EngineConfig(window=window, sinks=sinks))

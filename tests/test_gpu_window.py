@@ -296,3 +296,17 @@ def test_window_many_rows(D, Hq, Hkv, Q, splits, dtype):
     q, kv = _case(60 + D, lens, Hq, Hkv, D, Q, 4, 4, dtype=dtype)
     for window, sinks in ((100, 4), (33, 0)):
         _check(_run(q, kv, D ** -0.5, window, sinks, num_splits=splits), q, kv, D ** -0.5, window, sinks, dtype)
+
+
+@pytest.mark.parametrize("single", [False, True])
+@pytest.mark.parametrize("D,bwk,bwv", [(128, 4, 4), (128, 8, 3), (64, 4, 4), (64, 5, 6), (32, 4, 4), (32, 2, 8), (16, 4, 4), (16, 3, 3)])
+@pytest.mark.parametrize("Q", [61, 64])
+def test_window_blocks_of_256_rows(D, bwk, bwv, Q, single):
+    """Enough (sequence, kv head) pairs of 244 and 256 rows for the widest row blocks, every kind of kernel:
+    lengths of nothing, of part of the queries, across chunks; windows that begin and end inside one."""
+    lens = (Q + 300, 0, Q // 2, Q + 7, 2 * Q, 777)
+    q, kv = _case(70 + D + Q, lens, 24, 6, D, Q, bwk, bwv)
+    dkv, scale = to_device(kv, DEV), D ** -0.5
+    for window, sinks, splits in ((100, 5, None), (1, 0, 2), (2 ** 31, 0, 1), (64, 66, 7)):
+        got = _run(q, dkv, scale, window, sinks, num_splits=splits, allow_tf32=single)
+        _check(got, q, kv, scale, window, sinks, torch.float32, single=single)

@@ -49,6 +49,7 @@ import torch
 
 from winnow_amd.logits import MAX_BIASES, adjust_logits, mask_words, pack_allowed
 from winnow_amd.logprobs import MAX_TOP, token_logprobs
+from winnow_amd.packed_attention import check_window
 from winnow_amd.packed_backend import PagedPackedCache, fuse_rotary
 from winnow_amd.page_pool import PoolExhausted, default_fence
 
@@ -165,6 +166,8 @@ class Engine:
         self.cfg = config or EngineConfig()
         if self.cfg.window is None and self.cfg.sinks:
             raise ValueError("sinks stay in view beside a window: give one")
+        if self.cfg.window is not None:
+            check_window(self.cfg.window, self.cfg.sinks)
         self.clock = clock
         self.device = next(model.parameters()).device
         self.closed = False
