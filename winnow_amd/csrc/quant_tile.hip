@@ -49,6 +49,9 @@
 // eleven instructions per code to find its bucket, and the float64 norms and flagged
 // dot products; a launch of one pass per wave adds the staging and the latency of its
 // loads. Measured without gain: a touch of the next pass's rows ahead of it (40 us).
+//
+// With the rotation (ROT; wn_append_rotated_kv) the same 8,191 tokens, 32 query heads rotated beside them,
+// 4 bits bf16, take 61 us: 181 MB, 38 us at the rate of a copy; vector instructions issue in 63% of the cycles.
 #include <algorithm>
 #include <type_traits>
 

@@ -9,7 +9,8 @@
 // * the tree attention's (wn_tree.h, wn_tree_kernels.h), compiled for this choice of keys: q' = q Pi_K^T
 //   once, a scan of the chunks that some query of a row block sees (window_span), split where there are
 //   few blocks, and a merge with Pi_V. It serves every shape. 512 queries at a window of 4,096, 32 heads
-//   over 8, fp32 accuracy: 149 us of the call's 158, 0.7 PFLOP/s of fp16 products (three a factor).
+//   over 8, fp32 accuracy: 113 us of the call's 133 (125 of 157 in the first calls after a pause), 0.9 PFLOP/s of fp16 products (three a factor). Vector instructions (softmax, decoding) issue in
+//   54% of its cycles, products in 45%.
 // * one query at head_dim 128: the decode's row scan (wn_decode_rows.h) over the pages in view, laid out
 //   side by side by the launch that rotates the query (window_view, decode.hip). Between the last sink
 //   and the window's first position lie fewer than two pages of it, which it masks. 32 sequences at a
