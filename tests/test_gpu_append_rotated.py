@@ -198,3 +198,30 @@ def test_graph_replays_and_own_stream():
             graph.replay()
             want = call(eager)
             assert torch.equal(out, want) and all(torch.equal(x, y) for x, y in zip(pages, eager))
+
+
+@pytest.mark.parametrize("dtype,rot", [("bf16", "bf16"), ("fp16", "fp32"), ("fp32", "fp16"), ("fp32", "fp32")])
+@pytest.mark.parametrize("B,n,R,bwk,bwv", [(1, 1, 256, 4, 4), (3, 1, 64, 8, 8), (2, 17, 6, 3, 5), (2, 700, 256, 4, 6), (5, 33, 128, 2, 8)])
+def test_head_dim_256(B, n, R, bwk, bwv, dtype, rot):
+    """The matrix cores against ``append_kv``'s vector ALU: one vector, parts of a work-group's sixteen, many;
+    rotations that 16-byte loads read and ones that they do not."""
+    case = (B, 8, 2, n, 256, R, bwk, bwv, 16, dtype, rot)
+    q, k, v, *_ = _run(case, seed=B + n + R)
+    _run(case, seed=B + n, k=_misaligned(k), v=v)
+    _run(case, seed=B + n + 1, has_v=False, has_q=False)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_head_dim_256_extremes(dtype):
+    """Zero vectors, one channel, tiny and huge norms, values that are not finite."""
+    (_, k, v), _, _ = _inputs(2, 2, 2, 40, 256, 256, TYPES[dtype], TYPES[dtype], 3)
+    k, v = k.clone(), v.clone()
+    for x in (k, v):
+        x[:, :, 0] = 0
+        x[:, :, 1] = 0
+        x[:, :, 1, 77] = 3.0
+        x[:, :, 2] *= 1e-20
+        x[:, :, 3] *= 1e15
+        x[0, 0, 4, 9] = float("inf")
+        x[0, 1, 5, 200] = float("nan")
+    _run((2, 2, 2, 40, 256, 256, 4, 4, 16, dtype, dtype), seed=3, k=k, v=v, has_q=False)
