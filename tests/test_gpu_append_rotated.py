@@ -225,3 +225,21 @@ def test_head_dim_256_extremes(dtype):
         x[0, 0, 4, 9] = float("inf")
         x[0, 1, 5, 200] = float("nan")
     _run((2, 2, 2, 40, 256, 256, 4, 4, 16, dtype, dtype), seed=3, k=k, v=v, has_q=False)
+
+
+@pytest.mark.parametrize("rotated", [False, True])
+def test_start_positions_with_gaps_are_refused(rotated):
+    """They are read as a contiguous row."""
+    from winnow_amd.packed_attention import UnsupportedLayout
+    from winnow_amd.packed_backend import append_kv, append_rotated_kv
+    (q, k, v), cos, sin = _inputs(3, 4, 2, 2, 64, 64, torch.float32, torch.float32, 1)
+    table, start, (kp, vp, kn, vn) = _pool([1, 20, 33], 2, 2, 16, 64, 4, 4, 1)
+    before = kp.clone()
+    gaps = torch.stack([start, start + 7], 1)[:, 0]
+    kq, vq = _quantizers(4, 4, 64)
+    with pytest.raises(UnsupportedLayout, match="contiguous"):
+        if rotated:
+            append_rotated_kv(q, k, v, cos, sin, kq, vq, kp, vp, kn, vn, table, gaps)
+        else:
+            append_kv(k, v, kq, vq, kp, vp, kn, vn, table, gaps)
+    assert torch.equal(kp, before)

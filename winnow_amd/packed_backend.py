@@ -199,8 +199,8 @@ class AppendPlan:
         if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != B \
                 or page_table.stride(-1) != 1:
             raise pa.UnsupportedLayout("append: page_table must be (B, max_pages) int32 with contiguous rows")
-        if start_pos.dtype != torch.int32 or start_pos.shape != (B,):
-            raise pa.UnsupportedLayout("append: start_pos must be (B,) int32")
+        if start_pos.dtype != torch.int32 or start_pos.shape != (B,) or not start_pos.is_contiguous():
+            raise pa.UnsupportedLayout("append: start_pos must be (B,) int32, contiguous")
         return (k, v, page_table, start_pos, B, n)
 
     def launch(self, bound: tuple, timing_events=None) -> None:
