@@ -327,8 +327,9 @@ _here = contextlib.nullcontext()
 
 
 def on(device: torch.device):
-    """``torch.cuda.device(device)``, or nothing where that is the current one already."""
-    return _here if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    """``torch.cuda.device(device)`` of a tensor's device, or nothing where that is the current one already
+    (asked for directly: a tensor there means that the runtime is up)."""
+    return _here if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 def host_int32(t: torch.Tensor) -> bool:

@@ -53,7 +53,7 @@ def _whole(name: str, t: torch.Tensor, shape: tuple, device: torch.device) -> to
     if t.dtype == torch.int64:
         # of no vocabulary and no length that is served, and so where the type holds them
         t = t.clamp(-1, 2 ** 31 - 1).to(torch.int32)
-    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
 def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, lengths: torch.Tensor | None = None,
@@ -126,12 +126,16 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, 
         raise UnsupportedLayout("out shares memory with another operand")
     if N == 0:
         return out
+    (rep_t, rep_x), (pres_t, pres_x), (freq_t, freq_x) = rep, pres, freq
     with _lib.on(dev):
         _lib.call("wn_adjust_logits", logits.data_ptr(), _lib.DTYPE_CODE[logits.dtype], logits.stride(0), out.data_ptr(), out.stride(0), N, V,
-                  _lib.ptr(history), history.stride(0) if H else 0, H, _lib.ptr(lengths), _lib.ptr(prompt_lengths),
-                  _lib.ptr(rep[0]), _lib.ptr(pres[0]), _lib.ptr(freq[0]), rep[1], pres[1], freq[1],
-                  _lib.ptr(bias_ids), bias_ids.stride(0) if J else 0, _lib.ptr(bias), bias.stride(0) if J else 0, J,
-                  _lib.ptr(allowed), allowed.stride(0) if allowed is not None else 0, _lib.stream_of(dev))
+                  None if history is None else history.data_ptr(), history.stride(0) if H else 0, H,
+                  None if lengths is None else lengths.data_ptr(), None if prompt_lengths is None else prompt_lengths.data_ptr(),
+                  None if rep_t is None else rep_t.data_ptr(), None if pres_t is None else pres_t.data_ptr(),
+                  None if freq_t is None else freq_t.data_ptr(), rep_x, pres_x, freq_x,
+                  None if bias is None else bias_ids.data_ptr(), bias_ids.stride(0) if J else 0,
+                  None if bias is None else bias.data_ptr(), bias.stride(0) if J else 0, J,
+                  None if allowed is None else allowed.data_ptr(), 0 if allowed is None else allowed.stride(0), _lib.stream_of(dev))
     return out
 
 
