@@ -51,7 +51,8 @@
 // loads. Measured without gain: a touch of the next pass's rows ahead of it (40 us).
 //
 // With the rotation (ROT; wn_append_rotated_kv) the same 8,191 tokens, 32 query heads rotated beside them,
-// 4 bits bf16, take 61 us: 181 MB, 38 us at the rate of a copy; vector instructions issue in 63% of the cycles.
+// 4 bits bf16, take 61 us (68 where the 181 MB come from HBM, 38 us at the rate of a copy); vector
+// instructions issue in 63% of the cycles.
 #include <algorithm>
 #include <type_traits>
 
@@ -579,17 +580,21 @@ int launch_quantize_tiles(const QuantArgs& a, int sides, int D, hipStream_t st) 
   return launch_tiles<false>(D == 64 ? pick_tile<64, false>(a.x_dtype) : pick_tile<128, false>(a.x_dtype), a, sides, st);
 }
 
-// One work-group a CU, as many of them for K, V and q as their work takes of it: a vector of K, rotated,
-// counts 6.5, one of V 5.2, a row of q 1, one in fp32 2.2. (The 65,528 vectors each and 262,112 rows of an 8,191-token prompt, 128
-// bf16 at 4 bits, on 256 CUs by shares of K, V and q, us: 107, 86 and 63: 58; 86, 86, 84: 64; 128, 64, 64: 63; 86, 64,
-// 106: 66; 128, 86, 42: 75. A wave's passes are whole, so neighbours of the best are not always near it.)
+// One work-group a CU, as many of them for K, V and q as their work takes of it: a vector of K, rotated, counts
+// 6 and 0.035 per level of its codebook at head_dim 128, one of V 5 and 0.018 (a code near a level's end takes
+// a float64 product of its row, K's rotated again; with the width of what is near and the product's
+// length that share goes by D^2), a row of q 1.2, one in fp32 2.2. An 8,191-token prompt, 65,528 vectors each
+// and 262,112 rows, 128 bf16, on 256 CUs, from HBM, us by these weights and by 6.5, 5.2 and 1 for every width: 4 bits
+// 68 and 73, 6 bits 75 and 80, 8 bits 112 and 133, 8 and 4 101 and 132, 4 and 8 87 and 106. (From the 256 MB cache 61
+// at 4 bits, both. A wave's passes are whole, so neighbours of the best are not always near it.)
 int launch_quantize_tiles(const QuantRotArgs& args, int sides, int D, hipStream_t st) {
   const int cus = device_cus();
   if (cus <= 0) return WN_E_LAUNCH;
   QuantRotArgs a = args;
   const int64_t most = (a.total + kTileVecs - 1) / kTileVecs;  // passes of a side
-  const double k = 6.5 * double(a.total), v = sides > 1 ? 5.2 * double(a.total) : 0.0,
-               q = a.rot.q ? double(a.rot.B) * a.rot.Hq * a.n * (a.rot.q_dtype == WN_F32 ? 2.2 : 1.0) : 0.0, all = k + v + q;
+  const double d2 = double(D) * D / 16384.0, k = (6.0 + 0.035 * d2 * double(1 << a.side[0].bw)) * double(a.total),
+               v = sides > 1 ? (5.0 + 0.018 * d2 * double(1 << a.side[1].bw)) * double(a.total) : 0.0,
+               q = a.rot.q ? double(a.rot.B) * a.rot.Hq * a.n * (a.rot.q_dtype == WN_F32 ? 2.2 : 1.2) : 0.0, all = k + v + q;
   const auto share = [&](double w) { return int(std::min<double>(double(most), std::max(1.0, w / all * cus + 0.5))); };
   a.split[0] = share(k);
   a.split[1] = a.split[0] + (sides > 1 ? share(v) : 0);
