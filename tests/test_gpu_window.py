@@ -310,3 +310,20 @@ def test_window_blocks_of_256_rows(D, bwk, bwv, Q, single):
     for window, sinks, splits in ((100, 5, None), (1, 0, 2), (2 ** 31, 0, 1), (64, 66, 7)):
         got = _run(q, dkv, scale, window, sinks, num_splits=splits, allow_tf32=single)
         _check(got, q, kv, scale, window, sinks, torch.float32, single=single)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D,Hq,Hkv,Q", [(128, 16, 4, 150), (256, 8, 2, 131)])
+def test_window_many_rows_strided(D, Hq, Hkv, Q, dtype):
+    """As (B, Q, Hq, D) memory, aligned, and with rows of an odd length; the same bits."""
+    lens = (Q + 40, Q // 2, 300 + Q, Q, 90 + Q, Q + 7, 2 * Q, 1, 0, Q + 129, Q, Q) * 3
+    q, kv = _case(33 + D, lens, Hq, Hkv, D, Q, 4, 6, dtype=dtype)
+    dkv = to_device(kv, DEV)
+    want = _run(q, dkv, 0.1, 70, 3)
+    _check(want, q, kv, 0.1, 70, 3, dtype)
+    heads = q.to(DEV).transpose(1, 2).contiguous().transpose(1, 2)
+    odd = torch.zeros(len(lens), Q, Hq, D + 3, dtype=dtype, device=DEV)[..., 1:D + 1].transpose(1, 2)
+    odd.copy_(q)
+    for view in (heads, odd):
+        got = _pa().packed_window_attention(view, dkv, 0.1, window=70, sinks=3)
+        assert torch.equal(got.view(torch.uint8), want.view(torch.uint8))

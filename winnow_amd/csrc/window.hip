@@ -199,7 +199,11 @@ extern "C" int wn_window_attention(
   ra.exact = exact != 0;
   const int per = q_dtype == WN_F32 ? 4 : 8;  // elements of 16 bytes
   ra.vec = aligned(q, 16) && q_stride_b % per == 0 && q_stride_h % per == 0 && q_stride_q % per == 0;
-  hipLaunchKernelGGL(k.rotate, dim3(unsigned(tiles)), dim3(k.rotate_threads), 0, st, ra);
+  const int threads = window_row_threads(D);
+  const int64_t stay = int64_t(std::max(1, device_cus())) * (1024 / threads);  // 1,024 threads a compute unit
+  if (k.rotate_many && tiles * D >= (1 << 17))  // wn_window_rows.h has both sides
+    hipLaunchKernelGGL(k.rotate_many, dim3(unsigned(std::min(tiles, stay))), dim3(threads), 0, st, ra, int(tiles));
+  else hipLaunchKernelGGL(k.rotate, dim3(unsigned(tiles)), dim3(k.rotate_threads), 0, st, ra);
 
   WindowArgs a{};
   a.qh = ra.qh;
@@ -263,9 +267,7 @@ extern "C" int wn_window_attention(
   ma.chunk = window_chunk(D);
   const int64_t wide = int64_t(B) * Hkv * ((rows + 15) / 16);
   ma.tiles = int(wide);
-  const int threads = window_merge_threads(D);
-  const int64_t stay = int64_t(std::max(1, device_cus())) * (1024 / threads);  // 1,024 threads a compute unit
-  // few splits, or many rows: wn_window_merge.h has both sides
+  // few splits, or many rows: wn_window_rows.h has both sides
   if (num_splits <= 8 || wide >= 128)
     hipLaunchKernelGGL(k.merge[1], dim3(unsigned(std::min(wide, stay))), dim3(threads), 0, st, ma);
   else hipLaunchKernelGGL(k.merge[0], dim3(unsigned(int64_t(B) * Hkv * ((rows + 3) / 4))), dim3(1024), 0, st, ma);

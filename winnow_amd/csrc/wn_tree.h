@@ -240,8 +240,8 @@ struct WindowMergeArgs : TreeMergeArgs {
   int tiles;  // of sixteen rows of a unit, over all of them
 };
 
-// Of window_merge_kernel: a wave per 16 columns, four at least.
-__host__ __device__ constexpr int window_merge_threads(int D) { return 4 * D > 256 ? 4 * D : 256; }
+// Of window_rotate_kernel and window_merge_kernel: a wave per 16 columns, four at least.
+__host__ __device__ constexpr int window_row_threads(int D) { return 4 * D > 256 ? 4 * D : 256; }
 
 // The chunks that the queries of rows r0 .. r0 + rows - 1 of a (sequence, kv head) look at: those that
 // hold sinks, then those from the first query's window to the last query. `total` of them, counted as
@@ -270,7 +270,9 @@ __host__ __device__ inline WindowSpan window_span(int L, int T, int n_rep, int r
   return w;
 }
 
-using WindowKernels = TreeKernelsOf<WindowArgs, WindowMergeArgs>;
+struct WindowKernels : TreeKernelsOf<WindowArgs, WindowMergeArgs> {
+  void (*rotate_many)(TreeRotArgs, int) = nullptr;  // of many tiles of sixteen rows, from head_dim 128 on
+};
 WindowKernels window_kernels_16(bool exact, int bw_k, int bw_v);
 WindowKernels window_kernels_32(bool exact, int bw_k, int bw_v);
 WindowKernels window_kernels_64(bool exact, int bw_k, int bw_v);

@@ -929,7 +929,7 @@ __global__ __launch_bounds__(1024) void tree_merge_kernel(std::conditional_t<WIN
 template <bool WIN>
 using TreeArgsOf = std::conditional_t<WIN, WindowArgs, TreeArgs>;
 template <bool WIN>
-using TreeKernelSet = std::conditional_t<WIN, WindowKernels, TreeKernels>;
+using TreeKernelSet = std::conditional_t<WIN, TreeKernelsOf<WindowArgs, WindowMergeArgs>, TreeKernels>;
 
 template <int D, bool EX, int NCT, int RG, int TG, int W, bool WIN>
 TreeScanOf<TreeArgsOf<WIN>> tree_scan() {

@@ -1,4 +1,6 @@
-// Merge of the windowed attention's partials by work-groups that stay: each keeps its part of the
+// Rotation and merge of the windowed attention's rows by work-groups that stay (the rotation: below).
+//
+// The merge: each keeps its part of the
 // rotation in registers and takes tile after tile of sixteen rows, the next tile's partials on their way
 // while one is multiplied. tree_merge_kernel<D, 4> reads the 4 D^2 bytes of the rotation once for every four rows, but
 // joins the splits of a row by a whole wave. us in traces, it and this, by head_dim, tiles and splits:
@@ -18,10 +20,79 @@
 namespace wn {
 namespace {
 
+// q' of every row, as tree_rotate_kernel writes it, for many tiles of sixteen rows: a work-group keeps its
+// part of Pi_K and takes tile after tile, the next one's rows on their way while one is multiplied.
+// us in traces, a work-group a tile and this: head_dim 256, 504 tiles 25.8 and 21.3, 7,104 297 and 158 (fp32 matrix cores: 93); head_dim
+// 128, 512 tiles 8.1 and 8.5, 1,024 13.8 and 13.6, 4,000 39 and 34, 7,700 62 and 54. At head_dim 64 a rotation is 16 KB, and 4,000 tiles
+// take 15.9 and 16.3.
+template <int D>
+__global__ __launch_bounds__(window_row_threads(D)) void window_rotate_kernel(TreeRotArgs a, int tiles) {
+  constexpr int XS = D + 4, EPT = 16 * D / window_row_threads(D), DPT = D / 16;
+  static_assert(EPT == 4 && DPT >= 8, "16 or 8 bytes a load, 16 a store");
+  __shared__ __align__(16) float x[16 * XS];
+  __shared__ __align__(16) float y[16 * XS];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, per = a.nrp / 16, rows = a.n_rep * a.T;
+  TreeProduct<D> pi;
+  pi.load(wave, lane, [&](int j, int k) { return *reinterpret_cast<const f32x4*>(a.pi + j * D + k); });
+  const int rr = tid * EPT / D, d0 = tid * EPT % D;  // the thread's elements of a tile
+  f32x4 v;
+  const auto fetch = [&](int tile) {
+    const int unit = tile / per, r = 16 * (tile % per) + rr, kvh = unit % a.Hkv;
+    v = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (r >= rows) return;  // padding
+    const int64_t o = int64_t(unit / a.Hkv) * a.qsb + (kvh * a.n_rep + r % a.n_rep) * a.qsh + (r / a.n_rep) * a.qsq + d0;
+    if (a.vec && a.q_dtype == WN_F32) {
+      v = *reinterpret_cast<const f32x4*>(static_cast<const float*>(a.q) + o);
+    } else if (a.vec) {
+      const uint2 h = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.q) + o);
+      const uint32_t w[4] = {h.x & 0xffffu, h.x >> 16, h.y & 0xffffu, h.y >> 16};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = a.q_dtype == WN_BF16 ? bf16_to_f32(uint16_t(w[e])) : f16_to_f32(uint16_t(w[e]));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = load_elem(a.q, o + e, a.q_dtype);
+    }
+  };
+  fetch(blockIdx.x);
+  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    *reinterpret_cast<f32x4*>(x + rr * XS + d0) = v;
+    __syncthreads();  // x; and y of the tile before is read
+    if (tile + int(gridDim.x) < tiles) fetch(tile + gridDim.x);
+    const int g = lane >> 4, c = lane & 15;
+    *reinterpret_cast<f32x4*>(y + c * XS + 16 * wave + 4 * g) = pi.run(x + c * XS, lane);
+    __syncthreads();  // y; and x is read
+    if (tid < 256) {
+      // sixteen threads a row: its largest magnitude, then the fp16 terms of q' 2^e (below 2^15)
+      const int r = tid >> 4, k = tid & 15;
+      float w[DPT], top = 0.f;
+      __builtin_memcpy(w, __builtin_assume_aligned(y + r * XS + DPT * k, 16), 4 * DPT);
+#pragma unroll
+      for (int d = 0; d < DPT; ++d) top = fmaxf(top, fabsf(w[d]));
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 16));
+      int qe;
+      frexpf(fminf(top, 3.0e38f), &qe);
+      const int e = min(15 - qe, 120);
+      const float up = ldexpf(1.f, e);
+      const int64_t row = int64_t(tile) * 16 + r;  // a unit's rows are nrp, a multiple of sixteen
+      if (k == 0) a.qs[row] = ldexpf(a.scale, -(e + 8));
+      _Float16 h[DPT], l[DPT];
+#pragma unroll
+      for (int d = 0; d < DPT; ++d) {
+        const float t = w[d] * up;
+        h[d] = _Float16(t);
+        l[d] = _Float16(t - float(h[d]));
+      }
+      __builtin_memcpy(__builtin_assume_aligned(a.qh + row * D + DPT * k, 16), h, 2 * DPT);
+      if (a.exact) __builtin_memcpy(__builtin_assume_aligned(a.ql + row * D + DPT * k, 16), l, 2 * DPT);
+    }
+  }
+}
+
 // A lane takes EPT elements of one row, its splits one after the other.
 template <int D>
-__global__ __launch_bounds__(window_merge_threads(D)) void window_merge_kernel(WindowMergeArgs a) {
-  constexpr int XS = D + 4, EPT = 16 * D / window_merge_threads(D);
+__global__ __launch_bounds__(window_row_threads(D)) void window_merge_kernel(WindowMergeArgs a) {
+  constexpr int XS = D + 4, EPT = 16 * D / window_row_threads(D);
   constexpr int U = D == 256 ? 1 : 8;  // splits loaded at once (at 256 the rotation takes half of the 128 registers)
   __shared__ __align__(16) float x[2][16 * XS];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, rows = a.n_rep * a.T, blocks = (rows + 15) / 16, Hq = a.Hkv * a.n_rep;
@@ -90,8 +161,10 @@ __global__ __launch_bounds__(window_merge_threads(D)) void window_merge_kernel(W
 
 template <int D>
 WindowKernels window_kernels_for(bool exact, int bw_k, int bw_v) {
-  WindowKernels k = tree_kernels_for<D, true>(exact, bw_k, bw_v);
+  WindowKernels k;
+  static_cast<TreeKernelsOf<WindowArgs, WindowMergeArgs>&>(k) = tree_kernels_for<D, true>(exact, bw_k, bw_v);
   k.merge[1] = window_merge_kernel<D>;
+  if constexpr (D >= 128) k.rotate_many = window_rotate_kernel<D>;
   return k;
 }
 
