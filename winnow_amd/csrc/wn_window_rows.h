@@ -1,9 +1,8 @@
 // Rotation and merge of the windowed attention's rows by work-groups that stay (the rotation: below).
 //
-// The merge: each keeps its part of the
-// rotation in registers and takes tile after tile of sixteen rows, the next tile's partials on their way
-// while one is multiplied. tree_merge_kernel<D, 4> reads the 4 D^2 bytes of the rotation once for every four rows, but
-// joins the splits of a row by a whole wave. us in traces, it and this, by head_dim, tiles and splits:
+// The merge: each keeps its part of the rotation in registers and takes tile after tile of sixteen rows, the
+// next tile's partials on their way while one is multiplied. tree_merge_kernel<D, 4> reads the 4 D^2 bytes of
+// the rotation once for every four rows, but joins the splits of a row by a whole wave. us in traces, it and this, by head_dim, tiles and splits:
 //   128    8 tiles   2 splits  6.4   4.8     8 splits  6.1   5.3     32 splits  6.0   9.4
 //   128  128 tiles   2 splits 12.5   5.1     8 splits 12.6   6.1     32 splits 14.6  12.8
 //   128  384 tiles   2 splits 34     8.0     8 splits 34    10.4     32 splits 37    26
