@@ -524,7 +524,7 @@ int wn_append_rotated_kv(
 
 /* Attention over paged packed K/V under a sliding window with sinks, Q >= 1 queries per sequence, which
  * are its last Q positions: the query at position p sees the positions j <= p with p - j < window
- * or j < sinks; one that sees none (p < 0) gives 0.
+ * or j < sinks; one that sees none (p < 0) gives 0, one that is NaN or sees a norm that is gives NaN.
  *   q    (B, Hq, Q, D) with element strides, last dim contiguous, type q_dtype
  *   out  (B, Hq, Q, D) contiguous, type out_dtype
  * The algebra, pages, norms, table, rotations, `exact` and alignments are those of wn_tree_attention;

@@ -1,0 +1,64 @@
+"""``packed_window_attention`` at the edges of what it is given: queries and norms that are not finite.
+
+Tolerances as in test_gpu_window.py, whose checks these are.
+"""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from cases import to_device
+from test_gpu_window import DEV, _case, _check, _run
+
+pytestmark = pytest.mark.gpu
+
+# D, Hq, Hkv, Q, splits: rows merged sixteen at a time from few splits and from many, by fours, and the row scan
+ROWS = [(128, 8, 2, 12, None), (128, 8, 2, 12, 13), (128, 8, 2, 200, None), (64, 14, 2, 5, 1), (64, 8, 8, 33, 12), (256, 4, 2, 9, 2),
+        (32, 8, 2, 7, None), (16, 8, 4, 3, 2), (128, 32, 8, 1, None), (64, 8, 2, 1, None)]
+
+
+@pytest.mark.parametrize("single", [False, True])
+@pytest.mark.parametrize("D,Hq,Hkv,Q,splits", ROWS)
+def test_a_query_that_is_not_finite_has_no_finite_answer(D, Hq, Hkv, Q, splits, single):
+    """Every score of its row is NaN, in every split; no other row shows it."""
+    q, kv = _case(900 + D + Q, (Q + 300, Q + 5, Q + 77), Hq, Hkv, D, Q, 4, 4)
+    dkv = to_device(kv, DEV)
+    bad = q.clone()
+    for b, h, i in ((0, 1, Q // 2), (1, Hq - 1, Q - 1), (2, 0, 0)):
+        bad[b, h, i, (b + 5) % D] = float("nan")
+    for window, sinks in ((100, 4), (1, 0), (2 ** 31, 0)):
+        got = _run(bad, dkv, 0.1, window, sinks, num_splits=splits, allow_tf32=single)
+        hit = bad.isnan().any(-1)
+        assert not torch.isfinite(got.cpu()[hit]).any()
+        clean = _run(q, dkv, 0.1, window, sinks, num_splits=splits, allow_tf32=single)
+        got[hit.to(DEV)] = clean[hit.to(DEV)]
+        _check(got, q, kv, 0.1, window, sinks, torch.float32, single=single)
+
+
+@pytest.mark.parametrize("D,Hq,Hkv,Q,splits", ROWS)
+def test_the_only_key_in_view_is_not_finite(D, Hq, Hkv, Q, splits):
+    """A window of one position: the row whose own key's norm is NaN has nothing else to answer with."""
+    q, kv = _case(950 + D + Q, (Q + 130, Q + 5), Hq, Hkv, D, Q, 4, 4)
+    clean = _run(q, kv, 0.1, 1, 0, num_splits=splits)
+    _check(clean, q, kv, 0.1, 1, 0, torch.float32)
+    at = Q + 130 - 1 - Q // 2
+    kv.k_norms[kv.page_table[0, at // 16], :, at % 16] = float("nan")
+    got = _run(q, kv, 0.1, 1, 0, num_splits=splits)
+    row = Q - 1 - Q // 2
+    assert not torch.isfinite(got[0, :, row]).any()
+    got[0, :, row] = clean[0, :, row]
+    assert torch.equal(got, clean)
+
+
+def test_one_query_of_many_sequences():
+    """Enough (sequence, kv head) pairs for the merge of four heads at once."""
+    lens = tuple(20 + 3 * b for b in range(72))
+    q, kv = _case(71, lens, 16, 8, 128, 1, 4, 4)
+    bad = q.clone()
+    bad[3, 5], bad[70, 15] = float("nan"), float("nan")
+    got, clean = _run(bad, kv, 0.1, 30, 2).cpu(), _run(q, kv, 0.1, 30, 2).cpu()
+    _check(clean, q, kv, 0.1, 30, 2, torch.float32)
+    hit = bad.isnan().any(-1)
+    assert got[hit].isnan().all()
+    got[hit] = clean[hit]
+    _check(got, q, kv, 0.1, 30, 2, torch.float32)

@@ -155,7 +155,13 @@ struct MergeArgs {
   void* out;
   int out_dtype, Hq, Hkv, n_rep;
   int log2_units;  // partial maxima are in log2 units (weights 2^(m - M))
+  int keep_nan;    // a sum that is NaN gives NaN (windows); else 0, as where no key was seen
 };
+
+// Whether a head's merged sums are an answer.
+__device__ __forceinline__ bool merged(const MergeArgs& a, int n, float den) {
+  return n > 0 && (den > 0.f || (a.keep_nan && __builtin_isnan(den)));
+}
 
 constexpr int kMergeBatch = 32;  // partial rows whose loads are in flight together
 
@@ -231,7 +237,7 @@ __global__ __launch_bounds__(merge_threads<D>()) void merge_kernel(MergeArgs a) 
       }
     }
   }
-  if (tid < D) av[d] = (n > 0 && den > 0.f) ? num / fmaxf(den, 1e-30f) : 0.f;
+  if (tid < D) av[d] = merged(a, n, den) ? num / fmaxf(den, 1e-30f) : 0.f;
   __syncthreads();
   if (tid >= D) return;
   // out_j = sum_k a_k Pi_V[k, j]; (a / l) Pi_V == (a Pi_V) / l up to rounding
@@ -307,7 +313,7 @@ __global__ __launch_bounds__(64 * kMergeHeads) void merge4_kernel(MergeArgs a) {
         }
       }
     }
-    const bool some = n > 0 && den > 0.f;
+    const bool some = merged(a, n, den);
     av[wave][2 * lane] = some ? num.x / fmaxf(den, 1e-30f) : 0.f;
     av[wave][2 * lane + 1] = some ? num.y / fmaxf(den, 1e-30f) : 0.f;
   }
@@ -885,7 +891,7 @@ int window_rows_attention(const WindowStep& s) {
   hipLaunchKernelGGL(sk.fn, dim3(unsigned((s.num_splits + sk.wpb - 1) / sk.wpb)), dim3(sk.block), 0, st, da);
   if (s.ev_end) (void)hipEventRecord(static_cast<hipEvent_t>(s.ev_end), st);
 
-  MergeArgs ma{da.part_acc, da.part_ml, s.pi_v, ra.unit_meta, s.out, s.out_dtype, s.Hq, Hkv_s, n_rep_s, 1};
+  MergeArgs ma{da.part_acc, da.part_ml, s.pi_v, ra.unit_meta, s.out, s.out_dtype, s.Hq, Hkv_s, n_rep_s, 1, 1};
   launch_merge(128, dim3(n_rep_s, Hkv_s, s.B), st, ma);
   return check_launch("wn_window_attention");
 }

@@ -127,8 +127,9 @@ __global__ __launch_bounds__(window_row_threads(D)) void window_merge_kernel(Win
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (s + u >= live) break;
-        if (ml[u].x == -INFINITY) continue;  // a split that saw no key
-        const float up = fmaxf(M, ml[u].x), old = __builtin_amdgcn_exp2f(M - up), w = __builtin_amdgcn_exp2f(ml[u].x - up);
+        // a split that saw no key has weight 0, and so has one whose every score is NaN: its sums are NaN, and stay so
+        const float up = fmaxf(M, ml[u].x), top = up == -INFINITY ? 0.f : up;
+        const float old = __builtin_amdgcn_exp2f(M - top), w = __builtin_amdgcn_exp2f(ml[u].x - top);
         den = den * old + w * ml[u].y;
 #pragma unroll
         for (int e = 0; e < EPT; ++e) num[e] = num[e] * old + w * v[u][e];

@@ -836,7 +836,8 @@ def packed_window_attention(q: torch.Tensor, kv: PackedKV, scale: float, *, wind
     The cache already holds the Q >= 1 queries' tokens, as after ``append_kv``: query i of a sequence of
     length L is position p = L - Q + i. It sees the positions j <= p with p - j < ``window`` or
     j < ``sinks``; a query with p < 0 sees none and gives 0. With a window of L or more it is the causal
-    mask of the decode and the prefill.
+    mask of the decode and the prefill. NaN in a query or in a norm that it sees gives NaN (where the
+    decode and the prefill give 0), in no other query.
 
     What no query sees is not read: a call costs the window, not the context, and page table entries
     wholly outside may be -1 (their pages released). Every head_dim, width pair, n_rep and page
