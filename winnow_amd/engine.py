@@ -47,7 +47,7 @@ from dataclasses import dataclass, field
 
 import torch
 
-from winnow_amd.logits import MAX_BIASES, adjust_logits, mask_words, pack_allowed
+from winnow_amd.logits import MAX_BIASES, adjust_logits, fp32, mask_words, pack_allowed
 from winnow_amd.logprobs import MAX_TOP, token_logprobs
 from winnow_amd.packed_attention import check_window
 from winnow_amd.packed_backend import PagedPackedCache, fuse_rotary
@@ -145,9 +145,9 @@ _RULES = (
      lambda e, r: f"must be 1..{e.cfg.max_new_tokens_cap}"),
     ("bad_top_logprobs", lambda e, r: r.top_logprobs is not None and not 0 <= r.top_logprobs <= MAX_TOP,
      lambda e, r: f"must be 0..{MAX_TOP}"),
-    ("bad_penalty", lambda e, r: not (math.isfinite(r.repetition_penalty) and r.repetition_penalty > 0
-                                      and math.isfinite(r.presence_penalty) and math.isfinite(r.frequency_penalty)),
-     lambda e, r: "penalties must be finite, the repetition's above 0"),
+    ("bad_penalty", lambda e, r: not (0 < fp32(r.repetition_penalty) < math.inf
+                                      and math.isfinite(fp32(r.presence_penalty)) and math.isfinite(fp32(r.frequency_penalty))),
+     lambda e, r: "penalties must be finite in fp32, the repetition's above 0"),
     ("bad_logit_bias", lambda e, r: len(r.logit_bias) > MAX_BIASES or any(math.isnan(x) for x in r.logit_bias.values()),
      lambda e, r: f"at most {MAX_BIASES} biases, none of them NaN"),
     ("exceeds_request_cap", lambda e, r: e._worst_pages(r) > e.pool.max_pages_per_request,

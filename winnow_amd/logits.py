@@ -7,6 +7,7 @@ their ``repetition_penalty``, ``presence_penalty``, ``frequency_penalty``, ``log
 ``allowed_tokens``. There is no host fallback."""
 from __future__ import annotations
 
+import ctypes
 import math
 
 import torch
@@ -31,14 +32,22 @@ def pack_allowed(allowed: torch.Tensor) -> torch.Tensor:
     return torch.where(words >= 2 ** 31, words - 2 ** 32, words).to(torch.int32)
 
 
+def fp32(value) -> float:
+    """What a number becomes in the type that it is applied in: infinite past fp32's range, 0 below it."""
+    try:
+        return ctypes.c_float(float(value)).value
+    except OverflowError:
+        return math.inf if value > 0 else -math.inf
+
+
 def _penalty(name: str, value, N: int, device: torch.device) -> tuple:
     """(tensor or None, scalar) of a penalty given as a number or one per row."""
     if not isinstance(value, torch.Tensor):
         if type(value) is float and (value == 0.0 if name != "repetition" else value == 1.0):
             return None, value
-        value = float(value)
+        value = fp32(value)
         if not math.isfinite(value) or (name == "repetition" and value <= 0):
-            raise UnsupportedLayout(f"{name} must be finite{' and above 0' if name == 'repetition' else ''}, got {value}")
+            raise UnsupportedLayout(f"{name} must be finite{' and above 0' if name == 'repetition' else ''} in fp32, got {value} there")
         return None, value
     if value.shape != (N,) or value.dtype != torch.float32 or value.device != device or not value.is_contiguous():
         raise UnsupportedLayout(f"{name} must be a number or ({N},) fp32 on {device}, contiguous, got "
@@ -69,7 +78,7 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, 
       (all H without it). A token that occurs has its logit divided by ``repetition`` where it is
       positive and multiplied by it elsewhere. Of those from ``prompt_lengths`` (N,) on (0 without
       it: all), one that occurs c > 0 times loses ``frequency`` c + ``presence``. The penalties are
-      numbers or (N,) fp32. Tokens outside [0, V) are ignored.
+      numbers (finite in fp32, ``repetition`` above 0) or (N,) fp32. Tokens outside [0, V) are ignored.
     * ``bias`` (N, J) fp32 is added to the logits of the tokens ``bias_ids`` (N, J), J <= 1024; ids
       outside [0, V) pad the list; a token listed more than once gets each of its biases, in order.
     * ``allowed`` (N, ceil(V / 32)) int32: the logit of token v becomes -inf where bit v % 32 of
