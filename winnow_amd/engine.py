@@ -135,6 +135,13 @@ class EngineConfig:
     fuse_rotary: bool = False      # packed_backend.fuse_rotary on the model
 
 
+def _biases_fit(bias: dict) -> bool:
+    try:
+        return len(bias) <= MAX_BIASES and not any(math.isnan(fp32(x)) for x in bias.values()) and all(int(t) is not None for t in bias)
+    except (TypeError, ValueError, OverflowError):
+        return False
+
+
 # Admission rules in the order they are checked: (reason, refused?, detail).
 _RULES = (
     ("shutting_down", lambda e, r: e.closed, lambda e, r: ""),
@@ -148,8 +155,8 @@ _RULES = (
     ("bad_penalty", lambda e, r: not (0 < fp32(r.repetition_penalty) < math.inf
                                       and math.isfinite(fp32(r.presence_penalty)) and math.isfinite(fp32(r.frequency_penalty))),
      lambda e, r: "penalties must be finite in fp32, the repetition's above 0"),
-    ("bad_logit_bias", lambda e, r: len(r.logit_bias) > MAX_BIASES or any(math.isnan(x) for x in r.logit_bias.values()),
-     lambda e, r: f"at most {MAX_BIASES} biases, none of them NaN"),
+    ("bad_logit_bias", lambda e, r: not _biases_fit(r.logit_bias),
+     lambda e, r: f"at most {MAX_BIASES} biases, none of them NaN, of tokens by their ids"),
     ("exceeds_request_cap", lambda e, r: e._worst_pages(r) > e.pool.max_pages_per_request,
      lambda e, r: f"{e._worst_pages(r)} pages > {e.pool.max_pages_per_request}"),
 )
@@ -388,9 +395,10 @@ class Engine:
                 kw["repetition"], kw["presence"], kw["frequency"] = pen[0], pen[1], pen[2]
             J = max(len(r.logit_bias) for r in asked)
             if J:
-                pad = [list(r.logit_bias.items()) + [(-1, 0.0)] * (J - len(r.logit_bias)) for r in asked]
-                kw["bias_ids"] = torch.tensor([[int(t) for t, _ in row] for row in pad], dtype=torch.int64).to(dev)
-                kw["bias"] = torch.tensor([[float(x) for _, x in row] for row in pad], dtype=torch.float32).to(dev)
+                pad = [[(int(t), fp32(x)) for t, x in r.logit_bias.items()] + [(-1, 0.0)] * (J - len(r.logit_bias)) for r in asked]
+                # an id outside the vocabulary pads the list: some integer type may not hold it
+                kw["bias_ids"] = torch.tensor([[t if 0 <= t < vocab else -1 for t, _ in row] for row in pad], dtype=torch.int32).to(dev)
+                kw["bias"] = torch.tensor([[x for _, x in row] for row in pad], dtype=torch.float32).to(dev)
             if words is not None:
                 kw["allowed"] = words.to(dev)
             at = torch.tensor(rows, device=dev)
