@@ -26,6 +26,17 @@ def test_biases_that_are_none(monkeypatch, bias):
     assert err.value.reason == "bad_logit_bias"
 
 
+@pytest.mark.parametrize("prompt", [(9, 10, 11, 12, 10), range(4, 9)])
+def test_prompts_that_are_other_sequences(monkeypatch, prompt):
+    e = _engine(monkeypatch)
+    a = e.submit(Request("a", prompt, 5, repetition_penalty=1.7))
+    b = e.submit(Request("b", [1, 2, 3], 5, presence_penalty=0.5))
+    e.run_until_idle(50)
+    a.prompt_ids = list(prompt)
+    for r in (a, b):
+        assert r.status == "length" and r.generated == _expected(r, 5), (r.request_id, r.detail)
+
+
 def test_biases_by_text_keys(monkeypatch):
     """As a request in JSON has them."""
     e = _engine(monkeypatch)

@@ -340,7 +340,7 @@ class Engine:
             held = self._history_of[slot]
             have = held[1] if held is not None and held[0] is r else 0
             total = len(r.prompt_ids) + len(r.generated)
-            tokens = (r.prompt_ids[have:] if have < len(r.prompt_ids) else []) + r.generated[max(0, have - len(r.prompt_ids)):]
+            tokens = [*r.prompt_ids[have:], *r.generated[max(0, have - len(r.prompt_ids)):]]
             slots.append(slot)
             at += [slot * self._history.shape[1] + k for k in range(have, total)]
             new += tokens
