@@ -44,3 +44,18 @@ def test_biases_by_text_keys(monkeypatch):
     e.run_until_idle(20)
     r.logit_bias = {33: 2.5}
     assert r.generated == _expected(r, 3)
+
+
+@pytest.mark.parametrize("ask", [dict(repetition_penalty=2.0), dict(frequency_penalty=3.0, presence_penalty=1.0)])
+def test_a_request_object_that_is_used_again(monkeypatch, ask):
+    """In the slot that it had, with a shorter prompt: its tokens of the first time, which the second run would
+    make next, are not held against it."""
+    e = _engine(monkeypatch, max_batch=1)
+    r = Request("r", [42, 60, 43, 44, 44, 44, 60], 4, **ask)
+    e.submit(r)
+    e.run_until_idle(50)
+    assert r.status == "length" and r.generated == _expected(r, 4)
+    vars(r).update(vars(Request("r", [40, 41], 4, **ask)))
+    e.submit(r)
+    e.run_until_idle(50)
+    assert r.status == "length" and r.generated == _expected(r, 4) == [42, 43, 44, 45]
