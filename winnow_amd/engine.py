@@ -50,7 +50,7 @@ import torch
 from winnow_amd.logits import MAX_BIASES, adjust_logits, fp32, mask_words, pack_allowed
 from winnow_amd.logprobs import MAX_TOP, token_logprobs
 from winnow_amd.packed_attention import check_window
-from winnow_amd.packed_backend import PagedPackedCache, fuse_rotary
+from winnow_amd.packed_backend import PagedPackedCache, rotary_layers
 from winnow_amd.page_pool import PoolExhausted, default_fence
 
 
@@ -132,7 +132,9 @@ class EngineConfig:
     # not in the reference: attend to the last ``window`` positions and the first ``sinks`` only
     window: int | None = None
     sinks: int = 0
-    fuse_rotary: bool = False      # packed_backend.fuse_rotary on the model
+    # the position rotation in the cache's append, for this engine's requests (None: as
+    # packed_backend.fuse_rotary left the model)
+    fuse_rotary: bool | None = None
 
 
 def _biases_fit(bias: dict) -> bool:
@@ -190,7 +192,7 @@ class Engine:
         self._history: torch.Tensor | None = None    # (max_batch, ...) int32: a row's tokens, of the request below
         self._history_of: list[tuple[Request, int] | None] = [None] * self.cfg.max_batch    # ... and how many of them
         if self.cfg.fuse_rotary:
-            fuse_rotary(model)
+            rotary_layers(model)
 
     def _worst_pages(self, req: Request) -> int:
         return self.pool.pages_for(len(req.prompt_ids) + req.max_new_tokens)
@@ -318,7 +320,7 @@ class Engine:
         cache = PagedPackedCache(self.pool, [r.request_id for r in reqs], [r.stored for r in reqs],
                                  k_quant=self.kq, v_quant=self.vq, head_dim=self.head_dim,
                                  decode_backend=self.cfg.decode_backend, allow_tf32=self.cfg.allow_tf32,
-                                 window=self.cfg.window, sinks=self.cfg.sinks)
+                                 window=self.cfg.window, sinks=self.cfg.sinks, fuse_rotary=self.cfg.fuse_rotary)
         out = self.model(input_ids=ids, position_ids=positions, past_key_values=cache, use_cache=True,
                          logits_to_keep=1)
         for r, stored in zip(reqs, cache.lengths):

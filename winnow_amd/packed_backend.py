@@ -485,11 +485,15 @@ class PagedPackedCache:
     ``window`` limits what the new tokens attend to: the last ``window`` positions up to their own and
     the sequence's first ``sinks`` (``packed_attention.packed_window_attention``). Positions are
     those of the whole sequence, and the cache keeps all of it.
+
+    ``fuse_rotary`` says whether attention layers that ``fuse_rotary(model)`` has given their class let the
+    append apply the position rotation; without it they do as that call left them. Layers without the
+    class rotate by themselves.
     """
 
     def __init__(self, pool: PagePool, owners, lengths, *, k_quant, v_quant,
                  head_dim: int, decode_backend: str = "auto", allow_tf32: bool = False, tree=None,
-                 window: int | None = None, sinks: int = 0):
+                 window: int | None = None, sinks: int = 0, fuse_rotary: bool | None = None):
         if len(owners) != len(lengths):
             raise ValueError("one length per owner")
         if window is None and sinks:
@@ -497,6 +501,7 @@ class PagedPackedCache:
         if window is not None and tree is not None:
             raise ValueError("a tree of drafted tokens attends to the whole history: no window")
         self.window, self.sinks = (None, 0) if window is None else pa.check_window(window, sinks)
+        self.fuse_rotary = fuse_rotary
         self.tree = None if tree is None else _tree_parents(tree, len(owners))
         self._tree_device: torch.Tensor | None = None
         self.pool = pool
@@ -1017,9 +1022,10 @@ _ROTATED: dict[type, type] = {}
 
 def _rotated_class(base: type) -> type:
     """The class of a Qwen2 attention module whose rotation the cache's append applies: one launch writes K and
-    V and rotates q, in place of the rotation's elementary operations and an append. Calls that it does
-    not serve (no paged packed cache, another attention implementation, gradients, traces, autocast to
-    another type) go through the base's forward. A class, and no function set on the module: a copy
+    V and rotates q, in place of the rotation's elementary operations and an append. Calls that do not ask for
+    it (``PagedPackedCache.fuse_rotary``, or where that is None the layer's ``rotary_fused``) and those that
+    it does not serve (no paged packed cache, another attention implementation, gradients, traces, autocast
+    to another type) go through the base's forward. A class, and no function set on the module: a copy
     of the model then runs with its own weights."""
     if base in _ROTATED:
         return _ROTATED[base]
@@ -1027,6 +1033,7 @@ def _rotated_class(base: type) -> type:
     def forward(self, hidden_states, position_embeddings=None, attention_mask=None, past_key_values=None, **kwargs):
         cache = past_key_values
         if not isinstance(cache, PagedPackedCache) or cache.pool.dense or position_embeddings is None \
+                or not (self.rotary_fused if cache.fuse_rotary is None else cache.fuse_rotary) \
                 or self.config._attn_implementation != ATTN_NAME or torch.is_grad_enabled() or not _plain(hidden_states):
             return base.forward(self, hidden_states=hidden_states, position_embeddings=position_embeddings, attention_mask=attention_mask,
                                 past_key_values=past_key_values, **kwargs)
@@ -1036,23 +1043,31 @@ def _rotated_class(base: type) -> type:
         out, weights = winnow_packed_attention(self, q, handle, handle, attention_mask, scaling=self.scaling)
         return self.o_proj(out.reshape(*shape, -1)), weights
 
-    _ROTATED[base] = type("Rotated" + base.__name__, (base,), {"forward": forward, "__module__": __name__})
+    _ROTATED[base] = type("Rotated" + base.__name__, (base,), {"forward": forward, "rotary_fused": False, "__module__": __name__})
     return _ROTATED[base]
 
 
-def fuse_rotary(model) -> int:
-    """Let the cache's append apply the position rotation in every attention layer of ``model``
-    (``append_rotated_kv``): K is then quantized from its fp32 rotation, not from one rounded to the
-    model's type. Returns the number of layers; a layer that has it already keeps it. Raises
-    ``UnsupportedModel`` for an architecture that this path does not serve."""
+def rotary_layers(model) -> list:
+    """The attention layers of ``model``, each with a class whose forward can let the cache's append apply the
+    position rotation; what they do by themselves does not change. Raises ``UnsupportedModel`` for an
+    architecture that this path does not serve."""
     if _arch(model.config) not in SUPPORTED_ARCH:
         raise UnsupportedModel(f"{_arch(model.config)} is not a supported architecture {SUPPORTED_ARCH}")
-    count = 0
     for m in model.modules():
         if type(m).__name__ == "Qwen2Attention":
             m.__class__ = _rotated_class(type(m))
-        count += type(m) in _ROTATED.values()
-    return count
+    return [m for m in model.modules() if type(m) in _ROTATED.values()]
+
+
+def fuse_rotary(model, on: bool = True) -> int:
+    """Let the cache's append apply the position rotation in every attention layer of ``model``
+    (``append_rotated_kv``), for every ``PagedPackedCache`` that does not say otherwise: K is then quantized
+    from its fp32 rotation, not from one rounded to the model's type. ``on=False`` takes it back. Returns
+    the number of layers. Raises ``UnsupportedModel`` for an architecture that this path does not serve."""
+    layers = rotary_layers(model)
+    for m in layers:
+        m.rotary_fused = on
+    return len(layers)
 
 
 def register() -> None:
