@@ -4,8 +4,9 @@
 // quantize (turboquant_kv/cache.py:108-115):
 //   n = max(||x||_2, 1e-10);  y = (x / n) Pi^T;  code = #{boundaries < y}
 // A work-group quantizes sixteen vectors (quantize_kernel on the float64 matrix
-// cores at head_dim 64 and 128, with K's rotation at 256 too; quantize_any_kernel on the vector ALU at
-// the others); many vectors at 64 and 128 run on quant_tile.hip, with the same codes. The squared norm and the rotation are
+// cores at head_dim 64, 128 and 256; quantize_any_kernel on the vector ALU at 16 and 32); many
+// vectors at 64 and 128 run on quant_tile.hip, with the same codes. A head_dim's sums are formed in one
+// order, whatever the entry point, so equal vectors have equal codes. The squared norm and the rotation are
 // accumulated in float64 from exact fp32 inputs and rounded once to fp32, and
 // x / n is the correctly rounded fp32 quotient, so every code is the bucket of
 // the correctly rounded fp32 y; an fp32 GEMM elsewhere can differ from it only
@@ -60,7 +61,9 @@ __device__ __forceinline__ uint8_t packed_byte(const uint8_t* codes, int k, int 
 template <bool ROT>
 using AppendArgs = std::conditional_t<ROT, QuantRotArgs, QuantArgs>;
 
-// Threads of quantize_kernel: at head_dim 256 a wave keeps 32 rows of Pi, as at 128.
+// Threads of quantize_kernel: at head_dim 256 a wave keeps 32 rows of Pi, as at 128. K and V of 8 heads there,
+// 4 bits, calls: one token of one or two sequences 19.5 us, of 64 20; 2 x 2,000 tokens 299, 8.4
+// GFLOP in float64 (on the vector ALU, as quantize_any_kernel: 35 to 38, 39, 474).
 constexpr int quantize_threads(int D) { return D > 128 ? 2 * kQBlock : kQBlock; }
 
 template <int D, bool ROT>
@@ -238,10 +241,10 @@ __global__ __launch_bounds__(quantize_threads(D)) void quantize_kernel(AppendArg
   }
 }
 
-// The same computation for the head dims without the matrix-core kernel (16, 32,
-// 256), on the vector ALU: a work-group quantizes sixteen vectors; norms as above
-// (float64 sums of squares, x / n rounded once to fp32 into LDS), then thread j
-// forms output dims j, j + 256, ... of every vector as float64 dot products with the
+// The same computation for the head dims without the matrix-core kernel (16 and 32),
+// on the vector ALU: a work-group quantizes sixteen vectors; norms as above
+// (float64 sums of squares, x / n rounded once to fp32 into LDS), then thread j < D
+// forms output dim j of every vector as float64 dot products with the
 // rows of Pi (each product exact, the sum in float64, rounded once to fp32),
 // bucketizes them into the LDS codes, and the store phase packs and scatters as
 // quantize_kernel does.
@@ -488,12 +491,7 @@ static int launch_quantize(AppendArgs<ROT>& a, int sides, int D, hipStream_t st,
     case 32: hipLaunchKernelGGL(HIP_KERNEL_NAME(quantize_any_kernel<32, ROT>), grid, dim3(kQBlock), 0, st, a); break;
     case 64: hipLaunchKernelGGL(HIP_KERNEL_NAME(quantize_kernel<64, ROT>), grid, dim3(kQBlock), 0, st, a); break;
     case 128: hipLaunchKernelGGL(HIP_KERNEL_NAME(quantize_kernel<128, ROT>), grid, dim3(kQBlock), 0, st, a); break;
-    case 256:
-      // one token of two sequences, 8 heads, on the matrix cores 20 us and on the vector ALU 45; 2,000
-      // tokens 163 and 248 (without q and the rotation)
-      if constexpr (ROT) hipLaunchKernelGGL(HIP_KERNEL_NAME(quantize_kernel<256, true>), grid, dim3(quantize_threads(256)), 0, st, a);
-      else hipLaunchKernelGGL(HIP_KERNEL_NAME(quantize_any_kernel<256, false>), grid, dim3(kQBlock), 0, st, a);
-      break;
+    case 256: hipLaunchKernelGGL(HIP_KERNEL_NAME(quantize_kernel<256, ROT>), grid, dim3(quantize_threads(256)), 0, st, a); break;
   }
   if (ev_end) (void)hipEventRecord(static_cast<hipEvent_t>(ev_end), st);
   return check_launch(what);
