@@ -62,3 +62,18 @@ def test_one_query_of_many_sequences():
     assert got[hit].isnan().all()
     got[hit] = clean[hit]
     _check(got, q, kv, 0.1, 30, 2, torch.float32)
+
+
+@pytest.mark.parametrize("L,Q,window", [(9000, 129, 64), (9000, 130, 1), (9000, 257, 16), (9000, 400, 700), (300, 200, 64), (9000, 128, 64)])
+def test_a_plan_has_splits_for_its_longest_row_block(L, Q, window):
+    """Full row blocks span more positions than a partial last one. Planned for one sequence on an idle
+    device, every chunk of the longest block has a split of its own."""
+    from winnow_amd import packed_attention as pa
+    q, kv = _case(7, (L,), 2, 2, 128, Q, 4, 4)
+    splits, span = pa.window_plan_for(q.to(DEV), to_device(kv, DEV), window, 4, True)
+    rows, longest = 32 if Q <= 32 else 64 if Q <= 64 else 128, 0
+    for r0 in range(0, Q, rows):
+        p = range(L - Q + r0, L - Q + min(r0 + rows, Q))
+        lo, hi = max(p[0] - window + 1, 0), p[-1] + 1
+        longest = max(longest, len({j // 64 for j in range(lo, hi)} | {0}))
+    assert span == 64 and splits >= longest

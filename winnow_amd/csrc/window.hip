@@ -82,10 +82,14 @@ extern "C" int wn_window_plan(int B, int Hq, int Hkv, int Q, int D, int S, int b
   const int blocks = tree_nrp(scan, rows) / scan.rows;
   const int n = lens ? B : 1;
   const int64_t each = (lens ? 1 : std::max(B, 1)) * int64_t(Hkv) * blocks;  // work-groups per entry of lens and split
-  // chunks of a sequence's last row block: the others have as many, or fewer
+  // chunks of a sequence's last row block, or, where rows fill only part of that and so span fewer positions,
+  // the more of its and the one's before: the others have as many, fewer, or by where they begin one more
   auto chunks = [&](int b) {
     const int L = int(std::min<int64_t>(std::max(lens ? lens[b] : max_pages * S, 0), int64_t(max_pages) * S));
-    return int64_t(std::max(window_span(L, Q, n_rep, (blocks - 1) * scan.rows, scan.rows, ch, window, sinks, 1, ch).total, 1));
+    int64_t most = 1;
+    for (int blk = blocks - 1; blk >= 0 && blk >= blocks - (rows % scan.rows ? 2 : 1); --blk)
+      most = std::max<int64_t>(most, window_span(L, Q, n_rep, blk * scan.rows, scan.rows, ch, window, sinks, 1, ch).total);
+    return most;
   };
   int64_t longest = 1;
   for (int b = 0; b < n; ++b) longest = std::max(longest, chunks(b));
