@@ -529,7 +529,8 @@ int wn_append_rotated_kv(
  *   out  (B, Hq, Q, D) contiguous, type out_dtype
  * The algebra, pages, norms, table, rotations, `exact` and alignments are those of wn_tree_attention;
  * n_rep * Q <= 2^20, S a power of two >= 16. Pages that no query of the call sees are not used: their
- * ids may be any value. num_splits and span come from wn_window_plan; any num_splits 1 .. 4096 and
+ * ids may be any value. (The row scan reads a page whole that is partly in view; the tile scan chunks of 64
+ * positions, 32 at head_dim 256.) num_splits and span come from wn_window_plan; any num_splits 1 .. 4096 and
  * any span > 0 that is a multiple of 64 are valid for any lengths. span 0 is the row scan of one query
  * at head_dim 128, num_splits waves of it (any number >= 1): the plan chooses it where `wide` says
  * that pages and norms meet wn_decode_attention's alignments and stride limits, which the call

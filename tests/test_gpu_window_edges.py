@@ -77,3 +77,13 @@ def test_a_plan_has_splits_for_its_longest_row_block(L, Q, window):
         lo, hi = max(p[0] - window + 1, 0), p[-1] + 1
         longest = max(longest, len({j // 64 for j in range(lo, hi)} | {0}))
     assert span == 64 and splits >= longest
+
+
+@pytest.mark.parametrize("Q", [1, 9])
+@pytest.mark.parametrize("S", [1024, 4096])
+@pytest.mark.parametrize("D,bw", [(128, 4), (64, 8)])
+def test_pages_of_many_chunks(D, bw, S, Q):
+    """Views that begin and end inside a page much longer than the window."""
+    q, kv = _case(40 + S + Q, (9, S + 1, 2 * S + 700, 3 * S), 4, 2, D, Q, bw, bw, S=S)
+    for window, sinks in ((1, 0), (64, 4), (200, 1100), (5000, 65)):
+        _check(_run(q, kv, 0.1, window, sinks), q, kv, 0.1, window, sinks, torch.float32)

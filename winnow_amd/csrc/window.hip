@@ -3,8 +3,8 @@
 // p - j < window or j < sinks,
 //   out = softmax(scale q . k_hat) v_hat,   k_hat = n_K (c_K Pi_K),   v_hat = n_V (c_V Pi_V).
 //
-// Host side. What lies between the sinks and the window is not read: a call costs the window, not the
-// context. Two scans:
+// Host side. What lies between the sinks and the window is passed over, in chunks of 64 positions or in pages:
+// a call costs the window and up to three of these, not the context. Two scans:
 //
 // * the tree attention's (wn_tree.h, wn_tree_kernels.h), compiled for this choice of keys: q' = q Pi_K^T
 //   once, a scan of the chunks that some query of a row block sees (window_span), split where there are
@@ -12,10 +12,11 @@
 //   over 8, fp32 accuracy: 113 us of the call's 133 (125 of 157 in the first calls after a pause), 0.9 PFLOP/s of fp16 products (three a factor). Vector instructions (softmax, decoding) issue in
 //   54% of its cycles, products in 45%.
 // * one query at head_dim 128: the decode's row scan (wn_decode_rows.h) over the pages in view, laid out
-//   side by side by the launch that rotates the query (window_view, decode.hip). Between the last sink
-//   and the window's first position lie fewer than two pages of it, which it masks. 32 sequences at a
-//   window of 8,192, 32 heads over 8, 4 bits: 75 us, 3.7 TB/s; a step of one user at 1,024: 20 us, three
-//   launches' latency.
+//   side by side by the launch that rotates the query (window_view, decode.hip). It reads these pages whole
+//   and masks what is out of view of them. 32 sequences at a window of 8,192, 32 heads over 8, 4 bits,
+//   pages of 16: 69 us, 4.0 TB/s; a step of one user at 1,024: 20 us, three launches' latency. Pages much
+//   longer than the window are where the tile scan, which passes over chunks, would read less: 32 sequences at
+//   a window of 64, us by row scan and tile scan: pages of 16 23 and 28, of 1,024 33 and 28, of 4,096 48 and 28.
 #include "wn_decode.h"
 #include "wn_tree_host.h"
 

@@ -839,8 +839,10 @@ def packed_window_attention(q: torch.Tensor, kv: PackedKV, scale: float, *, wind
     mask of the decode and the prefill. NaN in a query or in a norm that it sees gives NaN (where the
     decode and the prefill give 0), in no other query.
 
-    What no query sees is not read: a call costs the window, not the context, and page table entries
-    wholly outside may be -1 (their pages released). Every head_dim, width pair, n_rep and page
+    What no query sees is passed over, by chunks of 64 positions (32 at head_dim 256) or, for one query on the
+    row scan, by whole pages, of which those partly in view are read whole: a call costs the window, up
+    to three of these units, and not the context. Page table entries wholly outside may be -1 (their pages
+    released). Every head_dim, width pair, n_rep and page
     size of ``packed_decode_attention`` is served, Q up to 2^20 / n_rep. Products have fp32 accuracy
     whatever the query's type, or, where ``allow_tf32`` is given, TF32-class accuracy (single fp16
     operands, fp32 accumulation), as in the decode. ``num_splits`` asks for so many splits of the
