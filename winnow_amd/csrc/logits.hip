@@ -298,7 +298,7 @@ extern "C" int wn_adjust_logits(const void* logits, int dtype, int64_t stride, v
              WN_E_INVALID, "adjust_logits: operands aligned to their type");
   const LogitsPlan plan = pick_logits(dtype, N, V, H, J);
   const int nseg = (V - 1) / plan.seg + 1;
-  WN_REQUIRE(N <= INT32_MAX / nseg, WN_E_INVALID, "adjust_logits: grid too large");
+  WN_REQUIRE(N <= INT32_MAX / nseg && grid_fits(N * nseg, plan.threads), WN_E_INVALID, "adjust_logits: grid too large");
   LogitsArgs a;
   a.x = logits;
   a.out = out;

@@ -476,10 +476,11 @@ static int launch_quantize(AppendArgs<ROT>& a, int sides, int D, hipStream_t st,
     q = a.rot.q != nullptr;
     if (q) groups = std::max<int64_t>(groups, std::min<int64_t>((int64_t(a.rot.B) * a.rot.Hq * a.n * (D / 8) + kQBlock - 1) / kQBlock, 2048));
   }
-  dim3 grid(unsigned(groups), sides + q);
-  if (ev_begin) (void)hipEventRecord(static_cast<hipEvent_t>(ev_begin), st);
   bool tiles = quantize_tiles_ok(a, sides, D);
   if constexpr (ROT) tiles = tiles && a.rot.k_vec;
+  WN_REQUIRE(tiles || grid_fits(groups, quantize_threads(D)), WN_E_INVALID, "%s: %lld vectors, the grid would be too large", what, (long long)a.total);
+  const dim3 grid(unsigned(groups), sides + q);
+  if (ev_begin) (void)hipEventRecord(static_cast<hipEvent_t>(ev_begin), st);
   if (tiles) {
     const int rc = launch_quantize_tiles(a, sides, D, st);
     if (rc != WN_OK) {

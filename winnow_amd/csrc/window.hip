@@ -180,7 +180,7 @@ extern "C" int wn_window_attention(
              "window: workspace needs %lld bytes, 256-aligned (got %lld)", (long long)lay.total, (long long)workspace_bytes);
   // work-groups in eights: a unit's row blocks, which read much the same rows, on one XCD
   const int64_t tiles = int64_t(B) * Hkv * (nrp / 16), groups = (int64_t(B) * num_splits * Hkv + 7) / 8 * 8 * ncg;
-  WN_REQUIRE(tiles < (int64_t(1) << 31) && groups < (int64_t(1) << 31), WN_E_INVALID, "window: grid too large");
+  WN_REQUIRE(grid_fits(tiles, k.rotate_threads) && grid_fits(groups, scan.threads), WN_E_INVALID, "window: grid too large");
   const int lds = tree_lds(scan, bw_k, bw_v);
   WN_REQUIRE(tree_slots(scan, lds) > 0, WN_E_LAUNCH, "window: cannot query the device occupancy");
 

@@ -28,6 +28,9 @@ int check_launch(const char* what);
 // Compute units of the current device, asked for once per device; 0: the query failed.
 int device_cus();
 
+// Whether a launch of so many work-groups along x is one: HIP takes fewer than 2^32 threads.
+inline bool grid_fits(int64_t groups, int64_t threads) { return groups < (int64_t(1) << 32) && groups * threads < (int64_t(1) << 32); }
+
 inline bool is_pow2(int64_t x) { return x > 0 && (x & (x - 1)) == 0; }
 inline int ilog2(int64_t x) {
   int r = 0;
