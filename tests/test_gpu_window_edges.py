@@ -87,3 +87,40 @@ def test_pages_of_many_chunks(D, bw, S, Q):
     q, kv = _case(40 + S + Q, (9, S + 1, 2 * S + 700, 3 * S), 4, 2, D, Q, bw, bw, S=S)
     for window, sinks in ((1, 0), (64, 4), (200, 1100), (5000, 65)):
         _check(_run(q, kv, 0.1, window, sinks), q, kv, 0.1, window, sinks, torch.float32)
+
+
+@pytest.mark.parametrize("value", [float("inf"), -float("inf")])
+@pytest.mark.parametrize("D,Hq,Hkv,Q,splits", ROWS)
+@pytest.mark.parametrize("single", [False, True])
+def test_an_infinite_query_beside_large_ones(D, Hq, Hkv, Q, splits, single, value):
+    """A head of infinities does not move its neighbours."""
+    q, kv = _case(300 + D + Q, (Q + 300, Q + 5), Hq, Hkv, D, Q, 4, 4, q_scale=30.0)
+    dkv = to_device(kv, DEV)
+    bad = q.clone()
+    bad[0, 1, Q // 2, 3:] = value
+    bad[1, Hq - 1, Q - 1, :] = value
+    got = _run(bad, dkv, 0.1, 100, 4, num_splits=splits, allow_tf32=single)
+    clean = _run(q, dkv, 0.1, 100, 4, num_splits=splits, allow_tf32=single)
+    hit = (bad != q).any(-1).to(DEV)
+    assert not torch.isfinite(got[hit]).any()
+    got[hit] = clean[hit]
+    _check(got, q, kv, 0.1, 100, 4, torch.float32, single=single)
+
+
+@pytest.mark.parametrize("side", ["k_norms", "v_norms"])
+@pytest.mark.parametrize("D,Hq,Hkv,Q,splits", ROWS)
+def test_a_norm_in_view_that_is_nan(D, Hq, Hkv, Q, splits, side):
+    """Among many other keys: the rows that see it are NaN, the others' bits are those without it."""
+    L = Q + 300
+    q, kv = _case(350 + D + Q, (L, Q + 5), Hq, Hkv, D, Q, 4, 4)
+    clean = _run(q, kv, 0.1, 64, 2, num_splits=splits)
+    at = L - 32 - (Q + 1) // 2
+    getattr(kv, side)[kv.page_table[0, at // 16], :, at % 16] = float("nan")
+    got = _run(q, kv, 0.1, 64, 2, num_splits=splits)
+    for i in range(Q):
+        p = L - Q + i
+        if at <= p < at + 64:
+            assert got[0, :, i].isnan().all()
+        else:
+            assert torch.equal(got[0, :, i], clean[0, :, i])
+    assert torch.equal(got[1], clean[1])
