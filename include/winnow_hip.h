@@ -503,8 +503,9 @@ int wn_token_logprobs(const void* logits, int dtype, int64_t stride_outer, int64
  *   q         (B, Hq, n, D) with element strides, last dim contiguous, type q_dtype; or null
  *   q_out     (B, Hq, n, D) contiguous, type q_dtype, 16-byte aligned; may not be q
  * Channel d < rot_dim / 2 becomes x_d cos_d - x_(d + rot_dim / 2) sin_d, d < rot_dim
- * x_d cos_d + x_(d - rot_dim / 2) sin_d: exact products, the sum rounded once to fp32. K is quantized
- * as that fp32 value, with wn_append_kv's codes and norms of it; q is rounded to its type. Other
+ * x_d cos_d + x_(d - rot_dim / 2) sin_d: exact products, their sum formed in float64 and rounded to fp32
+ * (for two 16-bit types rounded to fp32 at once, to the same value). K is quantized as that fp32 value, with
+ * wn_append_kv's codes and norms of it; q is rounded to its type. Other
  * operands, preconditions and errors as wn_append_kv. B * Hq * n * D < 2^33. */
 int wn_append_rotated_kv(
     const void* q, int64_t qs_b, int64_t qs_h, int64_t qs_n, int q_dtype, int Hq, void* q_out,

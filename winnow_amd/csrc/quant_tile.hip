@@ -52,7 +52,11 @@
 //
 // With the rotation (ROT; wn_append_rotated_kv) the same 8,191 tokens, 32 query heads rotated beside them,
 // 4 bits bf16, take 61 us (68 where the 181 MB come from HBM, 38 us at the rate of a copy); vector
-// instructions issue in 63% of the cycles.
+// instructions issue in 63% of the cycles. What they do beyond the kernel without it: V is carried as fp32,
+// whose low term is zero for 16-bit rows and still takes its product, and every instantiation spills, 19 of 128
+// VGPRs at head_dim 64 and 27 to 47 at 128, with reloads in the pass. q's part of the kernel, which holds the
+// code of every type, has a share in it: compiled without that none spills at 64, 7 to 24 VGPRs at 128. (The
+// kernels without any rotation spill none.)
 #include <algorithm>
 #include <type_traits>
 
@@ -280,7 +284,7 @@ __global__ __launch_bounds__(64 * tile_waves<G2>()) void quantize_tile_kernel(Ti
 #pragma unroll
         for (int k = 0; k < 8; ++k) y[k] = elem<DT>(x, k);
       }
-      __builtin_amdgcn_sched_barrier(0);  // one eight's operands at a time: of all four they would spill
+      __builtin_amdgcn_sched_barrier(0);  // one eight's operands at a time: of all four more would spill
       return __builtin_bit_cast(Raw8<XT>, y);
     } else {
       return load8<DT>(sd.x, xo + d);
@@ -586,7 +590,8 @@ int launch_quantize_tiles(const QuantArgs& a, int sides, int D, hipStream_t st) 
 // length that share goes by D^2), a row of q 1.2, one in fp32 2.2. An 8,191-token prompt, 65,528 vectors each
 // and 262,112 rows, 128 bf16, on 256 CUs, from HBM, us by these weights and by 6.5, 5.2 and 1 for every width: 4 bits
 // 68 and 73, 6 bits 75 and 80, 8 bits 112 and 133, 8 and 4 101 and 132, 4 and 8 87 and 106. (From the 256 MB cache 61
-// at 4 bits, both. A wave's passes are whole, so neighbours of the best are not always near it.)
+// at 4 bits, both. A wave's passes are whole, so neighbours of the best are not always near it.) This is the one
+// head layout that was measured; that the shares carry over to others and to head_dim 64 is arithmetic.
 int launch_quantize_tiles(const QuantRotArgs& args, int sides, int D, hipStream_t st) {
   const int cus = device_cus();
   if (cus <= 0) return WN_E_LAUNCH;

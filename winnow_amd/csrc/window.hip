@@ -14,7 +14,7 @@
 // * one query at head_dim 128: the decode's row scan (wn_decode_rows.h) over the pages in view, laid out
 //   side by side by the launch that rotates the query (window_view, decode.hip). It reads these pages whole
 //   and masks what is out of view of them. 32 sequences at a window of 8,192, 32 heads over 8, 4 bits,
-//   pages of 16: 69 us, 4.0 TB/s; a step of one user at 1,024: 20 us, three launches' latency. Pages much
+//   pages of 16: 71 us, 3.9 TB/s; a step of one user at 1,024: 20 us, three launches' latency. Pages much
 //   longer than the window are where the tile scan, which passes over chunks, would read less: 32 sequences at
 //   a window of 64, us by row scan and tile scan: pages of 16 23 and 28, of 1,024 33 and 28, of 4,096 48 and 28.
 #include "wn_decode.h"

@@ -10,10 +10,6 @@
 
 namespace wn {
 
-// Tiles of 16 rows from which a work-group merges a whole one (4 rows each below: 16 tiles merged from
-// 10 splits took 7.7 us a tile to a work-group, 6.0 us in fours).
-constexpr int64_t kMergeTiles = 256;
-
 // Query rows per kv head, padded to whole work-groups.
 template <class Args>
 int tree_nrp(const TreeScanOf<Args>& s, int64_t rows) { return int((rows + s.rows - 1) / s.rows * s.rows); }

@@ -342,8 +342,9 @@ def append_rotated_kv(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor |
 
         x_d cos_d - x_(d + R/2) sin_d  (d < R/2),    x_d cos_d + x_(d - R/2) sin_d  (R/2 <= d < R)
 
-    Each product is exact and the sum is rounded once to fp32: the pages hold what ``append_kv``
-    writes for that fp32 K, bit for bit, and the returned q, (B, Hq, n, D) contiguous, is rounded
+    Each product is exact, and their sum is formed in float64 and rounded to fp32 (for two 16-bit types
+    rounded to fp32 at once, to the same value): the pages hold what ``append_kv`` writes for that fp32 K,
+    bit for bit, and the returned q, (B, Hq, n, D) contiguous, is rounded
     once more to its type (None without q). A model that rotates K itself rounds it to its own
     type before it is quantized.
 
