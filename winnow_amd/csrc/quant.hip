@@ -61,6 +61,10 @@ __device__ __forceinline__ uint8_t packed_byte(const uint8_t* codes, int k, int 
 template <bool ROT>
 using AppendArgs = std::conditional_t<ROT, QuantRotArgs, QuantArgs>;
 
+// Most work-groups that rotate q beside the quantizing ones: an item and a stride of the threads of all of
+// them, below 2^30 and 2^29, do not pass 2^32 together.
+constexpr uint32_t kRotGroups = 1u << 20;
+
 // Threads of quantize_kernel: at head_dim 256 a wave keeps 32 rows of Pi, as at 128. K and V of 8 heads there,
 // 4 bits, calls: one token of one or two sequences 19.5 us, of 64 20; 2 x 2,000 tokens 299, 8.4
 // GFLOP in float64 (on the vector ALU, as quantize_any_kernel: 35 to 38, 39, 474).
@@ -84,7 +88,8 @@ __global__ __launch_bounds__(quantize_threads(D)) void quantize_kernel(AppendArg
 
   if constexpr (ROT) {
     if (blockIdx.y == gridDim.y - 1 && a.rot.q) {
-      rotate_queries<D, NT>(a.rot, a.n, blockIdx.x, gridDim.x, threadIdx.x);
+      const uint32_t groups = min(gridDim.x, kRotGroups);
+      if (blockIdx.x < groups) rotate_queries<D, NT>(a.rot, a.n, blockIdx.x, groups, threadIdx.x);
       return;
     }
   }
@@ -261,7 +266,8 @@ __global__ __launch_bounds__(kQBlock) void quantize_any_kernel(AppendArgs<ROT> a
 
   if constexpr (ROT) {
     if (blockIdx.y == gridDim.y - 1 && a.rot.q) {
-      rotate_queries<D, kQBlock>(a.rot, a.n, blockIdx.x, gridDim.x, threadIdx.x);
+      const uint32_t groups = min(gridDim.x, kRotGroups);
+      if (blockIdx.x < groups) rotate_queries<D, kQBlock>(a.rot, a.n, blockIdx.x, groups, threadIdx.x);
       return;
     }
   }
